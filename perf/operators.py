@@ -259,8 +259,7 @@ def work(case):
 def _exact_e4m3(v):
     """Nearest E4M3 value of float64 v, ties to even, from the format's definition."""
     a = v.abs()
-    e = torch.floor(torch.log2(a.clamp_min(2.0 ** -20))).clamp(-6, 8)
-    step = torch.pow(2.0, e - 3)
+    step = torch.ldexp(torch.ones_like(a), torch.frexp(a)[1].clamp(-5, 9) - 4)
     return torch.sign(v) * (torch.round(a / step) * step).clamp_max(448.0)
 
 
@@ -274,7 +273,8 @@ def _exact_product(x, w):
     for b in range(0, k, 128):
         xb = x[:, b:b + 128].double()
         amax = xb.abs().amax(1, keepdim=True).clamp_min(2.0 ** -100)
-        sx = torch.pow(2.0, torch.ceil(torch.log2(amax / 448.0)))
+        m, e = torch.frexp(amax / 448.0)
+        sx = torch.ldexp(torch.ones_like(m), e - (m == 0.5).int())
         y += (_exact_e4m3(xb / sx) @ codes[:, b:b + 128].double().T) * sx * scale[block_of, b // 128].double()
     return y
 
