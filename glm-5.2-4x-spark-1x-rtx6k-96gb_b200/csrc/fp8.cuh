@@ -1,0 +1,47 @@
+// Number formats and the activation quantiser's block arithmetic of the 8-bit products (fp8.cu).
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace glmrt {
+
+constexpr int kFp8Block = 128;   // columns per activation scale, rows and columns per weight scale
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float fp8_input(uint16_t v) { return bf16_bits_to_f32(v); }
+__device__ __forceinline__ float fp8_input(float v) { return v; }
+__device__ __forceinline__ void fp8_store(uint16_t* p, float v) { *p = f32_to_bf16_rne(v); }
+__device__ __forceinline__ void fp8_store(float* p, float v) { *p = v; }
+
+__device__ __forceinline__ float e4m3_to_f32_nan(uint8_t b) {
+  return (b & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : e4m3_to_f32(b);
+}
+
+// Scale of a block whose largest magnitude has the bits `amax`: the smallest power of two with
+// amax / scale <= 448 = 1.75 * 2^8, so one exponent comparison decides it.  Blocks below 2^-100 are
+// scaled as if they reached it (their codes are then zero or tiny); a block with an infinity or a NaN gets
+// the scale NaN, which makes every output of its row NaN.
+__device__ __forceinline__ float fp8_block_scale(uint32_t amax, float* inv) {
+  if (amax >= 0x7f800000u) {
+    *inv = 0.0f;
+    return __uint_as_float(0x7fc00000u);
+  }
+  amax = max(amax, (127u - 100u) << 23);
+  const int e = static_cast<int>(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);   // -108 .. 120
+  *inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+// Four values to E4M3, nearest even (the inputs are at most 448 in magnitude).
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+__device__ __forceinline__ float fp8_swiglu(float g, float u) {
+  // fast exponential and division: a few units in the last place, against codes of four bits
+  return __fdividef(g, 1.0f + __expf(-g)) * u;
+}
+#endif
+
+}  // namespace glmrt

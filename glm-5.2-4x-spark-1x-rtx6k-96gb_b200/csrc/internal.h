@@ -300,4 +300,21 @@ bool pair_tiles_supported(const FfnArgs& a, int sm_count);
 glmrt_status_t launch_fc1_tc_pair(const FfnArgs& a, const TensorMaps& maps, int sm_count, cudaStream_t stream);
 glmrt_status_t launch_fc2_tc_pair(const FfnArgs& a, const TensorMaps& maps, int sm_count, cudaStream_t stream);
 
+// ---- few.cu (a whole layer for a few tokens on bf16 activations) ----
+constexpr int kFewMaxRows = 16;
+struct FewArgs {
+  const uint16_t* hidden_rows;                              // [rows, hidden] bf16
+  const uint16_t *residual, *shared;                        // [rows, hidden] bf16 or nullptr
+  uint16_t* out;                                            // [rows, hidden] bf16
+  const uint8_t *gate_codes, *up_codes, *down_codes;        // stacked experts, as in FfnArgs
+  const uint8_t *gate_sf, *up_sf, *down_sf;                 // tiled scales
+  const float* scale2;                                      // [experts][3]
+  uint32_t* topk_idx;                                       // [rows * top_k]
+  float* topk_w;
+  float* act;                                               // [rows * top_k, inter] weighted SwiGLU rows
+  uint32_t* error_word;
+  int rows, top_k, experts, hidden, inter;
+};
+glmrt_status_t launch_few_simt(const FewArgs& a, cudaStream_t stream);
+
 }  // namespace glmrt

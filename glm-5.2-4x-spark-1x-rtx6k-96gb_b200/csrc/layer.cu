@@ -81,6 +81,7 @@ struct Layer {
   uint16_t* route_rows = nullptr;
   uint16_t** slot_out = nullptr;
   uint32_t* slot_weight = nullptr;   // route weight per slot (fused combine of large batches)
+  float* few_act = nullptr;          // weighted SwiGLU rows of the few-token path
   uint32_t* fc_sync = nullptr;       // hand-over words between the decode FC1 and FC2 kernels
   uint16_t *hidden_stage = nullptr, *out_stage = nullptr;
   // scratch for weight loading
@@ -469,6 +470,7 @@ glmrt_status_t alloc_workspace(Layer* l) {
   // destinations start out null: a slot nobody dispatched to is skipped by the FC2 epilogues
   A(dev_alloc(b, &l->slot_out, static_cast<size_t>(l->max_slots), true));
   if (c.max_tokens > 256 && c.ep_world == 1) A(dev_alloc(b, &l->slot_weight, static_cast<size_t>(l->max_slots), true));
+  if (c.ep_world == 1) A(dev_alloc(b, &l->few_act, std::min<size_t>(T, kFewMaxRows) * K * I));
   A(dev_alloc(b, &l->hidden_stage, T * H));
   A(dev_alloc(b, &l->out_stage, T * H));
   A(dev_alloc(b, &l->wtmp, std::max(I * H, static_cast<size_t>(1))));
@@ -742,6 +744,97 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_routed_async(
   GLMRT_RETURN_IF_ERROR(run_routed(l, static_cast<const uint16_t*>(hidden_bf16.ptr), rows,
                                    static_cast<uint16_t*>(output_bf16.ptr), s));
   l->launches_last = static_cast<uint32_t>(launches_total() - before);
+  return ok();
+}
+
+namespace {
+
+// Checks what both few-token entry points share and fills the kernel's arguments.
+glmrt_status_t few_args(Layer* l, const glmrt_device_buffer_t& hidden, size_t rows, const glmrt_device_buffer_t& residual,
+                        const glmrt_device_buffer_t& shared, const glmrt_device_buffer_t& output, FewArgs* out) {
+  GLMRT_RETURN_IF_ERROR(validate_forward(l, rows));
+  const auto& c = l->cfg;
+  if (c.ep_world != 1) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "forward_few: this entry point needs ep_world == 1");
+  if (rows > static_cast<size_t>(kFewMaxRows))
+    return fail(GLMRT_STATUS_INVALID_ARGUMENT, "forward_few: at most GLMRT_B200_FEW_MAX_ROWS rows");
+  const size_t bytes = rows * static_cast<size_t>(c.hidden_dim) * 2;
+  GLMRT_RETURN_IF_ERROR(check_buf(hidden, bytes, "forward_few hidden"));
+  GLMRT_RETURN_IF_ERROR(check_buf(output, bytes, "forward_few output"));
+  if (residual.ptr != nullptr) GLMRT_RETURN_IF_ERROR(check_buf(residual, bytes, "forward_few residual"));
+  if (shared.ptr != nullptr) GLMRT_RETURN_IF_ERROR(check_buf(shared, bytes, "forward_few shared_delta"));
+  for (const void* p : {hidden.ptr, residual.ptr, shared.ptr, output.ptr})
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
+      return fail(GLMRT_STATUS_INVALID_ARGUMENT, "forward_few: buffers must be 16-byte aligned");
+  const uintptr_t o = reinterpret_cast<uintptr_t>(output.ptr);
+  for (const void* p : {hidden.ptr, residual.ptr, shared.ptr}) {
+    // the rows are read until the last result is written; residual and shared may be the output, value for value
+    const uintptr_t i = reinterpret_cast<uintptr_t>(p);
+    if (p != nullptr && i < o + bytes && o < i + bytes && (p == hidden.ptr || i != o))
+      return fail(GLMRT_STATUS_INVALID_ARGUMENT, "forward_few: the output overlaps an input");
+  }
+  FewArgs a{};
+  a.hidden_rows = static_cast<const uint16_t*>(hidden.ptr);
+  a.residual = static_cast<const uint16_t*>(residual.ptr);
+  a.shared = static_cast<const uint16_t*>(shared.ptr);
+  a.out = static_cast<uint16_t*>(output.ptr);
+  a.gate_codes = l->gate_codes; a.up_codes = l->up_codes; a.down_codes = l->down_codes;
+  a.gate_sf = l->gate_sf; a.up_sf = l->up_sf; a.down_sf = l->down_sf;
+  a.scale2 = l->scale2;
+  a.topk_idx = l->topk_idx; a.topk_w = l->topk_w; a.act = l->few_act;
+  a.error_word = l->counters + kCntError;
+  a.rows = static_cast<int>(rows); a.top_k = static_cast<int>(c.top_k); a.experts = static_cast<int>(c.experts);
+  a.hidden = static_cast<int>(c.hidden_dim); a.inter = static_cast<int>(c.intermediate_dim);
+  *out = a;
+  return GLMRT_STATUS_OK;
+}
+
+}  // namespace
+
+extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_async(
+    void* layer, glmrt_device_buffer_t hidden_bf16, size_t rows, glmrt_device_buffer_t residual_bf16,
+    glmrt_device_buffer_t shared_delta_bf16, glmrt_device_buffer_t output_bf16, glmrt_device_buffer_t topk_indices,
+    glmrt_device_buffer_t topk_weights, void* cuda_stream) {
+  Layer* l = static_cast<Layer*>(layer);
+  FewArgs a{};
+  GLMRT_RETURN_IF_ERROR(few_args(l, hidden_bf16, rows, residual_bf16, shared_delta_bf16, output_bf16, &a));
+  const size_t routes = rows * l->cfg.top_k;
+  if (topk_indices.ptr != nullptr) GLMRT_RETURN_IF_ERROR(check_buf(topk_indices, routes * 4, "forward_few topk_indices"));
+  if (topk_weights.ptr != nullptr) GLMRT_RETURN_IF_ERROR(check_buf(topk_weights, routes * 4, "forward_few topk_weights"));
+  cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  const uint64_t before = launches_total();
+  cudaError_t err = cudaMemsetAsync(l->counters + kCntError, 0, 4, s);
+  if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "forward_few clear", err);
+  GLMRT_RETURN_IF_ERROR(run_router(l, hidden_bf16.ptr, rows, s));
+  GLMRT_RETURN_IF_ERROR(launch_few_simt(a, s));
+  l->launches_last = static_cast<uint32_t>(launches_total() - before);
+  if (topk_indices.ptr != nullptr)
+    err = cudaMemcpyAsync(topk_indices.ptr, l->topk_idx, routes * 4, cudaMemcpyDeviceToDevice, s);
+  if (err == cudaSuccess && topk_weights.ptr != nullptr)
+    err = cudaMemcpyAsync(topk_weights.ptr, l->topk_w, routes * 4, cudaMemcpyDeviceToDevice, s);
+  if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "forward_few route copy", err);
+  l->last_rows = static_cast<uint32_t>(rows);
+  return ok();
+}
+
+extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_routed_async(
+    void* layer, glmrt_device_buffer_t hidden_bf16, size_t rows, glmrt_device_buffer_t topk_indices,
+    glmrt_device_buffer_t topk_weights, glmrt_device_buffer_t residual_bf16, glmrt_device_buffer_t shared_delta_bf16,
+    glmrt_device_buffer_t output_bf16, void* cuda_stream) {
+  Layer* l = static_cast<Layer*>(layer);
+  FewArgs a{};
+  GLMRT_RETURN_IF_ERROR(few_args(l, hidden_bf16, rows, residual_bf16, shared_delta_bf16, output_bf16, &a));
+  const size_t routes = rows * l->cfg.top_k;
+  GLMRT_RETURN_IF_ERROR(check_buf(topk_indices, routes * 4, "forward_few_routed topk_indices"));
+  GLMRT_RETURN_IF_ERROR(check_buf(topk_weights, routes * 4, "forward_few_routed topk_weights"));
+  cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  const uint64_t before = launches_total();
+  cudaError_t err = cudaMemsetAsync(l->counters + kCntError, 0, 4, s);
+  if (err == cudaSuccess) err = cudaMemcpyAsync(l->topk_idx, topk_indices.ptr, routes * 4, cudaMemcpyDeviceToDevice, s);
+  if (err == cudaSuccess) err = cudaMemcpyAsync(l->topk_w, topk_weights.ptr, routes * 4, cudaMemcpyDeviceToDevice, s);
+  if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "forward_few_routed route copy", err);
+  GLMRT_RETURN_IF_ERROR(launch_few_simt(a, s));
+  l->launches_last = static_cast<uint32_t>(launches_total() - before);
+  l->last_rows = static_cast<uint32_t>(rows);
   return ok();
 }
 

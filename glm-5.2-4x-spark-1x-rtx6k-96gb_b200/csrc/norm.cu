@@ -1,0 +1,319 @@
+// The boundary between two blocks of a layer in one pass over the rows:
+//
+//   d = delta                                       the finished block's output (optional)
+//   d = d * rsqrt(mean(d^2) + eps) * post_weight    norm after the block (optional)
+//   d = d * gate                                    per row, per channel or per value (optional)
+//   r = residual + scale * d                        -> residual_out
+//   y = r * rsqrt(mean(r^2) + eps) * norm_weight    -> normalized, the next block's input
+//
+// The sparse layer's own use is the plain form (no post norm, no gate, scale 1): attention's result
+// joins the residual stream and the rows the router, the experts and the shared expert read come out
+// normalised (python/reference/glmrt_reference/glm_moe_dsa_layer_ref.py:157-206).
+//
+// Arithmetic is float32 throughout; each output is rounded once (nearest even), and `y` is formed
+// from the unrounded r, so it does not inherit the rounding of the stored residual.
+//
+// Bound by memory: each value is read once and written once and does about ten operations.  One row
+// belongs to one group of threads that keeps all of it in registers (at most 32 values a thread)
+// between the loads and the second statistic, so nothing is read twice.
+#include "common.cuh"
+#include "internal.h"
+
+namespace glmrt {
+namespace {
+
+constexpr int kMaxWidth = 32768;      // 1024 threads x 32 values
+
+struct NormArgs {
+  const void *residual, *delta, *norm_w, *post_w, *gate;
+  void *residual_out, *normalized;
+  size_t residual_stride, delta_stride, gate_rs, gate_cs, residual_out_stride, normalized_stride;
+  int rows, width;
+  float scale, eps;
+};
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<uint16_t>(uint16_t v) { return bf16_bits_to_f32(v); }
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ uint16_t from_f32<uint16_t>(float v) { return f32_to_bf16_rne(v); }
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+
+// kVec consecutive values as they lie in memory: 16 aligned bytes, or one value.
+template <typename T, int kVec>
+struct alignas(kVec == 1 ? sizeof(T) : 16) Piece {
+  T t[kVec];
+  __device__ __forceinline__ static Piece load(const T* p) { return *reinterpret_cast<const Piece*>(p); }
+  __device__ __forceinline__ void unpack(float (&v)[kVec]) const {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[i] = to_f32(t[i]);
+  }
+};
+template <typename T, int kVec>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[kVec]) { Piece<T, kVec>::load(p).unpack(v); }
+template <typename T, int kVec>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[kVec]) {
+  Piece<T, kVec> q;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) q.t[i] = from_f32<T>(v[i]);
+  *reinterpret_cast<Piece<T, kVec>*>(p) = q;
+}
+// Weights may be wider or narrower than the rows: kVec of them, vectorised where they are whole 16-byte pieces.
+template <typename W, int kVec>
+__device__ __forceinline__ void load_weight(const W* p, float (&v)[kVec]) {
+  constexpr int kPer = 16 / sizeof(W);
+  if constexpr (kVec % kPer == 0 && kVec > 1) {
+#pragma unroll
+    for (int i = 0; i < kVec; i += kPer) {
+      float t[kPer];
+      load_vec<W, kPer>(p + i, t);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[i + j] = t[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[i] = to_f32(p[i]);
+  }
+}
+
+// Sum over the threads of one row (blockDim.x of them); every thread gets it.
+__device__ __forceinline__ float row_sum(float v, float* scratch) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int warps = blockDim.x / 32;
+  if (warps == 1) return v;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  __syncthreads();                    // an earlier use of scratch has been read
+  if (lane == 0) scratch[warp] = v;
+  __syncthreads();
+  v = lane < warps ? scratch[lane] : 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// T rows' type, W weights' type, kVec values per access, kNv accesses per thread.
+template <typename T, typename W, int kVec, int kNv>
+__global__ void __launch_bounds__(1024) block_norm_kernel(NormArgs a) {
+  __shared__ float scratch[32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row_i = blockIdx.x * blockDim.y + threadIdx.y;
+  if (row_i >= a.rows) return;        // blockDim.y > 1 only with one warp per row: whole warps leave
+  const size_t row = static_cast<size_t>(row_i);
+  const T* res = static_cast<const T*>(a.residual) + row * a.residual_stride;
+  const float inv_width = 1.0f / static_cast<float>(a.width);
+  auto column = [&](int n) { return (n * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * kVec; };
+  // The residual is asked for with the branch, before the branch's statistic, where a thread has the
+  // registers to hold it as it lies (widest float32 rows: after the statistic).
+  constexpr bool kEarly = sizeof(T) * kVec * kNv <= 64;
+  Piece<T, kVec> early[kEarly ? kNv : 1];
+  if constexpr (kEarly) {
+#pragma unroll
+    for (int n = 0; n < kNv; ++n)
+      if (column(n) < a.width) early[n] = Piece<T, kVec>::load(res + column(n));
+  }
+  float v[kNv][kVec];                 // the branch, then the new residual; zero past the width
+  if (a.delta != nullptr) {
+    const T* del = static_cast<const T*>(a.delta) + row * a.delta_stride;
+#pragma unroll
+    for (int n = 0; n < kNv; ++n) {
+      if (column(n) < a.width) load_vec<T, kVec>(del + column(n), v[n]);
+      else
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[n][i] = 0.0f;
+    }
+    if (a.post_w != nullptr) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int n = 0; n < kNv; ++n)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) ss += v[n][i] * v[n][i];
+      const float rs = rsqrtf(row_sum(ss, scratch) * inv_width + a.eps);
+#pragma unroll
+      for (int n = 0; n < kNv; ++n) {
+        if (column(n) >= a.width) continue;
+        float w[kVec];
+        load_weight<W, kVec>(static_cast<const W*>(a.post_w) + column(n), w);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[n][i] *= rs * w[i];
+      }
+    }
+    if (a.gate != nullptr) {
+      const T* g = static_cast<const T*>(a.gate) + row * a.gate_rs;
+#pragma unroll
+      for (int n = 0; n < kNv; ++n) {
+        if (column(n) >= a.width) continue;
+        float s[kVec];
+        if (a.gate_cs == 0) {
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) s[i] = to_f32(*g);
+        } else {
+          load_vec<T, kVec>(g + column(n), s);
+        }
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[n][i] *= s[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < kNv; ++n) {
+    float r[kVec];
+    if (column(n) < a.width) {
+      if constexpr (kEarly) early[n].unpack(r);
+      else load_vec<T, kVec>(res + column(n), r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) r[i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[n][i] = a.delta != nullptr ? fmaf(a.scale, v[n][i], r[i]) : r[i];
+    if (a.delta != nullptr && column(n) < a.width)
+      store_vec<T, kVec>(static_cast<T*>(a.residual_out) + row * a.residual_out_stride + column(n), v[n]);
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int n = 0; n < kNv; ++n)
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) ss += v[n][i] * v[n][i];
+  const float rs = rsqrtf(row_sum(ss, scratch) * inv_width + a.eps);
+  T* out = static_cast<T*>(a.normalized) + row * a.normalized_stride;
+#pragma unroll
+  for (int n = 0; n < kNv; ++n) {
+    if (column(n) >= a.width) continue;
+    float w[kVec];
+    load_weight<W, kVec>(static_cast<const W*>(a.norm_w) + column(n), w);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) w[i] *= v[n][i] * rs;
+    store_vec<T, kVec>(out + column(n), w);
+  }
+}
+
+template <typename T, typename W, int kVec, int kNv>
+void launch(const NormArgs& a, int threads, cudaStream_t s) {
+  const int ty = threads == 32 ? 8 : 1;
+  launch_pdl(block_norm_kernel<T, W, kVec, kNv>, dim3(static_cast<unsigned>((a.rows + ty - 1) / ty)),
+             dim3(static_cast<unsigned>(threads), static_cast<unsigned>(ty)), 0, s, a);
+}
+
+template <typename T, typename W, int kVec>
+void dispatch(const NormArgs& a, cudaStream_t s) {
+  const int pieces = (a.width + kVec - 1) / kVec;
+  constexpr int kMost = 32 / kVec;            // accesses per thread at 32 values
+  // A few rows: as many threads per row as it has pieces, for the latency.  Many rows: a quarter of
+  // that, so that several rows share an SM and their loads overlap each other's reductions.
+  int nv = 1;
+  while (nv < kMost && (pieces + nv - 1) / nv > 1024) nv *= 2;
+  if (a.rows > 2 * 148)
+    while (nv < kMost && nv < 4 && (pieces + 2 * nv - 1) / (2 * nv) >= 128) nv *= 2;
+  const int threads = ((pieces + nv - 1) / nv + 31) / 32 * 32;
+  if (nv == 1) return launch<T, W, kVec, 1>(a, threads, s);
+  if (nv == 2) return launch<T, W, kVec, 2>(a, threads, s);
+  if (nv == 4) return launch<T, W, kVec, 4>(a, threads, s);
+  if constexpr (kMost >= 8)
+    if (nv == 8) return launch<T, W, kVec, 8>(a, threads, s);
+  if constexpr (kMost >= 32) {
+    if (nv == 16) return launch<T, W, kVec, 16>(a, threads, s);
+    return launch<T, W, kVec, 32>(a, threads, s);
+  }
+}
+
+template <typename T, typename W>
+void dispatch_vec(const NormArgs& a, bool vec, cudaStream_t s) {
+  if (vec) dispatch<T, W, 16 / static_cast<int>(sizeof(T))>(a, s);
+  else dispatch<T, W, 1>(a, s);
+}
+
+struct Span { uintptr_t lo, hi; size_t stride; };
+bool overlap(const Span& x, const Span& y) { return x.lo < y.hi && y.lo < x.hi; }
+
+}  // namespace
+}  // namespace glmrt
+
+using namespace glmrt;
+
+extern "C" glmrt_status_t glmrt_b200_block_norm_async(const glmrt_b200_block_norm_args_t* p, void* cuda_stream) {
+  if (p == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm: null arguments");
+  if (p->dtype > GLMRT_B200_DTYPE_F32 || p->weight_dtype > GLMRT_B200_DTYPE_F32)
+    return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm: dtype must be GLMRT_B200_DTYPE_BF16 or _F32");
+  if (p->width == 0 || p->width > kMaxWidth)
+    return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm: width must be 1..32768");
+  if (p->rows > 0x7fffffffu) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm: too many rows");
+  if (!(p->eps >= 0.0f) || !isfinite(p->eps) || !isfinite(p->scale))
+    return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm: eps must be finite and not negative, scale finite");
+  if (p->rows == 0) return ok();
+  const size_t size = p->dtype == GLMRT_B200_DTYPE_BF16 ? 2 : 4, wsize = p->weight_dtype == GLMRT_B200_DTYPE_BF16 ? 2 : 4;
+  const bool branch = p->delta.ptr != nullptr;
+  if (!branch && (p->post_weight.ptr != nullptr || p->gate.ptr != nullptr || p->residual_out.ptr != nullptr))
+    return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm: post_weight, gate and residual_out need a delta");
+  bool vec = p->width % (16 / size) == 0;
+  Span spans[4];                              // residual, delta, residual_out, normalized
+  auto rows_ok = [&](const glmrt_device_buffer_t& b, size_t row_stride, Span* span, const char* what) {
+    if (b.ptr == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string("block_norm ") + what + ": null buffer");
+    if (row_stride < p->width) return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string("block_norm ") + what + ": row stride below width");
+    size_t need = 0;
+    if (!checked_mul(p->rows - 1, row_stride, &need) || need > (SIZE_MAX >> 3) || b.bytes < (need + p->width) * size)
+      return fail(GLMRT_STATUS_BUFFER_TOO_SMALL, std::string("block_norm ") + what + ": buffer too small");
+    const uintptr_t at = reinterpret_cast<uintptr_t>(b.ptr);
+    if (at % size != 0) return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string("block_norm ") + what + ": misaligned");
+    vec = vec && at % 16 == 0 && row_stride % (16 / size) == 0;
+    *span = Span{at, at + (need + p->width) * size, row_stride};
+    return GLMRT_STATUS_OK;
+  };
+  GLMRT_RETURN_IF_ERROR(rows_ok(p->residual, p->residual_stride, &spans[0], "residual"));
+  GLMRT_RETURN_IF_ERROR(rows_ok(p->normalized, p->normalized_stride, &spans[3], "normalized"));
+  if (branch) {
+    GLMRT_RETURN_IF_ERROR(rows_ok(p->delta, p->delta_stride, &spans[1], "delta"));
+    GLMRT_RETURN_IF_ERROR(rows_ok(p->residual_out, p->residual_out_stride, &spans[2], "residual_out"));
+    if (overlap(spans[2], spans[3]))
+      return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm: residual_out and normalized overlap");
+  }
+  // an output may take the place of an input, row for row; any other overlap would be read after it was written
+  for (int out : {2, 3})
+    for (int in : {0, 1}) {
+      if (!branch && (out == 2 || in == 1)) continue;
+      if (overlap(spans[out], spans[in]) && (spans[out].lo != spans[in].lo || (spans[out].stride != spans[in].stride && p->rows > 1)))
+        return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm: an output overlaps an input without being it");
+    }
+  auto weight_ok = [&](const glmrt_device_buffer_t& b, const char* what) {
+    if (b.bytes < p->width * wsize) return fail(GLMRT_STATUS_BUFFER_TOO_SMALL, std::string("block_norm ") + what + ": buffer too small");
+    const uintptr_t at = reinterpret_cast<uintptr_t>(b.ptr);
+    if (at % wsize != 0) return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string("block_norm ") + what + ": misaligned");
+    const Span s{at, at + p->width * wsize, 0};
+    if (overlap(s, spans[3]) || (branch && overlap(s, spans[2])))
+      return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string("block_norm ") + what + ": overlaps an output");
+    vec = vec && at % 16 == 0;
+    return GLMRT_STATUS_OK;
+  };
+  if (p->norm_weight.ptr == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm norm_weight: null buffer");
+  GLMRT_RETURN_IF_ERROR(weight_ok(p->norm_weight, "norm_weight"));
+  if (p->post_weight.ptr != nullptr) GLMRT_RETURN_IF_ERROR(weight_ok(p->post_weight, "post_weight"));
+  if (p->gate.ptr != nullptr) {
+    if (p->gate_col_stride > 1) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm gate: column stride must be 0 or 1");
+    size_t need = 0;
+    if (!checked_mul(p->rows - 1, p->gate_row_stride, &need) || need > (SIZE_MAX >> 3) ||
+        p->gate.bytes < (need + (p->gate_col_stride ? p->width : 1)) * size)
+      return fail(GLMRT_STATUS_BUFFER_TOO_SMALL, "block_norm gate: buffer too small");
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p->gate.ptr);
+    if (at % size != 0) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm gate: misaligned");
+    const Span s{at, at + (need + (p->gate_col_stride ? p->width : 1)) * size, 0};
+    if (overlap(s, spans[2]) || overlap(s, spans[3]))
+      return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm gate: overlaps an output");
+    if (p->gate_col_stride != 0) vec = vec && at % 16 == 0 && p->gate_row_stride % (16 / size) == 0;
+  }
+  GLMRT_RETURN_IF_ERROR(require_cuda());
+  NormArgs a{};
+  a.residual = p->residual.ptr; a.delta = p->delta.ptr; a.norm_w = p->norm_weight.ptr; a.post_w = p->post_weight.ptr;
+  a.gate = p->gate.ptr; a.residual_out = p->residual_out.ptr; a.normalized = p->normalized.ptr;
+  a.residual_stride = p->residual_stride; a.delta_stride = p->delta_stride; a.gate_rs = p->gate_row_stride;
+  a.gate_cs = p->gate_col_stride; a.residual_out_stride = p->residual_out_stride; a.normalized_stride = p->normalized_stride;
+  a.rows = static_cast<int>(p->rows); a.width = static_cast<int>(p->width);
+  a.scale = p->scale; a.eps = p->eps;
+  cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  if (size == 2 && wsize == 2) dispatch_vec<uint16_t, uint16_t>(a, vec, s);
+  else if (size == 2) dispatch_vec<uint16_t, float>(a, vec, s);
+  else if (wsize == 2) dispatch_vec<float, uint16_t>(a, vec, s);
+  else dispatch_vec<float, float>(a, vec, s);
+  GLMRT_LAUNCH_CHECK("block_norm_kernel");
+  return ok();
+}

@@ -1,0 +1,133 @@
+"""Dense products in 8-bit floating point with a scale for each block of 128 (csrc/fp8.cu).
+
+Weights: E4M3 ``[n, k]`` with one float32 scale per 128 x 128 block, ``[ceil(n/128), ceil(k/128)]``.
+Activations: bf16 rows, quantised in the call with one power-of-two scale per row and 128 columns
+(the smallest with ``amax / scale <= 448``).  Sums are float32.  ``k`` is a multiple of 16; rows, ``n``
+and the last block may be ragged.  A row with a NaN or an infinity gives NaN outputs in that row only.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import native as N
+
+BLOCK = 128
+E4M3 = torch.float8_e4m3fn
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _buf(t: torch.Tensor) -> N.DeviceBuffer:
+    return N.DeviceBuffer.of(t.data_ptr(), t.numel() * t.element_size(), t.device.index)
+
+
+def _stream() -> C.c_void_p:
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _check_rows(x: torch.Tensor, k: int, types: tuple, what: str) -> tuple[N.DeviceBuffer, int]:
+    if x.dim() != 2 or x.shape[1] != k or x.dtype not in types:
+        raise ValueError(f"{what} must be [rows, {k}] of type {' or '.join(str(t) for t in types)}")
+    if not x.is_cuda:
+        raise ValueError(f"{what} must be on a CUDA device")
+    if k > 1 and x.stride(1) != 1:
+        raise ValueError(f"{what} must be contiguous along its rows")
+    rows = x.shape[0]
+    stride = x.stride(0) if rows > 1 else k
+    nbytes = ((rows - 1) * stride + k) * x.element_size() if rows else 0
+    return N.DeviceBuffer.of(x.data_ptr(), nbytes, x.device.index), stride
+
+
+def _check_weight(codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, device: torch.device, what: str) -> None:
+    if codes.shape != (n, k) or codes.dtype not in (E4M3, torch.uint8) or not codes.is_contiguous():
+        raise ValueError(f"{what} codes must be a contiguous E4M3 (or uint8) tensor [{n}, {k}]")
+    if scales.shape != (_blocks(n), _blocks(k)) or scales.dtype != torch.float32 or not scales.is_contiguous():
+        raise ValueError(f"{what} scales must be a contiguous float32 tensor [{_blocks(n)}, {_blocks(k)}]")
+    if codes.device != device or scales.device != device:
+        raise ValueError(f"{what} must be on the device of the rows")
+
+
+def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales (amax / 448 per 128 x 128 block) of a weight; done once at load."""
+    n, k = weight.shape
+    pad = torch.nn.functional.pad(weight.float(), (0, -k % BLOCK, 0, -n % BLOCK))
+    b = pad.view(_blocks(n), BLOCK, _blocks(k), BLOCK)
+    amax = b.abs().amax(dim=(1, 3))
+    scales = torch.where(amax > 0, amax / 448.0, torch.ones_like(amax))
+    codes = (b / scales[:, None, :, None]).reshape(pad.shape)[:n, :k].clamp(-448, 448).to(E4M3)
+    return codes.contiguous(), scales
+
+
+def quantize_rows(x: torch.Tensor, lib: N.NativeLibrary | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows' codes ``[rows, k]`` (E4M3) and scales ``[ceil(k/128), rows]``; x bf16 or float32."""
+    rows, k = x.shape if x.dim() == 2 else (0, 0)
+    buf, stride = _check_rows(x, k, (torch.bfloat16, torch.float32), "quantize_rows: x")
+    codes = torch.empty((rows, k), dtype=E4M3, device=x.device)
+    scales = torch.empty((_blocks(k), rows), dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        (lib or N.library()).call("glmrt_b200_fp8_quantize_rows_async", buf, _buf(codes), _buf(scales), C.c_size_t(rows),
+                                  C.c_size_t(k), C.c_size_t(stride),
+                                  C.c_uint32(N.DTYPE_BF16 if x.dtype == torch.bfloat16 else N.DTYPE_F32), _stream())
+    return codes, scales
+
+
+def _workspace(lib: N.NativeLibrary, symbol: str, device: torch.device, *sizes: int) -> torch.Tensor:
+    need = C.c_size_t(0)
+    lib.call(symbol, *[C.c_size_t(v) for v in sizes], C.byref(need))
+    return torch.empty(max(need.value, 1), dtype=torch.uint8, device=device)
+
+
+def _output(out: torch.Tensor | None, rows: int, n: int, dtype: torch.dtype, x: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty((rows, n), dtype=dtype, device=x.device)
+    if out.shape != (rows, n) or out.dtype != dtype or out.device != x.device or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {dtype} tensor [{rows}, {n}] on the rows' device")
+    return out
+
+
+def block_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None = None,
+                 out_dtype: torch.dtype = torch.bfloat16, lib: N.NativeLibrary | None = None) -> torch.Tensor:
+    """``x @ weight.T`` of bf16 rows and an E4M3 weight ``[n, k]``; out bf16 or float32."""
+    lib = lib or N.library()
+    if codes.dim() != 2:
+        raise ValueError("block_linear: codes must be [n, k]")
+    n, k = codes.shape
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("block_linear: out_dtype must be bfloat16 or float32")
+    buf, stride = _check_rows(x, k, (torch.bfloat16,), "block_linear: x")
+    _check_weight(codes, scales, n, k, x.device, "block_linear: weight")
+    rows = x.shape[0]
+    out = _output(out, rows, n, out_dtype, x)
+    with torch.cuda.device(x.device):
+        ws = _workspace(lib, "glmrt_b200_fp8_block_linear_workspace", x.device, rows, n, k)
+        lib.call("glmrt_b200_fp8_block_linear_async", buf, _buf(codes), _buf(scales), _buf(out), _buf(ws),
+                 C.c_size_t(rows), C.c_size_t(n), C.c_size_t(k), C.c_size_t(stride),
+                 C.c_uint32(N.DTYPE_BF16 if out_dtype == torch.bfloat16 else N.DTYPE_F32), _stream())
+    return out
+
+
+def gated_mlp(x: torch.Tensor, gate_codes: torch.Tensor, gate_scales: torch.Tensor, up_codes: torch.Tensor,
+              up_scales: torch.Tensor, down_codes: torch.Tensor, down_scales: torch.Tensor,
+              out: torch.Tensor | None = None, lib: N.NativeLibrary | None = None) -> torch.Tensor:
+    """``down(silu(gate(x)) * up(x))`` with gate / up ``[inter, hidden]`` and down ``[hidden, inter]``; the
+    activation between the products stays float32 until it is quantised like the rows."""
+    lib = lib or N.library()
+    if gate_codes.dim() != 2:
+        raise ValueError("gated_mlp: gate codes must be [inter, hidden]")
+    inter, hidden = gate_codes.shape
+    buf, stride = _check_rows(x, hidden, (torch.bfloat16,), "gated_mlp: x")
+    _check_weight(gate_codes, gate_scales, inter, hidden, x.device, "gated_mlp: gate")
+    _check_weight(up_codes, up_scales, inter, hidden, x.device, "gated_mlp: up")
+    _check_weight(down_codes, down_scales, hidden, inter, x.device, "gated_mlp: down")
+    rows = x.shape[0]
+    out = _output(out, rows, hidden, torch.bfloat16, x)
+    with torch.cuda.device(x.device):
+        ws = _workspace(lib, "glmrt_b200_fp8_gated_mlp_workspace", x.device, rows, hidden, inter)
+        lib.call("glmrt_b200_fp8_gated_mlp_async", buf, _buf(gate_codes), _buf(gate_scales), _buf(up_codes),
+                 _buf(up_scales), _buf(down_codes), _buf(down_scales), _buf(out), _buf(ws), C.c_size_t(rows),
+                 C.c_size_t(hidden), C.c_size_t(inter), C.c_size_t(stride), _stream())
+    return out

@@ -168,6 +168,47 @@ class MoeLayer:
                       C.c_size_t(rows), _buf(residual_bf16), shared, _buf(out), _stream())
         return out
 
+    FEW_MAX_ROWS = 16
+
+    def forward_few(self, hidden_bf16: torch.Tensor, out: torch.Tensor | None = None,
+                    residual_bf16: torch.Tensor | None = None, shared_delta_bf16: torch.Tensor | None = None,
+                    want_routes: bool = False):
+        """The whole layer for at most ``FEW_MAX_ROWS`` rows on bf16 activations (no activation
+        quantisation), out = bf16(residual + shared_delta + routed), rounded once."""
+        rows = self._few_rows(hidden_bf16, residual_bf16, shared_delta_bf16, out)
+        if out is None:
+            out = torch.empty_like(hidden_bf16)
+        idx = w = None
+        if want_routes:
+            idx = torch.empty((rows, self.top_k), dtype=torch.int32, device=self.device)
+            w = torch.empty((rows, self.top_k), dtype=torch.float32, device=self.device)
+        opt = lambda t: N.DeviceBuffer.null() if t is None else _buf(t)  # noqa: E731
+        self.lib.call("glmrt_b200_moe_layer_forward_few_async", self.handle, _buf(hidden_bf16), C.c_size_t(rows),
+                      opt(residual_bf16), opt(shared_delta_bf16), _buf(out), opt(idx), opt(w), _stream())
+        return (out, idx, w) if want_routes else out
+
+    def forward_few_routed(self, hidden_bf16: torch.Tensor, idx: torch.Tensor, w: torch.Tensor,
+                           out: torch.Tensor | None = None, residual_bf16: torch.Tensor | None = None,
+                           shared_delta_bf16: torch.Tensor | None = None) -> torch.Tensor:
+        """``forward_few`` with the routes given; index -1 is no route."""
+        rows = self._few_rows(hidden_bf16, residual_bf16, shared_delta_bf16, out)
+        assert idx.shape == (rows, self.top_k) and w.shape == (rows, self.top_k)
+        if out is None:
+            out = torch.empty_like(hidden_bf16)
+        idx = idx.to(torch.int32).contiguous()
+        w = w.to(torch.float32).contiguous()
+        opt = lambda t: N.DeviceBuffer.null() if t is None else _buf(t)  # noqa: E731
+        self.lib.call("glmrt_b200_moe_layer_forward_few_routed_async", self.handle, _buf(hidden_bf16), C.c_size_t(rows),
+                      _buf(idx), _buf(w), opt(residual_bf16), opt(shared_delta_bf16), _buf(out), _stream())
+        return out
+
+    def _few_rows(self, hidden: torch.Tensor, *others) -> int:
+        assert hidden.dim() == 2 and hidden.dtype == torch.bfloat16 and hidden.shape[1] == self.hidden
+        for t in (hidden, *others):
+            if t is not None:
+                assert t.shape == hidden.shape and t.dtype == torch.bfloat16 and t.device == self.device
+        return hidden.shape[0]
+
     def forward_host(self, hidden_host: torch.Tensor, out_host: torch.Tensor) -> None:
         """Host buffers in, host buffers out (pinned memory recommended); synchronises."""
         assert not hidden_host.is_cuda and not out_host.is_cuda

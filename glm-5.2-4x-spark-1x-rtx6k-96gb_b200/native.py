@@ -95,6 +95,19 @@ class RouteShardReductionBuffers(C.Structure):
     _fields_ = [("local", DeviceBuffer), ("peers", DeviceBuffer * 3), ("output_f32", DeviceBuffer)]
 
 
+class BlockNormArgs(C.Structure):
+    """glmrt_b200_block_norm_args_t."""
+    _fields_ = ([(n, DeviceBuffer) for n in ("residual", "delta", "norm_weight", "post_weight", "gate",
+                                             "residual_out", "normalized")]
+                + [(n, C.c_size_t) for n in ("rows", "width", "residual_stride", "delta_stride", "gate_row_stride",
+                                             "gate_col_stride", "residual_out_stride", "normalized_stride")]
+                + [("dtype", C.c_uint32), ("weight_dtype", C.c_uint32), ("scale", C.c_float), ("eps", C.c_float)])
+
+
+DTYPE_BF16 = 0
+DTYPE_F32 = 1
+
+
 def declared_symbols(header_path: str = HEADER) -> list[str]:
     """Every function name declared in include/glmrt_b200.h."""
     text = open(header_path).read()

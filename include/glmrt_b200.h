@@ -383,6 +383,72 @@ glmrt_status_t glmrt_cuda_residual_add_shared_f32_delta_bf16_async(
     uint16_t* out, size_t count, void* cuda_stream);
 
 /* ------------------------------------------------------------------------ */
+/* Block boundary (addition): residual add and RMSNorms in one pass.           */
+/*   d = delta; with post_weight: d = d * rsqrt(mean(d^2) + eps) * post_weight;  */
+/*   with gate: d = d * gate;  r = residual + scale * d  -> residual_out;        */
+/*   r * rsqrt(mean(r^2) + eps) * norm_weight -> normalized                      */
+/* (python/reference/glmrt_reference/glm_moe_dsa_layer_ref.py:157-206 with a     */
+/* plain delta).  float32 arithmetic, each output rounded once to the rows'      */
+/* type.  Strides count elements; rows are contiguous inside.  gate: row stride  */
+/* 0 = one row for all rows, column stride 0 = one value per row, else 1.        */
+/* Without a delta (null) post_weight, gate and residual_out must be null and    */
+/* only normalized is written.  An output may be one of the row inputs (same     */
+/* address and stride); other overlaps are refused.  width 1..32768; rows 0 is   */
+/* accepted and does nothing.                                                    */
+/* ------------------------------------------------------------------------ */
+typedef enum glmrt_b200_dtype_t {
+  GLMRT_B200_DTYPE_BF16 = 0,
+  GLMRT_B200_DTYPE_F32 = 1,
+} glmrt_b200_dtype_t;
+typedef struct glmrt_b200_block_norm_args_t {
+  glmrt_device_buffer_t residual;     /* [rows, width] */
+  glmrt_device_buffer_t delta;        /* [rows, width] or null */
+  glmrt_device_buffer_t norm_weight;  /* [width] */
+  glmrt_device_buffer_t post_weight;  /* [width] or null */
+  glmrt_device_buffer_t gate;         /* rows' type, or null */
+  glmrt_device_buffer_t residual_out; /* [rows, width] */
+  glmrt_device_buffer_t normalized;   /* [rows, width] */
+  size_t rows, width;
+  size_t residual_stride, delta_stride, gate_row_stride, gate_col_stride, residual_out_stride, normalized_stride;
+  uint32_t dtype;        /* of the rows and the gate */
+  uint32_t weight_dtype; /* of norm_weight and post_weight */
+  float scale, eps;
+} glmrt_b200_block_norm_args_t;
+glmrt_status_t glmrt_b200_block_norm_async(const glmrt_b200_block_norm_args_t* args, void* cuda_stream);
+
+/* ------------------------------------------------------------------------ */
+/* 8-bit floating point products with a scale for each block of 128 (addition). */
+/* Weights: E4M3 [n, k] row-major and one float32 scale per 128 x 128 block,      */
+/* [ceil(n/128), ceil(k/128)].  Activations: one power-of-two scale per row and   */
+/* 128 columns, the smallest with amax / scale <= 448 (blocks below 2^-100 count  */
+/* as 2^-100; a block with a NaN or an infinity makes its row's outputs NaN).      */
+/* float32 sums.  k is a multiple of 16 and weight codes are 16-byte aligned;     */
+/* rows, n and the last block may be ragged, rows 0 is accepted.  `workspace` is   */
+/* 256-byte aligned device memory of the stated size; it carries nothing from one  */
+/* call to the next, and calls that may overlap need one each.                     */
+/* ------------------------------------------------------------------------ */
+/* bf16 / float32 rows (input_row_stride elements apart) -> codes [rows, cols], scales
+ * [ceil(cols/128), rows]. */
+glmrt_status_t glmrt_b200_fp8_quantize_rows_async(glmrt_device_buffer_t input, glmrt_device_buffer_t codes,
+                                                  glmrt_device_buffer_t scales, size_t rows, size_t cols,
+                                                  size_t input_row_stride, uint32_t dtype, void* cuda_stream);
+glmrt_status_t glmrt_b200_fp8_block_linear_workspace(size_t rows, size_t n, size_t k, size_t* out_bytes);
+/* output [rows, n] (bf16 or float32) = x [rows, k] weight^T, x quantised in the call. */
+glmrt_status_t glmrt_b200_fp8_block_linear_async(glmrt_device_buffer_t x_bf16, glmrt_device_buffer_t weight_codes,
+                                                 glmrt_device_buffer_t weight_scales, glmrt_device_buffer_t output,
+                                                 glmrt_device_buffer_t workspace, size_t rows, size_t n, size_t k,
+                                                 size_t x_row_stride, uint32_t out_dtype, void* cuda_stream);
+glmrt_status_t glmrt_b200_fp8_gated_mlp_workspace(size_t rows, size_t hidden, size_t inter, size_t* out_bytes);
+/* output [rows, hidden] = down (silu(gate x) * (up x)), gate / up [inter, hidden], down [hidden, inter]: the
+ * dense shared expert (python/reference/glmrt_reference/moe_ref.py:17-21) in this arithmetic.  The
+ * activation between the products is float32 until it is quantised like the rows. */
+glmrt_status_t glmrt_b200_fp8_gated_mlp_async(
+    glmrt_device_buffer_t x_bf16, glmrt_device_buffer_t gate_codes, glmrt_device_buffer_t gate_scales,
+    glmrt_device_buffer_t up_codes, glmrt_device_buffer_t up_scales, glmrt_device_buffer_t down_codes,
+    glmrt_device_buffer_t down_scales, glmrt_device_buffer_t output_bf16, glmrt_device_buffer_t workspace, size_t rows,
+    size_t hidden, size_t inter, size_t x_row_stride, void* cuda_stream);
+
+/* ------------------------------------------------------------------------ */
 /* Layer-level entry points (additions).                                      */
 /*                                                                            */
 /* A layer object owns the NVFP4 weights of its local experts in tensor-core   */
@@ -475,6 +541,25 @@ glmrt_status_t glmrt_b200_moe_layer_forward_async(
 glmrt_status_t glmrt_b200_moe_layer_forward_residual_async(
     void* layer, glmrt_device_buffer_t hidden_bf16, size_t rows, glmrt_device_buffer_t residual_bf16,
     glmrt_device_buffer_t shared_delta_bf16, glmrt_device_buffer_t output_bf16, void* cuda_stream);
+/* The whole sparse layer for a few rows (at most GLMRT_B200_FEW_MAX_ROWS and max_tokens) on bf16 activations:
+ * router, expert FFN with the NVFP4 weights and unquantised activations (W4A16: the arithmetic of the
+ * reference's decode kernels, native/cuda/kernels/b12x_direct.cu:171-201,989-1541), weighted combine;
+ * output = bf16(residual + shared_delta + routed), rounded once (nearest even).  residual, shared_delta,
+ * topk_indices and topk_weights may be null; output may be residual or shared_delta, and no other input.
+ * Needs ep_world == 1.  Results differ from glmrt_b200_moe_layer_forward_async, which quantises the
+ * activations; an expert's sums do not depend on the other rows of the call. */
+#define GLMRT_B200_FEW_MAX_ROWS 16
+glmrt_status_t glmrt_b200_moe_layer_forward_few_async(
+    void* layer, glmrt_device_buffer_t hidden_bf16, size_t rows, glmrt_device_buffer_t residual_bf16,
+    glmrt_device_buffer_t shared_delta_bf16, glmrt_device_buffer_t output_bf16, glmrt_device_buffer_t topk_indices,
+    glmrt_device_buffer_t topk_weights, void* cuda_stream);
+/* The same with the routes given: topk_indices [rows, top_k] (0xffffffff: no route; any other id outside the
+ * layer is skipped and reported by glmrt_b200_moe_layer_check), topk_weights [rows, top_k].  An expert may be
+ * named more than once in a row. */
+glmrt_status_t glmrt_b200_moe_layer_forward_few_routed_async(
+    void* layer, glmrt_device_buffer_t hidden_bf16, size_t rows, glmrt_device_buffer_t topk_indices,
+    glmrt_device_buffer_t topk_weights, glmrt_device_buffer_t residual_bf16, glmrt_device_buffer_t shared_delta_bf16,
+    glmrt_device_buffer_t output_bf16, void* cuda_stream);
 /* Same with host buffers: copies the rows in from `hidden_host`, runs the layer, copies the
  * result out to `output_host` and synchronises the stream.  Host memory may be pageable;
  * pinned memory makes the copies asynchronous. */

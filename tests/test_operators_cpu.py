@@ -1,0 +1,152 @@
+"""Refusals of the operators around the routed experts: nothing here reaches a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib(pkg):
+    from glmrt_b200 import native as N
+    return N.library()
+
+
+def norm_args(N, rows=4, width=64, **kw):
+    a = N.BlockNormArgs()
+    size = rows * width * 2
+    a.residual, a.delta = N.DeviceBuffer.of(0x10000, size), N.DeviceBuffer.of(0x20000, size)
+    a.norm_weight = N.DeviceBuffer.of(0x30000, width * 2)
+    a.residual_out, a.normalized = N.DeviceBuffer.of(0x40000, size), N.DeviceBuffer.of(0x50000, size)
+    a.rows, a.width, a.scale, a.eps = rows, width, 1.0, 1e-5
+    for n in ("residual", "delta", "residual_out", "normalized"):
+        setattr(a, n + "_stride", width)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_block_norm_refusals(lib):
+    from glmrt_b200 import native as N
+    buf = N.DeviceBuffer.of
+
+    def status(**kw):
+        return lib.call_status("glmrt_b200_block_norm_async", C.byref(norm_args(N, **kw)), None)
+
+    assert lib.call_status("glmrt_b200_block_norm_async", None, None) == 1
+    for bad in (dict(dtype=2), dict(weight_dtype=7), dict(width=32769), dict(eps=-1.0), dict(eps=float("nan")),
+                dict(scale=float("inf")), dict(rows=1 << 33), dict(residual_stride=63), dict(normalized_stride=0)):
+        assert status(**bad) == 1, bad
+    assert lib.call_status("glmrt_b200_block_norm_async", C.byref(norm_args(N, width=0)), None) == 1
+    assert lib.call_status("glmrt_b200_block_norm_async", C.byref(norm_args(N, rows=0)), None) == 0
+    for name in ("residual", "residual_out", "normalized", "norm_weight"):
+        assert status(**{name: N.DeviceBuffer.null()}) == 1, name
+    for name in ("residual", "delta", "residual_out", "normalized"):
+        assert status(**{name: buf(0x100000, 4 * 64 * 2 - 1)}) == 2, name
+        assert status(**{name: buf(0x100001, 4 * 64 * 2)}) == 1, name
+        assert status(**{name + "_stride": 1 << 62}) == 2, name
+    assert status(norm_weight=buf(0x30000, 127)) == 2
+    # a null delta takes no branch arguments
+    null = N.DeviceBuffer.null()
+    assert status(delta=null) == 1 and "need a delta" in lib.last_error()
+    # overlaps: outputs with each other, an output with part of an input, with a weight, with the gate
+    assert status(residual_out=buf(0x50000 + 64, 512)) == 1
+    assert status(normalized=buf(0x10000 + 16, 512)) == 1
+    assert status(normalized=buf(0x10000, 1024), normalized_stride=128) == 1
+    assert status(normalized=buf(0x30000, 512)) == 1
+    gate = buf(0x60000, 512)
+    assert status(gate=gate, gate_col_stride=2) == 1
+    assert status(gate=gate, gate_row_stride=64, gate_col_stride=1, residual_out=buf(0x60000, 512)) == 1
+    assert status(gate=buf(0x60000, 6), gate_row_stride=1) == 2
+    assert status(post_weight=buf(0x70000, 100)) == 2
+
+
+def test_fp8_refusals(lib):
+    from glmrt_b200 import native as N
+    Z = C.c_size_t
+    buf, null = N.DeviceBuffer.of, N.DeviceBuffer.null()
+    need = Z(0)
+    assert lib.call_status("glmrt_b200_fp8_block_linear_workspace", Z(4), Z(64), Z(128), None) == 1
+    for rows, n, k in ((4, 0, 128), (4, 64, 0), (4, 64, 120), (1 << 25, 64, 128), (4, 1 << 25, 128), (4, 64, 1 << 25)):
+        assert lib.call_status("glmrt_b200_fp8_block_linear_workspace", Z(rows), Z(n), Z(k), C.byref(need)) == 1
+    assert lib.call_status("glmrt_b200_fp8_block_linear_workspace", Z(4), Z(64), Z(128), C.byref(need)) == 0 and need.value > 0
+    ws = buf(0x100000, need.value)
+
+    def linear(x=buf(0x10000, 1024), c=buf(0x20000, 64 * 128), s=buf(0x30000, 4), o=buf(0x40000, 512), w=ws, rows=4, n=64, k=128,
+               stride=128, dtype=0):
+        return lib.call_status("glmrt_b200_fp8_block_linear_async", x, c, s, o, w, Z(rows), Z(n), Z(k), Z(stride), C.c_uint32(dtype), None)
+
+    assert linear(rows=0) == 0
+    assert linear(dtype=2) == 1 and linear(stride=127) == 1 and linear(k=120) == 1
+    for name in "xcsow":
+        assert linear(**{name: null}) == 1, name
+    assert linear(x=buf(0x10000, 1023)) == 2 and linear(c=buf(0x20000, 8191)) == 2 and linear(s=buf(0x30000, 3)) == 2
+    assert linear(o=buf(0x40000, 511)) == 2 and linear(w=buf(0x100000, need.value - 1)) == 2
+    assert linear(o=buf(0x40000, 512), dtype=1) == 2
+    assert linear(c=buf(0x20008, 64 * 128)) == 1 and linear(w=buf(0x100010, need.value)) == 1
+
+    def rows(x=buf(0x10000, 1024), c=buf(0x20000, 512), s=buf(0x30000, 16), n=4, cols=128, stride=128, dtype=0):
+        return lib.call_status("glmrt_b200_fp8_quantize_rows_async", x, c, s, Z(n), Z(cols), Z(stride), C.c_uint32(dtype), None)
+
+    assert rows(n=0) == 0 and rows(cols=100) == 1 and rows(dtype=3) == 1 and rows(stride=100) == 1
+    assert rows(x=null) == 1 and rows(dtype=1) == 2 and rows(c=buf(0x20000, 511)) == 2 and rows(s=buf(0x30000, 15)) == 2
+    assert rows(c=buf(0x20004, 512)) == 1
+
+    assert lib.call_status("glmrt_b200_fp8_gated_mlp_workspace", Z(4), Z(128), Z(72), C.byref(need)) == 1
+    assert lib.call_status("glmrt_b200_fp8_gated_mlp_workspace", Z(4), Z(128), Z(64), C.byref(need)) == 0
+    names = ["x", "gc", "gs", "uc", "us", "dc", "ds", "o", "w"]
+    good = dict(zip(names, (buf(0x10000, 1024), buf(0x20000, 8192), buf(0x30000, 4), buf(0x40000, 8192), buf(0x50000, 4),
+                            buf(0x60000, 8192), buf(0x70000, 4), buf(0x80000, 1024), buf(0x100000, need.value))))
+
+    def mlp(rows=4, stride=128, **kw):
+        b = {**good, **kw}
+        return lib.call_status("glmrt_b200_fp8_gated_mlp_async", *[b[n] for n in names], Z(rows), Z(128), Z(64), Z(stride), None)
+
+    assert mlp(rows=0) == 0 and mlp(stride=64) == 1
+    for name in names:
+        assert mlp(**{name: null}) == 1, name
+        assert mlp(**{name: buf(good[name].ptr, good[name].bytes - 1)}) == 2, name
+
+
+def test_few_refusals(lib):
+    from glmrt_b200 import native as N
+    null = N.DeviceBuffer.null()
+    for name, args in (("glmrt_b200_moe_layer_forward_few_async", (null, C.c_size_t(1), null, null, null, null, null, None)),
+                       ("glmrt_b200_moe_layer_forward_few_routed_async", (null, C.c_size_t(1), null, null, null, null, null, None))):
+        assert lib.call_status(name, None, *args) == 1 and "null" in lib.last_error()
+
+
+def test_wrappers_refuse_host_tensors_and_wrong_shapes(pkg):
+    from glmrt_b200 import block_norm, fp8
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    w = torch.ones(64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        block_norm.block_norm(x, norm_weight=w)
+    with pytest.raises(ValueError, match="bfloat16 or float32"):
+        block_norm.block_norm(x.half(), norm_weight=w)
+    with pytest.raises(ValueError, match="rows"):
+        block_norm.block_norm(x[0], norm_weight=w)
+    codes, scales = fp8.quantize_weight(torch.randn(70, 64))
+    assert codes.shape == (70, 64) and scales.shape == (1, 1)
+    with pytest.raises(ValueError, match="CUDA"):
+        fp8.block_linear(x, codes, scales)
+    with pytest.raises(ValueError, match="must be"):
+        fp8.block_linear(x[:, :32], codes, scales)
+    with pytest.raises(ValueError, match="out_dtype"):
+        fp8.block_linear(x, codes, scales, out_dtype=torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        fp8.quantize_rows(x)
+
+
+def test_quantize_weight_against_the_definition(pkg):
+    from glmrt_b200 import fp8
+    w = torch.randn(200, 272, generator=torch.Generator().manual_seed(1)) * 0.02
+    w[130:, :128] = 0
+    codes, scales = fp8.quantize_weight(w)
+    for i in range(2):
+        for j in range(3):
+            b = w[128 * i:128 * i + 128, 128 * j:128 * j + 128]
+            s = float(b.abs().max()) / 448 or 1.0
+            assert abs(float(scales[i, j]) - s) <= 2 ** -22 * s
+            back = codes[128 * i:128 * i + 128, 128 * j:128 * j + 128].float() * scales[i, j]
+            # half a step of E4M3: 2^-4 of the value, or half the smallest step (2^-10) of the scale
+            assert ((back - b).abs() <= 2 ** -4 * b.abs() * 1.001 + 2 ** -10 * s).all()
