@@ -7,6 +7,10 @@
 //
 // with W = E2M1 code * E4M3 block scale * scale_2.  Nothing is rounded between the bf16 rows and the
 // bf16 result except where a comment says so.
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
 #include "common.cuh"
 #include "internal.h"
 
@@ -17,6 +21,652 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// ------------------------------------------------------------------------------------------------
+// One cooperative kernel, one CTA per SM, three grid-wide barriers:
+//
+//   logits     every warp: one expert x one share of the hidden columns, float32 weights       | barrier
+//   selection  every CTA for itself: sigmoid, top-k, the list of (expert, up to `cap` tokens) entries
+//   gate / up  the entries' rows split evenly over the CTAs                                    | barrier
+//   down       the same; one float32 row per route                                             | barrier
+//   combine    residual + (shared + sum over the slots, in slot order)
+//
+// What bounds it is the experts' weights (9/16 byte each, read once); everything else is arranged so
+// that they never stop arriving.  Each lane copies its own pieces of the weights into shared memory
+// (cp.async), kRing pieces ahead, and only itself reads them back, so the stream needs no barrier
+// between warps; it runs on from the gate / up rows into the down rows while the CTA waits at the
+// barrier between them.
+//
+// A piece is 16 weight rows x 128 columns of one warp: 16 B of codes of each of two rows per lane (32
+// columns) and the scales of both.  E2M1 codes become fp16 pairs (one instruction for two), times
+// the E4M3 scale: the product has at most six significant bits, so it is exact.  The tensor cores multiply
+// (m16n8k16; tokens are the eight columns) and add in float32.  Which columns a lane holds does not
+// matter as long as both operands agree, so lane t of a row's four takes columns 32t .. 32t+31.
+//
+// The rows as fp16: times a power of two per token that brings the largest magnitude to 2^14, which is
+// exact for everything within 2^28 of it and off by 2^-39 of it below.  The SwiGLU rows likewise, rounded
+// from float32 to fp16's 11 bits (2^-12 of a value: a sixteenth of the bf16 result's rounding).
+// ------------------------------------------------------------------------------------------------
+constexpr int kWarps = 16;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kPieceBytes = 1280;            // per warp: two 16-byte codes and 8 scale bytes a lane
+constexpr int kMaxEntries = 256;             // (expert, token group) pairs: at most one per route
+constexpr int kMaxRoutes = 256;
+constexpr uint64_t kBarrierLimitNs = 2000000000ull;
+
+struct FewShared {
+  uint16_t ent_expert[kMaxEntries];
+  int16_t ent_route[kMaxEntries][8];         // column -> route, or -1
+  float ent_w[kMaxEntries][8];               // column -> weight
+  uint32_t route_expert[kMaxRoutes];
+  float route_w[kMaxRoutes];
+  int16_t route_entry[kMaxRoutes];           // entry that a starting route opens
+  uint32_t used[kFewMaxRows];                // slots of a token that own a result row
+  uint32_t act_amax[kFewMaxRows];
+  float col_inv[8];                          // undoes the power of two of a column's values
+  uint32_t col_amax[8];
+  int warp_count[kWarps];
+  int entries, distinct, bad, abort;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
+
+// Eight E2M1 codes -> four fp16 pairs, in order.
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&d)[4]) {
+  asm("{\n\t.reg .b8 x0, x1, x2, x3;\n\t"
+      "mov.b32 {x0, x1, x2, x3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, x0;\n\tcvt.rn.f16x2.e2m1x2 %1, x1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, x2;\n\tcvt.rn.f16x2.e2m1x2 %3, x3;\n\t}"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(w));
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// Two E4M3 bytes -> two fp16 pairs, each holding one of them twice.
+__device__ __forceinline__ void e4m3x2_to_pairs(uint32_t two, uint32_t& lo, uint32_t& hi) {
+  uint32_t h;
+  asm("{\n\t.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(h) : "r"(two));
+  lo = __byte_perm(h, 0, 0x1010);
+  hi = __byte_perm(h, 0, 0x3232);
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// All CTAs of the grid (co-resident: cooperative launch).  The last arrival frees the others and
+// leaves the counter at zero for the next use.  False when the wait ran out.
+__device__ bool grid_barrier(uint32_t* sync, int* abort) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t gen, now;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(gen) : "l"(sync + 1) : "memory");
+    __threadfence();
+    if (atomicAdd(sync, 1u) == gridDim.x - 1) {
+      *reinterpret_cast<volatile uint32_t*>(sync) = 0u;
+      __threadfence();
+      asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(sync + 1), "r"(gen + 1) : "memory");
+    } else {
+      uint64_t t0 = 0, t;
+      for (uint32_t spin = 0;; ++spin) {
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(sync + 1) : "memory");
+        if (now != gen) break;
+        if ((spin & 255u) == 255u) {
+          asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+          if (t0 == 0) t0 = t;
+          else if (t - t0 > kBarrierLimitNs) { *abort = 1; break; }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  return *reinterpret_cast<volatile int*>(abort) == 0;
+}
+
+// One of the two weight passes: which rows, and how the CTA's warps share a group of them.
+struct Pass {
+  int units;            // 128-column units of K
+  int kw, rw;           // warps along K, warps along the rows (kw * rw = kWarps)
+  int per_entry;        // items (rw row units of 16 rows) per entry
+  int begin, end;       // this CTA's items
+};
+__device__ __forceinline__ Pass make_pass(int k, int rows, int entries) {
+  Pass p;
+  p.units = k / 128;
+  p.kw = kWarps;
+  while (p.kw / 2 >= p.units) p.kw /= 2;
+  p.rw = kWarps / p.kw;
+  p.per_entry = rows / 16 / p.rw;
+  const long long items = static_cast<long long>(entries) * p.per_entry;
+  p.begin = static_cast<int>(items * blockIdx.x / gridDim.x);
+  p.end = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
+  return p;
+}
+// First row of a row unit: rows R .. R+7 and R+32 .. R+39 of a 128-row scale tile, whose scales lie
+// next to each other in pairs (sf_tile_offset).
+__device__ __forceinline__ int unit_row(int u) { return (u >> 3) * 128 + ((u >> 2) & 1) * 64 + (u & 3) * 8; }
+
+// Walks a warp's pieces of one pass in the order they are consumed: groups of items of one entry, in
+// each the warp's K units, in each unit the pieces of the group (gate / up: both matrices of one
+// item; down: up to two items).
+template <bool kGateUp>
+struct Cursor {
+  int item, size, k, m;
+  __device__ __forceinline__ bool start(const Pass& p, int kwi) {
+    item = p.begin;
+    return open(p, kwi);
+  }
+  __device__ __forceinline__ bool open(const Pass& p, int kwi) {
+    if (item >= p.end || kwi >= p.units) return false;
+    size = kGateUp ? 2 : min(2, min(p.end - item, p.per_entry - item % p.per_entry));
+    k = kwi;
+    m = 0;
+    return true;
+  }
+  __device__ __forceinline__ bool next(const Pass& p, int kwi) {
+    if (++m < size) return true;
+    m = 0;
+    k += p.kw;
+    if (k < p.units) return true;
+    item += kGateUp ? 1 : size;
+    return open(p, kwi);
+  }
+};
+
+template <bool kGateUp>
+__device__ __forceinline__ void issue_piece(const FewArgs& a, const FewShared& sh, const Pass& p, const Cursor<kGateUp>& c,
+                                            int rwi, uint32_t slot, int lane) {
+  const int it = kGateUp ? c.item : c.item + c.m;
+  const int j = it / p.per_entry, u = (it - j * p.per_entry) * p.rw + rwi;
+  const int g = lane >> 2, t = lane & 3;
+  const uint8_t* codes = kGateUp ? (c.m == 0 ? a.gate_codes : a.up_codes) : a.down_codes;
+  const uint8_t* sf = kGateUp ? (c.m == 0 ? a.gate_sf : a.up_sf) : a.down_sf;
+  const int row_bytes = (kGateUp ? a.hidden : a.inter) / 2, rows = kGateUp ? a.inter : a.hidden;
+  const size_t row = static_cast<size_t>(sh.ent_expert[j]) * rows + unit_row(u);
+  const uint8_t* src = codes + (row + g) * row_bytes + c.k * 64 + t * 16;
+  const uint32_t dst = slot + lane * 16;
+  cp_async16(dst, src);
+  cp_async16(dst + 512, src + static_cast<size_t>(32) * row_bytes);
+  cp_async8(slot + 1024 + lane * 8, sf + ((row >> 7) * (row_bytes >> 5) + c.k * 2 + (t >> 1)) * 512 +
+                                        ((u & 3) * 8 + g) * 16 + ((u >> 2) & 1) * 8);
+}
+
+// The warp's stream of pieces through both passes.
+struct Stream {
+  Cursor<true> c1;
+  Cursor<false> c2;
+  bool more1, more2;
+  int kw1, rw1, kw2, rw2;
+  uint32_t ring, head;      // shared address of the warp's ring, next slot to fill (bytes)
+  uint32_t ring_bytes;
+  __device__ __forceinline__ void issue(const FewArgs& a, const FewShared& sh, const Pass& p1, const Pass& p2, int lane) {
+    if (more1) {
+      issue_piece<true>(a, sh, p1, c1, rw1, ring + head, lane);
+      more1 = c1.next(p1, kw1);
+    } else if (more2) {
+      issue_piece<false>(a, sh, p2, c2, rw2, ring + head, lane);
+      more2 = c2.next(p2, kw2);
+    }
+    head = head + kPieceBytes == ring_bytes ? 0 : head + kPieceBytes;
+    cp_async_commit();        // one group per call, also when nothing is left: the count of pending groups stays exact
+  }
+};
+
+// acc += the piece's 16 x 128 weights times the unit's columns.
+__device__ __forceinline__ void multiply_piece(float (&acc)[4], uint32_t slot, const uint32_t (&b)[16], int lane) {
+  uint4 w0, w1;
+  uint32_t s0, s1;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w0.x), "=r"(w0.y), "=r"(w0.z), "=r"(w0.w) : "r"(slot + lane * 16));
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w1.x), "=r"(w1.y), "=r"(w1.z), "=r"(w1.w) : "r"(slot + 512 + lane * 16));
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(s0), "=r"(s1) : "r"(slot + 1024 + lane * 8));
+  const int shift = (lane & 1) * 16;
+  uint32_t r0[2], r1[2];      // scales of the lane's two blocks, rows g and g + 32
+  e4m3x2_to_pairs(s0 >> shift, r0[0], r0[1]);
+  e4m3x2_to_pairs(s1 >> shift, r1[0], r1[1]);
+  const uint32_t a0[4] = {w0.x, w0.y, w0.z, w0.w}, a1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t d0[4], d1[4];
+    e2m1x8_to_f16(a0[i], d0);
+    e2m1x8_to_f16(a1[i], d1);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      d0[v] = mul_f16x2(d0[v], r0[i / 2]);
+      d1[v] = mul_f16x2(d1[v], r1[i / 2]);
+    }
+    mma16816(acc, d0[0], d1[0], d0[1], d1[1], b[4 * i], b[4 * i + 1]);
+    mma16816(acc, d0[2], d1[2], d0[3], d1[3], b[4 * i + 2], b[4 * i + 3]);
+  }
+}
+
+// Power of two that brings a largest magnitude with these bits into [2^14, 2^15), and its inverse.
+// Zero, infinite and NaN maxima: 1.  Far below 2^-112 the largest factor, 2^126, is kept.
+__device__ __forceinline__ float f16_factor(uint32_t amax, float* inverse) {
+  if (amax == 0u || amax >= 0x7f800000u) {
+    *inverse = 1.0f;
+    return 1.0f;
+  }
+  const int e = max(static_cast<int>(amax >> 23), 1) - 127;
+  const int k = min(14 - e, 126);
+  *inverse = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+  return __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+}
+
+// Columns of `cols` tokens, as fp16 in the order the lanes read them: [unit][quarter i][column][t] pieces of
+// 16 B, piece (i, t) of a unit = its columns 32t + 8i .. + 7.
+// kAct: float32 SwiGLU rows (scaled by their token's amax), else bf16 hidden rows (amax found here).
+template <bool kAct>
+__device__ void load_columns(const FewArgs& a, FewShared& sh, uint8_t* dst, int entry, int cols, bool identity) {
+  const int k = kAct ? a.inter : a.hidden;
+  const int tid = threadIdx.x;
+  auto route_of = [&](int c) { return static_cast<int>(sh.ent_route[entry][c]); };
+  auto token_of = [&](int c) { return identity ? c : (route_of(c) < 0 ? -1 : route_of(c) / a.top_k); };
+  __syncthreads();                       // the previous columns have been read
+  if (!kAct) {
+    if (tid < 8) sh.col_amax[tid] = 0u;
+    __syncthreads();
+    // warps in turn over (column, 256-value piece)
+    const int pieces = k / 256;
+    for (int i = tid / 32; i < cols * pieces; i += kWarps) {
+      const int c = i / pieces, tok = token_of(c);
+      if (tok < 0) continue;
+      const uint4 q = *reinterpret_cast<const uint4*>(a.hidden_rows + static_cast<size_t>(tok) * k + (i - c * pieces) * 256 + (tid & 31) * 8);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+      uint32_t m = 0;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) m = max(m, max(w[v] << 16 & 0x7fffffffu, w[v] & 0x7fff0000u));
+      m = __reduce_max_sync(0xffffffffu, m);
+      if ((tid & 31) == 0) atomicMax(&sh.col_amax[c], m);
+    }
+    __syncthreads();
+  }
+  const int per_col = k / 8;
+  for (int i = tid; i < cols * per_col; i += kThreads) {
+    const int c = i / per_col, o = i - c * per_col;       // o: 8-value piece of the row
+    const int unit = o >> 4, t = (o >> 2) & 3, q = o & 3;
+    const int tok = token_of(c);
+    uint32_t h[4] = {0u, 0u, 0u, 0u};
+    if (tok >= 0 && (!kAct || route_of(c) >= 0)) {
+      float v[8], inv;
+      const float f = f16_factor(kAct ? sh.act_amax[tok] : sh.col_amax[c], &inv);
+      if (kAct) {
+        const float4* src = reinterpret_cast<const float4*>(a.act + static_cast<size_t>(route_of(c)) * k + o * 8);
+        const float4 x = __ldcg(src), y = __ldcg(src + 1);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(a.hidden_rows + static_cast<size_t>(tok) * k + o * 8);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          v[2 * n] = __uint_as_float(w[n] << 16);
+          v[2 * n + 1] = __uint_as_float(w[n] & 0xffff0000u);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const __half2 p = __floats2half2_rn(v[2 * n] * f, v[2 * n + 1] * f);
+        h[n] = *reinterpret_cast<const uint32_t*>(&p);
+      }
+    }
+    *reinterpret_cast<uint4*>(dst + ((unit * 4 + q) * cols * 4 + c * 4 + t) * static_cast<size_t>(16)) = make_uint4(h[0], h[1], h[2], h[3]);
+  }
+  if (tid < cols) {
+    const int tok = token_of(tid);
+    float inv = 1.0f;
+    if (tok >= 0) f16_factor(kAct ? sh.act_amax[tok] : sh.col_amax[tid], &inv);
+    sh.col_inv[tid] = inv;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void load_b(uint32_t (&b)[16], const uint8_t* columns, int unit, int cols, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint4 q = make_uint4(0u, 0u, 0u, 0u);
+    if (g < cols) q = *reinterpret_cast<const uint4*>(columns + ((unit * 4 + i) * cols * 4 + g * 4 + t) * static_cast<size_t>(16));
+    b[4 * i] = q.x; b[4 * i + 1] = q.y; b[4 * i + 2] = q.z; b[4 * i + 3] = q.w;
+  }
+}
+
+// Partial sums of a group: [warp][piece m][row][column], `pitch` columns (cap rounded up to two).
+__device__ __forceinline__ void store_partial(float* red, const float (&acc)[2][4], int warp, int lane, int pitch, int cols) {
+  const int g = lane >> 2, t = lane & 3;
+  if (2 * t >= cols) return;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    float* d = red + ((warp * 2 + m) * 16 + g) * pitch + 2 * t;
+    *reinterpret_cast<float2*>(d) = make_float2(acc[m][0], acc[m][1]);
+    *reinterpret_cast<float2*>(d + 8 * pitch) = make_float2(acc[m][2], acc[m][3]);
+  }
+}
+
+__device__ void route_and_select(const FewArgs& a, FewShared& sh, float* scratch, int cap, bool identity) {
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int routes = a.rows * a.top_k;
+  if (a.logits != nullptr) {
+    // scores of all rows, the column shares added in order
+    const int n = a.rows * a.experts;
+    for (int i = tid; i < n; i += kThreads) {
+      float s = 0.0f;
+      for (int p = 0; p < a.splits; ++p) s += __ldcg(a.logits + static_cast<size_t>(p) * n + i);
+      scratch[i] = sigmoid_f32(s);
+    }
+    __syncthreads();
+    if (warp < a.rows) {
+      // keys that order like (score + bias, lower id first); a NaN ranks last
+      const float* score = scratch + warp * a.experts;
+      uint32_t key[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int e = lane + 32 * i;
+        key[i] = 0u;
+        if (e < a.experts) {
+          const float s = score[e] + a.router_b[e];
+          const uint32_t u = __float_as_uint(s == 0.0f ? 0.0f : s);
+          key[i] = s != s ? 1u : ((u >> 31) ? ~u : u | 0x80000000u);
+        }
+      }
+      float sum = 0.0f;
+      uint32_t mine = 0;
+      for (int s = 0; s < a.top_k; ++s) {
+        uint32_t best = 0u;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i * 32 < a.experts) best = max(best, key[i]);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        uint32_t id = 0xffffffffu;
+        if (best == top)
+#pragma unroll
+          for (int i = 31; i >= 0; --i)
+            if (key[i] == top && lane + 32 * i < a.experts) id = lane + 32 * i;
+        id = __reduce_min_sync(0xffffffffu, id);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (lane + 32 * i == static_cast<int>(id)) key[i] = 0u;
+        sum += score[id];
+        if (lane == s) mine = id;
+      }
+      const float inv = a.scaling / fmaxf(sum, 1e-12f);
+      if (lane < a.top_k) {
+        const int r = warp * a.top_k + lane;
+        sh.route_expert[r] = mine;
+        sh.route_w[r] = score[mine] * inv;
+      }
+    }
+  } else if (tid < routes) {
+    sh.route_expert[tid] = a.topk_idx[tid];
+    sh.route_w[tid] = a.topk_w[tid];
+  }
+  if (tid < kFewMaxRows) {
+    sh.used[tid] = 0u;
+    sh.act_amax[tid] = 0u;
+  }
+  if (tid == 0) { sh.bad = 0; sh.distinct = 0; }
+  for (int i = tid; i < kMaxEntries * 8; i += kThreads) {
+    sh.ent_route[i / 8][i % 8] = -1;
+    sh.ent_w[i / 8][i % 8] = 0.0f;
+  }
+  __syncthreads();
+  if (a.out_idx != nullptr && blockIdx.x == 0 && tid < routes) {
+    a.out_idx[tid] = sh.route_expert[tid];
+    a.out_w[tid] = sh.route_w[tid];
+  }
+  // Entries, in the order of the first route that names each: an expert's tokens in groups of `cap`
+  // (identity: all rows are one group and a token's column is its row).
+  uint32_t e = kNoRoute;
+  int rank = 0, opener = tid, slot = 0, token = 0;
+  bool live = false;
+  float w = 0.0f;
+  if (tid < routes) {
+    e = sh.route_expert[tid];
+    token = tid / a.top_k; slot = tid - token * a.top_k;
+    live = e < static_cast<uint32_t>(a.experts);
+    if (!live && e != kNoRoute) sh.bad = 1;
+    w = sh.route_w[tid];
+    const int row0 = token * a.top_k;
+    int last_token = -1;
+    for (int r = 0; r < tid && live; ++r) {
+      if (sh.route_expert[r] != e) continue;
+      if (r >= row0) { live = false; break; }     // the row has named this expert before: its weight went there
+      const int tr = r / a.top_k;
+      if (tr == last_token) continue;             // a second mention in an earlier row
+      last_token = tr;
+      if (rank % cap == 0) opener = r;
+      ++rank;
+    }
+    if (rank % cap == 0) opener = tid;
+    for (int r = tid + 1; r < row0 + a.top_k && live; ++r)
+      if (sh.route_expert[r] == e) w += sh.route_w[r];
+  }
+  const bool opens = live && opener == tid;
+  const uint32_t votes = __ballot_sync(0xffffffffu, opens);
+  if (lane == 0) sh.warp_count[warp] = __popc(votes);
+  __syncthreads();
+  int before = __popc(votes & ((1u << lane) - 1u)), total = 0;
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) before += sh.warp_count[i];
+    total += sh.warp_count[i];
+  }
+  if (opens) {
+    sh.route_entry[tid] = static_cast<int16_t>(before);
+    sh.ent_expert[before] = static_cast<uint16_t>(e);
+    if (rank == 0) atomicAdd(&sh.distinct, 1);
+  }
+  if (live) atomicOr(&sh.used[token], 1u << slot);
+  if (tid == 0) sh.entries = total;
+  __syncthreads();
+  if (live) {
+    const int entry = sh.route_entry[opener], col = identity ? token : rank % cap;
+    sh.ent_route[entry][col] = static_cast<int16_t>(tid);
+    sh.ent_w[entry][col] = w;
+  }
+  __syncthreads();
+}
+
+template <int kRing>
+__global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int cap) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  FewShared& sh = *reinterpret_cast<FewShared*>(smem);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const bool identity = a.rows <= cap;
+  const int cols = identity ? a.rows : cap;
+  const int pitch = (cols + 1) & ~1;
+  uint8_t* ring = smem + ((sizeof(FewShared) + 127) & ~static_cast<size_t>(127));
+  float* red = reinterpret_cast<float*>(ring + kRing * kWarps * kPieceBytes);
+  const int red_floats = kWarps * 2 * 16 * pitch;
+  uint8_t* columns = reinterpret_cast<uint8_t*>(red + 2 * red_floats);
+  if (tid == 0) sh.abort = 0;
+
+  // ---- logits: task = (column share, expert), one warp each ----
+  if (a.logits != nullptr) {
+    const int units = a.hidden / 128, n = a.rows * a.experts;
+    for (int task = blockIdx.x * kWarps + warp; task < a.splits * a.experts; task += gridDim.x * kWarps) {
+      const int p = task / a.experts, e = task - p * a.experts;
+      const int u0 = units * p / a.splits, u1 = units * (p + 1) / a.splits;
+      const float* wrow = a.router_w + static_cast<size_t>(e) * a.hidden + lane * 4;
+      const uint16_t* xrow = a.hidden_rows + lane * 4;
+      float acc[kFewMaxRows];
+#pragma unroll
+      for (int t = 0; t < kFewMaxRows; ++t) acc[t] = 0.0f;
+#pragma unroll 2
+      for (int u = u0; u < u1; ++u) {
+        const float4 wv = __ldg(reinterpret_cast<const float4*>(wrow + u * 128));
+#pragma unroll
+        for (int t = 0; t < kFewMaxRows; ++t) {
+          if (t >= a.rows) break;
+          const uint2 x = __ldg(reinterpret_cast<const uint2*>(xrow + static_cast<size_t>(t) * a.hidden + u * 128));
+          acc[t] = fmaf(__uint_as_float(x.x << 16), wv.x, acc[t]);
+          acc[t] = fmaf(__uint_as_float(x.x & 0xffff0000u), wv.y, acc[t]);
+          acc[t] = fmaf(__uint_as_float(x.y << 16), wv.z, acc[t]);
+          acc[t] = fmaf(__uint_as_float(x.y & 0xffff0000u), wv.w, acc[t]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < kFewMaxRows; ++t) {
+        if (t >= a.rows) break;
+        const float s = warp_sum(acc[t]);
+        if (lane == 0) a.logits[static_cast<size_t>(p) * n + t * a.experts + e] = s;
+      }
+    }
+    if (!grid_barrier(a.sync, &sh.abort)) {
+      if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
+      return;
+    }
+  }
+  route_and_select(a, sh, reinterpret_cast<float*>(ring), cap, identity);
+  if (blockIdx.x == 0 && tid == 0) {
+    a.error_word[0] = sh.bad ? static_cast<uint32_t>(kErrBadExpert) : 0u;
+    a.counters[kCntChunks] = static_cast<uint32_t>(sh.entries);
+    a.counters[kCntDistinct] = static_cast<uint32_t>(sh.distinct);
+  }
+
+  // ---- the weight stream ----
+  const Pass p1 = make_pass(a.hidden, a.inter, sh.entries), p2 = make_pass(a.inter, a.hidden, sh.entries);
+  Stream st;
+  st.kw1 = warp % p1.kw; st.rw1 = warp / p1.kw;
+  st.kw2 = warp % p2.kw; st.rw2 = warp / p2.kw;
+  st.more1 = st.c1.start(p1, st.kw1);
+  st.more2 = st.c2.start(p2, st.kw2);
+  st.ring = smem_addr(ring) + warp * kRing * kPieceBytes;
+  st.ring_bytes = kRing * kPieceBytes;
+  st.head = 0;
+#pragma unroll 1
+  for (int i = 0; i < kRing - 1; ++i) st.issue(a, sh, p1, p2, lane);
+  uint32_t tail = 0;
+  int flip = 0;
+
+  // ---- gate and up ----
+  int entry = -1;
+  for (int it = p1.begin; it < p1.end; ++it) {
+    const int j = it / p1.per_entry;
+    if (j != entry) {
+      if (entry < 0 || !identity) load_columns<false>(a, sh, columns, j, cols, identity);
+      entry = j;
+    }
+    float acc[2][4] = {};
+    for (int k = st.kw1; k < p1.units; k += p1.kw) {
+      uint32_t b[16];
+      load_b(b, columns, k, cols, lane);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        cp_async_wait<kRing - 2>();
+        multiply_piece(acc[m], st.ring + tail, b, lane);
+        tail = tail + kPieceBytes == st.ring_bytes ? 0 : tail + kPieceBytes;
+        st.issue(a, sh, p1, p2, lane);
+      }
+    }
+    float* part = red + flip * red_floats;
+    flip ^= 1;
+    store_partial(part, acc, warp, lane, pitch, cols);
+    __syncthreads();
+    const uint32_t e = sh.ent_expert[j];
+    const float s2g = __ldg(a.scale2 + e * 3), s2u = __ldg(a.scale2 + e * 3 + 1);
+    const int u0 = (it - j * p1.per_entry) * p1.rw;
+    const int warps_k = min(p1.kw, p1.units);
+    for (int i = tid; i < p1.rw * 16 * cols; i += kThreads) {
+      const int c = i % cols, r = (i / cols) % 16, rw = i / (cols * 16);
+      const int route = sh.ent_route[j][c];
+      if (route < 0) continue;
+      float g = 0.0f, u = 0.0f;
+      for (int w = 0; w < warps_k; ++w) {
+        const float* src = part + ((rw * p1.kw + w) * 2 * 16 + r) * pitch + c;
+        g += src[0];
+        u += src[16 * pitch];
+      }
+      const float inv = sh.col_inv[c];
+      g *= s2g * inv;
+      u *= s2u * inv;
+      const float v = sh.ent_w[j][c] * (__fdividef(g, 1.0f + __expf(-g)) * u);
+      a.act[static_cast<size_t>(route) * a.inter + unit_row(u0 + rw) + (r & 7) + (r >> 3) * 32] = v;
+      atomicMax(&sh.act_amax[route / a.top_k], __float_as_uint(v) & 0x7fffffffu);
+    }
+  }
+  __syncthreads();
+  if (tid < a.rows && sh.act_amax[tid] != 0u) atomicMax(a.act_amax + tid, sh.act_amax[tid]);
+  bool alive = grid_barrier(a.sync, &sh.abort);
+
+  // ---- down ----
+  if (alive) {
+    if (tid < a.rows) sh.act_amax[tid] = __ldcg(a.act_amax + tid);
+    entry = -1;
+    for (int it = p2.begin; it < p2.end;) {
+      const int j = it / p2.per_entry;
+      const int size = min(2, min(p2.end - it, p2.per_entry - (it - j * p2.per_entry)));
+      if (j != entry) {
+        load_columns<true>(a, sh, columns, j, cols, identity);
+        entry = j;
+      }
+      float acc[2][4] = {};
+      for (int k = st.kw2; k < p2.units; k += p2.kw) {
+        uint32_t b[16];
+        load_b(b, columns, k, cols, lane);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          if (m < size) {
+            cp_async_wait<kRing - 2>();
+            multiply_piece(acc[m], st.ring + tail, b, lane);
+            tail = tail + kPieceBytes == st.ring_bytes ? 0 : tail + kPieceBytes;
+            st.issue(a, sh, p1, p2, lane);
+          }
+        }
+      }
+      float* part = red + flip * red_floats;
+      flip ^= 1;
+      store_partial(part, acc, warp, lane, pitch, cols);
+      __syncthreads();
+      const float s2 = __ldg(a.scale2 + sh.ent_expert[j] * 3 + 2);
+      const int warps_k = min(p2.kw, p2.units);
+      for (int i = tid; i < size * p2.rw * 16 * cols; i += kThreads) {
+        const int r = i % 16, c = (i / 16) % cols, rest = i / (16 * cols), rw = rest % p2.rw, m = rest / p2.rw;
+        const int route = sh.ent_route[j][c];
+        if (route < 0) continue;
+        float y = 0.0f;
+        for (int w = 0; w < warps_k; ++w) y += part[(((rw * p2.kw + w) * 2 + m) * 16 + r) * pitch + c];
+        const int u = (it + m - j * p2.per_entry) * p2.rw + rw;
+        a.route_out[static_cast<size_t>(route) * a.hidden + unit_row(u) + (r & 7) + (r >> 3) * 32] = y * (s2 * sh.col_inv[c]);
+      }
+      it += size;
+    }
+    alive = grid_barrier(a.sync, &sh.abort);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!alive) {
+    if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
+    return;
+  }
+
+  // ---- combine ----
+  if (blockIdx.x == 0 && tid < a.rows) a.act_amax[tid] = 0u;      // for the next call; read by all before the barrier
+  const int n = a.rows * a.hidden;
+  for (int i = blockIdx.x * kThreads + tid; i < n; i += gridDim.x * kThreads) {
+    const int t = i / a.hidden, h = i - t * a.hidden;
+    float y = 0.0f;
+    const uint32_t used = sh.used[t];
+    const float* src = a.route_out + static_cast<size_t>(t) * a.top_k * a.hidden + h;
+#pragma unroll 8
+    for (int s = 0; s < a.top_k; ++s)
+      if (used >> s & 1u) y += __ldcg(src + static_cast<size_t>(s) * a.hidden);
+    if (a.shared != nullptr) y += bf16_bits_to_f32(a.shared[i]);
+    if (a.residual != nullptr) y += bf16_bits_to_f32(a.residual[i]);
+    a.out[i] = f32_to_bf16_rne(y);
+  }
 }
 
 // Verification form: one warp per (route, intermediate row).
@@ -88,6 +738,56 @@ __global__ void few_fc2_simt_kernel(FewArgs a) {
 }
 
 }  // namespace
+
+int few_splits(int sm_count, int experts, int hidden) {
+  const int s = sm_count * kWarps / experts, most = hidden / 128;
+  return s < 1 ? 1 : (s > kFewMaxSplits ? kFewMaxSplits : s) > most ? most : (s > kFewMaxSplits ? kFewMaxSplits : s);
+}
+
+namespace {
+size_t few_smem(int ring, int cols, int k) {
+  const size_t fixed = (sizeof(FewShared) + 127) & ~static_cast<size_t>(127);
+  return fixed + static_cast<size_t>(ring) * kWarps * kPieceBytes + 2 * static_cast<size_t>(kWarps) * 2 * 16 * ((cols + 1) & ~1) * 4 +
+         static_cast<size_t>(cols) * k * 2;
+}
+constexpr size_t kSmemMost = 227 * 1024;
+
+template <int kRing>
+glmrt_status_t launch_ring(const FewArgs& a, int cap, size_t smem, int sm_count, cudaStream_t s) {
+  static std::atomic<uint64_t> configured{0};
+  GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, few_layer_kernel<kRing>, kSmemMost, "cudaFuncSetAttribute(few_layer_kernel)"));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(sm_count));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t err = cudaLaunchKernelEx(&cfg, few_layer_kernel<kRing>, a, cap);
+  if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "few_layer_kernel", err);
+  GLMRT_LAUNCH_CHECK("few_layer_kernel");
+  return GLMRT_STATUS_OK;
+}
+}  // namespace
+
+// Columns per pass over an expert and depth of the stream, from what fits into shared memory: the
+// selection's scores (rows * experts floats) are kept in the ring, and a ring of at least four pieces is needed.
+bool few_fused_supported(const FewArgs& a) {
+  return few_smem(4, 1, max(a.hidden, a.inter)) <= kSmemMost &&
+         static_cast<size_t>(a.rows) * a.experts * 4 <= 4 * static_cast<size_t>(kWarps) * kPieceBytes;
+}
+glmrt_status_t launch_few_fused(const FewArgs& a, int sm_count, cudaStream_t s) {
+  const int k = std::max(a.hidden, a.inter);
+  int cap = std::min(a.rows, 4);
+  while (cap > 1 && few_smem(4, cap, k) > kSmemMost) --cap;
+  const int cols = a.rows <= cap ? a.rows : cap;
+  if (few_smem(9, cols, k) <= kSmemMost) return launch_ring<9>(a, cap, few_smem(9, cols, k), sm_count, s);
+  if (few_smem(6, cols, k) <= kSmemMost) return launch_ring<6>(a, cap, few_smem(6, cols, k), sm_count, s);
+  return launch_ring<4>(a, cap, few_smem(4, cols, k), sm_count, s);
+}
 
 glmrt_status_t launch_few_simt(const FewArgs& a, cudaStream_t s) {
   launch_pdl(few_fc1_simt_kernel, dim3((a.inter + 7) / 8, a.rows * a.top_k), dim3(256), 0, s, a);

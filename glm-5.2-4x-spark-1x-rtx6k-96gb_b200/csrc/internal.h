@@ -314,7 +314,22 @@ struct FewArgs {
   float* act;                                               // [rows * top_k, inter] weighted SwiGLU rows
   uint32_t* error_word;
   int rows, top_k, experts, hidden, inter;
+  // the fused kernel only
+  const float *router_w, *router_b;                         // [experts, hidden], [experts] float32
+  float* logits;                                            // [splits][rows][experts] partial sums; nullptr: routes given
+  int splits;
+  float scaling;
+  uint32_t* out_idx;                                        // where the routes are written, or nullptr
+  float* out_w;
+  float* route_out;                                         // [rows * top_k, hidden] float32 result rows
+  uint32_t* act_amax;                                       // [kFewMaxRows] zero between calls
+  uint32_t* sync;                                           // barrier count (zero between calls) and generation
+  uint32_t* counters;
 };
+constexpr int kFewMaxSplits = 16;
+int few_splits(int sm_count, int experts, int hidden);      // column shares of the router's logits
+bool few_fused_supported(const FewArgs& a);
+glmrt_status_t launch_few_fused(const FewArgs& a, int sm_count, cudaStream_t stream);
 glmrt_status_t launch_few_simt(const FewArgs& a, cudaStream_t stream);
 
 }  // namespace glmrt

@@ -49,6 +49,8 @@ struct EpState {
   uint32_t global_rows = 0;   // rows of the whole batch over all ranks when the caller has said so, else 0
 };
 
+constexpr size_t kFewSyncWords = 32 + kFewMaxRows;   // barrier words in a line of their own, then the maxima
+
 struct Layer {
   glmrt_b200_moe_config_t cfg{};
   int device = 0;
@@ -81,7 +83,10 @@ struct Layer {
   uint16_t* route_rows = nullptr;
   uint16_t** slot_out = nullptr;
   uint32_t* slot_weight = nullptr;   // route weight per slot (fused combine of large batches)
-  float* few_act = nullptr;          // weighted SwiGLU rows of the few-token path
+  // few-token path: weighted SwiGLU rows, one float32 result row per route, partial logits, and the words
+  // its kernel leaves at zero (barrier, largest activations)
+  float *few_act = nullptr, *few_out = nullptr, *few_logits = nullptr;
+  uint32_t* few_sync = nullptr;
   uint32_t* fc_sync = nullptr;       // hand-over words between the decode FC1 and FC2 kernels
   uint16_t *hidden_stage = nullptr, *out_stage = nullptr;
   // scratch for weight loading
@@ -470,7 +475,13 @@ glmrt_status_t alloc_workspace(Layer* l) {
   // destinations start out null: a slot nobody dispatched to is skipped by the FC2 epilogues
   A(dev_alloc(b, &l->slot_out, static_cast<size_t>(l->max_slots), true));
   if (c.max_tokens > 256 && c.ep_world == 1) A(dev_alloc(b, &l->slot_weight, static_cast<size_t>(l->max_slots), true));
-  if (c.ep_world == 1) A(dev_alloc(b, &l->few_act, std::min<size_t>(T, kFewMaxRows) * K * I));
+  if (c.ep_world == 1) {
+    const size_t F = std::min<size_t>(T, kFewMaxRows);
+    A(dev_alloc(b, &l->few_act, F * K * I));
+    A(dev_alloc(b, &l->few_out, F * K * H));
+    A(dev_alloc(b, &l->few_logits, kFewMaxSplits * F * c.experts));
+    A(dev_alloc(b, &l->few_sync, kFewSyncWords, true));
+  }
   A(dev_alloc(b, &l->hidden_stage, T * H));
   A(dev_alloc(b, &l->out_stage, T * H));
   A(dev_alloc(b, &l->wtmp, std::max(I * H, static_cast<size_t>(1))));
@@ -784,8 +795,17 @@ glmrt_status_t few_args(Layer* l, const glmrt_device_buffer_t& hidden, size_t ro
   a.error_word = l->counters + kCntError;
   a.rows = static_cast<int>(rows); a.top_k = static_cast<int>(c.top_k); a.experts = static_cast<int>(c.experts);
   a.hidden = static_cast<int>(c.hidden_dim); a.inter = static_cast<int>(c.intermediate_dim);
+  a.router_w = l->router_w; a.router_b = l->router_b; a.scaling = c.routed_scaling;
+  a.route_out = l->few_out;
+  a.sync = l->few_sync; a.act_amax = l->few_sync + 32;
+  a.counters = l->counters;
   *out = a;
   return GLMRT_STATUS_OK;
+}
+
+// One fused kernel, except on the verification engine and for shapes beyond its shared memory.
+bool few_fused(const Layer* l, const FewArgs& a) {
+  return !(l->cfg.flags & GLMRT_B200_LAYER_ENGINE_SIMT) && few_fused_supported(a);
 }
 
 }  // namespace
@@ -802,16 +822,24 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_async(
   if (topk_weights.ptr != nullptr) GLMRT_RETURN_IF_ERROR(check_buf(topk_weights, routes * 4, "forward_few topk_weights"));
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   const uint64_t before = launches_total();
-  cudaError_t err = cudaMemsetAsync(l->counters + kCntError, 0, 4, s);
-  if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "forward_few clear", err);
-  GLMRT_RETURN_IF_ERROR(run_router(l, hidden_bf16.ptr, rows, s));
-  GLMRT_RETURN_IF_ERROR(launch_few_simt(a, s));
+  if (few_fused(l, a)) {
+    a.logits = l->few_logits;
+    a.splits = few_splits(l->sm_count, a.experts, a.hidden);
+    a.out_idx = static_cast<uint32_t*>(topk_indices.ptr);
+    a.out_w = static_cast<float*>(topk_weights.ptr);
+    GLMRT_RETURN_IF_ERROR(launch_few_fused(a, l->sm_count, s));
+  } else {
+    cudaError_t err = cudaMemsetAsync(l->counters + kCntError, 0, 4, s);
+    if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "forward_few clear", err);
+    GLMRT_RETURN_IF_ERROR(run_router(l, hidden_bf16.ptr, rows, s));
+    GLMRT_RETURN_IF_ERROR(launch_few_simt(a, s));
+    if (topk_indices.ptr != nullptr)
+      err = cudaMemcpyAsync(topk_indices.ptr, l->topk_idx, routes * 4, cudaMemcpyDeviceToDevice, s);
+    if (err == cudaSuccess && topk_weights.ptr != nullptr)
+      err = cudaMemcpyAsync(topk_weights.ptr, l->topk_w, routes * 4, cudaMemcpyDeviceToDevice, s);
+    if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "forward_few route copy", err);
+  }
   l->launches_last = static_cast<uint32_t>(launches_total() - before);
-  if (topk_indices.ptr != nullptr)
-    err = cudaMemcpyAsync(topk_indices.ptr, l->topk_idx, routes * 4, cudaMemcpyDeviceToDevice, s);
-  if (err == cudaSuccess && topk_weights.ptr != nullptr)
-    err = cudaMemcpyAsync(topk_weights.ptr, l->topk_w, routes * 4, cudaMemcpyDeviceToDevice, s);
-  if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "forward_few route copy", err);
   l->last_rows = static_cast<uint32_t>(rows);
   return ok();
 }
@@ -828,11 +856,15 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_routed_async(
   GLMRT_RETURN_IF_ERROR(check_buf(topk_weights, routes * 4, "forward_few_routed topk_weights"));
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   const uint64_t before = launches_total();
-  cudaError_t err = cudaMemsetAsync(l->counters + kCntError, 0, 4, s);
-  if (err == cudaSuccess) err = cudaMemcpyAsync(l->topk_idx, topk_indices.ptr, routes * 4, cudaMemcpyDeviceToDevice, s);
-  if (err == cudaSuccess) err = cudaMemcpyAsync(l->topk_w, topk_weights.ptr, routes * 4, cudaMemcpyDeviceToDevice, s);
-  if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "forward_few_routed route copy", err);
-  GLMRT_RETURN_IF_ERROR(launch_few_simt(a, s));
+  a.topk_idx = static_cast<uint32_t*>(topk_indices.ptr);
+  a.topk_w = static_cast<float*>(topk_weights.ptr);
+  if (few_fused(l, a)) {
+    GLMRT_RETURN_IF_ERROR(launch_few_fused(a, l->sm_count, s));
+  } else {
+    cudaError_t err = cudaMemsetAsync(l->counters + kCntError, 0, 4, s);
+    if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "forward_few_routed clear", err);
+    GLMRT_RETURN_IF_ERROR(launch_few_simt(a, s));
+  }
   l->launches_last = static_cast<uint32_t>(launches_total() - before);
   l->last_rows = static_cast<uint32_t>(rows);
   return ok();
@@ -915,6 +947,10 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_check(void* layer, void* cuda_str
   if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "layer check", err);
   const uint32_t e = host[kCntError] | host[kCntRouterError];
   if (e == 0) return ok();
+  // a few-token kernel that gave up leaves its barrier words behind: nothing runs now, so they are cleared
+  if ((e & kErrWaitTimeout) && l->few_sync != nullptr &&
+      (err = cudaMemset(l->few_sync, 0, kFewSyncWords * 4)) != cudaSuccess)
+    return fail_cuda(GLMRT_STATUS_COPY_FAILED, "layer check", err);
   std::string msg = "device reported:";
   if (e & kErrWaitTimeout) msg += " a bounded wait expired;";
   if (e & kErrSlotOverflow) msg += " route plan exceeds slot capacity;";
