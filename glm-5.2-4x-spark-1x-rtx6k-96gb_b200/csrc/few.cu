@@ -13,6 +13,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "tc_ptx.cuh"
 
 namespace glmrt {
 namespace {
@@ -34,12 +35,13 @@ __device__ __forceinline__ float warp_sum(float v) {
 //
 // What bounds it is the experts' weights (9/16 byte each, read once); everything else is arranged so
 // that they never stop arriving.  Each lane copies its own pieces of the weights into shared memory
-// (cp.async), kRing pieces ahead, and only itself reads them back, so the stream needs no barrier
+// (cp.async), kRing - 1 slots ahead, and only itself reads them back, so the stream needs no barrier
 // between warps; it runs on from the gate / up rows into the down rows while the CTA waits at the
 // barrier between them.
 //
 // A piece is 16 weight rows x 128 columns of one warp: 16 B of codes of each of two rows per lane (32
-// columns) and the scales of both.  E2M1 codes become fp16 pairs (one instruction for two), times
+// columns) and the scales of both.  A slot is two pieces at the same columns: the same rows of gate and up,
+// or 32 rows of down.  E2M1 codes become fp16 pairs (one instruction for two), times
 // the E4M3 scale: the product has at most six significant bits, so it is exact.  The tensor cores multiply
 // (m16n8k16; tokens are the eight columns) and add in float32.  Which columns a lane holds does not
 // matter as long as both operands agree, so lane t of a row's four takes columns 32t .. 32t+31.
@@ -48,9 +50,12 @@ __device__ __forceinline__ float warp_sum(float v) {
 // exact for everything within 2^28 of it and off by 2^-39 of it below.  The SwiGLU rows likewise, rounded
 // from float32 to fp16's 11 bits (2^-12 of a value: a sixteenth of the bf16 result's rounding).
 // ------------------------------------------------------------------------------------------------
-constexpr int kWarps = 16;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kPieceBytes = 1280;            // per warp: two 16-byte codes and 8 scale bytes a lane
+constexpr int kWarps = 16;                   // that multiply
+constexpr int kSumWarps = 4;                 // that add the warps' partial sums up and finish the rows
+constexpr int kMainThreads = 32 * kWarps;
+constexpr int kThreads = kMainThreads + 32 * kSumWarps;
+constexpr int kBufs = kSumWarps;             // items whose partial sums may be waiting, one per summing warp
+constexpr int kSlotBytes = 2560;             // per warp: two pieces of two 16-byte codes and 8 scale bytes a lane
 constexpr int kMaxEntries = 256;             // (expert, token group) pairs: at most one per route
 constexpr int kMaxRoutes = 256;
 constexpr uint64_t kBarrierLimitNs = 2000000000ull;
@@ -64,10 +69,11 @@ struct FewShared {
   int16_t route_entry[kMaxRoutes];           // entry that a starting route opens
   uint32_t used[kFewMaxRows];                // slots of a token that own a result row
   uint32_t act_amax[kFewMaxRows];
-  float col_inv[8];                          // undoes the power of two of a column's values
-  uint32_t col_amax[8];
-  int warp_count[kWarps];
-  int entries, distinct, bad, abort;
+  uint32_t x_amax[kFewMaxRows];
+  uint64_t full[kBufs], empty[kBufs];
+  int warp_count[kThreads / 32];
+  int entries, distinct, bad;
+  uint32_t abort;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -104,7 +110,7 @@ __device__ __forceinline__ void e4m3x2_to_pairs(uint32_t two, uint32_t& lo, uint
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -112,7 +118,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 
 // All CTAs of the grid (co-resident: cooperative launch).  The last arrival frees the others and
 // leaves the counter at zero for the next use.  False when the wait ran out.
-__device__ bool grid_barrier(uint32_t* sync, int* abort) {
+__device__ bool grid_barrier(uint32_t* sync, volatile uint32_t* abort) {
   __syncthreads();
   if (threadIdx.x == 0) {
     uint32_t gen, now;
@@ -130,129 +136,127 @@ __device__ bool grid_barrier(uint32_t* sync, int* abort) {
         if ((spin & 255u) == 255u) {
           asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
           if (t0 == 0) t0 = t;
-          else if (t - t0 > kBarrierLimitNs) { *abort = 1; break; }
+          else if (t - t0 > kBarrierLimitNs) { *abort = 1u; break; }
         }
       }
     }
   }
   __syncthreads();
-  return *reinterpret_cast<volatile int*>(abort) == 0;
+  return *abort == 0u;
 }
 
-// One of the two weight passes: which rows, and how the CTA's warps share a group of them.
+// One of the two weight passes: which rows, and how the CTA's warps share an item of them.  The split
+// follows from the shape alone, so that a row's sums do not depend on its batch.
 struct Pass {
   int units;            // 128-column units of K
   int kw, rw;           // warps along K, warps along the rows (kw * rw = kWarps)
-  int per_entry;        // items (rw row units of 16 rows) per entry
+  int per_entry;        // items (rw row groups: 16 rows of gate and up, 32 rows of down) per entry
   int begin, end;       // this CTA's items
 };
-__device__ __forceinline__ Pass make_pass(int k, int rows, int entries) {
+__device__ __forceinline__ Pass make_pass(int k, int groups, int entries) {
   Pass p;
   p.units = k / 128;
   p.kw = kWarps;
   while (p.kw / 2 >= p.units) p.kw /= 2;
   p.rw = kWarps / p.kw;
-  p.per_entry = rows / 16 / p.rw;
+  p.per_entry = groups / p.rw;
   const long long items = static_cast<long long>(entries) * p.per_entry;
   p.begin = static_cast<int>(items * blockIdx.x / gridDim.x);
   p.end = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
   return p;
 }
 // First row of a row unit: rows R .. R+7 and R+32 .. R+39 of a 128-row scale tile, whose scales lie
-// next to each other in pairs (sf_tile_offset).
+// next to each other in pairs (sf_tile_offset).  Units 2v and 2v+1 are 8 rows apart.
 __device__ __forceinline__ int unit_row(int u) { return (u >> 3) * 128 + ((u >> 2) & 1) * 64 + (u & 3) * 8; }
 
-// Walks a warp's pieces of one pass in the order they are consumed: groups of items of one entry, in
-// each the warp's K units, in each unit the pieces of the group (gate / up: both matrices of one
-// item; down: up to two items).
-template <bool kGateUp>
-struct Cursor {
-  int item, size, k, m;
-  __device__ __forceinline__ bool start(const Pass& p, int kwi) {
-    item = p.begin;
-    return open(p, kwi);
-  }
-  __device__ __forceinline__ bool open(const Pass& p, int kwi) {
-    if (item >= p.end || kwi >= p.units) return false;
-    size = kGateUp ? 2 : min(2, min(p.end - item, p.per_entry - item % p.per_entry));
-    k = kwi;
-    m = 0;
-    return true;
-  }
-  __device__ __forceinline__ bool next(const Pass& p, int kwi) {
-    if (++m < size) return true;
-    m = 0;
-    k += p.kw;
-    if (k < p.units) return true;
-    item += kGateUp ? 1 : size;
-    return open(p, kwi);
-  }
-};
-
-template <bool kGateUp>
-__device__ __forceinline__ void issue_piece(const FewArgs& a, const FewShared& sh, const Pass& p, const Cursor<kGateUp>& c,
-                                            int rwi, uint32_t slot, int lane) {
-  const int it = kGateUp ? c.item : c.item + c.m;
-  const int j = it / p.per_entry, u = (it - j * p.per_entry) * p.rw + rwi;
-  const int g = lane >> 2, t = lane & 3;
-  const uint8_t* codes = kGateUp ? (c.m == 0 ? a.gate_codes : a.up_codes) : a.down_codes;
-  const uint8_t* sf = kGateUp ? (c.m == 0 ? a.gate_sf : a.up_sf) : a.down_sf;
-  const int row_bytes = (kGateUp ? a.hidden : a.inter) / 2, rows = kGateUp ? a.inter : a.hidden;
-  const size_t row = static_cast<size_t>(sh.ent_expert[j]) * rows + unit_row(u);
-  const uint8_t* src = codes + (row + g) * row_bytes + c.k * 64 + t * 16;
-  const uint32_t dst = slot + lane * 16;
-  cp_async16(dst, src);
-  cp_async16(dst + 512, src + static_cast<size_t>(32) * row_bytes);
-  cp_async8(slot + 1024 + lane * 8, sf + ((row >> 7) * (row_bytes >> 5) + c.k * 2 + (t >> 1)) * 512 +
-                                        ((u & 3) * 8 + g) * 16 + ((u >> 2) & 1) * 8);
-}
-
-// The warp's stream of pieces through both passes.
+// The warp's stream of slots: its K units of each item in turn, through both passes.
 struct Stream {
-  Cursor<true> c1;
-  Cursor<false> c2;
-  bool more1, more2;
-  int kw1, rw1, kw2, rw2;
-  uint32_t ring, head;      // shared address of the warp's ring, next slot to fill (bytes)
-  uint32_t ring_bytes;
-  __device__ __forceinline__ void issue(const FewArgs& a, const FewShared& sh, const Pass& p1, const Pass& p2, int lane) {
-    if (more1) {
-      issue_piece<true>(a, sh, p1, c1, rw1, ring + head, lane);
-      more1 = c1.next(p1, kw1);
-    } else if (more2) {
-      issue_piece<false>(a, sh, p2, c2, rw2, ring + head, lane);
-      more2 = c2.next(p2, kw2);
+  const uint8_t *codes, *sf;          // of the next slot, this lane's
+  const uint8_t *codes0, *sf0;        // of the pass, this lane's share of the address included
+  size_t second, sf_second;           // from a slot's first piece to its second
+  int row_bytes, rows, units, kw, kwi, rw, rwi, per_entry, shift;
+  int k, u, j, left;                  // K unit, item within its entry, entry, items left (0: nothing more)
+  uint32_t ring, head, ring_bytes;
+
+  __device__ __forceinline__ void begin_pass(const FewArgs& a, const FewShared& sh, const Pass& p, bool gate_up, int warp, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    units = p.units; kw = p.kw; rw = p.rw; per_entry = p.per_entry;
+    kwi = warp % kw; rwi = warp / kw;
+    shift = gate_up ? 0 : 1;
+    row_bytes = (gate_up ? a.hidden : a.inter) / 2;
+    rows = gate_up ? a.inter : a.hidden;
+    second = gate_up ? static_cast<size_t>(a.up_codes - a.gate_codes) : static_cast<size_t>(8) * row_bytes;
+    sf_second = gate_up ? static_cast<size_t>(a.up_sf - a.gate_sf) : 128;
+    codes0 = (gate_up ? a.gate_codes : a.down_codes) + static_cast<size_t>(g) * row_bytes + kwi * 64 + t * 16;
+    sf0 = (gate_up ? a.gate_sf : a.down_sf) + (kwi * 2 + (t >> 1)) * 512 + g * 16;
+    left = kwi < units ? p.end - p.begin : 0;
+    j = p.begin / per_entry;
+    u = p.begin - j * per_entry;
+    if (left > 0) open(sh);
+  }
+  __device__ __forceinline__ void open(const FewShared& sh) {
+    const int unit = (u * rw + rwi) << shift;
+    const uint32_t row = sh.ent_expert[j] * static_cast<uint32_t>(rows) + unit_row(unit);     // < 2^32: experts * rows
+    codes = codes0 + static_cast<size_t>(row) * row_bytes;
+    sf = sf0 + static_cast<size_t>(row >> 7) * (row_bytes >> 5) * 512 + (unit & 3) * 128 + ((unit >> 2) & 1) * 8;
+    k = kwi;
+  }
+  __device__ __forceinline__ void issue(const FewShared& sh, int lane) {
+    if (left > 0) {
+      const uint32_t dst = ring + head + lane * 16, dsf = ring + head + 2048 + lane * 8;
+      const size_t low = static_cast<size_t>(32) * row_bytes;
+      cp_async16(dst, codes);
+      cp_async16(dst + 512, codes + low);
+      cp_async16(dst + 1024, codes + second);
+      cp_async16(dst + 1536, codes + second + low);
+      cp_async8(dsf, sf);
+      cp_async8(dsf + 256, sf + sf_second);
+      k += kw;
+      codes += kw * 64;
+      sf += kw * 1024;
+      if (k >= units && --left > 0) {
+        if (++u == per_entry) { u = 0; ++j; }
+        open(sh);
+      }
     }
-    head = head + kPieceBytes == ring_bytes ? 0 : head + kPieceBytes;
+    head = head + kSlotBytes == ring_bytes ? 0 : head + kSlotBytes;
     cp_async_commit();        // one group per call, also when nothing is left: the count of pending groups stays exact
   }
 };
 
-// acc += the piece's 16 x 128 weights times the unit's columns.
-__device__ __forceinline__ void multiply_piece(float (&acc)[4], uint32_t slot, const uint32_t (&b)[16], int lane) {
-  uint4 w0, w1;
-  uint32_t s0, s1;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w0.x), "=r"(w0.y), "=r"(w0.z), "=r"(w0.w) : "r"(slot + lane * 16));
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w1.x), "=r"(w1.y), "=r"(w1.z), "=r"(w1.w) : "r"(slot + 512 + lane * 16));
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(s0), "=r"(s1) : "r"(slot + 1024 + lane * 8));
+__device__ __forceinline__ void lds128(uint32_t (&v)[4], uint32_t at) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+}
+// acc[m] += piece m's 16 x 128 weights times the unit's columns; the two pieces' chains of
+// products run side by side.
+__device__ __forceinline__ void multiply_slot(float (&acc)[2][4], uint32_t slot, const uint32_t (&b)[16], int lane) {
+  uint32_t w[4][4];           // piece 0 rows g, g + 32; piece 1 the same
+  uint32_t scale[4][2];       // of the lane's two blocks in each
+#pragma unroll
+  for (int i = 0; i < 4; ++i) lds128(w[i], slot + i * 512 + lane * 16);
   const int shift = (lane & 1) * 16;
-  uint32_t r0[2], r1[2];      // scales of the lane's two blocks, rows g and g + 32
-  e4m3x2_to_pairs(s0 >> shift, r0[0], r0[1]);
-  e4m3x2_to_pairs(s1 >> shift, r1[0], r1[1]);
-  const uint32_t a0[4] = {w0.x, w0.y, w0.z, w0.w}, a1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t d0[4], d1[4];
-    e2m1x8_to_f16(a0[i], d0);
-    e2m1x8_to_f16(a1[i], d1);
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      d0[v] = mul_f16x2(d0[v], r0[i / 2]);
-      d1[v] = mul_f16x2(d1[v], r1[i / 2]);
-    }
-    mma16816(acc, d0[0], d1[0], d0[1], d1[1], b[4 * i], b[4 * i + 1]);
-    mma16816(acc, d0[2], d1[2], d0[3], d1[3], b[4 * i + 2], b[4 * i + 3]);
+  for (int m = 0; m < 2; ++m) {
+    uint32_t s0, s1;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(s0), "=r"(s1) : "r"(slot + 2048 + m * 256 + lane * 8));
+    e4m3x2_to_pairs(s0 >> shift, scale[2 * m][0], scale[2 * m][1]);
+    e4m3x2_to_pairs(s1 >> shift, scale[2 * m + 1][0], scale[2 * m + 1][1]);
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      uint32_t d0[4], d1[4];
+      e2m1x8_to_f16(w[2 * m][i], d0);
+      e2m1x8_to_f16(w[2 * m + 1][i], d1);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        d0[v] = mul_f16x2(d0[v], scale[2 * m][i / 2]);
+        d1[v] = mul_f16x2(d1[v], scale[2 * m + 1][i / 2]);
+      }
+      mma16816(acc[m], d0[0], d1[0], d0[1], d1[1], b[4 * i], b[4 * i + 1]);
+      mma16816(acc[m], d0[2], d1[2], d0[3], d1[3], b[4 * i + 2], b[4 * i + 3]);
+    }
 }
 
 // Power of two that brings a largest magnitude with these bits into [2^14, 2^15), and its inverse.
@@ -268,45 +272,25 @@ __device__ __forceinline__ float f16_factor(uint32_t amax, float* inverse) {
   return __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
 }
 
+// Barrier of the multiplying warps alone.
+__device__ __forceinline__ void main_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kMainThreads) : "memory"); }
+
 // Columns of `cols` tokens, as fp16 in the order the lanes read them: [unit][quarter i][column][t] pieces of
-// 16 B, piece (i, t) of a unit = its columns 32t + 8i .. + 7.
-// kAct: float32 SwiGLU rows (scaled by their token's amax), else bf16 hidden rows (amax found here).
+// 16 B, piece (i, t) of a unit = its columns 32t + 8i .. + 7.  kAct: float32 SwiGLU rows, else bf16 hidden rows.
 template <bool kAct>
-__device__ void load_columns(const FewArgs& a, FewShared& sh, uint8_t* dst, int entry, int cols, bool identity) {
-  const int k = kAct ? a.inter : a.hidden;
-  const int tid = threadIdx.x;
-  auto route_of = [&](int c) { return static_cast<int>(sh.ent_route[entry][c]); };
-  auto token_of = [&](int c) { return identity ? c : (route_of(c) < 0 ? -1 : route_of(c) / a.top_k); };
-  __syncthreads();                       // the previous columns have been read
-  if (!kAct) {
-    if (tid < 8) sh.col_amax[tid] = 0u;
-    __syncthreads();
-    // warps in turn over (column, 256-value piece)
-    const int pieces = k / 256;
-    for (int i = tid / 32; i < cols * pieces; i += kWarps) {
-      const int c = i / pieces, tok = token_of(c);
-      if (tok < 0) continue;
-      const uint4 q = *reinterpret_cast<const uint4*>(a.hidden_rows + static_cast<size_t>(tok) * k + (i - c * pieces) * 256 + (tid & 31) * 8);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-      uint32_t m = 0;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) m = max(m, max(w[v] << 16 & 0x7fffffffu, w[v] & 0x7fff0000u));
-      m = __reduce_max_sync(0xffffffffu, m);
-      if ((tid & 31) == 0) atomicMax(&sh.col_amax[c], m);
-    }
-    __syncthreads();
-  }
-  const int per_col = k / 8;
-  for (int i = tid; i < cols * per_col; i += kThreads) {
-    const int c = i / per_col, o = i - c * per_col;       // o: 8-value piece of the row
-    const int unit = o >> 4, t = (o >> 2) & 3, q = o & 3;
-    const int tok = token_of(c);
-    uint32_t h[4] = {0u, 0u, 0u, 0u};
-    if (tok >= 0 && (!kAct || route_of(c) >= 0)) {
-      float v[8], inv;
-      const float f = f16_factor(kAct ? sh.act_amax[tok] : sh.col_amax[c], &inv);
+__device__ void load_columns(const FewArgs& a, const FewShared& sh, uint8_t* dst, int entry, int cols, bool identity) {
+  const int k = kAct ? a.inter : a.hidden, per_col = k / 8;
+  main_sync();                           // the previous columns have been read
+  for (int c = 0; c < cols; ++c) {
+    const int route = sh.ent_route[entry][c], tok = identity ? c : (route < 0 ? -1 : route / a.top_k);
+    if (tok < 0 || (kAct && route < 0)) continue;      // nobody reads the column's results
+    float inv;
+    const float f = f16_factor(kAct ? sh.act_amax[tok] : sh.x_amax[tok], &inv);
+    for (int o = threadIdx.x; o < per_col; o += kMainThreads) {       // 8-value pieces of the row
+      const int unit = o >> 4, t = (o >> 2) & 3, q = o & 3;
+      float v[8];
       if (kAct) {
-        const float4* src = reinterpret_cast<const float4*>(a.act + static_cast<size_t>(route_of(c)) * k + o * 8);
+        const float4* src = reinterpret_cast<const float4*>(a.act + static_cast<size_t>(route) * k + o * 8);
         const float4 x = __ldcg(src), y = __ldcg(src + 1);
         v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
       } else {
@@ -318,42 +302,37 @@ __device__ void load_columns(const FewArgs& a, FewShared& sh, uint8_t* dst, int 
           v[2 * n + 1] = __uint_as_float(w[n] & 0xffff0000u);
         }
       }
+      uint32_t h[4];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const __half2 p = __floats2half2_rn(v[2 * n] * f, v[2 * n + 1] * f);
         h[n] = *reinterpret_cast<const uint32_t*>(&p);
       }
+      *reinterpret_cast<uint4*>(dst + ((unit * 4 + q) * cols * 4 + c * 4 + t) * static_cast<size_t>(16)) = make_uint4(h[0], h[1], h[2], h[3]);
     }
-    *reinterpret_cast<uint4*>(dst + ((unit * 4 + q) * cols * 4 + c * 4 + t) * static_cast<size_t>(16)) = make_uint4(h[0], h[1], h[2], h[3]);
   }
-  if (tid < cols) {
-    const int tok = token_of(tid);
-    float inv = 1.0f;
-    if (tok >= 0) f16_factor(kAct ? sh.act_amax[tok] : sh.col_amax[tid], &inv);
-    sh.col_inv[tid] = inv;
-  }
-  __syncthreads();
+  main_sync();
 }
 
-__device__ __forceinline__ void load_b(uint32_t (&b)[16], const uint8_t* columns, int unit, int cols, int lane) {
-  const int g = lane >> 2, t = lane & 3;
+// Lanes of columns past `cols` take the last one's values: their results are not read.
+__device__ __forceinline__ void load_b(uint32_t (&b)[16], uint32_t lane_columns, int unit, int cols) {
+  const uint32_t step = cols * 64, at = lane_columns + unit * 4 * step;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint4 q = make_uint4(0u, 0u, 0u, 0u);
-    if (g < cols) q = *reinterpret_cast<const uint4*>(columns + ((unit * 4 + i) * cols * 4 + g * 4 + t) * static_cast<size_t>(16));
-    b[4 * i] = q.x; b[4 * i + 1] = q.y; b[4 * i + 2] = q.z; b[4 * i + 3] = q.w;
+    uint32_t q[4];
+    lds128(q, at + i * step);
+    b[4 * i] = q[0]; b[4 * i + 1] = q[1]; b[4 * i + 2] = q[2]; b[4 * i + 3] = q[3];
   }
 }
 
-// Partial sums of a group: [warp][piece m][row][column], `pitch` columns (cap rounded up to two).
-__device__ __forceinline__ void store_partial(float* red, const float (&acc)[2][4], int warp, int lane, int pitch, int cols) {
+// Partial sums of an item: [warp][piece m][row][column], `pitch` columns (a power of two).
+__device__ __forceinline__ void store_partial(float* red, const float (&acc)[2][4], int lane, int pitch, int cols) {
   const int g = lane >> 2, t = lane & 3;
-  if (2 * t >= cols) return;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    float* d = red + ((warp * 2 + m) * 16 + g) * pitch + 2 * t;
-    *reinterpret_cast<float2*>(d) = make_float2(acc[m][0], acc[m][1]);
-    *reinterpret_cast<float2*>(d + 8 * pitch) = make_float2(acc[m][2], acc[m][3]);
+    float* d = red + (m * 16 + g) * pitch + 2 * t;
+    if (2 * t < cols) { d[0] = acc[m][0]; d[8 * pitch] = acc[m][2]; }
+    if (2 * t + 1 < cols) { d[1] = acc[m][1]; d[8 * pitch + 1] = acc[m][3]; }
   }
 }
 
@@ -460,7 +439,7 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, float* scratch
   if (lane == 0) sh.warp_count[warp] = __popc(votes);
   __syncthreads();
   int before = __popc(votes & ((1u << lane) - 1u)), total = 0;
-  for (int i = 0; i < kWarps; ++i) {
+  for (int i = 0; i < kMaxRoutes / 32; ++i) {
     if (i < warp) before += sh.warp_count[i];
     total += sh.warp_count[i];
   }
@@ -487,17 +466,25 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const bool identity = a.rows <= cap;
   const int cols = identity ? a.rows : cap;
-  const int pitch = (cols + 1) & ~1;
+  const int log_pitch = cols > 4 ? 3 : cols > 2 ? 2 : cols - 1, pitch = 1 << log_pitch;
   uint8_t* ring = smem + ((sizeof(FewShared) + 127) & ~static_cast<size_t>(127));
-  float* red = reinterpret_cast<float*>(ring + kRing * kWarps * kPieceBytes);
-  const int red_floats = kWarps * 2 * 16 * pitch;
-  uint8_t* columns = reinterpret_cast<uint8_t*>(red + 2 * red_floats);
-  if (tid == 0) sh.abort = 0;
+  float* red = reinterpret_cast<float*>(ring + kRing * kWarps * kSlotBytes);
+  const int red_floats = kWarps * 32 * pitch;
+  uint8_t* columns = reinterpret_cast<uint8_t*>(red + kBufs * red_floats);
+  if (tid == 0) {
+    sh.abort = 0u;
+    for (int i = 0; i < kBufs; ++i) {
+      tc::mbar_init(&sh.full[i], kWarps);
+      tc::mbar_init(&sh.empty[i], 1);
+    }
+  }
+  if (tid < kFewMaxRows) sh.x_amax[tid] = 0u;
+  __syncthreads();
 
   // ---- logits: task = (column share, expert), one warp each ----
   if (a.logits != nullptr) {
     const int units = a.hidden / 128, n = a.rows * a.experts;
-    for (int task = blockIdx.x * kWarps + warp; task < a.splits * a.experts; task += gridDim.x * kWarps) {
+    for (int task = blockIdx.x * (kThreads / 32) + warp; task < a.splits * a.experts; task += gridDim.x * (kThreads / 32)) {
       const int p = task / a.experts, e = task - p * a.experts;
       const int u0 = units * p / a.splits, u1 = units * (p + 1) / a.splits;
       const float* wrow = a.router_w + static_cast<size_t>(e) * a.hidden + lane * 4;
@@ -525,6 +512,19 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
         if (lane == 0) a.logits[static_cast<size_t>(p) * n + t * a.experts + e] = s;
       }
     }
+  }
+  // the rows' largest magnitudes, 256 values a warp
+  for (int i = warp; i < a.rows * (a.hidden / 256); i += kThreads / 32) {
+    const int t = i / (a.hidden / 256);
+    const uint4 q = *reinterpret_cast<const uint4*>(a.hidden_rows + static_cast<size_t>(i) * 256 + lane * 8);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) m = max(m, max((w[v] << 16) & 0x7fffffffu, w[v] & 0x7fff0000u));
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) atomicMax(&sh.x_amax[t], m);
+  }
+  if (a.logits != nullptr) {
     if (!grid_barrier(a.sync, &sh.abort)) {
       if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
       return;
@@ -537,116 +537,149 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
     a.counters[kCntDistinct] = static_cast<uint32_t>(sh.distinct);
   }
 
-  // ---- the weight stream ----
-  const Pass p1 = make_pass(a.hidden, a.inter, sh.entries), p2 = make_pass(a.inter, a.hidden, sh.entries);
-  Stream st;
-  st.kw1 = warp % p1.kw; st.rw1 = warp / p1.kw;
-  st.kw2 = warp % p2.kw; st.rw2 = warp / p2.kw;
-  st.more1 = st.c1.start(p1, st.kw1);
-  st.more2 = st.c2.start(p2, st.kw2);
-  st.ring = smem_addr(ring) + warp * kRing * kPieceBytes;
-  st.ring_bytes = kRing * kPieceBytes;
-  st.head = 0;
+  const Pass p1 = make_pass(a.hidden, a.inter / 16, sh.entries), p2 = make_pass(a.inter, a.hidden / 32, sh.entries);
+  int n = 0;                     // items so far: buffer n % kBufs, its round n / kBufs
+  bool alive = true;
+  if (warp < kWarps) {
+    // ---- the multiplying warps: the weight stream, gate and up ----
+    Stream st;
+    st.ring = smem_addr(ring) + warp * kRing * kSlotBytes;
+    st.ring_bytes = kRing * kSlotBytes;
+    st.head = 0;
+    st.begin_pass(a, sh, p1, true, warp, lane);
+    bool first_pass = true;
+    auto issue = [&] {
+      if (st.left == 0 && first_pass) {
+        st.begin_pass(a, sh, p2, false, warp, lane);
+        first_pass = false;
+      }
+      st.issue(sh, lane);
+    };
 #pragma unroll 1
-  for (int i = 0; i < kRing - 1; ++i) st.issue(a, sh, p1, p2, lane);
-  uint32_t tail = 0;
-  int flip = 0;
-
-  // ---- gate and up ----
-  int entry = -1;
-  for (int it = p1.begin; it < p1.end; ++it) {
-    const int j = it / p1.per_entry;
-    if (j != entry) {
-      if (entry < 0 || !identity) load_columns<false>(a, sh, columns, j, cols, identity);
-      entry = j;
-    }
-    float acc[2][4] = {};
-    for (int k = st.kw1; k < p1.units; k += p1.kw) {
-      uint32_t b[16];
-      load_b(b, columns, k, cols, lane);
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        cp_async_wait<kRing - 2>();
-        multiply_piece(acc[m], st.ring + tail, b, lane);
-        tail = tail + kPieceBytes == st.ring_bytes ? 0 : tail + kPieceBytes;
-        st.issue(a, sh, p1, p2, lane);
+    for (int i = 0; i < kRing - 1; ++i) issue();
+    uint32_t tail = st.ring;
+    const uint32_t ring_end = st.ring + st.ring_bytes;
+    const uint32_t lane_columns = smem_addr(columns) + (min(lane >> 2, cols - 1) * 4 + (lane & 3)) * 16;
+    // one slot; one item's partial sums handed over
+    auto slot = [&](float (&acc)[2][4], const uint32_t (&b)[16]) {
+      cp_async_wait<kRing - 2>();
+      multiply_slot(acc, tail, b, lane);
+      tail += kSlotBytes;
+      if (tail == ring_end) tail = st.ring;
+      issue();
+    };
+    auto hand_over = [&](const float (&acc)[2][4]) {
+      // A wait that ran out is seen by everybody at the grid's next barrier; until then the warp keeps
+      // step with the others, which meet it at the barriers around their columns.
+      const int buf = n % kBufs;
+      if (tc::mbar_wait_warp(&sh.empty[buf], ((n / kBufs) & 1) ^ 1u, &sh.abort)) {
+        store_partial(red + buf * red_floats + warp * 32 * pitch, acc, lane, pitch, cols);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sh.full[buf]);
       }
-    }
-    float* part = red + flip * red_floats;
-    flip ^= 1;
-    store_partial(part, acc, warp, lane, pitch, cols);
-    __syncthreads();
-    const uint32_t e = sh.ent_expert[j];
-    const float s2g = __ldg(a.scale2 + e * 3), s2u = __ldg(a.scale2 + e * 3 + 1);
-    const int u0 = (it - j * p1.per_entry) * p1.rw;
-    const int warps_k = min(p1.kw, p1.units);
-    for (int i = tid; i < p1.rw * 16 * cols; i += kThreads) {
-      const int c = i % cols, r = (i / cols) % 16, rw = i / (cols * 16);
-      const int route = sh.ent_route[j][c];
-      if (route < 0) continue;
-      float g = 0.0f, u = 0.0f;
-      for (int w = 0; w < warps_k; ++w) {
-        const float* src = part + ((rw * p1.kw + w) * 2 * 16 + r) * pitch + c;
-        g += src[0];
-        u += src[16 * pitch];
+      ++n;
+    };
+    int entry = -1, j = p1.begin / p1.per_entry, u = p1.begin - j * p1.per_entry;
+    for (int it = p1.begin; it < p1.end; ++it) {
+      if (j != entry) {
+        if (entry < 0 || !identity) load_columns<false>(a, sh, columns, j, cols, identity);
+        entry = j;
       }
-      const float inv = sh.col_inv[c];
-      g *= s2g * inv;
-      u *= s2u * inv;
-      const float v = sh.ent_w[j][c] * (__fdividef(g, 1.0f + __expf(-g)) * u);
-      a.act[static_cast<size_t>(route) * a.inter + unit_row(u0 + rw) + (r & 7) + (r >> 3) * 32] = v;
-      atomicMax(&sh.act_amax[route / a.top_k], __float_as_uint(v) & 0x7fffffffu);
+      float acc[2][4] = {};
+      for (int k = warp % p1.kw; k < p1.units; k += p1.kw) {
+        uint32_t b[16];
+        load_b(b, lane_columns, k, cols);
+        slot(acc, b);
+      }
+      hand_over(acc);
+      if (++u == p1.per_entry) { u = 0; ++j; }
     }
-  }
-  __syncthreads();
-  if (tid < a.rows && sh.act_amax[tid] != 0u) atomicMax(a.act_amax + tid, sh.act_amax[tid]);
-  bool alive = grid_barrier(a.sync, &sh.abort);
-
-  // ---- down ----
-  if (alive) {
+    // ---- down ----
+    grid_barrier(a.sync, &sh.abort);
     if (tid < a.rows) sh.act_amax[tid] = __ldcg(a.act_amax + tid);
     entry = -1;
-    for (int it = p2.begin; it < p2.end;) {
-      const int j = it / p2.per_entry;
-      const int size = min(2, min(p2.end - it, p2.per_entry - (it - j * p2.per_entry)));
-      if (j != entry) {
+    j = p2.begin / p2.per_entry;
+    u = p2.begin - j * p2.per_entry;
+    const bool one_unit = p2.units <= p2.kw;      // its columns stay in registers while the entry lasts
+    uint32_t b[16];
+    for (int it = p2.begin; it < p2.end; ++it) {
+      const bool fresh = j != entry;
+      if (fresh) {
         load_columns<true>(a, sh, columns, j, cols, identity);
         entry = j;
       }
       float acc[2][4] = {};
-      for (int k = st.kw2; k < p2.units; k += p2.kw) {
-        uint32_t b[16];
-        load_b(b, columns, k, cols, lane);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          if (m < size) {
-            cp_async_wait<kRing - 2>();
-            multiply_piece(acc[m], st.ring + tail, b, lane);
-            tail = tail + kPieceBytes == st.ring_bytes ? 0 : tail + kPieceBytes;
-            st.issue(a, sh, p1, p2, lane);
-          }
-        }
+      for (int k = warp % p2.kw; k < p2.units; k += p2.kw) {
+        if (fresh || !one_unit) load_b(b, lane_columns, k, cols);
+        slot(acc, b);
       }
-      float* part = red + flip * red_floats;
-      flip ^= 1;
-      store_partial(part, acc, warp, lane, pitch, cols);
-      __syncthreads();
+      hand_over(acc);
+      if (++u == p2.per_entry) { u = 0; ++j; }
+    }
+    cp_async_wait<0>();
+  } else {
+    // ---- the summing warps: every kSumWarps-th item each, the warps' shares added in order ----
+    const int mine = warp - kWarps;
+    const float* part = red + mine * red_floats;
+    const int items1 = p1.end - p1.begin, items2 = p2.end - p2.begin;
+    for (n = mine; n < items1 && alive; n += kSumWarps) {
+      alive = tc::mbar_wait_warp(&sh.full[mine], (n / kBufs) & 1, &sh.abort);
+      if (!alive) break;
+      const int it = p1.begin + n, j = it / p1.per_entry, u = it - j * p1.per_entry;
+      const uint32_t e = sh.ent_expert[j];
+      const float s2 = __ldg(a.scale2 + e * 3 + (lane >> 4));
+      const int warps_k = min(p1.kw, p1.units);
+      for (int rw = 0; rw < p1.rw; ++rw)
+        for (int c = 0; c < cols; ++c) {
+          const int route = sh.ent_route[j][c];
+          if (route < 0) continue;
+          const float* src = part + (rw * p1.kw * 32 + lane) * pitch + c;      // lanes 0..15 gate, 16..31 up
+          float sum = 0.0f;
+#pragma unroll 4
+          for (int w = 0; w < warps_k; ++w) sum += src[w * 32 * pitch];
+          const int token = route / a.top_k;
+          float inv;
+          f16_factor(sh.x_amax[token], &inv);
+          sum *= s2 * inv;
+          const float up = __shfl_down_sync(0xffffffffu, sum, 16);
+          const float v = sh.ent_w[j][c] * (__fdividef(sum, 1.0f + __expf(-sum)) * up);
+          if (lane < 16)
+            a.act[static_cast<size_t>(route) * a.inter + unit_row(u * p1.rw + rw) + (lane & 7) + (lane >> 3) * 32] = v;
+          const uint32_t m = __reduce_max_sync(0xffffffffu, lane < 16 ? __float_as_uint(v) & 0x7fffffffu : 0u);
+          if (lane == 0) atomicMax(&sh.act_amax[token], m);
+        }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sh.empty[mine]);
+    }
+    asm volatile("bar.sync 2, %0;" ::"n"(32 * kSumWarps) : "memory");
+    if (warp == kWarps && lane < a.rows && sh.act_amax[lane] != 0u) atomicMax(a.act_amax + lane, sh.act_amax[lane]);
+    grid_barrier(a.sync, &sh.abort);
+    // item n of the second pass is the (items1 + n)-th of the CTA
+    n = items1 + (mine - items1 % kSumWarps + kSumWarps) % kSumWarps;
+    for (; n < items1 + items2 && alive; n += kSumWarps) {
+      alive = tc::mbar_wait_warp(&sh.full[mine], (n / kBufs) & 1, &sh.abort);
+      if (!alive) break;
+      const int it = p2.begin + n - items1, j = it / p2.per_entry, u = it - j * p2.per_entry;
       const float s2 = __ldg(a.scale2 + sh.ent_expert[j] * 3 + 2);
       const int warps_k = min(p2.kw, p2.units);
-      for (int i = tid; i < size * p2.rw * 16 * cols; i += kThreads) {
-        const int r = i % 16, c = (i / 16) % cols, rest = i / (16 * cols), rw = rest % p2.rw, m = rest / p2.rw;
-        const int route = sh.ent_route[j][c];
-        if (route < 0) continue;
-        float y = 0.0f;
-        for (int w = 0; w < warps_k; ++w) y += part[(((rw * p2.kw + w) * 2 + m) * 16 + r) * pitch + c];
-        const int u = (it + m - j * p2.per_entry) * p2.rw + rw;
-        a.route_out[static_cast<size_t>(route) * a.hidden + unit_row(u) + (r & 7) + (r >> 3) * 32] = y * (s2 * sh.col_inv[c]);
-      }
-      it += size;
+      for (int rw = 0; rw < p2.rw; ++rw)
+        for (int c = 0; c < cols; ++c) {
+          const int route = sh.ent_route[j][c];
+          if (route < 0) continue;
+          const float* src = part + (rw * p2.kw * 32 + lane) * pitch + c;
+          float sum = 0.0f;
+#pragma unroll 4
+          for (int w = 0; w < warps_k; ++w) sum += src[w * 32 * pitch];
+          float inv;
+          f16_factor(sh.act_amax[route / a.top_k], &inv);
+          a.route_out[static_cast<size_t>(route) * a.hidden + unit_row((u * p2.rw + rw) * 2 + (lane >> 4)) + (lane & 7) +
+                      ((lane >> 3) & 1) * 32] = sum * (s2 * inv);
+        }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sh.empty[mine]);
     }
-    alive = grid_barrier(a.sync, &sh.abort);
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  alive = grid_barrier(a.sync, &sh.abort);
   if (!alive) {
     if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
     return;
@@ -654,8 +687,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
 
   // ---- combine ----
   if (blockIdx.x == 0 && tid < a.rows) a.act_amax[tid] = 0u;      // for the next call; read by all before the barrier
-  const int n = a.rows * a.hidden;
-  for (int i = blockIdx.x * kThreads + tid; i < n; i += gridDim.x * kThreads) {
+  const int values = a.rows * a.hidden;
+  for (int i = blockIdx.x * kThreads + tid; i < values; i += gridDim.x * kThreads) {
     const int t = i / a.hidden, h = i - t * a.hidden;
     float y = 0.0f;
     const uint32_t used = sh.used[t];
@@ -740,14 +773,15 @@ __global__ void few_fc2_simt_kernel(FewArgs a) {
 }  // namespace
 
 int few_splits(int sm_count, int experts, int hidden) {
-  const int s = sm_count * kWarps / experts, most = hidden / 128;
+  const int s = sm_count * (kThreads / 32) / experts, most = hidden / 128;
   return s < 1 ? 1 : (s > kFewMaxSplits ? kFewMaxSplits : s) > most ? most : (s > kFewMaxSplits ? kFewMaxSplits : s);
 }
 
 namespace {
 size_t few_smem(int ring, int cols, int k) {
   const size_t fixed = (sizeof(FewShared) + 127) & ~static_cast<size_t>(127);
-  return fixed + static_cast<size_t>(ring) * kWarps * kPieceBytes + 2 * static_cast<size_t>(kWarps) * 2 * 16 * ((cols + 1) & ~1) * 4 +
+  const int pitch = cols > 4 ? 8 : cols > 2 ? 4 : cols;
+  return fixed + static_cast<size_t>(ring) * kWarps * kSlotBytes + static_cast<size_t>(kBufs) * kWarps * 32 * pitch * 4 +
          static_cast<size_t>(cols) * k * 2;
 }
 constexpr size_t kSmemMost = 227 * 1024;
@@ -774,19 +808,19 @@ glmrt_status_t launch_ring(const FewArgs& a, int cap, size_t smem, int sm_count,
 }  // namespace
 
 // Columns per pass over an expert and depth of the stream, from what fits into shared memory: the
-// selection's scores (rows * experts floats) are kept in the ring, and a ring of at least four pieces is needed.
+// selection's scores (rows * experts floats) are kept in the ring, and at least two slots are needed.
 bool few_fused_supported(const FewArgs& a) {
-  return few_smem(4, 1, max(a.hidden, a.inter)) <= kSmemMost &&
-         static_cast<size_t>(a.rows) * a.experts * 4 <= 4 * static_cast<size_t>(kWarps) * kPieceBytes;
+  return few_smem(2, 1, std::max(a.hidden, a.inter)) <= kSmemMost &&
+         static_cast<size_t>(a.rows) * a.experts * 4 <= 2 * static_cast<size_t>(kWarps) * kSlotBytes &&
+         static_cast<uint64_t>(a.experts) * std::max(a.hidden, a.inter) < (uint64_t{1} << 32);
 }
 glmrt_status_t launch_few_fused(const FewArgs& a, int sm_count, cudaStream_t s) {
   const int k = std::max(a.hidden, a.inter);
   int cap = std::min(a.rows, 4);
-  while (cap > 1 && few_smem(4, cap, k) > kSmemMost) --cap;
-  const int cols = a.rows <= cap ? a.rows : cap;
-  if (few_smem(9, cols, k) <= kSmemMost) return launch_ring<9>(a, cap, few_smem(9, cols, k), sm_count, s);
-  if (few_smem(6, cols, k) <= kSmemMost) return launch_ring<6>(a, cap, few_smem(6, cols, k), sm_count, s);
-  return launch_ring<4>(a, cap, few_smem(4, cols, k), sm_count, s);
+  while (cap > 1 && few_smem(3, cap, k) > kSmemMost) --cap;
+  if (few_smem(4, cap, k) <= kSmemMost) return launch_ring<4>(a, cap, few_smem(4, cap, k), sm_count, s);
+  if (few_smem(3, cap, k) <= kSmemMost) return launch_ring<3>(a, cap, few_smem(3, cap, k), sm_count, s);
+  return launch_ring<2>(a, cap, few_smem(2, cap, k), sm_count, s);
 }
 
 glmrt_status_t launch_few_simt(const FewArgs& a, cudaStream_t s) {

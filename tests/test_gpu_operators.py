@@ -447,6 +447,8 @@ def test_few_rows_do_not_depend_on_their_batch_and_repeat(mods):
     want = layer.forward_few(x)
     for _ in range(5):
         assert torch.equal(layer.forward_few(x), want)
+    for rows in (1, 2, 3, 4, 5, 7, 8, 9, 15):
+        assert torch.equal(layer.forward_few(x[:rows]), want[:rows]), rows
     layer.check()
     layer.close()
 
