@@ -66,9 +66,8 @@ struct FewShared {
   float ent_w[kMaxEntries][8];               // column -> weight
   uint32_t route_expert[kMaxRoutes];
   float route_w[kMaxRoutes];
-  int16_t route_entry[kMaxRoutes];           // entry that a starting route opens
   uint32_t used[kFewMaxRows];                // slots of a token that own a result row
-  uint32_t act_amax[kFewMaxRows];
+  uint32_t act_amax[kWarps][8];              // by warp along K and column
   uint32_t x_amax[kFewMaxRows];
   uint64_t full[kBufs], empty[kBufs];
   int warp_count[kThreads / 32];
@@ -116,28 +115,23 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// All CTAs of the grid (co-resident: cooperative launch).  The last arrival frees the others and
-// leaves the counter at zero for the next use.  False when the wait ran out.
-__device__ bool grid_barrier(uint32_t* sync, volatile uint32_t* abort) {
+// All CTAs of the grid (co-resident: cooperative launch).  The count only grows, by the grid's size at
+// each barrier, so an arrival's own value tells which multiple to wait for and nothing has to be
+// reset (64 bits: 32 would run over within minutes).  False when the wait ran out.
+__device__ bool grid_barrier(unsigned long long* count, volatile uint32_t* abort) {
   __syncthreads();
   if (threadIdx.x == 0) {
-    uint32_t gen, now;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(gen) : "l"(sync + 1) : "memory");
-    __threadfence();
-    if (atomicAdd(sync, 1u) == gridDim.x - 1) {
-      *reinterpret_cast<volatile uint32_t*>(sync) = 0u;
-      __threadfence();
-      asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(sync + 1), "r"(gen + 1) : "memory");
-    } else {
-      uint64_t t0 = 0, t;
-      for (uint32_t spin = 0;; ++spin) {
-        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(sync + 1) : "memory");
-        if (now != gen) break;
-        if ((spin & 255u) == 255u) {
-          asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-          if (t0 == 0) t0 = t;
-          else if (t - t0 > kBarrierLimitNs) { *abort = 1u; break; }
-        }
+    unsigned long long old, now;
+    asm volatile("atom.add.acq_rel.gpu.global.u64 %0, [%1], %2;" : "=l"(old) : "l"(count), "l"(1ull) : "memory");
+    const unsigned long long target = (old / gridDim.x + 1) * gridDim.x;
+    uint64_t t0 = 0, t;
+    for (uint32_t spin = 0;; ++spin) {
+      asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(count) : "memory");
+      if (now >= target) break;
+      if ((spin & 255u) == 255u) {
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+        if (t0 == 0) t0 = t;
+        else if (t - t0 > kBarrierLimitNs) { *abort = 1u; break; }
       }
     }
   }
@@ -157,10 +151,10 @@ __device__ __forceinline__ Pass make_pass(int k, int groups, int entries) {
   Pass p;
   p.units = k / 128;
   p.kw = kWarps;
-  while (p.kw / 2 >= p.units) p.kw /= 2;
+  while (p.kw > 2 && p.kw * 2 > p.units) p.kw /= 2;      // two units a warp or more, so that handing a sum over is rare
   p.rw = kWarps / p.kw;
   p.per_entry = groups / p.rw;
-  const long long items = static_cast<long long>(entries) * p.per_entry;
+  const uint32_t items = static_cast<uint32_t>(entries) * p.per_entry;    // items * grid < 2^32 (few_fused_supported)
   p.begin = static_cast<int>(items * blockIdx.x / gridDim.x);
   p.end = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
   return p;
@@ -276,40 +270,74 @@ __device__ __forceinline__ float f16_factor(uint32_t amax, float* inverse) {
 __device__ __forceinline__ void main_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kMainThreads) : "memory"); }
 
 // Columns of `cols` tokens, as fp16 in the order the lanes read them: [unit][quarter i][column][t] pieces of
-// 16 B, piece (i, t) of a unit = its columns 32t + 8i .. + 7.  kAct: float32 SwiGLU rows, else bf16 hidden rows.
-template <bool kAct>
-__device__ void load_columns(const FewArgs& a, const FewShared& sh, uint8_t* dst, int entry, int cols, bool identity) {
-  const int k = kAct ? a.inter : a.hidden, per_col = k / 8;
+// 16 B, piece (i, t) of a unit = its columns 32t + 8i .. + 7.
+// The hidden rows' power of two is the row's (x_amax).
+__device__ void load_hidden_columns(const FewArgs& a, const FewShared& sh, uint8_t* dst, int entry, int cols, bool identity) {
+  const int k = a.hidden, per_col = k / 8;
   main_sync();                           // the previous columns have been read
   for (int c = 0; c < cols; ++c) {
-    const int route = sh.ent_route[entry][c], tok = identity ? c : (route < 0 ? -1 : route / a.top_k);
-    if (tok < 0 || (kAct && route < 0)) continue;      // nobody reads the column's results
+    int tok = c;
+    if (!identity) {
+      const int route = sh.ent_route[entry][c];
+      if (route < 0) continue;           // nobody reads the column's results
+      tok = route / a.top_k;
+    }
     float inv;
-    const float f = f16_factor(kAct ? sh.act_amax[tok] : sh.x_amax[tok], &inv);
+    const float f = f16_factor(sh.x_amax[tok], &inv);
     for (int o = threadIdx.x; o < per_col; o += kMainThreads) {       // 8-value pieces of the row
       const int unit = o >> 4, t = (o >> 2) & 3, q = o & 3;
-      float v[8];
-      if (kAct) {
-        const float4* src = reinterpret_cast<const float4*>(a.act + static_cast<size_t>(route) * k + o * 8);
-        const float4 x = __ldcg(src), y = __ldcg(src + 1);
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-      } else {
-        const uint4 x = *reinterpret_cast<const uint4*>(a.hidden_rows + static_cast<size_t>(tok) * k + o * 8);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          v[2 * n] = __uint_as_float(w[n] << 16);
-          v[2 * n + 1] = __uint_as_float(w[n] & 0xffff0000u);
-        }
-      }
+      const uint4 x = *reinterpret_cast<const uint4*>(a.hidden_rows + static_cast<size_t>(tok) * k + o * 8);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
       uint32_t h[4];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const __half2 p = __floats2half2_rn(v[2 * n] * f, v[2 * n + 1] * f);
+        const __half2 p = __floats2half2_rn(__uint_as_float(w[n] << 16) * f, __uint_as_float(w[n] & 0xffff0000u) * f);
         h[n] = *reinterpret_cast<const uint32_t*>(&p);
       }
       *reinterpret_cast<uint4*>(dst + ((unit * 4 + q) * cols * 4 + c * 4 + t) * static_cast<size_t>(16)) = make_uint4(h[0], h[1], h[2], h[3]);
     }
+  }
+  main_sync();
+}
+// The SwiGLU rows' is that of the units one warp adds up (units kw apart): they alone share an accumulator.
+__device__ void load_act_columns(const FewArgs& a, FewShared& sh, uint8_t* dst, int entry, int cols, int kw) {
+  const int k = a.inter, per_col = k / 8;
+  main_sync();
+  for (int i = threadIdx.x; i < kWarps * 8; i += kMainThreads) sh.act_amax[i >> 3][i & 7] = 0u;
+  main_sync();
+  auto read = [&](int route, int o, float (&v)[8]) {
+    const float4* src = reinterpret_cast<const float4*>(a.act + static_cast<size_t>(route) * k + o * 8);
+    const float4 x = __ldcg(src), y = __ldcg(src + 1);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+  };
+  for (int i = threadIdx.x; i < cols * per_col; i += kMainThreads) {        // a unit is 16 neighbouring lanes (k % 256 == 0)
+    const int c = i / per_col, o = i - c * per_col, route = sh.ent_route[entry][c];
+    uint32_t m = 0u;
+    if (route >= 0) {
+      float v[8];
+      read(route, o, v);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) m = max(m, __float_as_uint(v[n]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
+    if ((threadIdx.x & 15) == 0) atomicMax(&sh.act_amax[(o >> 4) & (kw - 1)][c], m);
+  }
+  main_sync();
+  for (int i = threadIdx.x; i < cols * per_col; i += kMainThreads) {
+    const int c = i / per_col, o = i - c * per_col, route = sh.ent_route[entry][c];
+    if (route < 0) continue;
+    const int unit = o >> 4, t = (o >> 2) & 3, q = o & 3;
+    float v[8], inv;
+    read(route, o, v);
+    const float f = f16_factor(sh.act_amax[unit & (kw - 1)][c], &inv);
+    uint32_t h[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const __half2 p = __floats2half2_rn(v[2 * n] * f, v[2 * n + 1] * f);
+      h[n] = *reinterpret_cast<const uint32_t*>(&p);
+    }
+    *reinterpret_cast<uint4*>(dst + ((unit * 4 + q) * cols * 4 + c * 4 + t) * static_cast<size_t>(16)) = make_uint4(h[0], h[1], h[2], h[3]);
   }
   main_sync();
 }
@@ -325,134 +353,151 @@ __device__ __forceinline__ void load_b(uint32_t (&b)[16], uint32_t lane_columns,
   }
 }
 
-// Partial sums of an item: [warp][piece m][row][column], `pitch` columns (a power of two).
-__device__ __forceinline__ void store_partial(float* red, const float (&acc)[2][4], int lane, int pitch, int cols) {
+// Partial sums of an item: [warp][piece m][row][column], `pitch` columns (a power of two), times what undoes
+// the powers of two of the lane's two columns.
+__device__ __forceinline__ void store_partial(float* red, const float (&acc)[2][4], float f0, float f1, int lane, int pitch, int cols) {
   const int g = lane >> 2, t = lane & 3;
+  float* d = red + g * pitch + 2 * t;
+  if (2 * t < cols) {
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    float* d = red + (m * 16 + g) * pitch + 2 * t;
-    if (2 * t < cols) { d[0] = acc[m][0]; d[8 * pitch] = acc[m][2]; }
-    if (2 * t + 1 < cols) { d[1] = acc[m][1]; d[8 * pitch + 1] = acc[m][3]; }
+    for (int m = 0; m < 2; ++m) {
+      d[m * 16 * pitch] = acc[m][0] * f0;
+      d[(m * 16 + 8) * pitch] = acc[m][2] * f0;
+    }
+  }
+  if (2 * t + 1 < cols) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      d[m * 16 * pitch + 1] = acc[m][1] * f1;
+      d[(m * 16 + 8) * pitch + 1] = acc[m][3] * f1;
+    }
   }
 }
 
-__device__ void route_and_select(const FewArgs& a, FewShared& sh, float* scratch, int cap, bool identity) {
+// Top-k of one row by one warp: keys order like (score + bias, lower id first); a NaN ranks last.
+template <int kKeys>
+__device__ __forceinline__ void select_row(const FewArgs& a, FewShared& sh, const float* score, int row, int lane) {
+  uint32_t key[kKeys];
+#pragma unroll
+  for (int i = 0; i < kKeys; ++i) {
+    const int e = lane + 32 * i;
+    key[i] = 0u;
+    if (e < a.experts) {
+      const float s = score[e] + __ldg(a.router_b + e);
+      const uint32_t u = __float_as_uint(s == 0.0f ? 0.0f : s);
+      key[i] = s != s ? 1u : ((u >> 31) ? ~u : u | 0x80000000u);
+    }
+  }
+  float sum = 0.0f;
+  uint32_t mine = 0;
+  for (int s = 0; s < a.top_k; ++s) {
+    uint32_t best = key[0];
+    int at = 0;
+#pragma unroll
+    for (int i = 1; i < kKeys; ++i)
+      if (key[i] > best) { best = key[i]; at = i; }              // the first of equal ones: the lower id
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t id = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(lane + 32 * at) : 0xffffffffu);
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i)
+      if (lane + 32 * i == static_cast<int>(id)) key[i] = 0u;
+    sum += score[id];
+    if (lane == s) mine = id;
+  }
+  const float inv = a.scaling / fmaxf(sum, 1e-12f);
+  if (lane < a.top_k) {
+    const int r = row * a.top_k + lane;
+    sh.route_expert[r] = mine;
+    sh.route_w[r] = score[mine] * inv;
+  }
+}
+
+// Routes of all rows, then the list of entries (sh.ent_*).  `scratch`: rows * experts floats, and for
+// every expert a word and 16 half-words.
+__device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scratch, int cap, bool identity) {
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int routes = a.rows * a.top_k;
+  uint32_t* mask = reinterpret_cast<uint32_t*>(scratch);                            // rows that name an expert
+  uint16_t* entry_of = reinterpret_cast<uint16_t*>(mask + a.experts);               // [expert][16]
+  float* scores = reinterpret_cast<float*>(entry_of + a.experts * 16);
+  for (int i = tid; i < a.experts; i += kThreads) mask[i] = 0u;
+  for (int i = tid; i < kMaxEntries * 8; i += kThreads) {
+    sh.ent_route[i >> 3][i & 7] = -1;
+    sh.ent_w[i >> 3][i & 7] = 0.0f;
+  }
+  if (tid < kFewMaxRows) sh.used[tid] = 0u;
+  if (tid == 0) { sh.bad = 0; sh.distinct = 0; }
   if (a.logits != nullptr) {
     // scores of all rows, the column shares added in order
     const int n = a.rows * a.experts;
     for (int i = tid; i < n; i += kThreads) {
-      float s = 0.0f;
-      for (int p = 0; p < a.splits; ++p) s += __ldcg(a.logits + static_cast<size_t>(p) * n + i);
-      scratch[i] = sigmoid_f32(s);
+      float part[kFewMaxSplits];
+#pragma unroll
+      for (int p = 0; p < kFewMaxSplits; ++p) part[p] = p < a.splits ? __ldcg(a.logits + static_cast<size_t>(p) * n + i) : 0.0f;
+      float s = part[0];
+#pragma unroll
+      for (int p = 1; p < kFewMaxSplits; ++p) s += part[p];
+      scores[i] = sigmoid_f32(s);
     }
     __syncthreads();
     if (warp < a.rows) {
-      // keys that order like (score + bias, lower id first); a NaN ranks last
-      const float* score = scratch + warp * a.experts;
-      uint32_t key[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const int e = lane + 32 * i;
-        key[i] = 0u;
-        if (e < a.experts) {
-          const float s = score[e] + a.router_b[e];
-          const uint32_t u = __float_as_uint(s == 0.0f ? 0.0f : s);
-          key[i] = s != s ? 1u : ((u >> 31) ? ~u : u | 0x80000000u);
-        }
-      }
-      float sum = 0.0f;
-      uint32_t mine = 0;
-      for (int s = 0; s < a.top_k; ++s) {
-        uint32_t best = 0u;
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i * 32 < a.experts) best = max(best, key[i]);
-        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-        uint32_t id = 0xffffffffu;
-        if (best == top)
-#pragma unroll
-          for (int i = 31; i >= 0; --i)
-            if (key[i] == top && lane + 32 * i < a.experts) id = lane + 32 * i;
-        id = __reduce_min_sync(0xffffffffu, id);
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (lane + 32 * i == static_cast<int>(id)) key[i] = 0u;
-        sum += score[id];
-        if (lane == s) mine = id;
-      }
-      const float inv = a.scaling / fmaxf(sum, 1e-12f);
-      if (lane < a.top_k) {
-        const int r = warp * a.top_k + lane;
-        sh.route_expert[r] = mine;
-        sh.route_w[r] = score[mine] * inv;
-      }
+      if (a.experts <= 256) select_row<8>(a, sh, scores + warp * a.experts, warp, lane);
+      else select_row<32>(a, sh, scores + warp * a.experts, warp, lane);
     }
   } else if (tid < routes) {
     sh.route_expert[tid] = a.topk_idx[tid];
     sh.route_w[tid] = a.topk_w[tid];
   }
-  if (tid < kFewMaxRows) {
-    sh.used[tid] = 0u;
-    sh.act_amax[tid] = 0u;
-  }
-  if (tid == 0) { sh.bad = 0; sh.distinct = 0; }
-  for (int i = tid; i < kMaxEntries * 8; i += kThreads) {
-    sh.ent_route[i / 8][i % 8] = -1;
-    sh.ent_w[i / 8][i % 8] = 0.0f;
-  }
   __syncthreads();
-  if (a.out_idx != nullptr && blockIdx.x == 0 && tid < routes) {
-    a.out_idx[tid] = sh.route_expert[tid];
-    a.out_w[tid] = sh.route_w[tid];
-  }
-  // Entries, in the order of the first route that names each: an expert's tokens in groups of `cap`
-  // (identity: all rows are one group and a token's column is its row).
+  // Entries, in the order of the first route that names each: an expert's rows in groups of `cap`
+  // (identity: all rows are one group and a row's column is its number).
   uint32_t e = kNoRoute;
-  int rank = 0, opener = tid, slot = 0, token = 0;
+  int slot = 0, token = 0;
   bool live = false;
   float w = 0.0f;
   if (tid < routes) {
     e = sh.route_expert[tid];
+    w = sh.route_w[tid];
     token = tid / a.top_k; slot = tid - token * a.top_k;
     live = e < static_cast<uint32_t>(a.experts);
     if (!live && e != kNoRoute) sh.bad = 1;
-    w = sh.route_w[tid];
-    const int row0 = token * a.top_k;
-    int last_token = -1;
-    for (int r = 0; r < tid && live; ++r) {
-      if (sh.route_expert[r] != e) continue;
-      if (r >= row0) { live = false; break; }     // the row has named this expert before: its weight went there
-      const int tr = r / a.top_k;
-      if (tr == last_token) continue;             // a second mention in an earlier row
-      last_token = tr;
-      if (rank % cap == 0) opener = r;
-      ++rank;
+    const uint32_t* row = sh.route_expert + token * a.top_k;
+    for (int s = 0; s < a.top_k; ++s) {
+      if (s == slot || row[s] != e) continue;
+      if (s < slot) live = false;                 // the row has named this expert before: its weight went there
+      else w += sh.route_w[token * a.top_k + s];
     }
-    if (rank % cap == 0) opener = tid;
-    for (int r = tid + 1; r < row0 + a.top_k && live; ++r)
-      if (sh.route_expert[r] == e) w += sh.route_w[r];
+    if (a.out_idx != nullptr && blockIdx.x == 0) {
+      a.out_idx[tid] = e;
+      a.out_w[tid] = sh.route_w[tid];
+    }
+    if (live) {
+      atomicOr(&mask[e], 1u << token);
+      atomicOr(&sh.used[token], 1u << slot);
+    }
   }
-  const bool opens = live && opener == tid;
+  __syncthreads();
+  const int rank = live ? __popc(mask[e] & ((1u << token) - 1u)) : 0;
+  const bool opens = live && (identity ? rank == 0 : rank % cap == 0);
   const uint32_t votes = __ballot_sync(0xffffffffu, opens);
   if (lane == 0) sh.warp_count[warp] = __popc(votes);
   __syncthreads();
   int before = __popc(votes & ((1u << lane) - 1u)), total = 0;
+#pragma unroll
   for (int i = 0; i < kMaxRoutes / 32; ++i) {
     if (i < warp) before += sh.warp_count[i];
     total += sh.warp_count[i];
   }
+  const int group = identity ? 0 : rank / cap;
   if (opens) {
-    sh.route_entry[tid] = static_cast<int16_t>(before);
+    entry_of[e * 16 + group] = static_cast<uint16_t>(before);
     sh.ent_expert[before] = static_cast<uint16_t>(e);
     if (rank == 0) atomicAdd(&sh.distinct, 1);
   }
-  if (live) atomicOr(&sh.used[token], 1u << slot);
   if (tid == 0) sh.entries = total;
   __syncthreads();
   if (live) {
-    const int entry = sh.route_entry[opener], col = identity ? token : rank % cap;
+    const int entry = entry_of[e * 16 + group], col = identity ? token : rank - group * cap;
     sh.ent_route[entry][col] = static_cast<int16_t>(tid);
     sh.ent_w[entry][col] = w;
   }
@@ -492,17 +537,31 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
       float acc[kFewMaxRows];
 #pragma unroll
       for (int t = 0; t < kFewMaxRows; ++t) acc[t] = 0.0f;
-#pragma unroll 2
-      for (int u = u0; u < u1; ++u) {
-        const float4 wv = __ldg(reinterpret_cast<const float4*>(wrow + u * 128));
+      for (int ub = u0; ub < u1; ub += 4) {            // four units and four rows of loads in flight
+        float4 wv[4];
 #pragma unroll
-        for (int t = 0; t < kFewMaxRows; ++t) {
-          if (t >= a.rows) break;
-          const uint2 x = __ldg(reinterpret_cast<const uint2*>(xrow + static_cast<size_t>(t) * a.hidden + u * 128));
-          acc[t] = fmaf(__uint_as_float(x.x << 16), wv.x, acc[t]);
-          acc[t] = fmaf(__uint_as_float(x.x & 0xffff0000u), wv.y, acc[t]);
-          acc[t] = fmaf(__uint_as_float(x.y << 16), wv.z, acc[t]);
-          acc[t] = fmaf(__uint_as_float(x.y & 0xffff0000u), wv.w, acc[t]);
+        for (int i = 0; i < 4; ++i)
+          wv[i] = ub + i < u1 ? __ldg(reinterpret_cast<const float4*>(wrow + (ub + i) * 128)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int tb = 0; tb < kFewMaxRows; tb += 4) {
+          if (tb >= a.rows) break;
+          uint2 x[4][4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (tb + t < a.rows && ub + i < u1)
+                x[t][i] = __ldg(reinterpret_cast<const uint2*>(xrow + static_cast<size_t>(tb + t) * a.hidden + (ub + i) * 128));
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (tb + t < a.rows && ub + i < u1) {
+                acc[tb + t] = fmaf(__uint_as_float(x[t][i].x << 16), wv[i].x, acc[tb + t]);
+                acc[tb + t] = fmaf(__uint_as_float(x[t][i].x & 0xffff0000u), wv[i].y, acc[tb + t]);
+                acc[tb + t] = fmaf(__uint_as_float(x[t][i].y << 16), wv[i].z, acc[tb + t]);
+                acc[tb + t] = fmaf(__uint_as_float(x[t][i].y & 0xffff0000u), wv[i].w, acc[tb + t]);
+              }
         }
       }
 #pragma unroll
@@ -524,13 +583,15 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) atomicMax(&sh.x_amax[t], m);
   }
+  __syncthreads();
+  if (identity && warp < kWarps) load_hidden_columns(a, sh, columns, 0, cols, true);    // needs no routes
   if (a.logits != nullptr) {
     if (!grid_barrier(a.sync, &sh.abort)) {
       if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
       return;
     }
   }
-  route_and_select(a, sh, reinterpret_cast<float*>(ring), cap, identity);
+  route_and_select(a, sh, ring, cap, identity);
   if (blockIdx.x == 0 && tid == 0) {
     a.error_word[0] = sh.bad ? static_cast<uint32_t>(kErrBadExpert) : 0u;
     a.counters[kCntChunks] = static_cast<uint32_t>(sh.entries);
@@ -568,12 +629,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
       if (tail == ring_end) tail = st.ring;
       issue();
     };
-    auto hand_over = [&](const float (&acc)[2][4]) {
+    auto hand_over = [&](const float (&acc)[2][4], float f0, float f1) {
       // A wait that ran out is seen by everybody at the grid's next barrier; until then the warp keeps
       // step with the others, which meet it at the barriers around their columns.
       const int buf = n % kBufs;
       if (tc::mbar_wait_warp(&sh.empty[buf], ((n / kBufs) & 1) ^ 1u, &sh.abort)) {
-        store_partial(red + buf * red_floats + warp * 32 * pitch, acc, lane, pitch, cols);
+        store_partial(red + buf * red_floats + warp * 32 * pitch, acc, f0, f1, lane, pitch, cols);
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&sh.full[buf]);
       }
@@ -582,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
     int entry = -1, j = p1.begin / p1.per_entry, u = p1.begin - j * p1.per_entry;
     for (int it = p1.begin; it < p1.end; ++it) {
       if (j != entry) {
-        if (entry < 0 || !identity) load_columns<false>(a, sh, columns, j, cols, identity);
+        if (!identity) load_hidden_columns(a, sh, columns, j, cols, false);
         entry = j;
       }
       float acc[2][4] = {};
@@ -591,29 +652,30 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
         load_b(b, lane_columns, k, cols);
         slot(acc, b);
       }
-      hand_over(acc);
+      hand_over(acc, 1.0f, 1.0f);
       if (++u == p1.per_entry) { u = 0; ++j; }
     }
     // ---- down ----
     grid_barrier(a.sync, &sh.abort);
-    if (tid < a.rows) sh.act_amax[tid] = __ldcg(a.act_amax + tid);
     entry = -1;
     j = p2.begin / p2.per_entry;
     u = p2.begin - j * p2.per_entry;
-    const bool one_unit = p2.units <= p2.kw;      // its columns stay in registers while the entry lasts
-    uint32_t b[16];
+    const int kw2 = warp % p2.kw;
+    float f0 = 1.0f, f1 = 1.0f;
     for (int it = p2.begin; it < p2.end; ++it) {
-      const bool fresh = j != entry;
-      if (fresh) {
-        load_columns<true>(a, sh, columns, j, cols, identity);
+      if (j != entry) {
+        load_act_columns(a, sh, columns, j, cols, p2.kw);
         entry = j;
+        f16_factor(sh.act_amax[kw2][2 * (lane & 3)], &f0);
+        f16_factor(sh.act_amax[kw2][2 * (lane & 3) + 1], &f1);
       }
       float acc[2][4] = {};
-      for (int k = warp % p2.kw; k < p2.units; k += p2.kw) {
-        if (fresh || !one_unit) load_b(b, lane_columns, k, cols);
+      for (int k = kw2; k < p2.units; k += p2.kw) {
+        uint32_t b[16];
+        load_b(b, lane_columns, k, cols);
         slot(acc, b);
       }
-      hand_over(acc);
+      hand_over(acc, f0, f1);
       if (++u == p2.per_entry) { u = 0; ++j; }
     }
     cp_async_wait<0>();
@@ -637,22 +699,17 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
           float sum = 0.0f;
 #pragma unroll 4
           for (int w = 0; w < warps_k; ++w) sum += src[w * 32 * pitch];
-          const int token = route / a.top_k;
           float inv;
-          f16_factor(sh.x_amax[token], &inv);
+          f16_factor(sh.x_amax[route / a.top_k], &inv);
           sum *= s2 * inv;
           const float up = __shfl_down_sync(0xffffffffu, sum, 16);
           const float v = sh.ent_w[j][c] * (__fdividef(sum, 1.0f + __expf(-sum)) * up);
           if (lane < 16)
             a.act[static_cast<size_t>(route) * a.inter + unit_row(u * p1.rw + rw) + (lane & 7) + (lane >> 3) * 32] = v;
-          const uint32_t m = __reduce_max_sync(0xffffffffu, lane < 16 ? __float_as_uint(v) & 0x7fffffffu : 0u);
-          if (lane == 0) atomicMax(&sh.act_amax[token], m);
         }
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&sh.empty[mine]);
     }
-    asm volatile("bar.sync 2, %0;" ::"n"(32 * kSumWarps) : "memory");
-    if (warp == kWarps && lane < a.rows && sh.act_amax[lane] != 0u) atomicMax(a.act_amax + lane, sh.act_amax[lane]);
     grid_barrier(a.sync, &sh.abort);
     // item n of the second pass is the (items1 + n)-th of the CTA
     n = items1 + (mine - items1 % kSumWarps + kSumWarps) % kSumWarps;
@@ -670,10 +727,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
           float sum = 0.0f;
 #pragma unroll 4
           for (int w = 0; w < warps_k; ++w) sum += src[w * 32 * pitch];
-          float inv;
-          f16_factor(sh.act_amax[route / a.top_k], &inv);
           a.route_out[static_cast<size_t>(route) * a.hidden + unit_row((u * p2.rw + rw) * 2 + (lane >> 4)) + (lane & 7) +
-                      ((lane >> 3) & 1) * 32] = sum * (s2 * inv);
+                      ((lane >> 3) & 1) * 32] = sum * s2;
         }
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&sh.empty[mine]);
@@ -686,7 +741,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
   }
 
   // ---- combine ----
-  if (blockIdx.x == 0 && tid < a.rows) a.act_amax[tid] = 0u;      // for the next call; read by all before the barrier
   const int values = a.rows * a.hidden;
   for (int i = blockIdx.x * kThreads + tid; i < values; i += gridDim.x * kThreads) {
     const int t = i / a.hidden, h = i - t * a.hidden;
@@ -808,19 +862,18 @@ glmrt_status_t launch_ring(const FewArgs& a, int cap, size_t smem, int sm_count,
 }  // namespace
 
 // Columns per pass over an expert and depth of the stream, from what fits into shared memory: the
-// selection's scores (rows * experts floats) are kept in the ring, and at least two slots are needed.
+// selection's scratch (36 bytes an expert and a float per row and expert) lies in the ring, and at least
+// three slots are needed.
 bool few_fused_supported(const FewArgs& a) {
-  return few_smem(2, 1, std::max(a.hidden, a.inter)) <= kSmemMost &&
-         static_cast<size_t>(a.rows) * a.experts * 4 <= 2 * static_cast<size_t>(kWarps) * kSlotBytes &&
-         static_cast<uint64_t>(a.experts) * std::max(a.hidden, a.inter) < (uint64_t{1} << 32);
+  static_assert(1024 * 36 + 1024 * kFewMaxRows * 4 <= 3 * kWarps * kSlotBytes, "selection scratch fits the ring");
+  return few_smem(3, 1, std::max(a.hidden, a.inter)) <= kSmemMost && a.experts <= 1024;
 }
 glmrt_status_t launch_few_fused(const FewArgs& a, int sm_count, cudaStream_t s) {
   const int k = std::max(a.hidden, a.inter);
   int cap = std::min(a.rows, 4);
   while (cap > 1 && few_smem(3, cap, k) > kSmemMost) --cap;
   if (few_smem(4, cap, k) <= kSmemMost) return launch_ring<4>(a, cap, few_smem(4, cap, k), sm_count, s);
-  if (few_smem(3, cap, k) <= kSmemMost) return launch_ring<3>(a, cap, few_smem(3, cap, k), sm_count, s);
-  return launch_ring<2>(a, cap, few_smem(2, cap, k), sm_count, s);
+  return launch_ring<3>(a, cap, few_smem(3, cap, k), sm_count, s);
 }
 
 glmrt_status_t launch_few_simt(const FewArgs& a, cudaStream_t s) {

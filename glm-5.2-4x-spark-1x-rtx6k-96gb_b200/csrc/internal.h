@@ -322,8 +322,7 @@ struct FewArgs {
   uint32_t* out_idx;                                        // where the routes are written, or nullptr
   float* out_w;
   float* route_out;                                         // [rows * top_k, hidden] float32 result rows
-  uint32_t* act_amax;                                       // [kFewMaxRows] zero between calls
-  uint32_t* sync;                                           // barrier count (zero between calls) and generation
+  unsigned long long* sync;                                 // barrier count: a multiple of the grid's size between calls
   uint32_t* counters;
 };
 constexpr int kFewMaxSplits = 16;

@@ -49,8 +49,6 @@ struct EpState {
   uint32_t global_rows = 0;   // rows of the whole batch over all ranks when the caller has said so, else 0
 };
 
-constexpr size_t kFewSyncWords = 32 + kFewMaxRows;   // barrier words in a line of their own, then the maxima
-
 struct Layer {
   glmrt_b200_moe_config_t cfg{};
   int device = 0;
@@ -83,10 +81,10 @@ struct Layer {
   uint16_t* route_rows = nullptr;
   uint16_t** slot_out = nullptr;
   uint32_t* slot_weight = nullptr;   // route weight per slot (fused combine of large batches)
-  // few-token path: weighted SwiGLU rows, one float32 result row per route, partial logits, and the words
-  // its kernel leaves at zero (barrier, largest activations)
+  // few-token path: weighted SwiGLU rows, one float32 result row per route, partial logits, the count of
+  // its kernel's barriers
   float *few_act = nullptr, *few_out = nullptr, *few_logits = nullptr;
-  uint32_t* few_sync = nullptr;
+  unsigned long long* few_sync = nullptr;
   uint32_t* fc_sync = nullptr;       // hand-over words between the decode FC1 and FC2 kernels
   uint16_t *hidden_stage = nullptr, *out_stage = nullptr;
   // scratch for weight loading
@@ -480,7 +478,7 @@ glmrt_status_t alloc_workspace(Layer* l) {
     A(dev_alloc(b, &l->few_act, F * K * I));
     A(dev_alloc(b, &l->few_out, F * K * H));
     A(dev_alloc(b, &l->few_logits, kFewMaxSplits * F * c.experts));
-    A(dev_alloc(b, &l->few_sync, kFewSyncWords, true));
+    A(dev_alloc(b, &l->few_sync, 1, true));
   }
   A(dev_alloc(b, &l->hidden_stage, T * H));
   A(dev_alloc(b, &l->out_stage, T * H));
@@ -797,7 +795,7 @@ glmrt_status_t few_args(Layer* l, const glmrt_device_buffer_t& hidden, size_t ro
   a.hidden = static_cast<int>(c.hidden_dim); a.inter = static_cast<int>(c.intermediate_dim);
   a.router_w = l->router_w; a.router_b = l->router_b; a.scaling = c.routed_scaling;
   a.route_out = l->few_out;
-  a.sync = l->few_sync; a.act_amax = l->few_sync + 32;
+  a.sync = l->few_sync;
   a.counters = l->counters;
   *out = a;
   return GLMRT_STATUS_OK;
@@ -947,9 +945,9 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_check(void* layer, void* cuda_str
   if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "layer check", err);
   const uint32_t e = host[kCntError] | host[kCntRouterError];
   if (e == 0) return ok();
-  // a few-token kernel that gave up leaves its barrier words behind: nothing runs now, so they are cleared
+  // a few-token kernel that gave up leaves its barrier count uneven: nothing runs now, so it is cleared
   if ((e & kErrWaitTimeout) && l->few_sync != nullptr &&
-      (err = cudaMemset(l->few_sync, 0, kFewSyncWords * 4)) != cudaSuccess)
+      (err = cudaMemset(l->few_sync, 0, sizeof(*l->few_sync))) != cudaSuccess)
     return fail_cuda(GLMRT_STATUS_COPY_FAILED, "layer check", err);
   std::string msg = "device reported:";
   if (e & kErrWaitTimeout) msg += " a bounded wait expired;";
