@@ -19,9 +19,9 @@ constexpr int kBlock = kFp8Block;
 // One warp per (row, 128-column block): four values a lane.
 template <typename T>
 __global__ void fp8_quantize_rows_kernel(const T* __restrict__ in, size_t stride, uint8_t* __restrict__ codes,
-                                         float* __restrict__ scales, int rows, int cols) {
-  pdl_launch_dependents();
+                                         float* __restrict__ scales, int rows, int cols, int scale_stride) {
   pdl_wait();
+  pdl_launch_dependents();      // after the wait: a successor may then rely on everything before this kernel
   const int blocks = (cols + kBlock - 1) / kBlock;
   const size_t w = blockIdx.x * static_cast<size_t>(blockDim.x / 32) + threadIdx.x / 32;
   if (w >= static_cast<size_t>(rows) * blocks) return;
@@ -39,87 +39,13 @@ __global__ void fp8_quantize_rows_kernel(const T* __restrict__ in, size_t stride
   const float scale = fp8_block_scale(amax, &inv);
   const uint32_t q = fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
   if (c < cols) *reinterpret_cast<uint32_t*>(codes + row * cols + c) = q;   // cols % 16 == 0
-  if (lane == 0) scales[static_cast<size_t>(b) * rows + row] = scale;
-}
-
-// 64 x 64 outputs a CTA, 4 x 4 a thread, one 128-block of K at a time in two halves.
-template <typename O>
-__global__ void __launch_bounds__(256) fp8_linear_simt_kernel(const uint8_t* __restrict__ x, const float* __restrict__ xs,
-                                                              const uint8_t* __restrict__ w, const float* __restrict__ ws,
-                                                              O* __restrict__ out, int rows, int n, int k) {
-  __shared__ float sa[64][65], sb[64][65];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-  const int blocks = (k + kBlock - 1) / kBlock;
-  float acc[4][4] = {};
-  for (int b = 0; b < blocks; ++b) {
-    float part[4][4] = {};
-    for (int half = 0; half < 2; ++half) {
-      const int k0 = b * kBlock + half * 64;
-      __syncthreads();
-      for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = i / 64, c = i % 64;
-        const bool in_k = k0 + c < k;
-        sa[r][c] = in_k && m0 + r < rows ? e4m3_to_f32_nan(x[static_cast<size_t>(m0 + r) * k + k0 + c]) : 0.0f;
-        sb[r][c] = in_k && n0 + r < n ? e4m3_to_f32_nan(w[static_cast<size_t>(n0 + r) * k + k0 + c]) : 0.0f;
-      }
-      __syncthreads();
-      for (int c = 0; c < 64; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) part[i][j] = fmaf(sa[tm * 4 + i][c], sb[tn * 4 + j][c], part[i][j]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int m = m0 + tm * 4 + i;
-      const float sx = m < rows ? xs[static_cast<size_t>(b) * rows + m] : 0.0f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = n0 + tn * 4 + j;
-        const float s = c < n ? sx * ws[static_cast<size_t>(c / kBlock) * blocks + b] : 0.0f;
-        acc[i][j] = fmaf(part[i][j], s, acc[i][j]);
-      }
-    }
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + tm * 4 + i, c = n0 + tn * 4 + j;
-      if (m < rows && c < n) fp8_store(out + static_cast<size_t>(m) * n + c, acc[i][j]);
-    }
-}
-
-// act = silu(gate) * up, quantised like the rows: one warp per (row, block).
-__global__ void fp8_swiglu_quantize_kernel(const float* __restrict__ g, const float* __restrict__ u,
-                                           uint8_t* __restrict__ codes, float* __restrict__ scales, int rows, int cols) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int blocks = (cols + kBlock - 1) / kBlock;
-  const size_t w = blockIdx.x * static_cast<size_t>(blockDim.x / 32) + threadIdx.x / 32;
-  if (w >= static_cast<size_t>(rows) * blocks) return;
-  const size_t row = w / blocks;
-  const int b = static_cast<int>(w % blocks), lane = threadIdx.x % 32, c = b * kBlock + lane * 4;
-  float v[4];
-  uint32_t amax = 0u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = c + i < cols ? fp8_swiglu(g[row * cols + c + i], u[row * cols + c + i]) : 0.0f;
-    amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  float inv;
-  const float scale = fp8_block_scale(amax, &inv);
-  const uint32_t q = fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-  if (c < cols) *reinterpret_cast<uint32_t*>(codes + row * cols + c) = q;
-  if (lane == 0) scales[static_cast<size_t>(b) * rows + row] = scale;
+  if (lane == 0) scales[static_cast<size_t>(b) * scale_stride + row] = scale;
 }
 
 size_t round256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 size_t blocks_of(size_t k) { return (k + kBlock - 1) / kBlock; }
-size_t rows_bytes(size_t rows, size_t k) { return round256(rows * k) + round256(rows * blocks_of(k) * 4); }
+size_t padded(size_t rows) { return (rows + 127) & ~static_cast<size_t>(127); }
+size_t rows_bytes(size_t rows, size_t k) { return round256(rows * k) + padded(rows) * blocks_of(k) * 4; }
 
 glmrt_status_t check_dims(size_t rows, size_t n, size_t k, const char* what) {
   if (n == 0 || k == 0 || k % 16 != 0)
@@ -137,29 +63,16 @@ glmrt_status_t check_buffer(const glmrt_device_buffer_t& b, size_t need, size_t 
 }
 
 glmrt_status_t launch_quantize(const void* in, uint32_t dtype, size_t stride, uint8_t* codes, float* scales, size_t rows,
-                               size_t cols, cudaStream_t s) {
+                               size_t cols, size_t scale_stride, cudaStream_t s) {
   const size_t warps = rows * blocks_of(cols);
   const dim3 grid(static_cast<unsigned>((warps + 7) / 8)), block(256);
   if (dtype == GLMRT_B200_DTYPE_BF16)
     launch_pdl(fp8_quantize_rows_kernel<uint16_t>, grid, block, 0, s, static_cast<const uint16_t*>(in), stride, codes,
-               scales, static_cast<int>(rows), static_cast<int>(cols));
+               scales, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(scale_stride));
   else
     launch_pdl(fp8_quantize_rows_kernel<float>, grid, block, 0, s, static_cast<const float*>(in), stride, codes, scales,
-               static_cast<int>(rows), static_cast<int>(cols));
+               static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(scale_stride));
   GLMRT_LAUNCH_CHECK("fp8_quantize_rows_kernel");
-  return GLMRT_STATUS_OK;
-}
-
-glmrt_status_t launch_product(const uint8_t* x, const float* xs, const uint8_t* w, const float* ws, void* out,
-                              uint32_t out_dtype, size_t rows, size_t n, size_t k, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((n + 63) / 64), static_cast<unsigned>((rows + 63) / 64)), block(256);
-  if (out_dtype == GLMRT_B200_DTYPE_BF16)
-    launch_pdl(fp8_linear_simt_kernel<uint16_t>, grid, block, 0, s, x, xs, w, ws, static_cast<uint16_t*>(out),
-               static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k));
-  else
-    launch_pdl(fp8_linear_simt_kernel<float>, grid, block, 0, s, x, xs, w, ws, static_cast<float*>(out),
-               static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k));
-  GLMRT_LAUNCH_CHECK("fp8_linear_simt_kernel");
   return GLMRT_STATUS_OK;
 }
 
@@ -181,7 +94,7 @@ extern "C" glmrt_status_t glmrt_b200_fp8_quantize_rows_async(glmrt_device_buffer
   GLMRT_RETURN_IF_ERROR(check_buffer(scales, rows * blocks_of(cols) * 4, 4, "fp8_quantize_rows scales"));
   GLMRT_RETURN_IF_ERROR(require_cuda());
   GLMRT_RETURN_IF_ERROR(launch_quantize(input.ptr, dtype, input_row_stride, static_cast<uint8_t*>(codes.ptr),
-                                        static_cast<float*>(scales.ptr), rows, cols, static_cast<cudaStream_t>(cuda_stream)));
+                                        static_cast<float*>(scales.ptr), rows, cols, rows, static_cast<cudaStream_t>(cuda_stream)));
   return ok();
 }
 
@@ -210,9 +123,11 @@ extern "C" glmrt_status_t glmrt_b200_fp8_block_linear_async(glmrt_device_buffer_
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   uint8_t* codes = static_cast<uint8_t*>(workspace.ptr);
   float* scales = reinterpret_cast<float*>(codes + round256(rows * k));
-  GLMRT_RETURN_IF_ERROR(launch_quantize(x_bf16.ptr, GLMRT_B200_DTYPE_BF16, x_row_stride, codes, scales, rows, k, s));
-  GLMRT_RETURN_IF_ERROR(launch_product(codes, scales, static_cast<const uint8_t*>(weight_codes.ptr),
-                                       static_cast<const float*>(weight_scales.ptr), output.ptr, out_dtype, rows, n, k, s));
+  GLMRT_RETURN_IF_ERROR(launch_quantize(x_bf16.ptr, GLMRT_B200_DTYPE_BF16, x_row_stride, codes, scales, rows, k, padded(rows), s));
+  Fp8Gemm g{codes, scales, static_cast<const uint8_t*>(weight_codes.ptr), nullptr, static_cast<const float*>(weight_scales.ptr),
+            nullptr, output.ptr, nullptr, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k),
+            static_cast<int>(padded(rows)), 0};
+  GLMRT_RETURN_IF_ERROR(launch_fp8_gemm(g, out_dtype == GLMRT_B200_DTYPE_BF16 ? 0 : 1, s));
   return ok();
 }
 
@@ -220,7 +135,7 @@ extern "C" glmrt_status_t glmrt_b200_fp8_gated_mlp_workspace(size_t rows, size_t
   if (out_bytes == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "fp8_gated_mlp_workspace: null output");
   GLMRT_RETURN_IF_ERROR(check_dims(rows, inter, hidden, "fp8_gated_mlp"));
   GLMRT_RETURN_IF_ERROR(check_dims(rows, hidden, inter, "fp8_gated_mlp"));
-  *out_bytes = rows_bytes(rows, hidden) + rows_bytes(rows, inter) + 2 * round256(rows * inter * 4);
+  *out_bytes = rows_bytes(rows, hidden) + rows_bytes(rows, inter);
   return ok();
 }
 
@@ -250,18 +165,13 @@ extern "C" glmrt_status_t glmrt_b200_fp8_gated_mlp_async(
   float* xs = reinterpret_cast<float*>(xq + round256(rows * hidden));
   uint8_t* aq = xq + rows_bytes(rows, hidden);
   float* as = reinterpret_cast<float*>(aq + round256(rows * inter));
-  float* g = reinterpret_cast<float*>(aq + rows_bytes(rows, inter));
-  float* u = g + round256(rows * inter * 4) / 4;
-  GLMRT_RETURN_IF_ERROR(launch_quantize(x_bf16.ptr, GLMRT_B200_DTYPE_BF16, x_row_stride, xq, xs, rows, hidden, s));
-  GLMRT_RETURN_IF_ERROR(launch_product(xq, xs, static_cast<const uint8_t*>(gate_codes.ptr),
-                                       static_cast<const float*>(gate_scales.ptr), g, GLMRT_B200_DTYPE_F32, rows, inter, hidden, s));
-  GLMRT_RETURN_IF_ERROR(launch_product(xq, xs, static_cast<const uint8_t*>(up_codes.ptr),
-                                       static_cast<const float*>(up_scales.ptr), u, GLMRT_B200_DTYPE_F32, rows, inter, hidden, s));
-  launch_pdl(fp8_swiglu_quantize_kernel, dim3(static_cast<unsigned>((rows * blocks_of(inter) + 7) / 8)), dim3(256), 0, s, g, u,
-             aq, as, static_cast<int>(rows), static_cast<int>(inter));
-  GLMRT_LAUNCH_CHECK("fp8_swiglu_quantize_kernel");
-  GLMRT_RETURN_IF_ERROR(launch_product(aq, as, static_cast<const uint8_t*>(down_codes.ptr),
-                                       static_cast<const float*>(down_scales.ptr), output_bf16.ptr, GLMRT_B200_DTYPE_BF16,
-                                       rows, hidden, inter, s));
+  GLMRT_RETURN_IF_ERROR(launch_quantize(x_bf16.ptr, GLMRT_B200_DTYPE_BF16, x_row_stride, xq, xs, rows, hidden, padded(rows), s));
+  const int m = static_cast<int>(rows), h = static_cast<int>(hidden), i = static_cast<int>(inter), pad = static_cast<int>(padded(rows));
+  const Fp8Gemm up{xq, xs, static_cast<const uint8_t*>(gate_codes.ptr), static_cast<const uint8_t*>(up_codes.ptr),
+                   static_cast<const float*>(gate_scales.ptr), static_cast<const float*>(up_scales.ptr), aq, as, m, i, h, pad, pad};
+  const Fp8Gemm down{aq, as, static_cast<const uint8_t*>(down_codes.ptr), nullptr, static_cast<const float*>(down_scales.ptr),
+                     nullptr, output_bf16.ptr, nullptr, m, h, i, pad, 0};
+  GLMRT_RETURN_IF_ERROR(launch_fp8_gemm(up, 2, s));
+  GLMRT_RETURN_IF_ERROR(launch_fp8_gemm(down, 0, s));
   return ok();
 }

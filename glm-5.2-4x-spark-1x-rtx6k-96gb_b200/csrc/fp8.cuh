@@ -8,6 +8,21 @@ namespace glmrt {
 
 constexpr int kFp8Block = 128;   // columns per activation scale, rows and columns per weight scale
 
+// One product of quantised rows x [rows, k] (E4M3, scales [ceil(k / 128)][xs_stride], xs_stride whole tiles of
+// 128) with weights [n, k] (scales ws [ceil(n / 128)][ceil(k / 128)]).
+// mode 0: out bf16 [rows, n]; 1: float32; 2: silu(w0 x) * (w1 x) quantised: codes [rows, n], scales
+// out_scales [ceil(n / 128)][out_stride].
+struct Fp8Gemm {
+  const uint8_t* x;
+  const float* xs;
+  const uint8_t *w0, *w1;
+  const float *ws0, *ws1;
+  void* out;
+  float* out_scales;
+  int rows, n, k, xs_stride, out_stride;
+};
+glmrt_status_t launch_fp8_gemm(const Fp8Gemm& g, int mode, cudaStream_t stream);
+
 #ifdef __CUDACC__
 __device__ __forceinline__ float fp8_input(uint16_t v) { return bf16_bits_to_f32(v); }
 __device__ __forceinline__ float fp8_input(float v) { return v; }
@@ -37,6 +52,9 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  return static_cast<uint32_t>(f32_to_bf16_rne(lo)) | (static_cast<uint32_t>(f32_to_bf16_rne(hi)) << 16);
 }
 __device__ __forceinline__ float fp8_swiglu(float g, float u) {
   // fast exponential and division: a few units in the last place, against codes of four bits

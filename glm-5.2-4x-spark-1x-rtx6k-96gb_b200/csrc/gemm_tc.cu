@@ -495,12 +495,12 @@ bool fc_overlap(const FfnArgs& a) {
 
 }  // namespace
 
-glmrt_status_t make_codes_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes,
+glmrt_status_t make_bytes_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes,
                                      uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return fail(GLMRT_STATUS_CUDA_UNAVAILABLE, "cuTensorMapEncodeTiled is not available");
-  if (row_bytes % 128 != 0 || reinterpret_cast<uintptr_t>(base) % 16 != 0 || box_rows == 0 || box_rows > 256)
-    return fail(GLMRT_STATUS_INVALID_ARGUMENT, "tensor map: rows must be multiples of 128 bytes on a 16-byte aligned base");
+  if (row_bytes == 0 || row_bytes % 16 != 0 || reinterpret_cast<uintptr_t>(base) % 16 != 0 || box_rows == 0 || box_rows > 256)
+    return fail(GLMRT_STATUS_INVALID_ARGUMENT, "tensor map: rows must be multiples of 16 bytes on a 16-byte aligned base");
   const cuuint64_t dims[2] = {row_bytes, rows};
   const cuuint64_t strides[1] = {row_bytes};
   const cuuint32_t box[2] = {128, box_rows};
@@ -510,6 +510,12 @@ glmrt_status_t make_codes_tensor_map(CUtensorMap* out, const void* base, uint64_
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(GLMRT_STATUS_INTERNAL_ERROR, "cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)));
   return GLMRT_STATUS_OK;
+}
+
+glmrt_status_t make_codes_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes,
+                                     uint32_t box_rows) {
+  if (row_bytes % 128 != 0) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "tensor map: rows must be multiples of 128 bytes");
+  return make_bytes_tensor_map(out, base, rows, row_bytes, box_rows);
 }
 
 glmrt_status_t make_scale_tensor_map(CUtensorMap* out, const void* base, uint64_t bytes) {

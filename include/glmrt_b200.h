@@ -432,6 +432,9 @@ glmrt_status_t glmrt_b200_block_norm_async(const glmrt_b200_block_norm_args_t* a
 glmrt_status_t glmrt_b200_fp8_quantize_rows_async(glmrt_device_buffer_t input, glmrt_device_buffer_t codes,
                                                   glmrt_device_buffer_t scales, size_t rows, size_t cols,
                                                   size_t input_row_stride, uint32_t dtype, void* cuda_stream);
+/* Synchronises the stream and reports whether a bounded wait expired in any 8-bit product on the current
+ * device since the last check (its outputs are then not valid). */
+glmrt_status_t glmrt_b200_fp8_check(void* cuda_stream);
 glmrt_status_t glmrt_b200_fp8_block_linear_workspace(size_t rows, size_t n, size_t k, size_t* out_bytes);
 /* output [rows, n] (bf16 or float32) = x [rows, k] weight^T, x quantised in the call. */
 glmrt_status_t glmrt_b200_fp8_block_linear_async(glmrt_device_buffer_t x_bf16, glmrt_device_buffer_t weight_codes,
