@@ -44,7 +44,7 @@ __global__ void fp8_quantize_rows_kernel(const T* __restrict__ in, size_t stride
 
 size_t round256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 size_t blocks_of(size_t k) { return (k + kBlock - 1) / kBlock; }
-size_t padded(size_t rows) { return (rows + 127) & ~static_cast<size_t>(127); }
+size_t padded(size_t rows) { return (rows + 255) & ~static_cast<size_t>(255); }   // whole tiles of the products
 size_t rows_bytes(size_t rows, size_t k) { return round256(rows * k) + padded(rows) * blocks_of(k) * 4; }
 
 glmrt_status_t check_dims(size_t rows, size_t n, size_t k, const char* what) {

@@ -9,7 +9,7 @@ namespace glmrt {
 constexpr int kFp8Block = 128;   // columns per activation scale, rows and columns per weight scale
 
 // One product of quantised rows x [rows, k] (E4M3, scales [ceil(k / 128)][xs_stride], xs_stride whole tiles of
-// 128) with weights [n, k] (scales ws [ceil(n / 128)][ceil(k / 128)]).
+// 256) with weights [n, k] (scales ws [ceil(n / 128)][ceil(k / 128)]).
 // mode 0: out bf16 [rows, n]; 1: float32; 2: silu(w0 x) * (w1 x) quantised: codes [rows, n], scales
 // out_scales [ceil(n / 128)][out_stride].
 struct Fp8Gemm {

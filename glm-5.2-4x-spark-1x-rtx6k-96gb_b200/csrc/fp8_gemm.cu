@@ -5,8 +5,8 @@
 // each one out, scale it and add it to float32 sums in their registers while the next block is
 // multiplied into the other half of tensor memory.
 //
-//   rows on the MMA's 128 lanes (fp8_rows_kernel)      many rows: tiles of 128 rows x 256 weight rows;
-//       a thread owns a row and 128 of its columns, so a block costs it one scale and 128 FMAs.
+//   rows on the MMA's lanes (fp8_rows_kernel)          many rows: tiles of 256 rows x 256 weight rows on CTA
+//       pairs; a thread owns a row and 128 of its columns, so a block costs it one scale and 128 FMAs.
 //   weights on the lanes (fp8_weights_kernel)          few rows: tiles of 128 weight rows x 16..128
 //       rows, the K blocks of a tile split over a cluster of up to eight CTAs, whose sums meet in
 //       shared memory.  Bound by the weight bytes, so what counts is that every SM streams.
@@ -43,43 +43,79 @@ __device__ __forceinline__ uint32_t idesc_fp8(uint32_t n) { return (1u << 4) | (
 constexpr int kTileBytes = 128 * kFp8Block;            // 128 rows of one K block
 
 // ---------------------------------------------------------------------------------------------------
-// Many rows
+// Many rows: tiles of 256 rows x 256 weight rows on CTA pairs (cta_group::2)
 // ---------------------------------------------------------------------------------------------------
-constexpr int kRowsStages = 4;
-constexpr int kRowsEpiWarps = 8;
-constexpr int kRowsThreads = 32 * (2 + kRowsEpiWarps);
-constexpr int kRowsN = 256;
-constexpr int kRowsStageBytes = kTileBytes + 2 * kTileBytes;
-constexpr size_t kRowsSmem = static_cast<size_t>(kRowsStages) * kRowsStageBytes + 1024 + 256 + 128 * 2 * 4;
+// Each CTA of a pair holds 128 of the rows and half of the weight rows, one M = 256 MMA of the leader
+// fills a 128 x 256 block sum in each CTA's tensor memory.  A CTA alone would have to take in 48 KB per block's
+// 512 cycles of multiplication, more than the 62 bytes a cycle that an SM gets from the L2; the pair needs 32 KB.
+//
+// Twelve warps: producer, issuer, two idle, eight epilogue warps (two per tensor-memory quadrant) that hold
+// 128 sums a thread; registers move from the first four to them (3 x 128 threads x 168 = 128 x (40 + 2 x 232)).
+constexpr int kPairStages = 5;
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairThreads = 32 * (4 + kPairEpiWarps);
+constexpr int kPairStageBytes = 2 * kTileBytes;                   // this CTA's rows and its half of the weight rows
+constexpr int kPairN = 256;
+constexpr int kParkWords = 33;                                    // a parked row: 32 words and one against bank conflicts
+constexpr size_t kPairSmem = static_cast<size_t>(kPairStages) * kPairStageBytes + 1024 + 256 + 2 * 128 * 4 +
+                             static_cast<size_t>(kPairEpiWarps) * 32 * kParkWords * 4;
 
 struct RowsArgs {
-  const float* xs;            // [blocks][xs_stride]
+  const float* xs;            // [blocks][xs_stride], whole tiles of 256 readable
   const float *ws0, *ws1;     // weight scales (gate / up: both)
   void* out;                  // product: [rows, n] bf16 or float32; SwiGLU: codes [rows, n]
   float* out_scales;          // SwiGLU: [ceil(n / 128)][out_stride]
   int rows, n, k, xs_stride, out_stride;
-  int vector_out;             // rows of the output start on 16-byte boundaries
 };
+
+__device__ __forceinline__ void tc_mma_fp8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrival on the leader's barrier after reading tensor memory: the reads are complete (wait::ld) and ordered by the
+// tcgen05 fence before it, no other memory has to become visible.  With .release.cluster the same arrival made the
+// kernel wait for a memory barrier at every block (a third of its time).
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
+__device__ __forceinline__ void tc_load32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]),
+        "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
+        "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
 
 // kMode 0: bf16 product, 1: float32 product, 2: SwiGLU of gate / up, quantised
 template <int kMode>
-__global__ void __launch_bounds__(kRowsThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
 fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w0,
                 const __grid_constant__ CUtensorMap map_w1) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(kRowsStages) * kRowsStageBytes);
-  uint64_t* empty_bar = full_bar + kRowsStages;
-  uint64_t* acc_full = empty_bar + kRowsStages;
-  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(kPairStages) * kPairStageBytes);   // leader's count
+  uint64_t* empty_bar = full_bar + kPairStages;      // one set per CTA
+  uint64_t* acc_full = empty_bar + kPairStages;      // one pair per CTA
+  uint64_t* acc_empty = acc_full + 2;                // leader's count
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  float* amax_x = reinterpret_cast<float*>(smem + static_cast<size_t>(kRowsStages) * kRowsStageBytes + 256);   // [2][128]
+  uint32_t* amax_x = reinterpret_cast<uint32_t*>(smem + static_cast<size_t>(kPairStages) * kPairStageBytes + 256);   // [2][128]
+  uint32_t* park_all = amax_x + 256;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_ctarank();           // 0: leader
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int blocks = (a.k + kFp8Block - 1) / kFp8Block;
-  const int per_tile = kMode == 2 ? 128 : kRowsN;                 // output columns of a tile
-  const int n_tiles = (a.n + per_tile - 1) / per_tile, m_tiles = (a.rows + 127) / 128;
+  const int per_tile = kMode == 2 ? 128 : kPairN;                 // output columns of a tile
+  const int n_tiles = (a.n + per_tile - 1) / per_tile, m_tiles = (a.rows + 255) / 256;
   const int tiles = n_tiles * m_tiles;
 
   if (threadIdx.x == 32) {
@@ -88,118 +124,128 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
     if (kMode == 2) prefetch_tensormap(&map_w1);
   }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kRowsStages; ++s) {
+    for (int s = 0; s < kPairStages; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], kRowsEpiWarps);
+      mbar_init(&acc_empty[b], 2 * kPairEpiWarps);
     }
     *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before();
-  __syncthreads();
+  cluster_sync_all();           // barriers of both CTAs initialised, tensor memory of both allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
   pdl_launch_dependents();      // after the wait: a successor may then rely on everything before this kernel
 
-  // tiles of one column of weight tiles follow each other, so that the rows stay in L2 and the weights are read once
-  auto tile_m = [&](int tile) { return tile % m_tiles; };
-  auto tile_n = [&](int tile) { return tile / m_tiles; };
-
-  if (warp == 0) {
-    const uint64_t pol = policy_evict_last();
-    int stage = 0;
-    uint32_t phase = 0;
-    bool alive = true;
-    for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
-      const int m0 = tile_m(tile) * 128, n0 = tile_n(tile) * per_tile;
-      for (int b = 0; b < blocks; ++b) {
-        if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1u, abort_flag)) { alive = false; break; }
-        if (elect_one()) {
-          const uint32_t s_a = smem_u32(smem + static_cast<size_t>(stage) * kRowsStageBytes), s_b = s_a + kTileBytes;
-          mbar_expect_tx(&full_bar[stage], kRowsStageBytes);
-          tma_load_2d(s_a, &map_x, &full_bar[stage], b * kFp8Block, m0, pol);
-          if (kMode == 2) {
-            // 64 gate rows, the 64 up rows of the same features, and the same for the next 64
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              tma_load_2d(s_b + h * kTileBytes, &map_w0, &full_bar[stage], b * kFp8Block, n0 + 64 * h, pol);
-              tma_load_2d(s_b + h * kTileBytes + kTileBytes / 2, &map_w1, &full_bar[stage], b * kFp8Block, n0 + 64 * h, pol);
+  // tiles of one column of weight tiles follow each other: the weights are read once, the rows stay in the L2
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      const uint64_t pol = policy_evict_last();
+      int stage = 0;
+      uint32_t phase = 0;
+      bool alive = true;
+      for (int tile = pair; tile < tiles && alive; tile += pairs) {
+        const int m0 = (tile % m_tiles) * 256 + 128 * static_cast<int>(rank), n0 = (tile / m_tiles) * per_tile;
+        for (int b = 0; b < blocks; ++b) {
+          if (!mbar_wait_hot(&empty_bar[stage], phase ^ 1u, abort_flag)) { alive = false; break; }
+          if (elect_one()) {
+            const uint32_t s_a = smem_u32(smem + static_cast<size_t>(stage) * kPairStageBytes), s_b = s_a + kTileBytes;
+            const uint32_t full = cluster_addr(smem_u32(&full_bar[stage]), 0);
+            if (rank == 0) mbar_expect_tx(&full_bar[stage], 2 * kPairStageBytes);
+            tma_load_2d_pair(s_a, &map_x, full, b * kFp8Block, m0, pol);
+            if (kMode == 2) {     // this CTA's 64 features: their gate rows, then their up rows
+              tma_load_2d_pair(s_b, &map_w0, full, b * kFp8Block, n0 + 64 * static_cast<int>(rank), pol);
+              tma_load_2d_pair(s_b + kTileBytes / 2, &map_w1, full, b * kFp8Block, n0 + 64 * static_cast<int>(rank), pol);
+            } else {
+              tma_load_2d_pair(s_b, &map_w0, full, b * kFp8Block, n0 + 128 * static_cast<int>(rank), pol);
             }
-          } else {
-            tma_load_2d(s_b, &map_w0, &full_bar[stage], b * kFp8Block, n0, pol);
           }
+          __syncwarp();
+          if (++stage == kPairStages) { stage = 0; phase ^= 1u; }
         }
-        __syncwarp();
-        if (++stage == kRowsStages) { stage = 0; phase ^= 1u; }
       }
-    }
-  } else if (warp == 1) {
-    int stage = 0, abuf = 0;
-    uint32_t phase = 0, aphase = 0;
-    bool alive = true;
-    const uint32_t idesc = idesc_fp8(kRowsN);
-    for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
-      for (int b = 0; b < blocks; ++b) {
-        if (!mbar_wait_warp(&acc_empty[abuf], aphase ^ 1u, abort_flag) ||
-            !mbar_wait_warp(&full_bar[stage], phase, abort_flag)) { alive = false; break; }
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t s_a = smem_u32(smem + static_cast<size_t>(stage) * kRowsStageBytes), s_b = s_a + kTileBytes;
+    } else if (warp == 1 && rank == 0) {
+      int stage = 0, abuf = 0;
+      uint32_t phase = 0, aphase = 0;
+      bool alive = true;
+      const uint32_t idesc = (1u << 4) | ((static_cast<uint32_t>(kPairN) >> 3) << 17) | ((256u >> 4) << 24);
+      for (int tile = pair; tile < tiles && alive; tile += pairs)
+        for (int b = 0; b < blocks; ++b) {
+          if (!mbar_wait_hot(&acc_empty[abuf], aphase ^ 1u, abort_flag) ||
+              !mbar_wait_hot(&full_bar[stage], phase, abort_flag)) { alive = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t s_a = smem_u32(smem + static_cast<size_t>(stage) * kPairStageBytes), s_b = s_a + kTileBytes;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_fp8(tmem_base + abuf * kRowsN, desc_sw128(s_a + kk * 32), desc_sw128(s_b + kk * 32), idesc, kk != 0 ? 1u : 0u);
-          tc_commit(&empty_bar[stage]);
-          tc_commit(&acc_full[abuf]);
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_fp8_pair(tmem_base + abuf * kPairN, desc_sw128(s_a + kk * 32), desc_sw128(s_b + kk * 32), idesc, kk != 0 ? 1u : 0u);
+            tc_commit_pair(smem_u32(&empty_bar[stage]));
+            tc_commit_pair(cluster_addr(smem_u32(&empty_bar[stage]), 1));
+            tc_commit_pair(smem_u32(&acc_full[abuf]));
+            tc_commit_pair(cluster_addr(smem_u32(&acc_full[abuf]), 1));
+          }
+          __syncwarp();
+          if (++stage == kPairStages) { stage = 0; phase ^= 1u; }
+          abuf ^= 1;
+          if (abuf == 0) aphase ^= 1u;
         }
-        __syncwarp();
-        if (++stage == kRowsStages) { stage = 0; phase ^= 1u; }
-        abuf ^= 1;
-        if (abuf == 0) aphase ^= 1u;
-      }
     }
   } else {
-    const int quad = warp & 3, part = (warp - 2) >> 2;       // tensor-memory lanes, half of the tile's columns
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int quad = warp & 3, part = (warp - 4) >> 2;       // tensor-memory lanes, half of the tile's columns
     const int lane_row = quad * 32 + lane;
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + part * 128;
+    const uint32_t lead_acc_empty = cluster_addr(smem_u32(acc_empty), 0);
+    uint32_t* park = park_all + (warp - 4) * 32 * kParkWords;
     int abuf = 0;
     uint32_t aphase = 0;
     // A warp whose wait ran out keeps step with the others (they meet at barriers), computing nothing valid.
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-      const int row = tile_m(tile) * 128 + lane_row, n0 = tile_n(tile) * per_tile;
+    for (int tile = pair; tile < tiles; tile += pairs) {
+      const int row0 = (tile % m_tiles) * 256 + 128 * static_cast<int>(rank) + quad * 32, row = row0 + lane;
+      const int n0 = (tile / m_tiles) * per_tile;
       // the product's halves are two weight blocks; gate and up share the block number of their features
-      const int wb = kMode == 2 ? tile_n(tile) : min(tile_n(tile) * 2 + part, (a.n - 1) / kFp8Block);
-      const float* xs = a.xs + row;                          // padded to whole tiles
+      const int wb = kMode == 2 ? tile / m_tiles : min((tile / m_tiles) * 2 + part, (a.n - 1) / kFp8Block);
+      const float* xs = a.xs + row;
       const float* ws0 = a.ws0 + static_cast<size_t>(wb) * blocks;
-      const float* ws1 = kMode == 2 ? a.ws1 + static_cast<size_t>(wb) * blocks : nullptr;
+      const float* ws1 = kMode == 2 ? a.ws1 + static_cast<size_t>(wb) * blocks : ws0;
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+      float sx = __ldg(xs), w0 = __ldg(ws0), w1 = __ldg(ws1);
       for (int b = 0; b < blocks; ++b) {
-        const float sx = __ldg(xs + static_cast<size_t>(b) * a.xs_stride);
-        const float s0 = sx * __ldg(ws0 + b), s1 = kMode == 2 ? sx * __ldg(ws1 + b) : s0;
-        mbar_wait_warp(&acc_full[abuf], aphase, abort_flag);
-        tc_fence_after();
-        const uint32_t t = t_lane + abuf * kRowsN;
-        uint32_t v[2][16];
-        tc_load16(t, v[0]);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          tc_wait_ld();
-          if (c < 7) tc_load16(t + (c + 1) * 16, v[(c + 1) & 1]);
-          const float s = kMode == 2 && c >= 4 ? s1 : s0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(__uint_as_float(v[c & 1][i]), s, acc[c * 16 + i]);
+        const float s0 = sx * w0, s1 = sx * w1;
+        if (b + 1 < blocks) {       // the next block's scales come from the L2 under this block
+          sx = __ldg(xs + static_cast<size_t>(b + 1) * a.xs_stride);
+          w0 = __ldg(ws0 + b + 1);
+          if (kMode == 2) w1 = __ldg(ws1 + b + 1);
+          else w1 = w0;
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[abuf]);
+        mbar_wait_hot(&acc_full[abuf], aphase, abort_flag);
+        tc_fence_after();
+        const uint32_t t = t_lane + abuf * kPairN;
+        uint32_t v[2][32];
+        tc_load32(t, v[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tc_wait_ld();
+          if (c < 3) tc_load32(t + (c + 1) * 32, v[(c + 1) & 1]);
+          else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(lead_acc_empty + abuf * 8);
+          }
+          const float s = kMode == 2 && c >= 2 ? s1 : s0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(v[c & 1][i]), s, acc[c * 32 + i]);
+        }
         abuf ^= 1;
         if (abuf == 0) aphase ^= 1u;
       }
@@ -211,10 +257,10 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
           acc[i] = fp8_swiglu(acc[i], acc[64 + i]);
           amax = max(amax, __float_as_uint(acc[i]) & 0x7fffffffu);
         }
-        amax_x[part * 128 + lane_row] = __uint_as_float(amax);
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowsEpiWarps) : "memory");
-        amax = max(amax, __float_as_uint(amax_x[(part ^ 1) * 128 + lane_row]));
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowsEpiWarps) : "memory");   // read before the next tile writes
+        amax_x[part * 128 + lane_row] = amax;
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kPairEpiWarps) : "memory");
+        amax = max(amax, amax_x[(part ^ 1) * 128 + lane_row]);
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kPairEpiWarps) : "memory");   // read before the next tile writes
         float inv;
         const float scale = fp8_block_scale(amax, &inv);
         if (row < a.rows) {
@@ -230,29 +276,33 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
             if (n0 + 64 * part + 16 * c < a.n) *reinterpret_cast<uint4*>(dst + 16 * c) = q;      // n % 16 == 0
           }
         }
-      } else if (row < a.rows) {
-        const int c0 = n0 + 128 * part;
-        constexpr int kPer = kMode == 0 ? 8 : 4;             // values of 16 bytes
+      } else {
+        // Through shared memory, 32 words of each of the warp's rows at a time, so that a row leaves as 128
+        // consecutive bytes (a word is two bf16 or one float32).
+        constexpr int kPer = kMode == 0 ? 2 : 1;
 #pragma unroll
-        for (int c = 0; c < 128; c += kPer) {
-          if (c0 + c >= a.n) continue;
-          if (a.vector_out) {                                // n is a multiple of kPer
-            uint4 q;
+        for (int pass = 0; pass < 4 / kPer; ++pass) {
+          const int c0 = n0 + 128 * part + pass * 32 * kPer;
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            park[lane * kParkWords + i] = kMode == 0 ? pack_bf16x2(acc[pass * 32 * kPer + i * kPer], acc[pass * 32 * kPer + i * kPer + kPer - 1])
+                                                     : __float_as_uint(acc[pass * 32 * kPer + i]);
+          __syncwarp();
+          const int c = c0 + lane * kPer, valid = a.n - c;
+          for (int r = 0; r < 32 && row0 + r < a.rows; ++r) {
+            const uint32_t word = park[r * kParkWords + lane];
             if constexpr (kMode == 0) {
-              q.x = pack_bf16x2(acc[c], acc[c + 1]); q.y = pack_bf16x2(acc[c + 2], acc[c + 3]);
-              q.z = pack_bf16x2(acc[c + 4], acc[c + 5]); q.w = pack_bf16x2(acc[c + 6], acc[c + 7]);
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + static_cast<size_t>(row) * a.n + c0 + c) = q;
-            } else {
-              *reinterpret_cast<float4*>(static_cast<float*>(a.out) + static_cast<size_t>(row) * a.n + c0 + c) =
-                  make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-              if (c0 + c + i < a.n) {
-                if constexpr (kMode == 0) fp8_store(static_cast<uint16_t*>(a.out) + static_cast<size_t>(row) * a.n + c0 + c + i, acc[c + i]);
-                else fp8_store(static_cast<float*>(a.out) + static_cast<size_t>(row) * a.n + c0 + c + i, acc[c + i]);
+              uint16_t* dst = static_cast<uint16_t*>(a.out) + static_cast<size_t>(row0 + r) * a.n + c;
+              if (valid >= 2 && reinterpret_cast<uintptr_t>(dst) % 4 == 0) {
+                *reinterpret_cast<uint32_t*>(dst) = word;
+              } else {
+                if (valid >= 1) dst[0] = static_cast<uint16_t>(word);
+                if (valid >= 2) dst[1] = static_cast<uint16_t>(word >> 16);
               }
+            } else if (valid >= 1) {
+              static_cast<float*>(a.out)[static_cast<size_t>(row0 + r) * a.n + c] = __uint_as_float(word);
+            }
           }
         }
       }
@@ -265,7 +315,8 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem_base, 512);
+  cluster_sync_all();           // neither CTA frees tensor memory the other may still be written through
+  if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -283,17 +334,22 @@ template <int kMode, int kN>
 struct WCfg {
   static constexpr int kMats = kMode == 2 ? 2 : 1;
   static constexpr int kStageBytes = kMats * kTileBytes + kN * kFp8Block;
-  static constexpr int kStages = 184320 / kStageBytes < 10 ? 184320 / kStageBytes : 10;
   static constexpr int kAccCols = kMats * kN;                       // of one block
+  // Two CTAs on an SM where the sums leave the registers for it: twice as many chains of copy, product and
+  // read-out side by side, and twice as many splits of a tile.
+  static constexpr int kPerSm = kAccCols <= 64 ? 2 : 1;
+  static constexpr int kRingBytes = kPerSm == 2 ? 104448 : 184320;
+  static constexpr int kStages = kRingBytes / kStageBytes < 8 ? kRingBytes / kStageBytes : 8;
+  static constexpr int kScaleBlocks = 16;                           // blocks whose scales are kept in shared memory
   static constexpr int kTmemCols = 2 * kAccCols < 32 ? 32 : 2 * kAccCols;
   static constexpr int kThreads = 192;
-  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + 1024 + 512 + 4 * kN * 4;
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + 1024 + 512 + 4 * kN * 4 + kScaleBlocks * (kN + kMats) * 4;
   static_assert(static_cast<size_t>(kStages) * kStageBytes >= static_cast<size_t>(kMats + 1) * kN * 128 * 4, "partial sums and the activation reuse the ring");
 };
 
 // grid (weight tiles, splits, row tiles), cluster (1, splits, 1).
 template <int kMode, int kN>
-__global__ void __launch_bounds__(WCfg<kMode, kN>::kThreads, 1)
+__global__ void __launch_bounds__(WCfg<kMode, kN>::kThreads, WCfg<kMode, kN>::kPerSm)
 fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w0,
                    const __grid_constant__ CUtensorMap map_w1) {
   using C = WCfg<kMode, kN>;
@@ -306,6 +362,8 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   uint32_t* amax_x = reinterpret_cast<uint32_t*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes + 512);   // [4][kN]
+  float* sx_all = reinterpret_cast<float*>(amax_x + 4 * kN);                  // [kScaleBlocks][kN]
+  float* sw_all = sx_all + C::kScaleBlocks * kN;                              // [kMats][kScaleBlocks]
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int blocks = (a.k + kFp8Block - 1) / kFp8Block;
@@ -363,7 +421,7 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
     int stage = 0;
     uint32_t phase = 0;
     for (int b = b0 + ahead; b < b1; ++b) {
-      if (!mbar_wait_warp(&empty_bar[stage], phase, abort_flag)) break;
+      if (!mbar_wait_hot(&empty_bar[stage], phase, abort_flag)) break;
       if (elect_one()) {
         load_w(stage, b);
         load_x(stage, b);
@@ -377,8 +435,8 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
     uint32_t phase = 0, aphase = 0;
     const uint32_t idesc = idesc_fp8(kN);
     for (int b = b0; b < b1; ++b) {
-      if (!mbar_wait_warp(&acc_empty[abuf], aphase ^ 1u, abort_flag) ||
-          !mbar_wait_warp(&full_bar[stage], phase, abort_flag)) break;
+      if (!mbar_wait_hot(&acc_empty[abuf], aphase ^ 1u, abort_flag) ||
+          !mbar_wait_hot(&full_bar[stage], phase, abort_flag)) break;
       tc_fence_after();
       if (elect_one()) {
         const uint32_t s_a = smem_u32(smem + static_cast<size_t>(stage) * C::kStageBytes), s_x = s_a + C::kMats * kTileBytes;
@@ -409,27 +467,42 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
       for (int j = 0; j < kN; ++j) acc[mat][j] = 0.0f;
     int abuf = 0;
     uint32_t aphase = 0;
+    const int tid = threadIdx.x - 64;
     for (int b = b0; b < b1; ++b) {
-      const float* xs = a.xs + static_cast<size_t>(b) * a.xs_stride + m0;       // padded to whole tiles of 128
-      const float sw[2] = {__ldg(a.ws0 + wb + b), kMode == 2 ? __ldg(a.ws1 + wb + b) : 0.0f};
-      if (!mbar_wait_warp(&acc_full[abuf], aphase, abort_flag)) break;
+      const int at = (b - b0) % C::kScaleBlocks;
+      if (at == 0) {              // the scales of the next blocks (rows padded to whole tiles)
+        const int count = min(C::kScaleBlocks, b1 - b);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (int i = tid; i < count * (kN / 4); i += 128)
+          reinterpret_cast<float4*>(sx_all)[i] = *reinterpret_cast<const float4*>(
+              a.xs + static_cast<size_t>(b + i / (kN / 4)) * a.xs_stride + m0 + (i % (kN / 4)) * 4);
+        if (tid < count) {
+          sw_all[tid] = __ldg(a.ws0 + wb + b + tid);
+          if (kMode == 2) sw_all[(C::kMats - 1) * C::kScaleBlocks + tid] = __ldg(a.ws1 + wb + b + tid);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+      const float* xs = sx_all + at * kN;
+      mbar_wait_hot(&acc_full[abuf], aphase, abort_flag);      // on a time-out it keeps step, computing nothing valid
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < kN / 16; ++c) {
+        uint32_t v[C::kMats][16];
+#pragma unroll
+        for (int mat = 0; mat < C::kMats; ++mat) tc_load16(t_lane + abuf * C::kAccCols + mat * kN + c * 16, v[mat]);
         float sx[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float4 q = *reinterpret_cast<const float4*>(xs + c * 16 + i * 4);
           sx[4 * i] = q.x; sx[4 * i + 1] = q.y; sx[4 * i + 2] = q.z; sx[4 * i + 3] = q.w;
         }
+        tc_wait_ld();
 #pragma unroll
         for (int mat = 0; mat < C::kMats; ++mat) {
-          uint32_t v[16];
-          tc_load16(t_lane + abuf * C::kAccCols + mat * kN + c * 16, v);
-          tc_wait_ld();
+          const float sw = sw_all[mat * C::kScaleBlocks + at];
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            acc[mat][c * 16 + i] = fmaf(__uint_as_float(v[i]), sx[i] * sw[mat], acc[mat][c * 16 + i]);
+            acc[mat][c * 16 + i] = fmaf(__uint_as_float(v[mat][i]), sx[i] * sw, acc[mat][c * 16 + i]);
         }
       }
       tc_fence_before();
@@ -521,9 +594,12 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
   if (splits > 1) cluster_sync_all();       // nobody leaves while its sums may still be read
 }
 
+int weight_splits(int n_tiles, int row_tiles, int blocks, int room);
+
 template <int kMode, int kN>
-glmrt_status_t launch_weights(const Fp8Gemm& g, int splits, cudaStream_t s) {
+glmrt_status_t launch_weights(const Fp8Gemm& g, int sm_count, cudaStream_t s) {
   using C = WCfg<kMode, kN>;
+  const int splits = weight_splits((g.n + 127) / 128, (g.rows + kN - 1) / kN, (g.k + kFp8Block - 1) / kFp8Block, C::kPerSm * sm_count);
   CUtensorMap mx, m0, m1;
   GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&mx, g.x, g.rows, g.k, kN));
   GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&m0, g.w0, g.n, g.k, 128));
@@ -554,42 +630,49 @@ template <int kMode>
 glmrt_status_t launch_rows(const Fp8Gemm& g, int sm_count, cudaStream_t s) {
   CUtensorMap mx, m0, m1;
   GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&mx, g.x, g.rows, g.k, 128));
-  GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&m0, g.w0, g.n, g.k, kMode == 2 ? 64 : 256));
+  GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&m0, g.w0, g.n, g.k, kMode == 2 ? 64 : 128));
   if (kMode == 2) GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&m1, g.w1, g.n, g.k, 64));
   else m1 = m0;
-  const size_t per = kMode == 0 ? 8 : 4;
-  RowsArgs a{g.xs, g.ws0, g.ws1, g.out, g.out_scales, g.rows, g.n, g.k, g.xs_stride, g.out_stride,
-             g.n % per == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0};
+  RowsArgs a{g.xs, g.ws0, g.ws1, g.out, g.out_scales, g.rows, g.n, g.k, g.xs_stride, g.out_stride};
   static std::atomic<uint64_t> configured{0};
-  GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, fp8_rows_kernel<kMode>, kRowsSmem, "cudaFuncSetAttribute(fp8_rows_kernel)"));
-  const int per_tile = kMode == 2 ? 128 : kRowsN;
-  const long long tiles = static_cast<long long>((g.rows + 127) / 128) * ((g.n + per_tile - 1) / per_tile);
-  launch_pdl(fp8_rows_kernel<kMode>, dim3(static_cast<unsigned>(std::min<long long>(tiles, sm_count))), dim3(kRowsThreads), kRowsSmem, s,
-             a, mx, m0, m1);
+  GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, fp8_rows_kernel<kMode>, kPairSmem, "cudaFuncSetAttribute(fp8_rows_kernel)"));
+  const int per_tile = kMode == 2 ? 128 : kPairN;
+  const long long tiles = static_cast<long long>((g.rows + 255) / 256) * ((g.n + per_tile - 1) / per_tile);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<long long>(tiles, sm_count / 2)));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t err = cudaLaunchKernelEx(&cfg, fp8_rows_kernel<kMode>, a, mx, m0, m1);
+  if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "fp8_rows_kernel", err);
   GLMRT_LAUNCH_CHECK("fp8_rows_kernel");
   return GLMRT_STATUS_OK;
 }
 
-// CTAs of a cluster that share a tile's K blocks: as many as fill the SMs once, at most eight and one per block.
-int weight_splits(int n_tiles, int row_tiles, int blocks, int sm_count) {
-  return std::max(1, std::min({8, blocks, sm_count / (n_tiles * row_tiles)}));
+// CTAs of a cluster that share a tile's K blocks: as many as find room at once, at most eight and one per block.
+int weight_splits(int n_tiles, int row_tiles, int blocks, int room) {
+  return std::max(1, std::min({8, blocks, room / (n_tiles * row_tiles)}));
 }
+
+constexpr int kWeightsMostRows = 256;
 
 template <int kMode>
 glmrt_status_t launch_mode(const Fp8Gemm& g, cudaStream_t s) {
   int dev = 0, sm_count = 0;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev);
-  const int n_tiles = (g.n + 127) / 128, blocks = (g.k + kFp8Block - 1) / kFp8Block;
   constexpr int kMostN = kMode == 2 ? 64 : 128;
-  if (g.rows <= 128) {
-    const int kn = g.rows <= 16 ? 16 : g.rows <= 32 ? 32 : g.rows <= 64 ? 64 : kMostN;
-    const int splits = weight_splits(n_tiles, (g.rows + kn - 1) / kn, blocks, sm_count);
-    if (kn == 16) return launch_weights<kMode, 16>(g, splits, s);
-    if (kn == 32) return launch_weights<kMode, 32>(g, splits, s);
-    if (kn == 64) return launch_weights<kMode, 64>(g, splits, s);
-    if constexpr (kMode != 2) return launch_weights<kMode, 128>(g, splits, s);
-  }
+  if (g.rows <= 16) return launch_weights<kMode, 16>(g, sm_count, s);
+  if (g.rows <= 32) return launch_weights<kMode, 32>(g, sm_count, s);
+  if (g.rows <= 64) return launch_weights<kMode, 64>(g, sm_count, s);
+  if (g.rows <= kWeightsMostRows) return launch_weights<kMode, kMostN>(g, sm_count, s);
   return launch_rows<kMode>(g, sm_count, s);
 }
 

@@ -69,6 +69,23 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
   if (ok != 0u) (void)mbar_try_wait(bar, parity);
   return ok != 0u;
 }
+// The same for waits on the critical path of every block of a product: every lane polls, and the clock is read
+// only once 256 polls have failed (reading it costs a good part of a microsecond).
+__device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  uint64_t t0 = 0;
+  for (uint32_t spin = 1;; ++spin) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((spin & 255u) == 0u) {
+      if (*abort_flag != 0u) return false;
+      const uint64_t t = global_timer_ns();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > kWaitLimitNs) {
+        *abort_flag = 1u;
+        return false;
+      }
+    }
+  }
+}
 // One leader lane of a converged warp (the form the compiler recognises as warp-uniform issue).
 __device__ __forceinline__ bool elect_one() {
   uint32_t pred;
