@@ -56,6 +56,7 @@ constexpr int kPairEpiWarps = 8;
 constexpr int kPairThreads = 32 * (4 + kPairEpiWarps);
 constexpr int kPairStageBytes = 2 * kTileBytes;                   // this CTA's rows and its half of the weight rows
 constexpr int kPairN = 256;
+constexpr int kBand = 8;                                          // row tiles of a band
 constexpr int kParkWords = 33;                                    // a parked row: 32 words and one against bank conflicts
 constexpr size_t kPairSmem = static_cast<size_t>(kPairStages) * kPairStageBytes + 1024 + 256 + 2 * 128 * 4 +
                              static_cast<size_t>(kPairEpiWarps) * 32 * kParkWords * 4;
@@ -144,7 +145,14 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
   pdl_wait();
   pdl_launch_dependents();      // after the wait: a successor may then rely on everything before this kernel
 
-  // tiles of one column of weight tiles follow each other: the weights are read once, the rows stay in the L2
+  // Tiles in bands of eight row tiles, column by column inside a band, so that the tiles in flight (74 pairs) form
+  // a block of about 8 x 9 whose rows and weights stay in the L2 while they are read.
+  auto tile_at = [&](int tile, int& m, int& nt) {
+    const int band = tile / (kBand * n_tiles), in = tile - band * kBand * n_tiles;
+    const int high = min(kBand, m_tiles - band * kBand);
+    nt = in / high;
+    m = band * kBand + in - nt * high;
+  };
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
@@ -153,7 +161,9 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
       uint32_t phase = 0;
       bool alive = true;
       for (int tile = pair; tile < tiles && alive; tile += pairs) {
-        const int m0 = (tile % m_tiles) * 256 + 128 * static_cast<int>(rank), n0 = (tile / m_tiles) * per_tile;
+        int mt, nt;
+        tile_at(tile, mt, nt);
+        const int m0 = mt * 256 + 128 * static_cast<int>(rank), n0 = nt * per_tile;
         for (int b = 0; b < blocks; ++b) {
           if (!mbar_wait_hot(&empty_bar[stage], phase ^ 1u, abort_flag)) { alive = false; break; }
           if (elect_one()) {
@@ -209,10 +219,12 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
     uint32_t aphase = 0;
     // A warp whose wait ran out keeps step with the others (they meet at barriers), computing nothing valid.
     for (int tile = pair; tile < tiles; tile += pairs) {
-      const int row0 = (tile % m_tiles) * 256 + 128 * static_cast<int>(rank) + quad * 32, row = row0 + lane;
-      const int n0 = (tile / m_tiles) * per_tile;
+      int mt, nt;
+      tile_at(tile, mt, nt);
+      const int row0 = mt * 256 + 128 * static_cast<int>(rank) + quad * 32, row = row0 + lane;
+      const int n0 = nt * per_tile;
       // the product's halves are two weight blocks; gate and up share the block number of their features
-      const int wb = kMode == 2 ? tile / m_tiles : min((tile / m_tiles) * 2 + part, (a.n - 1) / kFp8Block);
+      const int wb = kMode == 2 ? nt : min(nt * 2 + part, (a.n - 1) / kFp8Block);
       const float* xs = a.xs + row;
       const float* ws0 = a.ws0 + static_cast<size_t>(wb) * blocks;
       const float* ws1 = kMode == 2 ? a.ws1 + static_cast<size_t>(wb) * blocks : ws0;
