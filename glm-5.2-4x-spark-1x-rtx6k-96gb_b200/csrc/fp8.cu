@@ -16,30 +16,61 @@ namespace {
 
 constexpr int kBlock = kFp8Block;
 
-// One warp per (row, 128-column block): four values a lane.
-template <typename T>
-__global__ void fp8_quantize_rows_kernel(const T* __restrict__ in, size_t stride, uint8_t* __restrict__ codes,
-                                         float* __restrict__ scales, int rows, int cols, int scale_stride) {
+// Half a warp per (row, 128-column block), eight values a lane.  Bound by memory (bf16: 3 bytes a value), so
+// each lane keeps two blocks' loads in flight.  kVec: the rows' pieces of eight values are 16-byte aligned.
+constexpr int kQuantPerLane = 2;
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256) fp8_quantize_rows_kernel(const T* __restrict__ in, size_t stride, uint8_t* __restrict__ codes,
+                                                                float* __restrict__ scales, int rows, int cols, int scale_stride) {
   pdl_wait();
   pdl_launch_dependents();      // after the wait: a successor may then rely on everything before this kernel
-  const int blocks = (cols + kBlock - 1) / kBlock;
-  const size_t w = blockIdx.x * static_cast<size_t>(blockDim.x / 32) + threadIdx.x / 32;
-  if (w >= static_cast<size_t>(rows) * blocks) return;
-  const size_t row = w / blocks;
-  const int b = static_cast<int>(w % blocks), lane = threadIdx.x % 32, c = b * kBlock + lane * 4;
-  float v[4];
+  const uint32_t blocks = (cols + kBlock - 1) / kBlock;
+  const uint32_t sub = threadIdx.x % 16, groups = gridDim.x * 16u;
+  const uint32_t first = blockIdx.x * 16u + threadIdx.x / 16;
+  const uint64_t total = static_cast<uint64_t>(rows) * blocks;
+  float v[kQuantPerLane][8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = c + i < cols ? fp8_input(in[row * stride + c + i]) : 0.0f;
-  uint32_t amax = 0u;
+  for (int p = 0; p < kQuantPerLane; ++p) {
+    const uint64_t unit = first + static_cast<uint64_t>(p) * groups;
+    const uint32_t row = static_cast<uint32_t>(unit / blocks), b = static_cast<uint32_t>(unit - static_cast<uint64_t>(row) * blocks);
+    const uint32_t c = b * kBlock + sub * 8;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
+    if (unit < total && c < static_cast<uint32_t>(cols)) {          // cols % 16 == 0: eight values or none
+      const T* src = in + row * stride + c;
+      if constexpr (kVec) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  float inv;
-  const float scale = fp8_block_scale(amax, &inv);
-  const uint32_t q = fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-  if (c < cols) *reinterpret_cast<uint32_t*>(codes + row * cols + c) = q;   // cols % 16 == 0
-  if (lane == 0) scales[static_cast<size_t>(b) * scale_stride + row] = scale;
+        for (int i = 0; i < 8; i += 16 / static_cast<int>(sizeof(T))) {
+          T t[16 / sizeof(T)];
+          *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(src + i);
+#pragma unroll
+          for (int j = 0; j < static_cast<int>(16 / sizeof(T)); ++j) v[p][i + j] = fp8_input(t[j]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[p][i] = fp8_input(src[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < kQuantPerLane; ++p) {
+    const uint64_t unit = first + static_cast<uint64_t>(p) * groups;
+    const uint32_t row = static_cast<uint32_t>(unit / blocks), b = static_cast<uint32_t>(unit - static_cast<uint64_t>(row) * blocks);
+    const uint32_t c = b * kBlock + sub * 8;
+    uint32_t amax = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(v[p][i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (unit >= total) continue;
+    float inv;
+    const float scale = fp8_block_scale(amax, &inv);
+    if (c < static_cast<uint32_t>(cols))
+      *reinterpret_cast<uint2*>(codes + static_cast<size_t>(row) * cols + c) =
+          make_uint2(fp8_pack4(v[p][0] * inv, v[p][1] * inv, v[p][2] * inv, v[p][3] * inv),
+                     fp8_pack4(v[p][4] * inv, v[p][5] * inv, v[p][6] * inv, v[p][7] * inv));
+    if (sub == 0) scales[static_cast<size_t>(b) * scale_stride + row] = scale;
+  }
 }
 
 size_t round256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
@@ -64,14 +95,15 @@ glmrt_status_t check_buffer(const glmrt_device_buffer_t& b, size_t need, size_t 
 
 glmrt_status_t launch_quantize(const void* in, uint32_t dtype, size_t stride, uint8_t* codes, float* scales, size_t rows,
                                size_t cols, size_t scale_stride, cudaStream_t s) {
-  const size_t warps = rows * blocks_of(cols);
-  const dim3 grid(static_cast<unsigned>((warps + 7) / 8)), block(256);
-  if (dtype == GLMRT_B200_DTYPE_BF16)
-    launch_pdl(fp8_quantize_rows_kernel<uint16_t>, grid, block, 0, s, static_cast<const uint16_t*>(in), stride, codes,
-               scales, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(scale_stride));
-  else
-    launch_pdl(fp8_quantize_rows_kernel<float>, grid, block, 0, s, static_cast<const float*>(in), stride, codes, scales,
-               static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(scale_stride));
+  const size_t size = dtype == GLMRT_B200_DTYPE_BF16 ? 2 : 4, units = rows * blocks_of(cols);
+  const bool vec = reinterpret_cast<uintptr_t>(in) % 16 == 0 && stride * size % 16 == 0;
+  const dim3 grid(static_cast<unsigned>((units + 16 * kQuantPerLane - 1) / (16 * kQuantPerLane))), block(256);
+  const int m = static_cast<int>(rows), n = static_cast<int>(cols), ss = static_cast<int>(scale_stride);
+  auto run = [&](auto kernel, auto* src) { launch_pdl(kernel, grid, block, 0, s, src, stride, codes, scales, m, n, ss); };
+  const auto* bf = static_cast<const uint16_t*>(in);
+  const auto* f = static_cast<const float*>(in);
+  if (size == 2) vec ? run(fp8_quantize_rows_kernel<uint16_t, true>, bf) : run(fp8_quantize_rows_kernel<uint16_t, false>, bf);
+  else vec ? run(fp8_quantize_rows_kernel<float, true>, f) : run(fp8_quantize_rows_kernel<float, false>, f);
   GLMRT_LAUNCH_CHECK("fp8_quantize_rows_kernel");
   return GLMRT_STATUS_OK;
 }

@@ -243,20 +243,26 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
         mbar_wait_hot(&acc_full[abuf], aphase, abort_flag);
         tc_fence_after();
         const uint32_t t = t_lane + abuf * kPairN;
+        // 64 columns in flight at a time; the buffer is free again before the last half is added
         uint32_t v[2][32];
         tc_load32(t, v[0]);
+        tc_load32(t + 32, v[1]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int half = 0; half < 2; ++half) {
           tc_wait_ld();
-          if (c < 3) tc_load32(t + (c + 1) * 32, v[(c + 1) & 1]);
-          else {
+          if (half == 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(lead_acc_empty + abuf * 8);
           }
-          const float s = kMode == 2 && c >= 2 ? s1 : s0;
+          const float s = kMode == 2 && half == 1 ? s1 : s0;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(v[c & 1][i]), s, acc[c * 32 + i]);
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              acc[half * 64 + c * 32 + i] = fmaf(__uint_as_float(v[c][i]), s, acc[half * 64 + c * 32 + i]);
+            if (half == 0) tc_load32(t + 64 + c * 32, v[c]);
+          }
         }
         abuf ^= 1;
         if (abuf == 0) aphase ^= 1u;
