@@ -16,6 +16,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "fp8.cuh"
@@ -57,7 +58,7 @@ constexpr int kPairThreads = 32 * (4 + kPairEpiWarps);
 constexpr int kPairStageBytes = 2 * kTileBytes;                   // this CTA's rows and its half of the weight rows
 constexpr int kPairN = 256;
 constexpr int kBand = 8;                                          // row tiles of a band
-constexpr int kParkWords = 33;                                    // a parked row: 32 words and one against bank conflicts
+constexpr int kParkWords = 36;                                    // a parked row: 32 words and four against bank conflicts
 constexpr size_t kPairSmem = static_cast<size_t>(kPairStages) * kPairStageBytes + 1024 + 256 + 2 * 128 * 4 +
                              static_cast<size_t>(kPairEpiWarps) * 32 * kParkWords * 4;
 
@@ -67,6 +68,7 @@ struct RowsArgs {
   void* out;                  // product: [rows, n] bf16 or float32; SwiGLU: codes [rows, n]
   float* out_scales;          // SwiGLU: [ceil(n / 128)][out_stride]
   int rows, n, k, xs_stride, out_stride;
+  int vector_out;             // whole 16-byte pieces: n and the output's address allow them
 };
 
 __device__ __forceinline__ void tc_mma_fp8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -296,31 +298,37 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
         }
       } else {
         // Through shared memory, 32 words of each of the warp's rows at a time, so that a row leaves as 128
-        // consecutive bytes (a word is two bf16 or one float32).
+        // consecutive bytes (a word is two bf16 or one float32), four rows an instruction.
         constexpr int kPer = kMode == 0 ? 2 : 1;
 #pragma unroll
         for (int pass = 0; pass < 4 / kPer; ++pass) {
           const int c0 = n0 + 128 * part + pass * 32 * kPer;
+          auto word = [&](int i) {
+            return kMode == 0 ? pack_bf16x2(acc[pass * 32 * kPer + i * kPer], acc[pass * 32 * kPer + i * kPer + kPer - 1])
+                              : __float_as_uint(acc[pass * 32 * kPer + i]);
+          };
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            park[lane * kParkWords + i] = kMode == 0 ? pack_bf16x2(acc[pass * 32 * kPer + i * kPer], acc[pass * 32 * kPer + i * kPer + kPer - 1])
-                                                     : __float_as_uint(acc[pass * 32 * kPer + i]);
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(park + lane * kParkWords + i) = make_uint4(word(i), word(i + 1), word(i + 2), word(i + 3));
           __syncwarp();
-          const int c = c0 + lane * kPer, valid = a.n - c;
-          for (int r = 0; r < 32 && row0 + r < a.rows; ++r) {
-            const uint32_t word = park[r * kParkWords + lane];
-            if constexpr (kMode == 0) {
-              uint16_t* dst = static_cast<uint16_t*>(a.out) + static_cast<size_t>(row0 + r) * a.n + c;
-              if (valid >= 2 && reinterpret_cast<uintptr_t>(dst) % 4 == 0) {
-                *reinterpret_cast<uint32_t*>(dst) = word;
-              } else {
-                if (valid >= 1) dst[0] = static_cast<uint16_t>(word);
-                if (valid >= 2) dst[1] = static_cast<uint16_t>(word >> 16);
-              }
-            } else if (valid >= 1) {
-              static_cast<float*>(a.out)[static_cast<size_t>(row0 + r) * a.n + c] = __uint_as_float(word);
+          using Out = typename std::conditional<kMode == 0, uint16_t, float>::type;
+          Out* out = static_cast<Out*>(a.out) + static_cast<size_t>(row0) * a.n + c0;
+          if (a.vector_out) {
+            const int c = (lane & 7) * 4 * kPer;
+            if (c0 + c < a.n) {
+#pragma unroll
+              for (int r = lane >> 3; r < 32; r += 4)
+                if (row0 + r < a.rows)
+                  *reinterpret_cast<uint4*>(out + static_cast<size_t>(r) * a.n + c) =
+                      *reinterpret_cast<const uint4*>(park + r * kParkWords + (lane & 7) * 4);
             }
+          } else {
+            const Out* src = reinterpret_cast<const Out*>(park);
+            for (int r = 0; r < 32 && row0 + r < a.rows; ++r)
+#pragma unroll
+              for (int c = lane; c < 32 * kPer; c += 32)
+                if (c0 + c < a.n) out[static_cast<size_t>(r) * a.n + c] = src[r * kParkWords * kPer + c];
           }
         }
       }
@@ -541,70 +549,66 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem_base, C::kTmemCols);
   float* part = reinterpret_cast<float*>(smem);
-  if (splits > 1) {
-    if (warp >= 2)
+  if (warp >= 2)
 #pragma unroll
-      for (int mat = 0; mat < C::kMats; ++mat)
+    for (int mat = 0; mat < C::kMats; ++mat)
 #pragma unroll
-        for (int j = 0; j < kN; ++j) part[(mat * kN + j) * 128 + lane_row] = acc[mat][j];
-    cluster_sync_all();
-  }
-  // this CTA finishes rows j0 .. j1 of the tile, the splits added in order
+      for (int j = 0; j < kN; ++j) part[(mat * kN + j) * 128 + lane_row] = acc[mat][j];
+  if (splits > 1) cluster_sync_all();
+  // This CTA finishes rows j0 .. j1 of the tile, the splits added in order, four rows' loads in flight (a load from
+  // another CTA's shared memory takes most of a microsecond).
   const int valid = min(kN, a.rows - m0);
   const int j0 = valid * split / splits, j1 = valid * (split + 1) / splits;
   const int feature = w0 + lane_row;
   if (warp >= 2) {
-    const uint32_t part_at = smem_u32(part);
-    auto total = [&](int mat, int j) {
-      float v[8];
+    const uint32_t part_at = smem_u32(part) + lane_row * 4;
+    constexpr int kBatch = 4;
+    float* act = part + C::kMats * kN * 128;              // [row of x][feature], behind the partial sums
+    for (int jb = j0; jb < j1; jb += kBatch) {
+      float y[C::kMats][kBatch];
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        v[r] = 0.0f;
-        if (r < splits)
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[r]) : "r"(cluster_addr(part_at + ((mat * kN + j) * 128 + lane_row) * 4, r)) : "memory");
-      }
-      float s = v[0];
+      for (int mat = 0; mat < C::kMats; ++mat) {
+        float v[kBatch][8];
 #pragma unroll
-      for (int r = 1; r < 8; ++r) s += v[r];
-      return s;
-    };
-    if constexpr (kMode != 2) {
-      if (splits == 1) {
+        for (int j = 0; j < kBatch; ++j)
 #pragma unroll
-        for (int j = 0; j < kN; ++j)
-          if (j < valid && feature < a.n) {
-            if constexpr (kMode == 0) fp8_store(static_cast<uint16_t*>(a.out) + static_cast<size_t>(m0 + j) * a.n + feature, acc[0][j]);
-            else fp8_store(static_cast<float*>(a.out) + static_cast<size_t>(m0 + j) * a.n + feature, acc[0][j]);
+          for (int r = 0; r < 8; ++r) {
+            v[j][r] = 0.0f;
+            if (r < splits && jb + j < j1)
+              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[j][r]) : "r"(cluster_addr(part_at + (mat * kN + jb + j) * 512, r)) : "memory");
           }
-      } else {
-        for (int j = j0; j < j1; ++j) {
-          const float y = total(0, j);
-          if (feature < a.n) {
-            if constexpr (kMode == 0) fp8_store(static_cast<uint16_t*>(a.out) + static_cast<size_t>(m0 + j) * a.n + feature, y);
-            else fp8_store(static_cast<float*>(a.out) + static_cast<size_t>(m0 + j) * a.n + feature, y);
-          }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          y[mat][j] = v[j][0];
+#pragma unroll
+          for (int r = 1; r < 8; ++r) y[mat][j] += v[j][r];
         }
       }
-    } else {
-      // SwiGLU, then the block's (128 features of one row) largest magnitude over the four warps
-      float* act = part + C::kMats * kN * 128;              // [row of x][feature], behind the partial sums
 #pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        if (j < j0 || j >= j1) continue;
-        const float v = splits == 1 ? fp8_swiglu(acc[0][j], acc[C::kMats - 1][j]) : fp8_swiglu(total(0, j), total(1, j));
-        act[j * 128 + lane_row] = v;
-        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu);
-        if (lane == 0) amax_x[quad * kN + j] = m;
+      for (int j = 0; j < kBatch; ++j) {
+        if (jb + j >= j1) break;
+        if constexpr (kMode == 2) {
+          // SwiGLU, then the block's (128 features of one row) largest magnitude over the four warps
+          const float f = fp8_swiglu(y[0][j], y[C::kMats - 1][j]);
+          act[(jb + j) * 128 + lane_row] = f;
+          const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(f) & 0x7fffffffu);
+          if (lane == 0) amax_x[quad * kN + jb + j] = m;
+        } else if (feature < a.n) {
+          const size_t at = static_cast<size_t>(m0 + jb + j) * a.n + feature;
+          if constexpr (kMode == 0) fp8_store(static_cast<uint16_t*>(a.out) + at, y[0][j]);
+          else fp8_store(static_cast<float*>(a.out) + at, y[0][j]);
+        }
       }
+    }
+    if constexpr (kMode == 2) {
       asm volatile("bar.sync 1, 128;" ::: "memory");
       for (int j = j0; j < j1; ++j) {
-        const float v = act[j * 128 + lane_row];
         const uint32_t m = max(max(amax_x[j], amax_x[kN + j]), max(amax_x[2 * kN + j], amax_x[3 * kN + j]));
         float inv;
         const float scale = fp8_block_scale(m, &inv);
         const size_t row = static_cast<size_t>(m0 + j);
         if (feature < a.n) static_cast<uint8_t*>(a.out)[row * a.n + feature] =
-            static_cast<uint8_t>(__nv_cvt_float_to_fp8(v * inv, __NV_SATFINITE, __NV_E4M3));
+            static_cast<uint8_t>(__nv_cvt_float_to_fp8(act[j * 128 + lane_row] * inv, __NV_SATFINITE, __NV_E4M3));
         if (lane_row == 0) a.out_scales[static_cast<size_t>(blockIdx.x) * a.out_stride + row] = scale;
       }
     }
@@ -651,7 +655,8 @@ glmrt_status_t launch_rows(const Fp8Gemm& g, int sm_count, cudaStream_t s) {
   GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&m0, g.w0, g.n, g.k, kMode == 2 ? 64 : 128));
   if (kMode == 2) GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&m1, g.w1, g.n, g.k, 64));
   else m1 = m0;
-  RowsArgs a{g.xs, g.ws0, g.ws1, g.out, g.out_scales, g.rows, g.n, g.k, g.xs_stride, g.out_stride};
+  RowsArgs a{g.xs, g.ws0, g.ws1, g.out, g.out_scales, g.rows, g.n, g.k, g.xs_stride, g.out_stride,
+             g.n % (kMode == 0 ? 8 : 4) == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0};
   static std::atomic<uint64_t> configured{0};
   GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, fp8_rows_kernel<kMode>, kPairSmem, "cudaFuncSetAttribute(fp8_rows_kernel)"));
   const int per_tile = kMode == 2 ? 128 : kPairN;
