@@ -369,8 +369,8 @@ struct WCfg {
   static constexpr int kScaleBlocks = 16;                           // blocks whose scales are kept in shared memory
   static constexpr int kTmemCols = 2 * kAccCols < 32 ? 32 : 2 * kAccCols;
   static constexpr int kThreads = 192;
-  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + 1024 + 512 + 4 * kN * 4 + kScaleBlocks * (kN + kMats) * 4;
-  static_assert(static_cast<size_t>(kStages) * kStageBytes >= static_cast<size_t>(kMats + 1) * kN * 128 * 4, "partial sums and the activation reuse the ring");
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + 1024 + 512 + kScaleBlocks * (kN + kMats) * 4;
+  static_assert(static_cast<size_t>(kStages) * kStageBytes >= static_cast<size_t>(kMats) * kN * 128 * 4, "partial sums reuse the ring");
 };
 
 // grid (weight tiles, splits, row tiles), cluster (1, splits, 1).
@@ -387,8 +387,7 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  uint32_t* amax_x = reinterpret_cast<uint32_t*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes + 512);   // [4][kN]
-  float* sx_all = reinterpret_cast<float*>(amax_x + 4 * kN);                  // [kScaleBlocks][kN]
+  float* sx_all = reinterpret_cast<float*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes + 512);   // [kScaleBlocks][kN]
   float* sw_all = sx_all + C::kScaleBlocks * kN;                              // [kMats][kScaleBlocks]
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -511,24 +510,27 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
       const float* xs = sx_all + at * kN;
       mbar_wait_hot(&acc_full[abuf], aphase, abort_flag);      // on a time-out it keeps step, computing nothing valid
       tc_fence_after();
+      constexpr int kChunk = kN >= 32 && C::kAccCols < 128 ? 32 : 16;        // columns in flight, per matrix
 #pragma unroll
-      for (int c = 0; c < kN / 16; ++c) {
-        uint32_t v[C::kMats][16];
+      for (int c = 0; c < kN / kChunk; ++c) {
+        uint32_t v[C::kMats][kChunk];
 #pragma unroll
-        for (int mat = 0; mat < C::kMats; ++mat) tc_load16(t_lane + abuf * C::kAccCols + mat * kN + c * 16, v[mat]);
-        float sx[16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 q = *reinterpret_cast<const float4*>(xs + c * 16 + i * 4);
-          sx[4 * i] = q.x; sx[4 * i + 1] = q.y; sx[4 * i + 2] = q.z; sx[4 * i + 3] = q.w;
+        for (int mat = 0; mat < C::kMats; ++mat) {
+          if constexpr (kChunk == 32) tc_load32(t_lane + abuf * C::kAccCols + mat * kN + c * kChunk, v[mat]);
+          else tc_load16(t_lane + abuf * C::kAccCols + mat * kN + c * kChunk, v[mat]);
         }
         tc_wait_ld();
 #pragma unroll
-        for (int mat = 0; mat < C::kMats; ++mat) {
-          const float sw = sw_all[mat * C::kScaleBlocks + at];
+        for (int i = 0; i < kChunk; i += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(xs + c * kChunk + i);
+          const float sx[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            acc[mat][c * 16 + i] = fmaf(__uint_as_float(v[mat][i]), sx[i] * sw, acc[mat][c * 16 + i]);
+          for (int mat = 0; mat < C::kMats; ++mat) {
+            const float sw = sw_all[mat * C::kScaleBlocks + at];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[mat][c * kChunk + i + e] = fmaf(__uint_as_float(v[mat][i + e]), sx[e] * sw, acc[mat][c * kChunk + i + e]);
+          }
         }
       }
       tc_fence_before();
@@ -555,61 +557,69 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
 #pragma unroll
       for (int j = 0; j < kN; ++j) part[(mat * kN + j) * 128 + lane_row] = acc[mat][j];
   if (splits > 1) cluster_sync_all();
-  // This CTA finishes rows j0 .. j1 of the tile, the splits added in order, four rows' loads in flight (a load from
-  // another CTA's shared memory takes most of a microsecond).
+  else if (warp >= 2) asm volatile("bar.sync 1, 128;" ::: "memory");
+  // This CTA finishes rows j0 .. j1 of the tile, one warp a row and four features a lane, the splits added in order.
+  // A load from another CTA's shared memory takes most of a microsecond, so a lane has all splits' in flight.
   const int valid = min(kN, a.rows - m0);
   const int j0 = valid * split / splits, j1 = valid * (split + 1) / splits;
-  const int feature = w0 + lane_row;
   if (warp >= 2) {
-    const uint32_t part_at = smem_u32(part) + lane_row * 4;
-    constexpr int kBatch = 4;
-    float* act = part + C::kMats * kN * 128;              // [row of x][feature], behind the partial sums
-    for (int jb = j0; jb < j1; jb += kBatch) {
-      float y[C::kMats][kBatch];
+    const uint32_t part_at = smem_u32(part) + lane * 16;
+    const int feature = w0 + lane * 4;
+    constexpr int kBatch = kMode == 2 ? 1 : 2;
+    for (int jb = j0 + (warp - 2) * kBatch; jb < j1; jb += 4 * kBatch) {
+      float v[C::kMats * kBatch][8][4];
 #pragma unroll
-      for (int mat = 0; mat < C::kMats; ++mat) {
-        float v[kBatch][8];
+      for (int q = 0; q < C::kMats * kBatch; ++q) {
+        const int j = kMode == 2 ? q * kN + jb : jb + q;       // gate and up of one row, or two rows
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            v[j][r] = 0.0f;
-            if (r < splits && jb + j < j1)
-              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[j][r]) : "r"(cluster_addr(part_at + (mat * kN + jb + j) * 512, r)) : "memory");
-          }
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          y[mat][j] = v[j][0];
-#pragma unroll
-          for (int r = 1; r < 8; ++r) y[mat][j] += v[j][r];
+        for (int r = 0; r < 8; ++r) {
+          v[q][r][0] = v[q][r][1] = v[q][r][2] = v[q][r][3] = 0.0f;
+          if (r < splits && (kMode == 2 || j < j1))
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[q][r][0]), "=f"(v[q][r][1]), "=f"(v[q][r][2]), "=f"(v[q][r][3])
+                         : "r"(cluster_addr(part_at + j * 512, r))
+                         : "memory");
         }
       }
+      float y[C::kMats * kBatch][4];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        if (jb + j >= j1) break;
-        if constexpr (kMode == 2) {
-          // SwiGLU, then the block's (128 features of one row) largest magnitude over the four warps
-          const float f = fp8_swiglu(y[0][j], y[C::kMats - 1][j]);
-          act[(jb + j) * 128 + lane_row] = f;
-          const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(f) & 0x7fffffffu);
-          if (lane == 0) amax_x[quad * kN + jb + j] = m;
-        } else if (feature < a.n) {
-          const size_t at = static_cast<size_t>(m0 + jb + j) * a.n + feature;
-          if constexpr (kMode == 0) fp8_store(static_cast<uint16_t*>(a.out) + at, y[0][j]);
-          else fp8_store(static_cast<float*>(a.out) + at, y[0][j]);
+      for (int q = 0; q < C::kMats * kBatch; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y[q][i] = v[q][0][i];
+#pragma unroll
+          for (int r = 1; r < 8; ++r) y[q][i] += v[q][r][i];
         }
-      }
-    }
-    if constexpr (kMode == 2) {
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      for (int j = j0; j < j1; ++j) {
-        const uint32_t m = max(max(amax_x[j], amax_x[kN + j]), max(amax_x[2 * kN + j], amax_x[3 * kN + j]));
+      if constexpr (kMode == 2) {
+        // SwiGLU, and the block's (128 features of one row) scale
+        uint32_t amax = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y[0][i] = fp8_swiglu(y[0][i], y[1][i]);
+          amax = max(amax, __float_as_uint(y[0][i]) & 0x7fffffffu);
+        }
         float inv;
-        const float scale = fp8_block_scale(m, &inv);
-        const size_t row = static_cast<size_t>(m0 + j);
-        if (feature < a.n) static_cast<uint8_t*>(a.out)[row * a.n + feature] =
-            static_cast<uint8_t>(__nv_cvt_float_to_fp8(act[j * 128 + lane_row] * inv, __NV_SATFINITE, __NV_E4M3));
-        if (lane_row == 0) a.out_scales[static_cast<size_t>(blockIdx.x) * a.out_stride + row] = scale;
+        const float scale = fp8_block_scale(__reduce_max_sync(0xffffffffu, amax), &inv);
+        const size_t row = static_cast<size_t>(m0 + jb);
+        if (feature < a.n)                                      // n % 16 == 0
+          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + row * a.n + feature) =
+              fp8_pack4(y[0][0] * inv, y[0][1] * inv, y[0][2] * inv, y[0][3] * inv);
+        if (lane == 0) a.out_scales[static_cast<size_t>(blockIdx.x) * a.out_stride + row] = scale;
+      } else {
+        using Out = typename std::conditional<kMode == 0, uint16_t, float>::type;
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+          if (jb + q >= j1) break;
+          Out* out = static_cast<Out*>(a.out) + static_cast<size_t>(m0 + jb + q) * a.n + feature;
+          if (feature + 3 < a.n && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(Out)) == 0) {
+            if constexpr (kMode == 0) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(y[q][0], y[q][1]), pack_bf16x2(y[q][2], y[q][3]));
+            else *reinterpret_cast<float4*>(out) = make_float4(y[q][0], y[q][1], y[q][2], y[q][3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (feature + i < a.n) fp8_store(out + i, y[q][i]);
+          }
+        }
       }
     }
   }
