@@ -368,7 +368,10 @@ struct WCfg {
   static constexpr int kStages = kRingBytes / kStageBytes < 8 ? kRingBytes / kStageBytes : 8;
   static constexpr int kScaleBlocks = 16;                           // blocks whose scales are kept in shared memory
   static constexpr int kTmemCols = 2 * kAccCols < 32 ? 32 : 2 * kAccCols;
-  static constexpr int kThreads = 192;
+  static constexpr int kParts = kAccCols > 64 ? 2 : 1;              // epilogue warps per tensor-memory quadrant, by columns
+  static constexpr int kEpiWarps = 4 * kParts;
+  static constexpr int kCols = kN / kParts;                         // of each matrix, per thread
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + 1024 + 512 + kScaleBlocks * (kN + kMats) * 4;
   static_assert(static_cast<size_t>(kStages) * kStageBytes >= static_cast<size_t>(kMats) * kN * 128 * 4, "partial sums reuse the ring");
 };
@@ -408,7 +411,7 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4);
+      mbar_init(&acc_empty[b], C::kEpiWarps);
     }
     *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -481,15 +484,16 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
     }
   }
   const int quad = warp & 3, lane_row = quad * 32 + lane;           // epilogue warps: weight row of the tile
-  float acc[C::kMats][kN];
+  const int part_col = ((warp - 2) >> 2) * C::kCols;                // first column of this warp's share
+  float acc[C::kMats][C::kCols];
   if (warp >= 2) {
     pdl_wait();
-    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + part_col;
     const size_t wb = static_cast<size_t>(blockIdx.x) * blocks;
 #pragma unroll
     for (int mat = 0; mat < C::kMats; ++mat)
 #pragma unroll
-      for (int j = 0; j < kN; ++j) acc[mat][j] = 0.0f;
+      for (int j = 0; j < C::kCols; ++j) acc[mat][j] = 0.0f;
     int abuf = 0;
     uint32_t aphase = 0;
     const int tid = threadIdx.x - 64;
@@ -497,22 +501,22 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
       const int at = (b - b0) % C::kScaleBlocks;
       if (at == 0) {              // the scales of the next blocks (rows padded to whole tiles)
         const int count = min(C::kScaleBlocks, b1 - b);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        for (int i = tid; i < count * (kN / 4); i += 128)
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kEpiWarps) : "memory");
+        for (int i = tid; i < count * (kN / 4); i += 32 * C::kEpiWarps)
           reinterpret_cast<float4*>(sx_all)[i] = *reinterpret_cast<const float4*>(
               a.xs + static_cast<size_t>(b + i / (kN / 4)) * a.xs_stride + m0 + (i % (kN / 4)) * 4);
         if (tid < count) {
           sw_all[tid] = __ldg(a.ws0 + wb + b + tid);
           if (kMode == 2) sw_all[(C::kMats - 1) * C::kScaleBlocks + tid] = __ldg(a.ws1 + wb + b + tid);
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kEpiWarps) : "memory");
       }
-      const float* xs = sx_all + at * kN;
+      const float* xs = sx_all + at * kN + part_col;
       mbar_wait_hot(&acc_full[abuf], aphase, abort_flag);      // on a time-out it keeps step, computing nothing valid
       tc_fence_after();
-      constexpr int kChunk = kN >= 32 && C::kAccCols < 128 ? 32 : 16;        // columns in flight, per matrix
+      constexpr int kChunk = C::kCols >= 32 ? 32 : 16;        // columns in flight, per matrix
 #pragma unroll
-      for (int c = 0; c < kN / kChunk; ++c) {
+      for (int c = 0; c < C::kCols / kChunk; ++c) {
         uint32_t v[C::kMats][kChunk];
 #pragma unroll
         for (int mat = 0; mat < C::kMats; ++mat) {
@@ -555,9 +559,9 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
 #pragma unroll
     for (int mat = 0; mat < C::kMats; ++mat)
 #pragma unroll
-      for (int j = 0; j < kN; ++j) part[(mat * kN + j) * 128 + lane_row] = acc[mat][j];
+      for (int j = 0; j < C::kCols; ++j) part[(mat * kN + part_col + j) * 128 + lane_row] = acc[mat][j];
   if (splits > 1) cluster_sync_all();
-  else if (warp >= 2) asm volatile("bar.sync 1, 128;" ::: "memory");
+  else if (warp >= 2) asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kEpiWarps) : "memory");
   // This CTA finishes rows j0 .. j1 of the tile, one warp a row and four features a lane, the splits added in order.
   // A load from another CTA's shared memory takes most of a microsecond, so a lane has all splits' in flight.
   const int valid = min(kN, a.rows - m0);
@@ -566,7 +570,7 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
     const uint32_t part_at = smem_u32(part) + lane * 16;
     const int feature = w0 + lane * 4;
     constexpr int kBatch = kMode == 2 ? 1 : 2;
-    for (int jb = j0 + (warp - 2) * kBatch; jb < j1; jb += 4 * kBatch) {
+    for (int jb = j0 + (warp - 2) * kBatch; jb < j1; jb += C::kEpiWarps * kBatch) {
       float v[C::kMats * kBatch][8][4];
 #pragma unroll
       for (int q = 0; q < C::kMats * kBatch; ++q) {
@@ -658,19 +662,20 @@ int active_clusters(int splits) {
 }
 
 // CTAs of a cluster that share a tile's K blocks: the number with the shortest estimated time.  A wave of CTAs
-// costs about 3 us beside its blocks (set-up, first copies, joining), a block 0.2 us and 0.0015 us per column of
-// the sum (measured at 16 to 128 rows and 2048 to 6144 columns).
+// costs about 3 us beside its blocks (set-up, first copies, joining), a block 0.42 us and 0.0015 us per column of
+// the sum (measured at 16 to 256 rows and 2048 to 6144 columns of K).
 template <int kMode, int kN>
-int weight_splits(int tiles, int blocks) {
+int weight_splits(int tiles, int blocks, float* estimate_us) {
   int best = 1;
   float best_us = 0.0f;
   for (int s = 1; s <= 8 && s <= blocks; ++s) {
     const int active = active_clusters<kMode, kN>(s);
     if (active <= 0) continue;
     const float us = static_cast<float>((tiles + active - 1) / active) *
-                     (3.0f + (s > 1 ? 0.7f : 0.0f) + static_cast<float>((blocks + s - 1) / s) * (0.2f + 0.0015f * WCfg<kMode, kN>::kAccCols));
+                     (3.0f + (s > 1 ? 0.7f : 0.0f) + static_cast<float>((blocks + s - 1) / s) * (0.42f + 0.0015f * WCfg<kMode, kN>::kAccCols));
     if (best_us == 0.0f || us < best_us) { best = s; best_us = us; }
   }
+  *estimate_us = best_us;
   return best;
 }
 
@@ -679,7 +684,8 @@ glmrt_status_t launch_weights(const Fp8Gemm& g, cudaStream_t s) {
   using C = WCfg<kMode, kN>;
   static std::atomic<uint64_t> configured{0};
   GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, fp8_weights_kernel<kMode, kN>, C::kSmem, "cudaFuncSetAttribute(fp8_weights_kernel)"));
-  const int splits = weight_splits<kMode, kN>((g.n + 127) / 128 * ((g.rows + kN - 1) / kN), (g.k + kFp8Block - 1) / kFp8Block);
+  float us = 0.0f;
+  const int splits = weight_splits<kMode, kN>((g.n + 127) / 128 * ((g.rows + kN - 1) / kN), (g.k + kFp8Block - 1) / kFp8Block, &us);
   CUtensorMap mx, m0, m1;
   GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&mx, g.x, g.rows, g.k, kN));
   GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&m0, g.w0, g.n, g.k, 128));
@@ -735,18 +741,33 @@ glmrt_status_t launch_rows(const Fp8Gemm& g, int sm_count, cudaStream_t s) {
   return GLMRT_STATUS_OK;
 }
 
-constexpr int kWeightsMostRows = 256;
+// Tiles of 16, 32 and 64 rows for batches that small.  Above, the larger of the weight-row tiles or the row tiles,
+// by their estimates: a wave of row tiles costs about 4 us and 0.48 us a block, whatever part of its 256 rows is
+// filled (measured: 256 rows, n = 6144, k = 2048: 14 against 20 us on weight-row tiles; n = 1500, k = 2000: 16
+// against 10 us).
+constexpr int kWeightsMostRows = 1024;
 
 template <int kMode>
 glmrt_status_t launch_mode(const Fp8Gemm& g, cudaStream_t s) {
-  int dev = 0, sm_count = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev);
   constexpr int kMostN = kMode == 2 ? 64 : 128;
   if (g.rows <= 16) return launch_weights<kMode, 16>(g, s);
   if (g.rows <= 32) return launch_weights<kMode, 32>(g, s);
   if (g.rows <= 64) return launch_weights<kMode, 64>(g, s);
-  if (g.rows <= kWeightsMostRows) return launch_weights<kMode, kMostN>(g, s);
+  int dev = 0, sm_count = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev);
+  if (g.rows <= kWeightsMostRows) {
+    using C = WCfg<kMode, kMostN>;
+    static std::atomic<uint64_t> configured{0};
+    GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, fp8_weights_kernel<kMode, kMostN>, C::kSmem, "cudaFuncSetAttribute(fp8_weights_kernel)"));
+    const int blocks = (g.k + kFp8Block - 1) / kFp8Block, per_tile = kMode == 2 ? 128 : kPairN;
+    const int tiles = (g.n + 127) / 128 * ((g.rows + kMostN - 1) / kMostN);
+    const int row_tiles = (g.n + per_tile - 1) / per_tile * ((g.rows + 255) / 256), pairs = sm_count / 2;
+    float us = 0.0f;
+    weight_splits<kMode, kMostN>(tiles, blocks, &us);
+    if (us < static_cast<float>((row_tiles + pairs - 1) / pairs) * (4.0f + 0.48f * static_cast<float>(blocks)))
+      return launch_weights<kMode, kMostN>(g, s);
+  }
   return launch_rows<kMode>(g, sm_count, s);
 }
 
