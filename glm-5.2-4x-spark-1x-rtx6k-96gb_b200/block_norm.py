@@ -9,25 +9,24 @@ residual stream (python/reference/glmrt_reference/glm_moe_dsa_layer_ref.py:157-2
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 
 import torch
 
+from . import launch
 from . import native as N
 
 _DTYPES = {torch.bfloat16: N.DTYPE_BF16, torch.float32: N.DTYPE_F32}
+_ARGS = struct.Struct("@" + launch.BUFFER * 7 + "8Q2I2f")      # glmrt_b200_block_norm_args_t
 
 
-def _rows(t: torch.Tensor, like: torch.Tensor, what: str) -> tuple[N.DeviceBuffer, int]:
-    """Buffer and row stride of a [rows, width] tensor whose rows are contiguous inside."""
+def _rows(t: torch.Tensor, like: torch.Tensor, rows: int, width: int, what: str) -> tuple[tuple, int]:
+    """Packed buffer and row stride of a [rows, width] tensor whose rows are contiguous inside."""
     if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"block_norm: {what} must have the shape, type and device of residual")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    if width > 1 and t.stride(1) != 1:
         raise ValueError(f"block_norm: {what} must be contiguous along its rows")
-    rows, width = t.shape
-    stride = t.stride(0) if rows > 1 else width
-    nbytes = ((rows - 1) * stride + width) * t.element_size() if rows else 0
-    return N.DeviceBuffer.of(t.data_ptr(), nbytes, t.device.index), stride
+    return launch.rows_buffer(t, rows, width)
 
 
 def block_norm(residual: torch.Tensor, delta: torch.Tensor | None = None, *, norm_weight: torch.Tensor,
@@ -40,49 +39,47 @@ def block_norm(residual: torch.Tensor, delta: torch.Tensor | None = None, *, nor
     ``normalized`` may be given, also in the place of ``residual`` or ``delta``.  Without ``delta``
     the residual comes back as it is.
     """
-    if residual.dim() != 2 or residual.dtype not in _DTYPES:
+    dtype = _DTYPES.get(residual.dtype)
+    if residual.dim() != 2 or dtype is None:
         raise ValueError("block_norm: residual must be [rows, width], bfloat16 or float32")
     if not residual.is_cuda:
         raise ValueError("block_norm: tensors must be on a CUDA device")
     rows, width = residual.shape
     if delta is None and (post_weight is not None or gate is not None or residual_out is not None):
         raise ValueError("block_norm: post_weight, gate and residual_out need a delta")
-    a = N.BlockNormArgs()
-    a.rows, a.width, a.scale, a.eps = rows, width, scale, eps
-    a.dtype = _DTYPES[residual.dtype]
+    wdtype = _DTYPES.get(norm_weight.dtype)
     for name, w in (("norm_weight", norm_weight), ("post_weight", post_weight)):
         if w is None:
             continue
-        if w.shape != (width,) or w.dtype not in _DTYPES or w.device != residual.device or not w.is_contiguous():
+        if w.shape != (width,) or wdtype is None or w.device != residual.device or not w.is_contiguous():
             raise ValueError(f"block_norm: {name} must be a contiguous [{width}] bfloat16 or float32 tensor on the rows' device")
         if w.dtype != norm_weight.dtype:
             raise ValueError("block_norm: norm_weight and post_weight must have one type")
-        setattr(a, name, N.DeviceBuffer.of(w.data_ptr(), width * w.element_size(), w.device.index))
-    a.weight_dtype = _DTYPES[norm_weight.dtype]
+    gate_buf, gate_rs, gate_cs = launch.NO_BUFFER, 0, 0
     if gate is not None:
         if gate.dim() != 2 or gate.shape[0] not in (1, rows) or gate.shape[1] not in (1, width):
             raise ValueError("block_norm: gate must be [rows, 1], [1, width] or [rows, width]")
         if gate.dtype != residual.dtype or gate.device != residual.device:
             raise ValueError("block_norm: gate must have the type and device of residual")
-        a.gate_row_stride = gate.stride(0) if gate.shape[0] > 1 else 0
-        a.gate_col_stride = gate.stride(1) if gate.shape[1] > 1 else 0
-        if a.gate_col_stride > 1:
+        gate_rs = gate.stride(0) if gate.shape[0] > 1 else 0
+        gate_cs = gate.stride(1) if gate.shape[1] > 1 else 0
+        if gate_cs > 1:
             raise ValueError("block_norm: gate must be contiguous along its rows")
-        span = (gate.shape[0] - 1) * a.gate_row_stride + (gate.shape[1] - 1) * a.gate_col_stride + 1
-        if a.gate_col_stride == 0 and gate.shape[1] == width and width > 1:
-            span = (gate.shape[0] - 1) * a.gate_row_stride + 1          # an expanded column
-        a.gate = N.DeviceBuffer.of(gate.data_ptr(), span * gate.element_size(), gate.device.index)
+        span = (gate.shape[0] - 1) * gate_rs + (gate.shape[1] - 1) * gate_cs + 1
+        gate_buf = (gate.data_ptr(), span * gate.element_size(), 0, 0)
     if normalized is None:
-        normalized = torch.empty((rows, width), dtype=residual.dtype, device=residual.device)
-    a.residual, a.residual_stride = _rows(residual, residual, "residual")
-    a.normalized, a.normalized_stride = _rows(normalized, residual, "normalized")
+        normalized = residual.new_empty((rows, width))
+    res, res_stride = _rows(residual, residual, rows, width, "residual")
+    norm, norm_stride = _rows(normalized, residual, rows, width, "normalized")
+    dlt, dlt_stride, out, out_stride = launch.NO_BUFFER, 0, launch.NO_BUFFER, 0
     if delta is not None:
         if residual_out is None:
-            residual_out = torch.empty((rows, width), dtype=residual.dtype, device=residual.device)
-        a.delta, a.delta_stride = _rows(delta, residual, "delta")
-        a.residual_out, a.residual_out_stride = _rows(residual_out, residual, "residual_out")
+            residual_out = residual.new_empty((rows, width))
+        dlt, dlt_stride = _rows(delta, residual, rows, width, "delta")
+        out, out_stride = _rows(residual_out, residual, rows, width, "residual_out")
     if rows:
-        with torch.cuda.device(residual.device):
-            (lib or N.library()).call("glmrt_b200_block_norm_async", C.byref(a),
-                                      C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        launch.call(lib, "glmrt_b200_block_norm_async",
+                    _ARGS.pack(*res, *dlt, *launch.buffer(norm_weight), *launch.buffer(post_weight), *gate_buf, *out, *norm,
+                               rows, width, res_stride, dlt_stride, gate_rs, gate_cs, out_stride, norm_stride,
+                               dtype, wdtype, scale, eps), residual.device)
     return (residual if delta is None else residual_out), normalized

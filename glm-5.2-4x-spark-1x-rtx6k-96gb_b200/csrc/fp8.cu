@@ -113,9 +113,9 @@ glmrt_status_t launch_quantize(const void* in, uint32_t dtype, size_t stride, ui
 
 using namespace glmrt;
 
-extern "C" glmrt_status_t glmrt_b200_fp8_quantize_rows_async(glmrt_device_buffer_t input, glmrt_device_buffer_t codes,
-                                                             glmrt_device_buffer_t scales, size_t rows, size_t cols,
-                                                             size_t input_row_stride, uint32_t dtype, void* cuda_stream) {
+extern "C" glmrt_status_t glmrt_b200_fp8_quantize_rows_async(const glmrt_b200_fp8_quantize_rows_args_t* args, void* cuda_stream) {
+  if (args == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "fp8_quantize_rows: null arguments");
+  const auto& [input, codes, scales, rows, cols, input_row_stride, dtype] = *args;
   GLMRT_RETURN_IF_ERROR(check_dims(rows, 1, cols, "fp8_quantize_rows"));
   if (dtype > GLMRT_B200_DTYPE_F32 || input_row_stride < cols || input_row_stride > (size_t{1} << 32))
     return fail(GLMRT_STATUS_INVALID_ARGUMENT, "fp8_quantize_rows: unknown dtype, or row stride below cols");
@@ -137,10 +137,9 @@ extern "C" glmrt_status_t glmrt_b200_fp8_block_linear_workspace(size_t rows, siz
   return ok();
 }
 
-extern "C" glmrt_status_t glmrt_b200_fp8_block_linear_async(glmrt_device_buffer_t x_bf16, glmrt_device_buffer_t weight_codes,
-                                                            glmrt_device_buffer_t weight_scales, glmrt_device_buffer_t output,
-                                                            glmrt_device_buffer_t workspace, size_t rows, size_t n, size_t k,
-                                                            size_t x_row_stride, uint32_t out_dtype, void* cuda_stream) {
+extern "C" glmrt_status_t glmrt_b200_fp8_block_linear_async(const glmrt_b200_fp8_block_linear_args_t* args, void* cuda_stream) {
+  if (args == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "fp8_block_linear: null arguments");
+  const auto& [x_bf16, weight_codes, weight_scales, output, workspace, rows, n, k, x_row_stride, out_dtype] = *args;
   GLMRT_RETURN_IF_ERROR(check_dims(rows, n, k, "fp8_block_linear"));
   if (out_dtype > GLMRT_B200_DTYPE_F32 || x_row_stride < k || x_row_stride > (size_t{1} << 32))
     return fail(GLMRT_STATUS_INVALID_ARGUMENT, "fp8_block_linear: unknown output dtype, or x row stride below k");
@@ -171,11 +170,10 @@ extern "C" glmrt_status_t glmrt_b200_fp8_gated_mlp_workspace(size_t rows, size_t
   return ok();
 }
 
-extern "C" glmrt_status_t glmrt_b200_fp8_gated_mlp_async(
-    glmrt_device_buffer_t x_bf16, glmrt_device_buffer_t gate_codes, glmrt_device_buffer_t gate_scales,
-    glmrt_device_buffer_t up_codes, glmrt_device_buffer_t up_scales, glmrt_device_buffer_t down_codes,
-    glmrt_device_buffer_t down_scales, glmrt_device_buffer_t output_bf16, glmrt_device_buffer_t workspace, size_t rows,
-    size_t hidden, size_t inter, size_t x_row_stride, void* cuda_stream) {
+extern "C" glmrt_status_t glmrt_b200_fp8_gated_mlp_async(const glmrt_b200_fp8_gated_mlp_args_t* args, void* cuda_stream) {
+  if (args == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "fp8_gated_mlp: null arguments");
+  const auto& [x_bf16, gate_codes, gate_scales, up_codes, up_scales, down_codes, down_scales, output_bf16, workspace, rows,
+               hidden, inter, x_row_stride] = *args;
   size_t need = 0;
   GLMRT_RETURN_IF_ERROR(glmrt_b200_fp8_gated_mlp_workspace(rows, hidden, inter, &need));
   if (x_row_stride < hidden || x_row_stride > (size_t{1} << 32))

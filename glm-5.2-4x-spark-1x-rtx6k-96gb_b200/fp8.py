@@ -8,38 +8,32 @@ and the last block may be ragged.  A row with a NaN or an infinity gives NaN out
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import struct
 
 import torch
 
+from . import launch
 from . import native as N
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
+_QUANT_ARGS = struct.Struct("@" + launch.BUFFER * 3 + "3QI4x")       # glmrt_b200_fp8_quantize_rows_args_t
+_LINEAR_ARGS = struct.Struct("@" + launch.BUFFER * 5 + "4QI4x")      # glmrt_b200_fp8_block_linear_args_t
+_MLP_ARGS = struct.Struct("@" + launch.BUFFER * 9 + "4Q")            # glmrt_b200_fp8_gated_mlp_args_t
 
 
 def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def _buf(t: torch.Tensor) -> N.DeviceBuffer:
-    return N.DeviceBuffer.of(t.data_ptr(), t.numel() * t.element_size(), t.device.index)
-
-
-def _stream() -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-def _check_rows(x: torch.Tensor, k: int, types: tuple, what: str) -> tuple[N.DeviceBuffer, int]:
+def _check_rows(x: torch.Tensor, k: int, types: tuple, what: str) -> None:
     if x.dim() != 2 or x.shape[1] != k or x.dtype not in types:
         raise ValueError(f"{what} must be [rows, {k}] of type {' or '.join(str(t) for t in types)}")
     if not x.is_cuda:
         raise ValueError(f"{what} must be on a CUDA device")
     if k > 1 and x.stride(1) != 1:
         raise ValueError(f"{what} must be contiguous along its rows")
-    rows = x.shape[0]
-    stride = x.stride(0) if rows > 1 else k
-    nbytes = ((rows - 1) * stride + k) * x.element_size() if rows else 0
-    return N.DeviceBuffer.of(x.data_ptr(), nbytes, x.device.index), stride
 
 
 def _check_weight(codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, device: torch.device, what: str) -> None:
@@ -65,20 +59,21 @@ def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def quantize_rows(x: torch.Tensor, lib: N.NativeLibrary | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The rows' codes ``[rows, k]`` (E4M3) and scales ``[ceil(k/128), rows]``; x bf16 or float32."""
     rows, k = x.shape if x.dim() == 2 else (0, 0)
-    buf, stride = _check_rows(x, k, (torch.bfloat16, torch.float32), "quantize_rows: x")
+    _check_rows(x, k, (torch.bfloat16, torch.float32), "quantize_rows: x")
+    buf, stride = launch.rows_buffer(x, rows, k)
     codes = torch.empty((rows, k), dtype=E4M3, device=x.device)
     scales = torch.empty((_blocks(k), rows), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        (lib or N.library()).call("glmrt_b200_fp8_quantize_rows_async", buf, _buf(codes), _buf(scales), C.c_size_t(rows),
-                                  C.c_size_t(k), C.c_size_t(stride),
-                                  C.c_uint32(N.DTYPE_BF16 if x.dtype == torch.bfloat16 else N.DTYPE_F32), _stream())
+    launch.call(lib, "glmrt_b200_fp8_quantize_rows_async",
+                _QUANT_ARGS.pack(*buf, *launch.buffer(codes), *launch.buffer(scales), rows, k, stride,
+                                 N.DTYPE_BF16 if x.dtype == torch.bfloat16 else N.DTYPE_F32), x.device)
     return codes, scales
 
 
-def _workspace(lib: N.NativeLibrary, symbol: str, device: torch.device, *sizes: int) -> torch.Tensor:
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(lib: N.NativeLibrary, symbol: str, *sizes: int) -> int:
     need = C.c_size_t(0)
     lib.call(symbol, *[C.c_size_t(v) for v in sizes], C.byref(need))
-    return torch.empty(max(need.value, 1), dtype=torch.uint8, device=device)
+    return max(need.value, 1)
 
 
 def _output(out: torch.Tensor | None, rows: int, n: int, dtype: torch.dtype, x: torch.Tensor) -> torch.Tensor:
@@ -98,15 +93,15 @@ def block_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out
     n, k = codes.shape
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("block_linear: out_dtype must be bfloat16 or float32")
-    buf, stride = _check_rows(x, k, (torch.bfloat16,), "block_linear: x")
+    _check_rows(x, k, (torch.bfloat16,), "block_linear: x")
     _check_weight(codes, scales, n, k, x.device, "block_linear: weight")
     rows = x.shape[0]
+    buf, stride = launch.rows_buffer(x, rows, k)
     out = _output(out, rows, n, out_dtype, x)
-    with torch.cuda.device(x.device):
-        ws = _workspace(lib, "glmrt_b200_fp8_block_linear_workspace", x.device, rows, n, k)
-        lib.call("glmrt_b200_fp8_block_linear_async", buf, _buf(codes), _buf(scales), _buf(out), _buf(ws),
-                 C.c_size_t(rows), C.c_size_t(n), C.c_size_t(k), C.c_size_t(stride),
-                 C.c_uint32(N.DTYPE_BF16 if out_dtype == torch.bfloat16 else N.DTYPE_F32), _stream())
+    ws = torch.empty(_workspace_bytes(lib, "glmrt_b200_fp8_block_linear_workspace", rows, n, k), dtype=torch.uint8, device=x.device)
+    launch.call(lib, "glmrt_b200_fp8_block_linear_async",
+                _LINEAR_ARGS.pack(*buf, *launch.buffer(codes), *launch.buffer(scales), *launch.buffer(out), *launch.buffer(ws),
+                                  rows, n, k, stride, N.DTYPE_BF16 if out_dtype == torch.bfloat16 else N.DTYPE_F32), x.device)
     return out
 
 
@@ -119,15 +114,21 @@ def gated_mlp(x: torch.Tensor, gate_codes: torch.Tensor, gate_scales: torch.Tens
     if gate_codes.dim() != 2:
         raise ValueError("gated_mlp: gate codes must be [inter, hidden]")
     inter, hidden = gate_codes.shape
-    buf, stride = _check_rows(x, hidden, (torch.bfloat16,), "gated_mlp: x")
+    _check_rows(x, hidden, (torch.bfloat16,), "gated_mlp: x")
     _check_weight(gate_codes, gate_scales, inter, hidden, x.device, "gated_mlp: gate")
     _check_weight(up_codes, up_scales, inter, hidden, x.device, "gated_mlp: up")
     _check_weight(down_codes, down_scales, hidden, inter, x.device, "gated_mlp: down")
     rows = x.shape[0]
+    buf, stride = launch.rows_buffer(x, rows, hidden)
     out = _output(out, rows, hidden, torch.bfloat16, x)
-    with torch.cuda.device(x.device):
-        ws = _workspace(lib, "glmrt_b200_fp8_gated_mlp_workspace", x.device, rows, hidden, inter)
-        lib.call("glmrt_b200_fp8_gated_mlp_async", buf, _buf(gate_codes), _buf(gate_scales), _buf(up_codes),
-                 _buf(up_scales), _buf(down_codes), _buf(down_scales), _buf(out), _buf(ws), C.c_size_t(rows),
-                 C.c_size_t(hidden), C.c_size_t(inter), C.c_size_t(stride), _stream())
+    ws = torch.empty(_workspace_bytes(lib, "glmrt_b200_fp8_gated_mlp_workspace", rows, hidden, inter), dtype=torch.uint8, device=x.device)
+    b = launch.buffer
+    launch.call(lib, "glmrt_b200_fp8_gated_mlp_async",
+                _MLP_ARGS.pack(*buf, *b(gate_codes), *b(gate_scales), *b(up_codes), *b(up_scales), *b(down_codes),
+                               *b(down_scales), *b(out), *b(ws), rows, hidden, inter, stride), x.device)
     return out
+
+
+def check(lib: N.NativeLibrary | None = None) -> None:
+    """Waits for the current stream and raises if a product on this device reported a wait that expired."""
+    (lib or N.library()).call("glmrt_b200_fp8_check", C.c_void_p(torch.cuda.current_stream().cuda_stream))

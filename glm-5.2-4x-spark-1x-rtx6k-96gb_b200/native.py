@@ -104,6 +104,25 @@ class BlockNormArgs(C.Structure):
                 + [("dtype", C.c_uint32), ("weight_dtype", C.c_uint32), ("scale", C.c_float), ("eps", C.c_float)])
 
 
+class Fp8QuantizeRowsArgs(C.Structure):
+    """glmrt_b200_fp8_quantize_rows_args_t."""
+    _fields_ = ([(n, DeviceBuffer) for n in ("input", "codes", "scales")]
+                + [(n, C.c_size_t) for n in ("rows", "cols", "input_row_stride")] + [("dtype", C.c_uint32)])
+
+
+class Fp8BlockLinearArgs(C.Structure):
+    """glmrt_b200_fp8_block_linear_args_t."""
+    _fields_ = ([(n, DeviceBuffer) for n in ("x_bf16", "weight_codes", "weight_scales", "output", "workspace")]
+                + [(n, C.c_size_t) for n in ("rows", "n", "k", "x_row_stride")] + [("out_dtype", C.c_uint32)])
+
+
+class Fp8GatedMlpArgs(C.Structure):
+    """glmrt_b200_fp8_gated_mlp_args_t."""
+    _fields_ = ([(n, DeviceBuffer) for n in ("x_bf16", "gate_codes", "gate_scales", "up_codes", "up_scales", "down_codes",
+                                             "down_scales", "output_bf16", "workspace")]
+                + [(n, C.c_size_t) for n in ("rows", "hidden", "inter", "x_row_stride")])
+
+
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
 

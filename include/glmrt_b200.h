@@ -429,27 +429,32 @@ glmrt_status_t glmrt_b200_block_norm_async(const glmrt_b200_block_norm_args_t* a
 /* ------------------------------------------------------------------------ */
 /* bf16 / float32 rows (input_row_stride elements apart) -> codes [rows, cols], scales
  * [ceil(cols/128), rows]. */
-glmrt_status_t glmrt_b200_fp8_quantize_rows_async(glmrt_device_buffer_t input, glmrt_device_buffer_t codes,
-                                                  glmrt_device_buffer_t scales, size_t rows, size_t cols,
-                                                  size_t input_row_stride, uint32_t dtype, void* cuda_stream);
+typedef struct glmrt_b200_fp8_quantize_rows_args_t {
+  glmrt_device_buffer_t input, codes, scales;
+  size_t rows, cols, input_row_stride;
+  uint32_t dtype; /* glmrt_b200_dtype_t of the input */
+} glmrt_b200_fp8_quantize_rows_args_t;
+glmrt_status_t glmrt_b200_fp8_quantize_rows_async(const glmrt_b200_fp8_quantize_rows_args_t* args, void* cuda_stream);
 /* Synchronises the stream and reports whether a bounded wait expired in any 8-bit product on the current
  * device since the last check (its outputs are then not valid). */
 glmrt_status_t glmrt_b200_fp8_check(void* cuda_stream);
 glmrt_status_t glmrt_b200_fp8_block_linear_workspace(size_t rows, size_t n, size_t k, size_t* out_bytes);
 /* output [rows, n] (bf16 or float32) = x [rows, k] weight^T, x quantised in the call. */
-glmrt_status_t glmrt_b200_fp8_block_linear_async(glmrt_device_buffer_t x_bf16, glmrt_device_buffer_t weight_codes,
-                                                 glmrt_device_buffer_t weight_scales, glmrt_device_buffer_t output,
-                                                 glmrt_device_buffer_t workspace, size_t rows, size_t n, size_t k,
-                                                 size_t x_row_stride, uint32_t out_dtype, void* cuda_stream);
+typedef struct glmrt_b200_fp8_block_linear_args_t {
+  glmrt_device_buffer_t x_bf16, weight_codes, weight_scales, output, workspace;
+  size_t rows, n, k, x_row_stride;
+  uint32_t out_dtype; /* glmrt_b200_dtype_t of the output */
+} glmrt_b200_fp8_block_linear_args_t;
+glmrt_status_t glmrt_b200_fp8_block_linear_async(const glmrt_b200_fp8_block_linear_args_t* args, void* cuda_stream);
 glmrt_status_t glmrt_b200_fp8_gated_mlp_workspace(size_t rows, size_t hidden, size_t inter, size_t* out_bytes);
 /* output [rows, hidden] = down (silu(gate x) * (up x)), gate / up [inter, hidden], down [hidden, inter]: the
  * dense shared expert (python/reference/glmrt_reference/moe_ref.py:17-21) in this arithmetic.  The
  * activation between the products is float32 until it is quantised like the rows. */
-glmrt_status_t glmrt_b200_fp8_gated_mlp_async(
-    glmrt_device_buffer_t x_bf16, glmrt_device_buffer_t gate_codes, glmrt_device_buffer_t gate_scales,
-    glmrt_device_buffer_t up_codes, glmrt_device_buffer_t up_scales, glmrt_device_buffer_t down_codes,
-    glmrt_device_buffer_t down_scales, glmrt_device_buffer_t output_bf16, glmrt_device_buffer_t workspace, size_t rows,
-    size_t hidden, size_t inter, size_t x_row_stride, void* cuda_stream);
+typedef struct glmrt_b200_fp8_gated_mlp_args_t {
+  glmrt_device_buffer_t x_bf16, gate_codes, gate_scales, up_codes, up_scales, down_codes, down_scales, output_bf16, workspace;
+  size_t rows, hidden, inter, x_row_stride;
+} glmrt_b200_fp8_gated_mlp_args_t;
+glmrt_status_t glmrt_b200_fp8_gated_mlp_async(const glmrt_b200_fp8_gated_mlp_args_t* args, void* cuda_stream);
 
 /* ------------------------------------------------------------------------ */
 /* Layer-level entry points (additions).                                      */

@@ -73,7 +73,7 @@ def test_fp8_refusals(lib):
 
     def linear(x=buf(0x10000, 1024), c=buf(0x20000, 64 * 128), s=buf(0x30000, 4), o=buf(0x40000, 512), w=ws, rows=4, n=64, k=128,
                stride=128, dtype=0):
-        return lib.call_status("glmrt_b200_fp8_block_linear_async", x, c, s, o, w, Z(rows), Z(n), Z(k), Z(stride), C.c_uint32(dtype), None)
+        return lib.call_status("glmrt_b200_fp8_block_linear_async", C.byref(N.Fp8BlockLinearArgs(x, c, s, o, w, rows, n, k, stride, dtype)), None)
 
     assert linear(rows=0) == 0
     assert linear(dtype=2) == 1 and linear(stride=127) == 1 and linear(k=120) == 1
@@ -85,7 +85,7 @@ def test_fp8_refusals(lib):
     assert linear(c=buf(0x20008, 64 * 128)) == 1 and linear(w=buf(0x100010, need.value)) == 1
 
     def rows(x=buf(0x10000, 1024), c=buf(0x20000, 512), s=buf(0x30000, 16), n=4, cols=128, stride=128, dtype=0):
-        return lib.call_status("glmrt_b200_fp8_quantize_rows_async", x, c, s, Z(n), Z(cols), Z(stride), C.c_uint32(dtype), None)
+        return lib.call_status("glmrt_b200_fp8_quantize_rows_async", C.byref(N.Fp8QuantizeRowsArgs(x, c, s, n, cols, stride, dtype)), None)
 
     assert rows(n=0) == 0 and rows(cols=100) == 1 and rows(dtype=3) == 1 and rows(stride=100) == 1
     assert rows(x=null) == 1 and rows(dtype=1) == 2 and rows(c=buf(0x20000, 511)) == 2 and rows(s=buf(0x30000, 15)) == 2
@@ -99,12 +99,33 @@ def test_fp8_refusals(lib):
 
     def mlp(rows=4, stride=128, **kw):
         b = {**good, **kw}
-        return lib.call_status("glmrt_b200_fp8_gated_mlp_async", *[b[n] for n in names], Z(rows), Z(128), Z(64), Z(stride), None)
+        return lib.call_status("glmrt_b200_fp8_gated_mlp_async", C.byref(N.Fp8GatedMlpArgs(*[b[n] for n in names], rows, 128, 64, stride)), None)
 
     assert mlp(rows=0) == 0 and mlp(stride=64) == 1
     for name in names:
         assert mlp(**{name: null}) == 1, name
         assert mlp(**{name: buf(good[name].ptr, good[name].bytes - 1)}) == 2, name
+
+
+def test_packed_arguments_have_the_layout_of_the_structs(pkg):
+    """The wrappers pack their arguments with struct; the C side reads the structs of the header."""
+    from glmrt_b200 import block_norm, fp8, native as N
+    import ctypes
+    for packer, cls, nbuf in ((block_norm._ARGS, N.BlockNormArgs, 7), (fp8._QUANT_ARGS, N.Fp8QuantizeRowsArgs, 3),
+                              (fp8._LINEAR_ARGS, N.Fp8BlockLinearArgs, 5), (fp8._MLP_ARGS, N.Fp8GatedMlpArgs, 9)):
+        assert packer.size == ctypes.sizeof(cls)
+        values = [0] * (4 * nbuf)
+        for i in range(nbuf):
+            values[4 * i:4 * i + 4] = [1000 + i, 2000 + i, 0, 0]
+        rest = [n for n, _ in cls._fields_[nbuf:]]
+        got = cls.from_buffer_copy(packer.pack(*values, *range(1, len(rest) + 1)))
+        assert [(getattr(got, n).ptr, getattr(got, n).bytes) for n, _ in cls._fields_[:nbuf]] == [(1000 + i, 2000 + i) for i in range(nbuf)]
+        assert [getattr(got, n) for n in rest] == list(range(1, len(rest) + 1))
+
+
+def test_null_argument_structs(lib):
+    for name in ("fp8_quantize_rows", "fp8_block_linear", "fp8_gated_mlp"):
+        assert lib.call_status(f"glmrt_b200_{name}_async", None, None) == 1
 
 
 def test_few_refusals(lib):
