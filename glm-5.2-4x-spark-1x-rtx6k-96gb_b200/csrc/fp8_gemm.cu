@@ -28,7 +28,7 @@ namespace {
 
 using namespace tc;
 
-__device__ uint32_t g_fp8_error;       // kErrWaitTimeout when a bounded wait ran out (glmrt_b200_fp8_check)
+__device__ uint32_t g_fp8_error;       // kErrWaitTimeout when a bounded wait ran out (glmrt_b200_operators_check)
 
 __device__ __forceinline__ void tc_mma_fp8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -776,17 +776,20 @@ glmrt_status_t launch_mode(const Fp8Gemm& g, cudaStream_t s) {
 glmrt_status_t launch_fp8_gemm(const Fp8Gemm& g, int mode, cudaStream_t s) {
   return mode == 0 ? launch_mode<0>(g, s) : mode == 1 ? launch_mode<1>(g, s) : launch_mode<2>(g, s);
 }
+glmrt_status_t fp8_take_error(uint32_t* out) { return take_error_word(g_fp8_error, out); }
 
 }  // namespace glmrt
 
 using namespace glmrt;
 
-extern "C" glmrt_status_t glmrt_b200_fp8_check(void* cuda_stream) {
+extern "C" glmrt_status_t glmrt_b200_operators_check(void* cuda_stream) {
   GLMRT_RETURN_IF_ERROR(require_cuda());
-  uint32_t e = 0, zero = 0;
+  uint32_t fp8 = 0, norm = 0;
   cudaError_t err = cudaStreamSynchronize(static_cast<cudaStream_t>(cuda_stream));
-  if (err == cudaSuccess) err = cudaMemcpyFromSymbol(&e, g_fp8_error, sizeof(e));
-  if (err == cudaSuccess && e != 0) err = cudaMemcpyToSymbol(g_fp8_error, &zero, sizeof(zero));
-  if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "fp8 check", err);
-  return e == 0 ? ok() : fail(GLMRT_STATUS_INTERNAL_ERROR, "device reported: a bounded wait expired in an 8-bit product; its outputs are not valid");
+  if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "operators check", err);
+  GLMRT_RETURN_IF_ERROR(fp8_take_error(&fp8));
+  GLMRT_RETURN_IF_ERROR(norm_take_error(&norm));
+  if ((fp8 | norm) == 0) return ok();
+  return fail(GLMRT_STATUS_INTERNAL_ERROR, std::string("device reported: a bounded wait expired in ") + (fp8 ? "an 8-bit product" : "a block norm") +
+                                               "; its outputs are not valid");
 }

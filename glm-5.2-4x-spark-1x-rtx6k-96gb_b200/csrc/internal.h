@@ -335,4 +335,34 @@ bool few_fused_supported(const FewArgs& a);
 glmrt_status_t launch_few_fused(const FewArgs& a, int sm_count, cudaStream_t stream);
 glmrt_status_t launch_few_simt(const FewArgs& a, cudaStream_t stream);
 
+// ---- error words of the operators without a layer (norm.cu, fp8_gemm.cu) ----
+// A kernel whose bounded wait ran out sets kErrWaitTimeout in its translation unit's word;
+// glmrt_b200_operators_check reads and clears them.
+glmrt_status_t norm_take_error(uint32_t* out);
+glmrt_status_t fp8_take_error(uint32_t* out);
+#ifdef __CUDACC__
+constexpr int kMaxErrorDevices = 64;
+template <typename Symbol>
+glmrt_status_t error_word_of(const Symbol& symbol, uint32_t** out) {
+  static std::atomic<void*> known[kMaxErrorDevices];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  void* p = dev >= 0 && dev < kMaxErrorDevices ? known[dev].load(std::memory_order_relaxed) : nullptr;
+  if (p == nullptr) {
+    cudaError_t err = cudaGetSymbolAddress(&p, symbol);
+    if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_INTERNAL_ERROR, "cudaGetSymbolAddress(error word)", err);
+    if (dev >= 0 && dev < kMaxErrorDevices) known[dev].store(p, std::memory_order_relaxed);
+  }
+  *out = static_cast<uint32_t*>(p);
+  return GLMRT_STATUS_OK;
+}
+template <typename Symbol>
+glmrt_status_t take_error_word(Symbol& symbol, uint32_t* out) {
+  const uint32_t zero = 0;
+  cudaError_t err = cudaMemcpyFromSymbol(out, symbol, sizeof(*out));
+  if (err == cudaSuccess && *out != 0) err = cudaMemcpyToSymbol(symbol, &zero, sizeof(zero));
+  return err == cudaSuccess ? GLMRT_STATUS_OK : fail_cuda(GLMRT_STATUS_COPY_FAILED, "error word", err);
+}
+#endif
+
 }  // namespace glmrt

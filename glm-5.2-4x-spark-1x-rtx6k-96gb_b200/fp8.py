@@ -127,8 +127,3 @@ def gated_mlp(x: torch.Tensor, gate_codes: torch.Tensor, gate_scales: torch.Tens
                 _MLP_ARGS.pack(*buf, *b(gate_codes), *b(gate_scales), *b(up_codes), *b(up_scales), *b(down_codes),
                                *b(down_scales), *b(out), *b(ws), rows, hidden, inter, stride), x.device)
     return out
-
-
-def check(lib: N.NativeLibrary | None = None) -> None:
-    """Waits for the current stream and raises if a product on this device reported a wait that expired."""
-    (lib or N.library()).call("glmrt_b200_fp8_check", C.c_void_p(torch.cuda.current_stream().cuda_stream))

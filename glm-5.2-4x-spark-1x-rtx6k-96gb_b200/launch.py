@@ -34,3 +34,9 @@ def call(lib: N.NativeLibrary | None, symbol: str, packed: bytes, device: torch.
     else:
         with torch.cuda.device(index):
             lib.call(symbol, packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
+
+
+def check(lib: N.NativeLibrary | None = None) -> None:
+    """Waits for the current stream and raises if a block norm or an 8-bit product on this device reported a wait
+    that expired (glmrt_b200_operators_check)."""
+    (lib or N.library()).call("glmrt_b200_operators_check", C.c_void_p(torch.cuda.current_stream().cuda_stream))

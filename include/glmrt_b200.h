@@ -415,6 +415,9 @@ typedef struct glmrt_b200_block_norm_args_t {
   float scale, eps;
 } glmrt_b200_block_norm_args_t;
 glmrt_status_t glmrt_b200_block_norm_async(const glmrt_b200_block_norm_args_t* args, void* cuda_stream);
+/* Synchronises the stream and reports whether a bounded device wait expired in a block norm or an 8-bit
+ * product (below) on the current device since the last check; the outputs of that call are then not valid. */
+glmrt_status_t glmrt_b200_operators_check(void* cuda_stream);
 
 /* ------------------------------------------------------------------------ */
 /* 8-bit floating point products with a scale for each block of 128 (addition). */
@@ -435,9 +438,6 @@ typedef struct glmrt_b200_fp8_quantize_rows_args_t {
   uint32_t dtype; /* glmrt_b200_dtype_t of the input */
 } glmrt_b200_fp8_quantize_rows_args_t;
 glmrt_status_t glmrt_b200_fp8_quantize_rows_async(const glmrt_b200_fp8_quantize_rows_args_t* args, void* cuda_stream);
-/* Synchronises the stream and reports whether a bounded wait expired in any 8-bit product on the current
- * device since the last check (its outputs are then not valid). */
-glmrt_status_t glmrt_b200_fp8_check(void* cuda_stream);
 glmrt_status_t glmrt_b200_fp8_block_linear_workspace(size_t rows, size_t n, size_t k, size_t* out_bytes);
 /* output [rows, n] (bf16 or float32) = x [rows, k] weight^T, x quantised in the call. */
 typedef struct glmrt_b200_fp8_block_linear_args_t {

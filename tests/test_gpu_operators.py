@@ -83,6 +83,27 @@ def test_block_norm_sizes(mods, dtype, wdtype, rows, width):
     assert ro is res
 
 
+@pytest.mark.parametrize("dtype,wdtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                          (torch.float32, torch.bfloat16), (torch.float32, torch.float32)])
+@pytest.mark.parametrize("rows,width", [(2368, 512), (2371, 520), (2500, 1032), (4737, 256), (2400, 4096), (2368, 8192), (3001, 6144)])
+def test_block_norm_many_rows(mods, dtype, wdtype, rows, width):
+    """The streaming form (rows in a ring of shared memory) at its borders, with every term and in place."""
+    res, delta = randn(1, rows, width, std=2.0, dtype=dtype), randn(2, rows, width, dtype=dtype)
+    nw, pw = (1 + randn(3, width, std=0.1)).to(wdtype), (1 + randn(4, width, std=0.1)).to(wdtype)
+    want = check_norm(mods, res, delta, nw)
+    check_norm(mods, res, delta, nw, pw, randn(5, 1, width, dtype=dtype), 0.25)
+    check_norm(mods, res, delta, nw, None, randn(6, rows, 1, dtype=dtype), -1.5)
+    check_norm(mods, res, delta, nw, pw, randn(7, rows, width, dtype=dtype), 1.0, eps=0.1)
+    check_norm(mods, res, None, nw)
+    r2, d2 = res.clone(), delta.clone()
+    got = mods["block_norm"].block_norm(r2, d2, norm_weight=nw, residual_out=r2, normalized=d2)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    pad = torch.nn.functional.pad(res, (0, 16))
+    out = torch.full((rows, width + 8), 7.0, device="cuda", dtype=dtype)
+    got = mods["block_norm"].block_norm(pad[:, :width], delta, norm_weight=nw, normalized=out[:, :width])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and (out[:, width:] == 7).all()
+
+
 def test_block_norm_strides_and_alignment(mods):
     """Padded rows, rows that start off a 16-byte boundary, an expanded gate."""
     rows, width = 9, 520
