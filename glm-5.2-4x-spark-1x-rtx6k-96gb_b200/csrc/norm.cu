@@ -192,13 +192,13 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(NormArgs a) {
   }
 }
 
-// Many rows: a CTA takes every gridDim-th row; bulk copies bring the next rows into a ring in shared memory while
-// one is worked on, and the weights stay in registers.  A row of the kernel above waits for its own loads, then for
-// the weights' (measured at 8192 x 6144 bf16: 98 us, or 87 with half the values a thread; here 4 streams of 100 MB
-// at the copy rate are 61).  Rows whose pieces are 16 bytes, aligned.
-template <typename T, typename W, int kNv>
+// Many wide bf16 rows: a CTA takes every gridDim-th row; bulk copies bring the next rows into a ring in shared
+// memory while one is worked on, and the weights stay in registers (8192 x 6144: 71 us; four streams of 100 MB at the
+// copy rate are 61).  Rows whose pieces are 16 bytes, aligned; two pieces a thread.
+template <typename W>
 __global__ void __launch_bounds__(512, 2) block_norm_stream_kernel(NormArgs a, int stages, uint32_t row_bytes, uint32_t* error_word) {
-  constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kPer = 16 / static_cast<int>(sizeof(W));
+  using T = uint16_t;
+  constexpr int kVec = 8, kNv = 2, kPer = 16 / static_cast<int>(sizeof(W));
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float scratch[32];
   __shared__ uint64_t full[8];
@@ -229,17 +229,12 @@ __global__ void __launch_bounds__(512, 2) block_norm_stream_kernel(NormArgs a, i
     }
   const float inv_width = 1.0f / static_cast<float>(a.width);
   auto column = [&](int n) { return (n * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * kVec; };
-  uint4 norm_w[kNv][kVec / kPer > 0 ? kVec / kPer : 1], post_w[kNv][kVec / kPer > 0 ? kVec / kPer : 1];
-  auto take = [&](const void* w, uint4 (&q)[kVec / kPer > 0 ? kVec / kPer : 1], int c) {
-    if constexpr (kVec >= kPer) {
+  uint4 norm_w[kNv][kVec / kPer], post_w[kNv][kVec / kPer];
+  auto take = [&](const void* w, uint4 (&q)[kVec / kPer], int c) {
 #pragma unroll
-      for (int i = 0; i < kVec / kPer; ++i) q[i] = *reinterpret_cast<const uint4*>(static_cast<const W*>(w) + c + i * kPer);
-    } else {                                            // float32 rows, bf16 weights: four of them are 8 bytes
-      const uint2 h = *reinterpret_cast<const uint2*>(static_cast<const W*>(w) + c);
-      q[0] = make_uint4(h.x, h.y, 0u, 0u);
-    }
+    for (int i = 0; i < kVec / kPer; ++i) q[i] = *reinterpret_cast<const uint4*>(static_cast<const W*>(w) + c + i * kPer);
   };
-  auto weight_at = [&](const uint4 (&q)[kVec / kPer > 0 ? kVec / kPer : 1], int i) { return to_f32(reinterpret_cast<const W*>(&q[i / kPer])[i % kPer]); };
+  auto weight_at = [&](const uint4 (&q)[kVec / kPer], int i) { return to_f32(reinterpret_cast<const W*>(&q[i / kPer])[i % kPer]); };
 #pragma unroll
   for (int n = 0; n < kNv; ++n)
     if (column(n) < a.width) {
@@ -338,14 +333,14 @@ void launch(const NormArgs& a, int threads, cudaStream_t s) {
 
 constexpr int kStreamRing = 104 * 1024;       // a CTA's rows in shared memory, two CTAs on an SM
 
-template <typename T, typename W, int kNv>
+template <typename W>
 glmrt_status_t launch_stream(const NormArgs& a, int stages, uint32_t row_bytes, int ctas, cudaStream_t s) {
   static std::atomic<uint64_t> configured{0};
-  GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, block_norm_stream_kernel<T, W, kNv>, kStreamRing, "cudaFuncSetAttribute(block_norm_stream_kernel)"));
+  GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, block_norm_stream_kernel<W>, kStreamRing, "cudaFuncSetAttribute(block_norm_stream_kernel)"));
   uint32_t* error_word = nullptr;
   GLMRT_RETURN_IF_ERROR(error_word_of(g_norm_error, &error_word));
-  const int pieces = a.width / (16 / static_cast<int>(sizeof(T)));
-  launch_pdl(block_norm_stream_kernel<T, W, kNv>, dim3(static_cast<unsigned>(ctas)), dim3(static_cast<unsigned>(((pieces + kNv - 1) / kNv + 31) / 32 * 32)),
+  const int pieces = a.width / 8;
+  launch_pdl(block_norm_stream_kernel<W>, dim3(static_cast<unsigned>(ctas)), dim3(static_cast<unsigned>(((pieces + 1) / 2 + 31) / 32 * 32)),
              static_cast<size_t>(stages) * row_bytes * (a.delta != nullptr ? 2 : 1), s, a, stages, row_bytes, error_word);
   return GLMRT_STATUS_OK;
 }
@@ -354,13 +349,13 @@ template <typename T, typename W, int kVec>
 glmrt_status_t dispatch(const NormArgs& a, cudaStream_t s) {
   const int pieces = (a.width + kVec - 1) / kVec;
   constexpr int kMost = 32 / kVec;            // accesses per thread at 32 values
-  if constexpr (kVec > 1) {
-    // Eight rows and more for each of the 296 CTAs, of a width that keeps two warps to 512 threads busy and two
-    // rows or more in the ring.
+  if constexpr (kVec == 8) {
+    // bf16 rows of 8 to 16 KB, at least four for each of the 296 CTAs: the kernel above holds 16 values a thread there
+    // and too few rows on an SM (measured, rows x width: 1200 x 6144 13.8 against 15.4 us, 8192 x 6144 71 / 87,
+    // 8192 x 8192 93 / 127, 8192 x 4096 55 / 62; but 8192 x 2048 47 / 30, and float32 8192 x 4096 90 / 80).
     const uint32_t row_bytes = static_cast<uint32_t>(a.width) * sizeof(T);
     const int ctas = 2 * 148, stages = std::min<int>(8, kStreamRing / (row_bytes * (a.delta != nullptr ? 2 : 1)));
-    if (a.rows >= 8 * ctas && stages >= 2 && pieces >= 64 && pieces <= 2 * 512)
-      return pieces <= 128 ? launch_stream<T, W, 1>(a, stages, row_bytes, ctas, s) : launch_stream<T, W, 2>(a, stages, row_bytes, ctas, s);
+    if (a.rows >= 4 * ctas && pieces >= 512 && pieces <= 1024) return launch_stream<W>(a, stages, row_bytes, ctas, s);
   }
   // A few rows: as many threads per row as it has pieces, for the latency.  More rows than SMs: two pieces a thread,
   // so that several rows share an SM and their loads overlap each other's reductions (measured at 333 x 5120 bf16
