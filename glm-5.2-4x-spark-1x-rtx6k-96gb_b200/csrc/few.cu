@@ -58,6 +58,8 @@ constexpr int kBufs = kSumWarps;             // items whose partial sums may be 
 constexpr int kSlotBytes = 2560;             // per warp: two pieces of two 16-byte codes and 8 scale bytes a lane
 constexpr int kMaxEntries = 256;             // (expert, token group) pairs: at most one per route
 constexpr int kMaxRoutes = 256;
+constexpr int kLogitExperts = 2;             // experts a CTA scores at a time, by kLogitShares warps each
+constexpr int kLogitShares = kThreads / 32 / kLogitExperts;
 constexpr uint64_t kBarrierLimitNs = 2000000000ull;
 
 struct FewShared {
@@ -66,9 +68,12 @@ struct FewShared {
   float ent_w[kMaxEntries][8];               // column -> weight
   uint32_t route_expert[kMaxRoutes];
   float route_w[kMaxRoutes];
+  uint8_t route_token[kMaxRoutes];
   uint32_t used[kFewMaxRows];                // slots of a token that own a result row
   uint32_t act_amax[kWarps][8];              // by warp along K and column
   uint32_t x_amax[kFewMaxRows];
+  float x_inv[kFewMaxRows];                  // undoes the power of two of a row
+  float logit_part[kLogitExperts][kLogitShares][kFewMaxRows];
   uint64_t full[kBufs], empty[kBufs];
   int warp_count[kThreads / 32];
   int entries, distinct, bad;
@@ -104,8 +109,12 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ void e4m3x2_to_pairs(uint32_t two, uint32_t& lo, uint32_t& hi) {
   uint32_t h;
   asm("{\n\t.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(h) : "r"(two));
-  lo = __byte_perm(h, 0, 0x1010);
-  hi = __byte_perm(h, 0, 0x3232);
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tmov.b32 %0, {a, a};\n\tmov.b32 %1, {b, b};\n\t}" : "=r"(lo), "=r"(hi) : "r"(h));
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+  return v;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -115,21 +124,21 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// All CTAs of the grid (co-resident: cooperative launch).  The count only grows, by the grid's size at
-// each barrier, so an arrival's own value tells which multiple to wait for and nothing has to be
-// reset (64 bits: 32 would run over within minutes).  False when the wait ran out.
-__device__ bool grid_barrier(unsigned long long* count, volatile uint32_t* abort) {
+// All CTAs of the grid (co-resident: cooperative launch).  The arrivals of one barrier add up to 2^31: every CTA
+// adds one, the first what is missing.  So the top bit flips when the last has come, and nothing has to be
+// reset.  False when the wait ran out.
+__device__ bool grid_barrier(uint32_t* count, volatile uint32_t* abort) {
   __syncthreads();
   if (threadIdx.x == 0) {
-    unsigned long long old, now;
-    asm volatile("atom.add.acq_rel.gpu.global.u64 %0, [%1], %2;" : "=l"(old) : "l"(count), "l"(1ull) : "memory");
-    const unsigned long long target = (old / gridDim.x + 1) * gridDim.x;
-    uint64_t t0 = 0, t;
-    for (uint32_t spin = 0;; ++spin) {
-      asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(count) : "memory");
-      if (now >= target) break;
-      if ((spin & 255u) == 255u) {
-        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    const uint32_t add = blockIdx.x == 0 ? 0x80000000u - (gridDim.x - 1) : 1u;
+    uint32_t old, now;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(old) : "l"(count), "r"(add) : "memory");
+    uint64_t t0 = 0;
+    for (uint32_t spin = 1;; ++spin) {
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(count) : "memory");
+      if ((old ^ now) >> 31) break;
+      if ((spin & 255u) == 0u) {
+        const uint64_t t = tc::global_timer_ns();
         if (t0 == 0) t0 = t;
         else if (t - t0 > kBarrierLimitNs) { *abort = 1u; break; }
       }
@@ -139,72 +148,69 @@ __device__ bool grid_barrier(unsigned long long* count, volatile uint32_t* abort
   return *abort == 0u;
 }
 
-// One of the two weight passes: which rows, and how the CTA's warps share an item of them.  The split
-// follows from the shape alone, so that a row's sums do not depend on its batch.
-struct Pass {
-  int units;            // 128-column units of K
-  int kw, rw;           // warps along K, warps along the rows (kw * rw = kWarps)
-  int per_entry;        // items (rw row groups: 16 rows of gate and up, 32 rows of down) per entry
-  int begin, end;       // this CTA's items
-};
-__device__ __forceinline__ Pass make_pass(int k, int groups, int entries) {
-  Pass p;
-  p.units = k / 128;
-  p.kw = kWarps;
-  while (p.kw > 2 && p.kw * 2 > p.units) p.kw /= 2;      // two units a warp or more, so that handing a sum over is rare
-  p.rw = kWarps / p.kw;
-  p.per_entry = groups / p.rw;
+// A CTA's share of one of the two weight passes.  How an item of rows is shared by the warps (FewPass: kw along K,
+// rw along the rows) follows from the shape alone, so that a row's sums do not depend on its batch.
+struct Share { int begin, end, entry, first; };        // items, and the first one's entry and place in it
+__device__ __forceinline__ Share share_of(const FewPass& p, int entries) {
   const uint32_t items = static_cast<uint32_t>(entries) * p.per_entry;    // items * grid < 2^32 (few_fused_supported)
-  p.begin = static_cast<int>(items * blockIdx.x / gridDim.x);
-  p.end = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
-  return p;
+  Share s;
+  s.begin = static_cast<int>(items * blockIdx.x / gridDim.x);
+  s.end = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
+  s.entry = s.begin / p.per_entry;
+  s.first = s.begin - s.entry * p.per_entry;
+  return s;
 }
 // First row of a row unit: rows R .. R+7 and R+32 .. R+39 of a 128-row scale tile, whose scales lie
 // next to each other in pairs (sf_tile_offset).  Units 2v and 2v+1 are 8 rows apart.
 __device__ __forceinline__ int unit_row(int u) { return (u >> 3) * 128 + ((u >> 2) & 1) * 64 + (u & 3) * 8; }
 
-// The warp's stream of slots: its K units of each item in turn, through both passes.
+// The warp's stream of slots: its K units of each item in turn, through both passes.  Everything but the two lane
+// offsets is the same for the whole warp.
 struct Stream {
-  const uint8_t *codes, *sf;          // of the next slot, this lane's
-  const uint8_t *codes0, *sf0;        // of the pass, this lane's share of the address included
+  const uint8_t *codes, *sf;          // of the next slot
+  const uint8_t *codes0, *sf0;        // of the pass, at this warp's first unit
   size_t second, sf_second;           // from a slot's first piece to its second
+  uint32_t lane_codes, lane_low, lane_sf;      // this lane's place in a piece: rows g and g + 32, scales
   int row_bytes, rows, units, kw, kwi, rw, rwi, per_entry, shift;
   int k, u, j, left;                  // K unit, item within its entry, entry, items left (0: nothing more)
-  uint32_t ring, head, ring_bytes;
+  uint32_t ring, head, ring_end;      // shared addresses, this lane's 16 bytes included
 
-  __device__ __forceinline__ void begin_pass(const FewArgs& a, const FewShared& sh, const Pass& p, bool gate_up, int warp, int lane) {
+  __device__ __forceinline__ void begin_pass(const FewArgs& a, const FewShared& sh, const FewPass& p, const Share& s, bool gate_up,
+                                             int warp, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    units = p.units; kw = p.kw; rw = p.rw; per_entry = p.per_entry;
-    kwi = warp % kw; rwi = warp / kw;
+    units = p.units; kw = p.kw; rw = kWarps / p.kw; per_entry = p.per_entry;
+    kwi = warp & (kw - 1); rwi = warp >> p.log_kw;
     shift = gate_up ? 0 : 1;
     row_bytes = (gate_up ? a.hidden : a.inter) / 2;
     rows = gate_up ? a.inter : a.hidden;
     second = gate_up ? static_cast<size_t>(a.up_codes - a.gate_codes) : static_cast<size_t>(8) * row_bytes;
     sf_second = gate_up ? static_cast<size_t>(a.up_sf - a.gate_sf) : 128;
-    codes0 = (gate_up ? a.gate_codes : a.down_codes) + static_cast<size_t>(g) * row_bytes + kwi * 64 + t * 16;
-    sf0 = (gate_up ? a.gate_sf : a.down_sf) + (kwi * 2 + (t >> 1)) * 512 + g * 16;
-    left = kwi < units ? p.end - p.begin : 0;
-    j = p.begin / per_entry;
-    u = p.begin - j * per_entry;
+    lane_codes = static_cast<uint32_t>(g) * row_bytes + t * 16;
+    lane_low = lane_codes + 32u * row_bytes;
+    lane_sf = (t >> 1) * 512 + g * 16;
+    codes0 = (gate_up ? a.gate_codes : a.down_codes) + kwi * 64;
+    sf0 = (gate_up ? a.gate_sf : a.down_sf) + kwi * 1024;
+    left = kwi < units ? s.end - s.begin : 0;
+    j = s.entry;
+    u = s.first;
     if (left > 0) open(sh);
   }
   __device__ __forceinline__ void open(const FewShared& sh) {
     const int unit = (u * rw + rwi) << shift;
-    const uint32_t row = sh.ent_expert[j] * static_cast<uint32_t>(rows) + unit_row(unit);     // < 2^32: experts * rows
+    const uint32_t expert = __shfl_sync(0xffffffffu, static_cast<uint32_t>(sh.ent_expert[j]), 0);
+    const uint32_t row = expert * static_cast<uint32_t>(rows) + unit_row(unit);     // < 2^32: experts * rows
     codes = codes0 + static_cast<size_t>(row) * row_bytes;
     sf = sf0 + static_cast<size_t>(row >> 7) * (row_bytes >> 5) * 512 + (unit & 3) * 128 + ((unit >> 2) & 1) * 8;
     k = kwi;
   }
   __device__ __forceinline__ void issue(const FewShared& sh, int lane) {
     if (left > 0) {
-      const uint32_t dst = ring + head + lane * 16, dsf = ring + head + 2048 + lane * 8;
-      const size_t low = static_cast<size_t>(32) * row_bytes;
-      cp_async16(dst, codes);
-      cp_async16(dst + 512, codes + low);
-      cp_async16(dst + 1024, codes + second);
-      cp_async16(dst + 1536, codes + second + low);
-      cp_async8(dsf, sf);
-      cp_async8(dsf + 256, sf + sf_second);
+      cp_async16(head, codes + lane_codes);
+      cp_async16(head + 512, codes + lane_low);
+      cp_async16(head + 1024, codes + second + lane_codes);
+      cp_async16(head + 1536, codes + second + lane_low);
+      cp_async8(head + 2048 - lane * 8, sf + lane_sf);
+      cp_async8(head + 2304 - lane * 8, sf + sf_second + lane_sf);
       k += kw;
       codes += kw * 64;
       sf += kw * 1024;
@@ -213,7 +219,8 @@ struct Stream {
         open(sh);
       }
     }
-    head = head + kSlotBytes == ring_bytes ? 0 : head + kSlotBytes;
+    head += kSlotBytes;
+    if (head == ring_end) head = ring;
     cp_async_commit();        // one group per call, also when nothing is left: the count of pending groups stays exact
   }
 };
@@ -221,21 +228,16 @@ struct Stream {
 __device__ __forceinline__ void lds128(uint32_t (&v)[4], uint32_t at) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
 }
-// acc[m] += piece m's 16 x 128 weights times the unit's columns; the two pieces' chains of
-// products run side by side.
-__device__ __forceinline__ void multiply_slot(float (&acc)[2][4], uint32_t slot, const uint32_t (&b)[16], int lane) {
+// acc[m] += piece m's 16 x 128 weights times the unit's columns; the two pieces' chains of products run side by
+// side.  `slot`: shared address of the slot, this lane's 16 bytes included; `scales`: of this lane's two scale bytes
+// of piece 0, row g (row g + 32: 4 further, piece 1: 256).
+__device__ __forceinline__ void multiply_slot(float (&acc)[2][4], uint32_t slot, uint32_t scales, const uint32_t (&b)[16]) {
   uint32_t w[4][4];           // piece 0 rows g, g + 32; piece 1 the same
   uint32_t scale[4][2];       // of the lane's two blocks in each
 #pragma unroll
-  for (int i = 0; i < 4; ++i) lds128(w[i], slot + i * 512 + lane * 16);
-  const int shift = (lane & 1) * 16;
+  for (int i = 0; i < 4; ++i) lds128(w[i], slot + i * 512);
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    uint32_t s0, s1;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(s0), "=r"(s1) : "r"(slot + 2048 + m * 256 + lane * 8));
-    e4m3x2_to_pairs(s0 >> shift, scale[2 * m][0], scale[2 * m][1]);
-    e4m3x2_to_pairs(s1 >> shift, scale[2 * m + 1][0], scale[2 * m + 1][1]);
-  }
+  for (int i = 0; i < 4; ++i) e4m3x2_to_pairs(lds_u16(scales + (i >> 1) * 256 + (i & 1) * 4), scale[i][0], scale[i][1]);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -280,7 +282,7 @@ __device__ void load_hidden_columns(const FewArgs& a, const FewShared& sh, uint8
     if (!identity) {
       const int route = sh.ent_route[entry][c];
       if (route < 0) continue;           // nobody reads the column's results
-      tok = route / a.top_k;
+      tok = sh.route_token[route];
     }
     float inv;
     const float f = f16_factor(sh.x_amax[tok], &inv);
@@ -376,73 +378,64 @@ __device__ __forceinline__ void store_partial(float* red, const float (&acc)[2][
 
 // Top-k of one row by one warp: keys order like (score + bias, lower id first); a NaN ranks last.
 template <int kKeys>
-__device__ __forceinline__ void select_row(const FewArgs& a, FewShared& sh, const float* score, int row, int lane) {
+__device__ __forceinline__ void select_row(const FewArgs& a, FewShared& sh, int row, int lane) {
   uint32_t key[kKeys];
+  float score[kKeys];
+#pragma unroll
+  for (int i = 0; i < kKeys; ++i) score[i] = lane + 32 * i < a.experts ? __ldcg(a.logits + row * a.experts + lane + 32 * i) : 0.0f;
 #pragma unroll
   for (int i = 0; i < kKeys; ++i) {
-    const int e = lane + 32 * i;
     key[i] = 0u;
-    if (e < a.experts) {
-      const float s = score[e] + __ldg(a.router_b + e);
+    score[i] = sigmoid_f32(score[i]);
+    if (lane + 32 * i < a.experts) {
+      const float s = score[i] + __ldg(a.router_b + lane + 32 * i);
       const uint32_t u = __float_as_uint(s == 0.0f ? 0.0f : s);
       key[i] = s != s ? 1u : ((u >> 31) ? ~u : u | 0x80000000u);
     }
   }
-  float sum = 0.0f;
+  float sum = 0.0f, my_score = 0.0f;
   uint32_t mine = 0;
+#pragma unroll 1
   for (int s = 0; s < a.top_k; ++s) {
     uint32_t best = key[0];
+    float best_score = score[0];
     int at = 0;
 #pragma unroll
     for (int i = 1; i < kKeys; ++i)
-      if (key[i] > best) { best = key[i]; at = i; }              // the first of equal ones: the lower id
+      if (key[i] > best) { best = key[i]; best_score = score[i]; at = i; }       // the first of equal ones: the lower id
     const uint32_t top = __reduce_max_sync(0xffffffffu, best);
     const uint32_t id = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(lane + 32 * at) : 0xffffffffu);
+    const float chosen = __shfl_sync(0xffffffffu, best_score, id & 31);
 #pragma unroll
     for (int i = 0; i < kKeys; ++i)
       if (lane + 32 * i == static_cast<int>(id)) key[i] = 0u;
-    sum += score[id];
-    if (lane == s) mine = id;
+    sum += chosen;
+    if (lane == s) { mine = id; my_score = chosen; }
   }
-  const float inv = a.scaling / fmaxf(sum, 1e-12f);
   if (lane < a.top_k) {
     const int r = row * a.top_k + lane;
     sh.route_expert[r] = mine;
-    sh.route_w[r] = score[mine] * inv;
+    sh.route_w[r] = my_score * (a.scaling / fmaxf(sum, 1e-12f));
   }
 }
 
-// Routes of all rows, then the list of entries (sh.ent_*).  `scratch`: rows * experts floats, and for
-// every expert a word and 16 half-words.
+// Routes of all rows, then the list of entries (sh.ent_*).  `scratch`: for every expert a word and 16 half-words.
 __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scratch, int cap, bool identity) {
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int routes = a.rows * a.top_k;
   uint32_t* mask = reinterpret_cast<uint32_t*>(scratch);                            // rows that name an expert
   uint16_t* entry_of = reinterpret_cast<uint16_t*>(mask + a.experts);               // [expert][16]
-  float* scores = reinterpret_cast<float*>(entry_of + a.experts * 16);
   for (int i = tid; i < a.experts; i += kThreads) mask[i] = 0u;
-  for (int i = tid; i < kMaxEntries * 8; i += kThreads) {
+  for (int i = tid; i < routes * 8; i += kThreads) {        // at most one entry per route
     sh.ent_route[i >> 3][i & 7] = -1;
     sh.ent_w[i >> 3][i & 7] = 0.0f;
   }
   if (tid < kFewMaxRows) sh.used[tid] = 0u;
   if (tid == 0) { sh.bad = 0; sh.distinct = 0; }
   if (a.logits != nullptr) {
-    // scores of all rows, the column shares added in order
-    const int n = a.rows * a.experts;
-    for (int i = tid; i < n; i += kThreads) {
-      float part[kFewMaxSplits];
-#pragma unroll
-      for (int p = 0; p < kFewMaxSplits; ++p) part[p] = p < a.splits ? __ldcg(a.logits + static_cast<size_t>(p) * n + i) : 0.0f;
-      float s = part[0];
-#pragma unroll
-      for (int p = 1; p < kFewMaxSplits; ++p) s += part[p];
-      scores[i] = sigmoid_f32(s);
-    }
-    __syncthreads();
     if (warp < a.rows) {
-      if (a.experts <= 256) select_row<8>(a, sh, scores + warp * a.experts, warp, lane);
-      else select_row<32>(a, sh, scores + warp * a.experts, warp, lane);
+      if (a.experts <= 256) select_row<8>(a, sh, warp, lane);
+      else select_row<32>(a, sh, warp, lane);
     }
   } else if (tid < routes) {
     sh.route_expert[tid] = a.topk_idx[tid];
@@ -459,6 +452,7 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
     e = sh.route_expert[tid];
     w = sh.route_w[tid];
     token = tid / a.top_k; slot = tid - token * a.top_k;
+    sh.route_token[tid] = static_cast<uint8_t>(token);
     live = e < static_cast<uint32_t>(a.experts);
     if (!live && e != kNoRoute) sh.bad = 1;
     const uint32_t* row = sh.route_expert + token * a.top_k;
@@ -504,11 +498,67 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
   __syncthreads();
 }
 
+// Logits of all rows, kLogitExperts experts of this CTA at a time: every warp one expert and one share of the
+// columns, the shares added in order.  (Complete logits in one place: adding partial ones from every CTA would cost
+// the selection an access to the L2 each.)
+__device__ void score_experts(const FewArgs& a, FewShared& sh, int warp, int lane) {
+  const int half = warp / kLogitShares, share = warp - half * kLogitShares, units = a.hidden / 128;
+  const int u0 = units * share / kLogitShares, u1 = units * (share + 1) / kLogitShares;
+#pragma unroll 1
+  for (int e0 = blockIdx.x; e0 < a.experts; e0 += kLogitExperts * gridDim.x) {
+    const int e = e0 + half * gridDim.x;
+    const float* wrow = a.router_w + static_cast<size_t>(e) * a.hidden + lane * 4;
+#pragma unroll 1
+    for (int t0 = 0; t0 < a.rows && e < a.experts; t0 += 4) {
+      const uint16_t* xrow = a.hidden_rows + static_cast<size_t>(t0) * a.hidden + lane * 4;
+      float acc[4] = {};
+#pragma unroll 1
+      for (int ub = u0; ub < u1; ub += 5) {            // five units of four rows in flight
+        float4 w[5];
+        uint2 x[4][5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          const bool in = ub + i < u1;
+          w[i] = in ? __ldg(reinterpret_cast<const float4*>(wrow + (ub + i) * 128)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            x[t][i] = in && t0 + t < a.rows ? __ldg(reinterpret_cast<const uint2*>(xrow + static_cast<size_t>(t) * a.hidden + (ub + i) * 128))
+                                            : make_uint2(0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            if (ub + i >= u1) continue;                // (zero times a weight that is not finite)
+            acc[t] = fmaf(__uint_as_float(x[t][i].x << 16), w[i].x, acc[t]);
+            acc[t] = fmaf(__uint_as_float(x[t][i].x & 0xffff0000u), w[i].y, acc[t]);
+            acc[t] = fmaf(__uint_as_float(x[t][i].y << 16), w[i].z, acc[t]);
+            acc[t] = fmaf(__uint_as_float(x[t][i].y & 0xffff0000u), w[i].w, acc[t]);
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float s = warp_sum(acc[t]);
+        if (lane == 0) sh.logit_part[half][share][t0 + t] = s;
+      }
+    }
+    __syncthreads();
+    const int h = threadIdx.x / kFewMaxRows, t = threadIdx.x % kFewMaxRows;
+    if (h < kLogitExperts && t < a.rows && e0 + h * static_cast<int>(gridDim.x) < a.experts) {
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kLogitShares; ++i) s += sh.logit_part[h][i][t];
+      a.logits[t * a.experts + e0 + h * gridDim.x] = s;
+    }
+    __syncthreads();
+  }
+}
+
 template <int kRing>
 __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int cap) {
   extern __shared__ __align__(128) uint8_t smem[];
   FewShared& sh = *reinterpret_cast<FewShared*>(smem);
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
   const bool identity = a.rows <= cap;
   const int cols = identity ? a.rows : cap;
   const int log_pitch = cols > 4 ? 3 : cols > 2 ? 2 : cols - 1, pitch = 1 << log_pitch;
@@ -526,64 +576,21 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
   if (tid < kFewMaxRows) sh.x_amax[tid] = 0u;
   __syncthreads();
 
-  // ---- logits: task = (column share, expert), one warp each ----
-  if (a.logits != nullptr) {
-    const int units = a.hidden / 128, n = a.rows * a.experts;
-    for (int task = blockIdx.x * (kThreads / 32) + warp; task < a.splits * a.experts; task += gridDim.x * (kThreads / 32)) {
-      const int p = task / a.experts, e = task - p * a.experts;
-      const int u0 = units * p / a.splits, u1 = units * (p + 1) / a.splits;
-      const float* wrow = a.router_w + static_cast<size_t>(e) * a.hidden + lane * 4;
-      const uint16_t* xrow = a.hidden_rows + lane * 4;
-      float acc[kFewMaxRows];
-#pragma unroll
-      for (int t = 0; t < kFewMaxRows; ++t) acc[t] = 0.0f;
-      for (int ub = u0; ub < u1; ub += 4) {            // four units and four rows of loads in flight
-        float4 wv[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          wv[i] = ub + i < u1 ? __ldg(reinterpret_cast<const float4*>(wrow + (ub + i) * 128)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int tb = 0; tb < kFewMaxRows; tb += 4) {
-          if (tb >= a.rows) break;
-          uint2 x[4][4];
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (tb + t < a.rows && ub + i < u1)
-                x[t][i] = __ldg(reinterpret_cast<const uint2*>(xrow + static_cast<size_t>(tb + t) * a.hidden + (ub + i) * 128));
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (tb + t < a.rows && ub + i < u1) {
-                acc[tb + t] = fmaf(__uint_as_float(x[t][i].x << 16), wv[i].x, acc[tb + t]);
-                acc[tb + t] = fmaf(__uint_as_float(x[t][i].x & 0xffff0000u), wv[i].y, acc[tb + t]);
-                acc[tb + t] = fmaf(__uint_as_float(x[t][i].y << 16), wv[i].z, acc[tb + t]);
-                acc[tb + t] = fmaf(__uint_as_float(x[t][i].y & 0xffff0000u), wv[i].w, acc[tb + t]);
-              }
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < kFewMaxRows; ++t) {
-        if (t >= a.rows) break;
-        const float s = warp_sum(acc[t]);
-        if (lane == 0) a.logits[static_cast<size_t>(p) * n + t * a.experts + e] = s;
-      }
-    }
-  }
+  if (a.logits != nullptr) score_experts(a, sh, warp, lane);
   // the rows' largest magnitudes, 256 values a warp
-  for (int i = warp; i < a.rows * (a.hidden / 256); i += kThreads / 32) {
-    const int t = i / (a.hidden / 256);
+  const int row_pieces = a.hidden / 256;
+#pragma unroll 1
+  for (int i = warp; i < a.rows * row_pieces; i += kThreads / 32) {
     const uint4 q = *reinterpret_cast<const uint4*>(a.hidden_rows + static_cast<size_t>(i) * 256 + lane * 8);
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
     uint32_t m = 0;
 #pragma unroll
     for (int v = 0; v < 4; ++v) m = max(m, max((w[v] << 16) & 0x7fffffffu, w[v] & 0x7fff0000u));
     m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) atomicMax(&sh.x_amax[t], m);
+    if (lane == 0) atomicMax(&sh.x_amax[i / row_pieces], m);
   }
   __syncthreads();
+  if (tid < a.rows) f16_factor(sh.x_amax[tid], &sh.x_inv[tid]);
   if (identity && warp < kWarps) load_hidden_columns(a, sh, columns, 0, cols, true);    // needs no routes
   if (a.logits != nullptr) {
     if (!grid_barrier(a.sync, &sh.abort)) {
@@ -592,26 +599,25 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
     }
   }
   route_and_select(a, sh, ring, cap, identity);
+  const int entries = __shfl_sync(0xffffffffu, sh.entries, 0);
   if (blockIdx.x == 0 && tid == 0) {
     a.error_word[0] = sh.bad ? static_cast<uint32_t>(kErrBadExpert) : 0u;
-    a.counters[kCntChunks] = static_cast<uint32_t>(sh.entries);
+    a.counters[kCntChunks] = static_cast<uint32_t>(entries);
     a.counters[kCntDistinct] = static_cast<uint32_t>(sh.distinct);
   }
 
-  const Pass p1 = make_pass(a.hidden, a.inter / 16, sh.entries), p2 = make_pass(a.inter, a.hidden / 32, sh.entries);
-  int n = 0;                     // items so far: buffer n % kBufs, its round n / kBufs
-  bool alive = true;
+  const Share s1 = share_of(a.pass[0], entries), s2 = share_of(a.pass[1], entries);
   if (warp < kWarps) {
-    // ---- the multiplying warps: the weight stream, gate and up ----
+    // ---- the multiplying warps: the weight stream, then gate and up (pass 0) and down (pass 1) ----
     Stream st;
-    st.ring = smem_addr(ring) + warp * kRing * kSlotBytes;
-    st.ring_bytes = kRing * kSlotBytes;
-    st.head = 0;
-    st.begin_pass(a, sh, p1, true, warp, lane);
+    st.ring = smem_addr(ring) + warp * kRing * kSlotBytes + lane * 16;
+    st.ring_end = st.ring + kRing * kSlotBytes;
+    st.head = st.ring;
+    st.begin_pass(a, sh, a.pass[0], s1, true, warp, lane);
     bool first_pass = true;
     auto issue = [&] {
       if (st.left == 0 && first_pass) {
-        st.begin_pass(a, sh, p2, false, warp, lane);
+        st.begin_pass(a, sh, a.pass[1], s2, false, warp, lane);
         first_pass = false;
       }
       st.issue(sh, lane);
@@ -619,123 +625,104 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
 #pragma unroll 1
     for (int i = 0; i < kRing - 1; ++i) issue();
     uint32_t tail = st.ring;
-    const uint32_t ring_end = st.ring + st.ring_bytes;
     const uint32_t lane_columns = smem_addr(columns) + (min(lane >> 2, cols - 1) * 4 + (lane & 3)) * 16;
-    // one slot; one item's partial sums handed over
-    auto slot = [&](float (&acc)[2][4], const uint32_t (&b)[16]) {
-      cp_async_wait<kRing - 2>();
-      multiply_slot(acc, tail, b, lane);
-      tail += kSlotBytes;
-      if (tail == ring_end) tail = st.ring;
-      issue();
-    };
-    auto hand_over = [&](const float (&acc)[2][4], float f0, float f1) {
-      // A wait that ran out is seen by everybody at the grid's next barrier; until then the warp keeps
-      // step with the others, which meet it at the barriers around their columns.
-      const int buf = n % kBufs;
-      if (tc::mbar_wait_warp(&sh.empty[buf], ((n / kBufs) & 1) ^ 1u, &sh.abort)) {
-        store_partial(red + buf * red_floats + warp * 32 * pitch, acc, f0, f1, lane, pitch, cols);
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sh.full[buf]);
+    const int scale_at = 2048 - lane * 8 + (lane & 1) * 2;
+    int n = 0;                     // items so far: buffer n % kBufs, its round n / kBufs
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+      if (pass == 1) grid_barrier(a.sync, &sh.abort);
+      const Share s = pass == 0 ? s1 : s2;
+      const FewPass p = a.pass[pass];
+      const int kwi = warp & (p.kw - 1);
+      int entry = -1, j = s.entry, u = s.first;
+      float f0 = 1.0f, f1 = 1.0f;
+#pragma unroll 1
+      for (int it = s.begin; it < s.end; ++it) {
+        if (j != entry) {
+          if (pass == 0) {
+            if (!identity) load_hidden_columns(a, sh, columns, j, cols, false);
+          } else {
+            load_act_columns(a, sh, columns, j, cols, p.kw);
+            f16_factor(sh.act_amax[kwi][2 * (lane & 3)], &f0);
+            f16_factor(sh.act_amax[kwi][2 * (lane & 3) + 1], &f1);
+          }
+          entry = j;
+        }
+        float acc[2][4] = {};
+#pragma unroll 1
+        for (int k = kwi; k < p.units; k += p.kw) {
+          uint32_t b[16];
+          load_b(b, lane_columns, k, cols);
+          cp_async_wait<kRing - 2>();
+          multiply_slot(acc, tail, tail + scale_at, b);
+          tail += kSlotBytes;
+          if (tail == st.ring_end) tail = st.ring;
+          issue();
+        }
+        // The item's partial sums go to a summing warp.  A wait that ran out is seen by everybody at the grid's next
+        // barrier; until then the warp keeps step with the others, which meet it at the barriers around their columns.
+        const int buf = n % kBufs;
+        if (tc::mbar_wait_warp(&sh.empty[buf], ((n / kBufs) & 1) ^ 1u, &sh.abort)) {
+          store_partial(red + buf * red_floats + warp * 32 * pitch, acc, f0, f1, lane, pitch, cols);
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&sh.full[buf]);
+        }
+        ++n;
+        if (++u == p.per_entry) { u = 0; ++j; }
       }
-      ++n;
-    };
-    int entry = -1, j = p1.begin / p1.per_entry, u = p1.begin - j * p1.per_entry;
-    for (int it = p1.begin; it < p1.end; ++it) {
-      if (j != entry) {
-        if (!identity) load_hidden_columns(a, sh, columns, j, cols, false);
-        entry = j;
-      }
-      float acc[2][4] = {};
-      for (int k = warp % p1.kw; k < p1.units; k += p1.kw) {
-        uint32_t b[16];
-        load_b(b, lane_columns, k, cols);
-        slot(acc, b);
-      }
-      hand_over(acc, 1.0f, 1.0f);
-      if (++u == p1.per_entry) { u = 0; ++j; }
-    }
-    // ---- down ----
-    grid_barrier(a.sync, &sh.abort);
-    entry = -1;
-    j = p2.begin / p2.per_entry;
-    u = p2.begin - j * p2.per_entry;
-    const int kw2 = warp % p2.kw;
-    float f0 = 1.0f, f1 = 1.0f;
-    for (int it = p2.begin; it < p2.end; ++it) {
-      if (j != entry) {
-        load_act_columns(a, sh, columns, j, cols, p2.kw);
-        entry = j;
-        f16_factor(sh.act_amax[kw2][2 * (lane & 3)], &f0);
-        f16_factor(sh.act_amax[kw2][2 * (lane & 3) + 1], &f1);
-      }
-      float acc[2][4] = {};
-      for (int k = kw2; k < p2.units; k += p2.kw) {
-        uint32_t b[16];
-        load_b(b, lane_columns, k, cols);
-        slot(acc, b);
-      }
-      hand_over(acc, f0, f1);
-      if (++u == p2.per_entry) { u = 0; ++j; }
     }
     cp_async_wait<0>();
   } else {
     // ---- the summing warps: every kSumWarps-th item each, the warps' shares added in order ----
     const int mine = warp - kWarps;
     const float* part = red + mine * red_floats;
-    const int items1 = p1.end - p1.begin, items2 = p2.end - p2.begin;
-    for (n = mine; n < items1 && alive; n += kSumWarps) {
-      alive = tc::mbar_wait_warp(&sh.full[mine], (n / kBufs) & 1, &sh.abort);
-      if (!alive) break;
-      const int it = p1.begin + n, j = it / p1.per_entry, u = it - j * p1.per_entry;
-      const uint32_t e = sh.ent_expert[j];
-      const float s2 = __ldg(a.scale2 + e * 3 + (lane >> 4));
-      const int warps_k = min(p1.kw, p1.units);
-      for (int rw = 0; rw < p1.rw; ++rw)
-        for (int c = 0; c < cols; ++c) {
+    bool alive = true;
+    int base = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+      const Share s = pass == 0 ? s1 : s2;
+      const FewPass p = a.pass[pass];
+      const int items = s.end - s.begin, rw = kWarps >> p.log_kw, warps_k = min(p.kw, p.units);
+      // the CTA's item number base + i is this warp's when it is `mine` modulo kSumWarps
+      int i = (mine - base % kSumWarps + kSumWarps) % kSumWarps;
+      int u = s.first, j = s.entry, at = 0;          // entry and place of item `at`
+#pragma unroll 1
+      for (; i < items && alive; i += kSumWarps) {
+        u += i - at;
+        at = i;
+        while (u >= p.per_entry) { u -= p.per_entry; ++j; }
+        const float* s2p = a.scale2 + sh.ent_expert[j] * 3 + (pass == 0 ? lane >> 4 : 2);
+        const float scale2 = __ldg(s2p);
+        alive = tc::mbar_wait_warp(&sh.full[mine], ((base + i) / kBufs) & 1, &sh.abort);
+        if (!alive) break;
+#pragma unroll 1
+        for (int q = 0; q < rw * cols; ++q) {
+          const int r = q / cols, c = q - r * cols;
           const int route = sh.ent_route[j][c];
           if (route < 0) continue;
-          const float* src = part + (rw * p1.kw * 32 + lane) * pitch + c;      // lanes 0..15 gate, 16..31 up
+          const float* src = part + (r * p.kw * 32 + lane) * pitch + c;
           float sum = 0.0f;
 #pragma unroll 4
           for (int w = 0; w < warps_k; ++w) sum += src[w * 32 * pitch];
-          float inv;
-          f16_factor(sh.x_amax[route / a.top_k], &inv);
-          sum *= s2 * inv;
-          const float up = __shfl_down_sync(0xffffffffu, sum, 16);
-          const float v = sh.ent_w[j][c] * (__fdividef(sum, 1.0f + __expf(-sum)) * up);
-          if (lane < 16)
-            a.act[static_cast<size_t>(route) * a.inter + unit_row(u * p1.rw + rw) + (lane & 7) + (lane >> 3) * 32] = v;
+          if (pass == 0) {                             // lanes 0..15 gate, 16..31 up
+            sum *= scale2 * sh.x_inv[sh.route_token[route]];
+            const float up = __shfl_down_sync(0xffffffffu, sum, 16);
+            const float v = sh.ent_w[j][c] * (__fdividef(sum, 1.0f + __expf(-sum)) * up);
+            if (lane < 16)
+              a.act[static_cast<size_t>(route) * a.inter + unit_row(u * rw + r) + (lane & 7) + (lane >> 3) * 32] = v;
+          } else {
+            a.route_out[static_cast<size_t>(route) * a.hidden + unit_row((u * rw + r) * 2 + (lane >> 4)) + (lane & 7) +
+                        ((lane >> 3) & 1) * 32] = sum * scale2;
+          }
         }
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sh.empty[mine]);
-    }
-    grid_barrier(a.sync, &sh.abort);
-    // item n of the second pass is the (items1 + n)-th of the CTA
-    n = items1 + (mine - items1 % kSumWarps + kSumWarps) % kSumWarps;
-    for (; n < items1 + items2 && alive; n += kSumWarps) {
-      alive = tc::mbar_wait_warp(&sh.full[mine], (n / kBufs) & 1, &sh.abort);
-      if (!alive) break;
-      const int it = p2.begin + n - items1, j = it / p2.per_entry, u = it - j * p2.per_entry;
-      const float s2 = __ldg(a.scale2 + sh.ent_expert[j] * 3 + 2);
-      const int warps_k = min(p2.kw, p2.units);
-      for (int rw = 0; rw < p2.rw; ++rw)
-        for (int c = 0; c < cols; ++c) {
-          const int route = sh.ent_route[j][c];
-          if (route < 0) continue;
-          const float* src = part + (rw * p2.kw * 32 + lane) * pitch + c;
-          float sum = 0.0f;
-#pragma unroll 4
-          for (int w = 0; w < warps_k; ++w) sum += src[w * 32 * pitch];
-          a.route_out[static_cast<size_t>(route) * a.hidden + unit_row((u * p2.rw + rw) * 2 + (lane >> 4)) + (lane & 7) +
-                      ((lane >> 3) & 1) * 32] = sum * s2;
-        }
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sh.empty[mine]);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sh.empty[mine]);
+      }
+      base += items;
+      if (pass == 0) grid_barrier(a.sync, &sh.abort);
     }
   }
-  alive = grid_barrier(a.sync, &sh.abort);
-  if (!alive) {
+  if (!grid_barrier(a.sync, &sh.abort)) {
     if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
     return;
   }
@@ -826,9 +813,17 @@ __global__ void few_fc2_simt_kernel(FewArgs a) {
 
 }  // namespace
 
-int few_splits(int sm_count, int experts, int hidden) {
-  const int s = sm_count * (kThreads / 32) / experts, most = hidden / 128;
-  return s < 1 ? 1 : (s > kFewMaxSplits ? kFewMaxSplits : s) > most ? most : (s > kFewMaxSplits ? kFewMaxSplits : s);
+FewPass few_pass(int k, int groups) {
+  FewPass p{};
+  p.units = k / 128;
+  p.kw = kWarps;
+  p.log_kw = 4;
+  while (p.kw > 2 && p.kw * 2 > p.units) {      // two units a warp or more, so that handing a sum over is rare
+    p.kw /= 2;
+    --p.log_kw;
+  }
+  p.per_entry = groups / (kWarps / p.kw);
+  return p;
 }
 
 namespace {
@@ -862,10 +857,10 @@ glmrt_status_t launch_ring(const FewArgs& a, int cap, size_t smem, int sm_count,
 }  // namespace
 
 // Columns per pass over an expert and depth of the stream, from what fits into shared memory: the
-// selection's scratch (36 bytes an expert and a float per row and expert) lies in the ring, and at least
+// selection's scratch (36 bytes an expert) lies in the ring, and at least
 // three slots are needed.
 bool few_fused_supported(const FewArgs& a) {
-  static_assert(1024 * 36 + 1024 * kFewMaxRows * 4 <= 3 * kWarps * kSlotBytes, "selection scratch fits the ring");
+  static_assert(1024 * 36 <= 3 * kWarps * kSlotBytes, "selection scratch fits the ring");
   return few_smem(3, 1, std::max(a.hidden, a.inter)) <= kSmemMost && a.experts <= 1024;
 }
 glmrt_status_t launch_few_fused(const FewArgs& a, int sm_count, cudaStream_t s) {

@@ -306,6 +306,9 @@ glmrt_status_t launch_fc2_tc_pair(const FfnArgs& a, const TensorMaps& maps, int 
 
 // ---- few.cu (a whole layer for a few tokens on bf16 activations) ----
 constexpr int kFewMaxRows = 16;
+// How the rows of one weight pass are worked on: items of 16 / kw groups of rows (16 rows of gate and up, 32 of down),
+// kw warps sharing the 128-column units of K.
+struct FewPass { int units, kw, log_kw, per_entry; };
 struct FewArgs {
   const uint16_t* hidden_rows;                              // [rows, hidden] bf16
   const uint16_t *residual, *shared;                        // [rows, hidden] bf16 or nullptr
@@ -320,17 +323,16 @@ struct FewArgs {
   int rows, top_k, experts, hidden, inter;
   // the fused kernel only
   const float *router_w, *router_b;                         // [experts, hidden], [experts] float32
-  float* logits;                                            // [splits][rows][experts] partial sums; nullptr: routes given
-  int splits;
+  float* logits;                                            // [rows][experts]; nullptr: routes given
+  FewPass pass[2];                                          // gate and up; down
   float scaling;
   uint32_t* out_idx;                                        // where the routes are written, or nullptr
   float* out_w;
   float* route_out;                                         // [rows * top_k, hidden] float32 result rows
-  unsigned long long* sync;                                 // barrier count: a multiple of the grid's size between calls
+  uint32_t* sync;                                           // barrier count
   uint32_t* counters;
 };
-constexpr int kFewMaxSplits = 16;
-int few_splits(int sm_count, int experts, int hidden);      // column shares of the router's logits
+FewPass few_pass(int k, int groups);
 bool few_fused_supported(const FewArgs& a);
 glmrt_status_t launch_few_fused(const FewArgs& a, int sm_count, cudaStream_t stream);
 glmrt_status_t launch_few_simt(const FewArgs& a, cudaStream_t stream);

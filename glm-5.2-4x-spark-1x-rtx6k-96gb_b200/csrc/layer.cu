@@ -81,10 +81,10 @@ struct Layer {
   uint16_t* route_rows = nullptr;
   uint16_t** slot_out = nullptr;
   uint32_t* slot_weight = nullptr;   // route weight per slot (fused combine of large batches)
-  // few-token path: weighted SwiGLU rows, one float32 result row per route, partial logits, the count of
+  // few-token path: weighted SwiGLU rows, one float32 result row per route, logits, the count of
   // its kernel's barriers
   float *few_act = nullptr, *few_out = nullptr, *few_logits = nullptr;
-  unsigned long long* few_sync = nullptr;
+  uint32_t* few_sync = nullptr;
   uint32_t* fc_sync = nullptr;       // hand-over words between the decode FC1 and FC2 kernels
   uint16_t *hidden_stage = nullptr, *out_stage = nullptr;
   // scratch for weight loading
@@ -477,7 +477,7 @@ glmrt_status_t alloc_workspace(Layer* l) {
     const size_t F = std::min<size_t>(T, kFewMaxRows);
     A(dev_alloc(b, &l->few_act, F * K * I));
     A(dev_alloc(b, &l->few_out, F * K * H));
-    A(dev_alloc(b, &l->few_logits, kFewMaxSplits * F * c.experts));
+    A(dev_alloc(b, &l->few_logits, F * c.experts));
     A(dev_alloc(b, &l->few_sync, 1, true));
   }
   A(dev_alloc(b, &l->hidden_stage, T * H));
@@ -795,6 +795,8 @@ glmrt_status_t few_args(Layer* l, const glmrt_device_buffer_t& hidden, size_t ro
   a.hidden = static_cast<int>(c.hidden_dim); a.inter = static_cast<int>(c.intermediate_dim);
   a.router_w = l->router_w; a.router_b = l->router_b; a.scaling = c.routed_scaling;
   a.route_out = l->few_out;
+  a.pass[0] = few_pass(a.hidden, a.inter / 16);
+  a.pass[1] = few_pass(a.inter, a.hidden / 32);
   a.sync = l->few_sync;
   a.counters = l->counters;
   *out = a;
@@ -822,7 +824,6 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_async(
   const uint64_t before = launches_total();
   if (few_fused(l, a)) {
     a.logits = l->few_logits;
-    a.splits = few_splits(l->sm_count, a.experts, a.hidden);
     a.out_idx = static_cast<uint32_t*>(topk_indices.ptr);
     a.out_w = static_cast<float*>(topk_weights.ptr);
     GLMRT_RETURN_IF_ERROR(launch_few_fused(a, l->sm_count, s));
