@@ -151,12 +151,16 @@ __device__ bool grid_barrier(uint32_t* count, volatile uint32_t* abort) {
 // A CTA's share of one of the two weight passes.  How an item of rows is shared by the warps (FewPass: kw along K,
 // rw along the rows) follows from the shape alone, so that a row's sums do not depend on its batch.
 struct Share { int begin, end, entry, first; };        // items, and the first one's entry and place in it
-__device__ __forceinline__ Share share_of(const FewPass& p, int entries) {
-  const uint32_t items = static_cast<uint32_t>(entries) * p.per_entry;    // items * grid < 2^32 (few_fused_supported)
+__device__ __forceinline__ Share share_of(const FewArgs& a, const FewPass& p, int entries) {
+  const uint32_t items = static_cast<uint32_t>(entries) * p.per_entry;
+  // items * i / grid without a division: a.grid_step is 2^32 / grid, rounded up, so the last share is cut at `items`
+  auto border = [&](uint32_t i) {
+    return min(items, static_cast<uint32_t>((static_cast<uint64_t>(items) * min(static_cast<uint64_t>(i) * a.grid_step, uint64_t{1} << 32)) >> 32));
+  };
   Share s;
-  s.begin = static_cast<int>(items * blockIdx.x / gridDim.x);
-  s.end = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
-  s.entry = s.begin / p.per_entry;
+  s.begin = static_cast<int>(border(blockIdx.x));
+  s.end = static_cast<int>(border(blockIdx.x + 1));
+  s.entry = static_cast<int>(__umulhi(static_cast<uint32_t>(s.begin), p.per_entry_inv));    // begin / per_entry (few_pass)
   s.first = s.begin - s.entry * p.per_entry;
   return s;
 }
@@ -376,41 +380,36 @@ __device__ __forceinline__ void store_partial(float* red, const float (&acc)[2][
   }
 }
 
-// Top-k of one row by one warp: keys order like (score + bias, lower id first); a NaN ranks last.
+// Top-k of one row by one warp: the largest keys, the lower id first among equal ones.
 template <int kKeys>
 __device__ __forceinline__ void select_row(const FewArgs& a, FewShared& sh, int row, int lane) {
-  uint32_t key[kKeys];
-  float score[kKeys];
+  uint2 v[kKeys];            // key, score
 #pragma unroll
-  for (int i = 0; i < kKeys; ++i) score[i] = lane + 32 * i < a.experts ? __ldcg(a.logits + row * a.experts + lane + 32 * i) : 0.0f;
-#pragma unroll
-  for (int i = 0; i < kKeys; ++i) {
-    key[i] = 0u;
-    score[i] = sigmoid_f32(score[i]);
-    if (lane + 32 * i < a.experts) {
-      const float s = score[i] + __ldg(a.router_b + lane + 32 * i);
-      const uint32_t u = __float_as_uint(s == 0.0f ? 0.0f : s);
-      key[i] = s != s ? 1u : ((u >> 31) ? ~u : u | 0x80000000u);
-    }
-  }
+  for (int i = 0; i < kKeys; ++i)
+    v[i] = lane + 32 * i < a.experts ? __ldcg(a.scores + row * a.experts + lane + 32 * i) : make_uint2(0u, 0u);
   float sum = 0.0f, my_score = 0.0f;
   uint32_t mine = 0;
 #pragma unroll 1
   for (int s = 0; s < a.top_k; ++s) {
-    uint32_t best = key[0];
-    float best_score = score[0];
-    int at = 0;
+    uint32_t best[kKeys];
 #pragma unroll
-    for (int i = 1; i < kKeys; ++i)
-      if (key[i] > best) { best = key[i]; best_score = score[i]; at = i; }       // the first of equal ones: the lower id
-    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    const uint32_t id = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(lane + 32 * at) : 0xffffffffu);
-    const float chosen = __shfl_sync(0xffffffffu, best_score, id & 31);
+    for (int i = 0; i < kKeys; ++i) best[i] = v[i].x;
+#pragma unroll
+    for (int h = kKeys / 2; h > 0; h /= 2)
+#pragma unroll
+      for (int i = 0; i < h; ++i) best[i] = max(best[i], best[i + h]);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best[0]);
+    uint32_t id = 0xffffffffu, score = 0u;
+#pragma unroll
+    for (int i = kKeys - 1; i >= 0; --i)
+      if (v[i].x == top) { id = lane + 32 * i; score = v[i].y; }
+    const uint32_t first = __reduce_min_sync(0xffffffffu, id);
+    const float chosen = __uint_as_float(__shfl_sync(0xffffffffu, score, first & 31));
 #pragma unroll
     for (int i = 0; i < kKeys; ++i)
-      if (lane + 32 * i == static_cast<int>(id)) key[i] = 0u;
+      if (lane + 32 * i == static_cast<int>(first)) v[i].x = 0u;
     sum += chosen;
-    if (lane == s) { mine = id; my_score = chosen; }
+    if (lane == s) { mine = first; my_score = chosen; }
   }
   if (lane < a.top_k) {
     const int r = row * a.top_k + lane;
@@ -432,7 +431,7 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
   }
   if (tid < kFewMaxRows) sh.used[tid] = 0u;
   if (tid == 0) { sh.bad = 0; sh.distinct = 0; }
-  if (a.logits != nullptr) {
+  if (a.scores != nullptr) {
     if (warp < a.rows) {
       if (a.experts <= 256) select_row<8>(a, sh, warp, lane);
       else select_row<32>(a, sh, warp, lane);
@@ -506,10 +505,10 @@ __device__ void score_experts(const FewArgs& a, FewShared& sh, int warp, int lan
   const int u0 = units * share / kLogitShares, u1 = units * (share + 1) / kLogitShares;
 #pragma unroll 1
   for (int e0 = blockIdx.x; e0 < a.experts; e0 += kLogitExperts * gridDim.x) {
-    const int e = e0 + half * gridDim.x;
-    const float* wrow = a.router_w + static_cast<size_t>(e) * a.hidden + lane * 4;
+    const int e_mine = e0 + half * gridDim.x;
+    const float* wrow = a.router_w + static_cast<size_t>(e_mine) * a.hidden + lane * 4;
 #pragma unroll 1
-    for (int t0 = 0; t0 < a.rows && e < a.experts; t0 += 4) {
+    for (int t0 = 0; t0 < a.rows && e_mine < a.experts; t0 += 4) {
       const uint16_t* xrow = a.hidden_rows + static_cast<size_t>(t0) * a.hidden + lane * 4;
       float acc[4] = {};
 #pragma unroll 1
@@ -544,11 +543,15 @@ __device__ void score_experts(const FewArgs& a, FewShared& sh, int warp, int lan
     }
     __syncthreads();
     const int h = threadIdx.x / kFewMaxRows, t = threadIdx.x % kFewMaxRows;
-    if (h < kLogitExperts && t < a.rows && e0 + h * static_cast<int>(gridDim.x) < a.experts) {
+    const int e = e0 + h * static_cast<int>(gridDim.x);
+    if (h < kLogitExperts && t < a.rows && e < a.experts) {
       float s = 0.0f;
 #pragma unroll
       for (int i = 0; i < kLogitShares; ++i) s += sh.logit_part[h][i][t];
-      a.logits[t * a.experts + e0 + h * gridDim.x] = s;
+      // a key that orders like score + bias (a NaN last, zero for no expert) and the score
+      const float score = sigmoid_f32(s), rank = score + __ldg(a.router_b + e);
+      const uint32_t u = __float_as_uint(rank == 0.0f ? 0.0f : rank);
+      a.scores[t * a.experts + e] = make_uint2(rank != rank ? 1u : ((u >> 31) ? ~u : u | 0x80000000u), __float_as_uint(score));
     }
     __syncthreads();
   }
@@ -576,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
   if (tid < kFewMaxRows) sh.x_amax[tid] = 0u;
   __syncthreads();
 
-  if (a.logits != nullptr) score_experts(a, sh, warp, lane);
+  if (a.scores != nullptr) score_experts(a, sh, warp, lane);
   // the rows' largest magnitudes, 256 values a warp
   const int row_pieces = a.hidden / 256;
 #pragma unroll 1
@@ -592,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
   __syncthreads();
   if (tid < a.rows) f16_factor(sh.x_amax[tid], &sh.x_inv[tid]);
   if (identity && warp < kWarps) load_hidden_columns(a, sh, columns, 0, cols, true);    // needs no routes
-  if (a.logits != nullptr) {
+  if (a.scores != nullptr) {
     if (!grid_barrier(a.sync, &sh.abort)) {
       if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
       return;
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
     a.counters[kCntDistinct] = static_cast<uint32_t>(sh.distinct);
   }
 
-  const Share s1 = share_of(a.pass[0], entries), s2 = share_of(a.pass[1], entries);
+  const Share s1 = share_of(a, a.pass[0], entries), s2 = share_of(a, a.pass[1], entries);
   if (warp < kWarps) {
     // ---- the multiplying warps: the weight stream, then gate and up (pass 0) and down (pass 1) ----
     Stream st;
@@ -823,6 +826,7 @@ FewPass few_pass(int k, int groups) {
     --p.log_kw;
   }
   p.per_entry = groups / (kWarps / p.kw);
+  p.per_entry_inv = static_cast<uint32_t>(((uint64_t{1} << 32) + p.per_entry - 1) / p.per_entry);
   return p;
 }
 
@@ -849,7 +853,9 @@ glmrt_status_t launch_ring(const FewArgs& a, int cap, size_t smem, int sm_count,
   attr[0].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t err = cudaLaunchKernelEx(&cfg, few_layer_kernel<kRing>, a, cap);
+  FewArgs args = a;
+  args.grid_step = static_cast<uint32_t>(((uint64_t{1} << 32) + sm_count - 1) / sm_count);
+  cudaError_t err = cudaLaunchKernelEx(&cfg, few_layer_kernel<kRing>, args, cap);
   if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "few_layer_kernel", err);
   GLMRT_LAUNCH_CHECK("few_layer_kernel");
   return GLMRT_STATUS_OK;
@@ -861,7 +867,9 @@ glmrt_status_t launch_ring(const FewArgs& a, int cap, size_t smem, int sm_count,
 // three slots are needed.
 bool few_fused_supported(const FewArgs& a) {
   static_assert(1024 * 36 <= 3 * kWarps * kSlotBytes, "selection scratch fits the ring");
-  return few_smem(3, 1, std::max(a.hidden, a.inter)) <= kSmemMost && a.experts <= 1024;
+  // (per_entry < 4096 makes the multiplication by its inverse exact: at most 256 entries)
+  return few_smem(3, 1, std::max(a.hidden, a.inter)) <= kSmemMost && a.experts <= 1024 && a.pass[0].per_entry > 1 &&
+         a.pass[0].per_entry < 4096 && a.pass[1].per_entry > 1 && a.pass[1].per_entry < 4096;
 }
 glmrt_status_t launch_few_fused(const FewArgs& a, int sm_count, cudaStream_t s) {
   const int k = std::max(a.hidden, a.inter);

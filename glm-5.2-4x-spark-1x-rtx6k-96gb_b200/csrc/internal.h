@@ -308,7 +308,8 @@ glmrt_status_t launch_fc2_tc_pair(const FfnArgs& a, const TensorMaps& maps, int 
 constexpr int kFewMaxRows = 16;
 // How the rows of one weight pass are worked on: items of 16 / kw groups of rows (16 rows of gate and up, 32 of down),
 // kw warps sharing the 128-column units of K.
-struct FewPass { int units, kw, log_kw, per_entry; };
+// per_entry items per entry, per_entry_inv = 2^32 / per_entry rounded up.
+struct FewPass { int units, kw, log_kw, per_entry; uint32_t per_entry_inv; };
 struct FewArgs {
   const uint16_t* hidden_rows;                              // [rows, hidden] bf16
   const uint16_t *residual, *shared;                        // [rows, hidden] bf16 or nullptr
@@ -323,7 +324,8 @@ struct FewArgs {
   int rows, top_k, experts, hidden, inter;
   // the fused kernel only
   const float *router_w, *router_b;                         // [experts, hidden], [experts] float32
-  float* logits;                                            // [rows][experts]; nullptr: routes given
+  uint2* scores;                                            // [rows][experts] ranking key and score; nullptr: routes given
+  uint32_t grid_step;                                       // 2^32 / grid, rounded up (set at the launch)
   FewPass pass[2];                                          // gate and up; down
   float scaling;
   uint32_t* out_idx;                                        // where the routes are written, or nullptr

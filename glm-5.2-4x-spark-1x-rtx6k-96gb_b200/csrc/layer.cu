@@ -81,9 +81,10 @@ struct Layer {
   uint16_t* route_rows = nullptr;
   uint16_t** slot_out = nullptr;
   uint32_t* slot_weight = nullptr;   // route weight per slot (fused combine of large batches)
-  // few-token path: weighted SwiGLU rows, one float32 result row per route, logits, the count of
+  // few-token path: weighted SwiGLU rows, one float32 result row per route, scores, the count of
   // its kernel's barriers
-  float *few_act = nullptr, *few_out = nullptr, *few_logits = nullptr;
+  float *few_act = nullptr, *few_out = nullptr;
+  uint2* few_scores = nullptr;
   uint32_t* few_sync = nullptr;
   uint32_t* fc_sync = nullptr;       // hand-over words between the decode FC1 and FC2 kernels
   uint16_t *hidden_stage = nullptr, *out_stage = nullptr;
@@ -477,7 +478,7 @@ glmrt_status_t alloc_workspace(Layer* l) {
     const size_t F = std::min<size_t>(T, kFewMaxRows);
     A(dev_alloc(b, &l->few_act, F * K * I));
     A(dev_alloc(b, &l->few_out, F * K * H));
-    A(dev_alloc(b, &l->few_logits, F * c.experts));
+    A(dev_alloc(b, &l->few_scores, F * c.experts));
     A(dev_alloc(b, &l->few_sync, 1, true));
   }
   A(dev_alloc(b, &l->hidden_stage, T * H));
@@ -823,7 +824,7 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_async(
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   const uint64_t before = launches_total();
   if (few_fused(l, a)) {
-    a.logits = l->few_logits;
+    a.scores = l->few_scores;
     a.out_idx = static_cast<uint32_t*>(topk_indices.ptr);
     a.out_w = static_cast<float*>(topk_weights.ptr);
     GLMRT_RETURN_IF_ERROR(launch_few_fused(a, l->sm_count, s));
