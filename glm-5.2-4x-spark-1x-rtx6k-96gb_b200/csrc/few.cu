@@ -28,7 +28,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 // One cooperative kernel, one CTA per SM, three grid-wide barriers:
 //
 //   logits     every warp: one expert x one share of the hidden columns, float32 weights       | barrier
-//   selection  every CTA for itself: sigmoid, top-k, the list of (expert, up to `cap` tokens) entries
+//   selection  every CTA for itself: sigmoid, top-k, the list of (expert, one or two tokens) entries
 //   gate / up  the entries' rows split evenly over the CTAs                                    | barrier
 //   down       the same; one float32 row per route                                             | barrier
 //   combine    residual + (shared + sum over the slots, in slot order)
@@ -41,10 +41,14 @@ __device__ __forceinline__ float warp_sum(float v) {
 //
 // A piece is 16 weight rows x 128 columns of one warp: 16 B of codes of each of two rows per lane (32
 // columns) and the scales of both.  A slot is two pieces at the same columns: the same rows of gate and up,
-// or 32 rows of down.  E2M1 codes become fp16 pairs (one instruction for two), times
-// the E4M3 scale: the product has at most six significant bits, so it is exact.  The tensor cores multiply
-// (m16n8k16; tokens are the eight columns) and add in float32.  Which columns a lane holds does not
-// matter as long as both operands agree, so lane t of a row's four takes columns 32t .. 32t+31.
+// or 32 rows of down.  E2M1 codes become fp16 pairs (one instruction for two) and the tensor cores multiply
+// them (m16n8k16, float32 sums).  Which columns a lane holds does not matter as long as both operands agree,
+// so lane t of a row's four takes columns 32t .. 32t+31, two scale blocks.  A product's four lanes thus lie in
+// four different blocks; to keep the blocks apart an entry has at most two tokens and a token four of the
+// eight columns, column t' holding the token's values of lane t' and zeros elsewhere.  So a sum of four products
+// is one block's, and the E4M3 scale is multiplied to it in float32: 16 FMAs a slot, where scaling the weights
+// themselves takes 64 fp16 multiplications on the pipe that the products run on (measured: 18.5 cycles a product
+// with them, 10.5 without; the conversions take 12 on another pipe).
 //
 // The rows as fp16: times a power of two per token that brings the largest magnitude to 2^14, which is
 // exact for everything within 2^28 of it and off by 2^-39 of it below.  The SwiGLU rows likewise, rounded
@@ -56,6 +60,7 @@ constexpr int kMainThreads = 32 * kWarps;
 constexpr int kThreads = kMainThreads + 32 * kSumWarps;
 constexpr int kBufs = kSumWarps;             // items whose partial sums may be waiting, one per summing warp
 constexpr int kSlotBytes = 2560;             // per warp: two pieces of two 16-byte codes and 8 scale bytes a lane
+constexpr int kCols = 2;                     // tokens of an entry at most
 constexpr int kMaxEntries = 256;             // (expert, token group) pairs: at most one per route
 constexpr int kMaxRoutes = 256;
 constexpr int kLogitExperts = 2;             // experts a CTA scores at a time, by kLogitShares warps each
@@ -64,13 +69,13 @@ constexpr uint64_t kBarrierLimitNs = 2000000000ull;
 
 struct FewShared {
   uint16_t ent_expert[kMaxEntries];
-  int16_t ent_route[kMaxEntries][8];         // column -> route, or -1
-  float ent_w[kMaxEntries][8];               // column -> weight
+  int16_t ent_route[kMaxEntries][kCols];     // column -> route, or -1
+  float ent_w[kMaxEntries][kCols];           // column -> weight
   uint32_t route_expert[kMaxRoutes];
   float route_w[kMaxRoutes];
   uint8_t route_token[kMaxRoutes];
   uint32_t used[kFewMaxRows];                // slots of a token that own a result row
-  uint32_t act_amax[kWarps][8];              // by warp along K and column
+  uint32_t act_amax[kWarps][kCols];          // by warp along K and column
   uint32_t x_amax[kFewMaxRows];
   float x_inv[kFewMaxRows];                  // undoes the power of two of a row
   float logit_part[kLogitExperts][kLogitShares][kFewMaxRows];
@@ -100,21 +105,12 @@ __device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&d)[4]) {
       : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
       : "r"(w));
 }
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-// Two E4M3 bytes -> two fp16 pairs, each holding one of them twice.
-__device__ __forceinline__ void e4m3x2_to_pairs(uint32_t two, uint32_t& lo, uint32_t& hi) {
-  uint32_t h;
-  asm("{\n\t.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(h) : "r"(two));
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tmov.b32 %0, {a, a};\n\tmov.b32 %1, {b, b};\n\t}" : "=r"(lo), "=r"(hi) : "r"(h));
-}
-__device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
-  return v;
+// Four E4M3 bytes -> float32.
+__device__ __forceinline__ void e4m3x4_to_f32(uint32_t four, float (&f)[4]) {
+  uint32_t lo, hi;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -191,7 +187,7 @@ struct Stream {
     sf_second = gate_up ? static_cast<size_t>(a.up_sf - a.gate_sf) : 128;
     lane_codes = static_cast<uint32_t>(g) * row_bytes + t * 16;
     lane_low = lane_codes + 32u * row_bytes;
-    lane_sf = (t >> 1) * 512 + g * 16;
+    lane_sf = (t & 1) * 512 + g * 16;          // the four blocks this lane scales (multiply_slot)
     codes0 = (gate_up ? a.gate_codes : a.down_codes) + kwi * 64;
     sf0 = (gate_up ? a.gate_sf : a.down_sf) + kwi * 1024;
     left = kwi < units ? s.end - s.begin : 0;
@@ -232,30 +228,45 @@ struct Stream {
 __device__ __forceinline__ void lds128(uint32_t (&v)[4], uint32_t at) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
 }
-// acc[m] += piece m's 16 x 128 weights times the unit's columns; the two pieces' chains of products run side by
-// side.  `slot`: shared address of the slot, this lane's 16 bytes included; `scales`: of this lane's two scale bytes
-// of piece 0, row g (row g + 32: 4 further, piece 1: 256).
-__device__ __forceinline__ void multiply_slot(float (&acc)[2][4], uint32_t slot, uint32_t scales, const uint32_t (&b)[16]) {
+// acc[m] += piece m's rows (g, g + 32) times the unit's columns, as far as this lane holds them: of token t / 2 (lane
+// t of the row's four), blocks 4 (t & 1) .. + 3.  `slot`: shared address of the slot, this lane's 16 bytes included;
+// `scales`: of the scale words of those blocks of rows g and g + 32, piece 0 (piece 1: 256 further).  The four sums (two
+// pieces, two blocks a lane) are chains of products side by side.
+__device__ __forceinline__ void multiply_slot(float (&acc)[2][2], uint32_t slot, uint32_t scales, const uint32_t (&b)[16]) {
   uint32_t w[4][4];           // piece 0 rows g, g + 32; piece 1 the same
-  uint32_t scale[4][2];       // of the lane's two blocks in each
 #pragma unroll
   for (int i = 0; i < 4; ++i) lds128(w[i], slot + i * 512);
+  uint32_t s[2][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) e4m3x2_to_pairs(lds_u16(scales + (i >> 1) * 256 + (i & 1) * 4), scale[i][0], scale[i][1]);
+  for (int m = 0; m < 2; ++m)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(s[m][0]), "=r"(s[m][1]) : "r"(scales + m * 256) : "memory");
+  float c[2][2][4];           // [piece][first or second block of each lane]
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int half = 0; half < 2; ++half)
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      uint32_t d0[4], d1[4];
-      e2m1x8_to_f16(w[2 * m][i], d0);
-      e2m1x8_to_f16(w[2 * m + 1][i], d1);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        d0[v] = mul_f16x2(d0[v], scale[2 * m][i / 2]);
-        d1[v] = mul_f16x2(d1[v], scale[2 * m + 1][i / 2]);
+      for (int i = 0; i < 4; ++i) c[m][half][i] = 0.0f;
+#pragma unroll
+      for (int i = 2 * half; i < 2 * half + 2; ++i) {
+        uint32_t d0[4], d1[4];
+        e2m1x8_to_f16(w[2 * m][i], d0);
+        e2m1x8_to_f16(w[2 * m + 1][i], d1);
+        mma16816(c[m][half], d0[0], d1[0], d0[1], d1[1], b[4 * i], b[4 * i + 1]);
+        mma16816(c[m][half], d0[2], d1[2], d0[3], d1[3], b[4 * i + 2], b[4 * i + 3]);
       }
-      mma16816(acc[m], d0[0], d1[0], d0[1], d1[1], b[4 * i], b[4 * i + 1]);
-      mma16816(acc[m], d0[2], d1[2], d0[3], d1[3], b[4 * i + 2], b[4 * i + 3]);
+    }
+  // columns 2t and 2t + 1 are lanes t' = 2 (t & 1) and the next: their first blocks are the word's bytes 0 and 2
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float f[4];
+      e4m3x4_to_f32(s[m][r], f);
+      acc[m][r] = fmaf(c[m][0][2 * r], f[0], acc[m][r]);
+      acc[m][r] = fmaf(c[m][1][2 * r], f[1], acc[m][r]);
+      acc[m][r] = fmaf(c[m][0][2 * r + 1], f[2], acc[m][r]);
+      acc[m][r] = fmaf(c[m][1][2 * r + 1], f[3], acc[m][r]);
     }
 }
 
@@ -309,7 +320,7 @@ __device__ void load_hidden_columns(const FewArgs& a, const FewShared& sh, uint8
 __device__ void load_act_columns(const FewArgs& a, FewShared& sh, uint8_t* dst, int entry, int cols, int kw) {
   const int k = a.inter, per_col = k / 8;
   main_sync();
-  for (int i = threadIdx.x; i < kWarps * 8; i += kMainThreads) sh.act_amax[i >> 3][i & 7] = 0u;
+  for (int i = threadIdx.x; i < kWarps * kCols; i += kMainThreads) sh.act_amax[i / kCols][i % kCols] = 0u;
   main_sync();
   auto read = [&](int route, int o, float (&v)[8]) {
     const float4* src = reinterpret_cast<const float4*>(a.act + static_cast<size_t>(route) * k + o * 8);
@@ -348,8 +359,10 @@ __device__ void load_act_columns(const FewArgs& a, FewShared& sh, uint8_t* dst, 
   main_sync();
 }
 
-// Lanes of columns past `cols` take the last one's values: their results are not read.
-__device__ __forceinline__ void load_b(uint32_t (&b)[16], uint32_t lane_columns, int unit, int cols) {
+// Lane (g, t) holds the values of lane t in product column g = 4 token + t': they are the token's where t' = t (`mine`),
+// else zero (and b stays as it was set).
+__device__ __forceinline__ void load_b(uint32_t (&b)[16], uint32_t lane_columns, int unit, int cols, bool mine) {
+  if (!mine) return;
   const uint32_t step = cols * 64, at = lane_columns + unit * 4 * step;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -359,25 +372,17 @@ __device__ __forceinline__ void load_b(uint32_t (&b)[16], uint32_t lane_columns,
   }
 }
 
-// Partial sums of an item: [warp][piece m][row][column], `pitch` columns (a power of two), times what undoes
-// the powers of two of the lane's two columns.
-__device__ __forceinline__ void store_partial(float* red, const float (&acc)[2][4], float f0, float f1, int lane, int pitch, int cols) {
-  const int g = lane >> 2, t = lane & 3;
-  float* d = red + g * pitch + 2 * t;
-  if (2 * t < cols) {
+// Partial sums of an item: [warp][piece m][row][column], times what undoes the power of two of the column.  Two lanes
+// share a token.
+__device__ __forceinline__ void store_partial(float* red, const float (&acc)[2][2], float factor, int lane, int cols) {
+  const int g = lane >> 2, c = (lane & 3) >> 1;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      d[m * 16 * pitch] = acc[m][0] * f0;
-      d[(m * 16 + 8) * pitch] = acc[m][2] * f0;
-    }
-  }
-  if (2 * t + 1 < cols) {
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      d[m * 16 * pitch + 1] = acc[m][1] * f1;
-      d[(m * 16 + 8) * pitch + 1] = acc[m][3] * f1;
+    for (int r = 0; r < 2; ++r) {
+      const float v = (acc[m][r] + __shfl_xor_sync(0xffffffffu, acc[m][r], 1)) * factor;
+      if ((lane & 1) == 0 && c < cols) red[(m * 16 + r * 8 + g) * cols + c] = v;
     }
-  }
 }
 
 // Top-k of one row by one warp: the largest keys, the lower id first among equal ones.
@@ -419,15 +424,15 @@ __device__ __forceinline__ void select_row(const FewArgs& a, FewShared& sh, int 
 }
 
 // Routes of all rows, then the list of entries (sh.ent_*).  `scratch`: for every expert a word and 16 half-words.
-__device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scratch, int cap, bool identity) {
+__device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scratch, bool identity) {
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int routes = a.rows * a.top_k;
   uint32_t* mask = reinterpret_cast<uint32_t*>(scratch);                            // rows that name an expert
   uint16_t* entry_of = reinterpret_cast<uint16_t*>(mask + a.experts);               // [expert][16]
   for (int i = tid; i < a.experts; i += kThreads) mask[i] = 0u;
-  for (int i = tid; i < routes * 8; i += kThreads) {        // at most one entry per route
-    sh.ent_route[i >> 3][i & 7] = -1;
-    sh.ent_w[i >> 3][i & 7] = 0.0f;
+  for (int i = tid; i < routes * kCols; i += kThreads) {    // at most one entry per route
+    sh.ent_route[i / kCols][i % kCols] = -1;
+    sh.ent_w[i / kCols][i % kCols] = 0.0f;
   }
   if (tid < kFewMaxRows) sh.used[tid] = 0u;
   if (tid == 0) { sh.bad = 0; sh.distinct = 0; }
@@ -441,7 +446,7 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
     sh.route_w[tid] = a.topk_w[tid];
   }
   __syncthreads();
-  // Entries, in the order of the first route that names each: an expert's rows in groups of `cap`
+  // Entries, in the order of the first route that names each: an expert's rows in groups of kCols
   // (identity: all rows are one group and a row's column is its number).
   uint32_t e = kNoRoute;
   int slot = 0, token = 0;
@@ -471,7 +476,7 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
   }
   __syncthreads();
   const int rank = live ? __popc(mask[e] & ((1u << token) - 1u)) : 0;
-  const bool opens = live && (identity ? rank == 0 : rank % cap == 0);
+  const bool opens = live && (identity ? rank == 0 : rank % kCols == 0);
   const uint32_t votes = __ballot_sync(0xffffffffu, opens);
   if (lane == 0) sh.warp_count[warp] = __popc(votes);
   __syncthreads();
@@ -481,7 +486,7 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
     if (i < warp) before += sh.warp_count[i];
     total += sh.warp_count[i];
   }
-  const int group = identity ? 0 : rank / cap;
+  const int group = identity ? 0 : rank / kCols;
   if (opens) {
     entry_of[e * 16 + group] = static_cast<uint16_t>(before);
     sh.ent_expert[before] = static_cast<uint16_t>(e);
@@ -490,7 +495,7 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
   if (tid == 0) sh.entries = total;
   __syncthreads();
   if (live) {
-    const int entry = entry_of[e * 16 + group], col = identity ? token : rank - group * cap;
+    const int entry = entry_of[e * 16 + group], col = identity ? token : rank - group * kCols;
     sh.ent_route[entry][col] = static_cast<int16_t>(tid);
     sh.ent_w[entry][col] = w;
   }
@@ -558,16 +563,15 @@ __device__ void score_experts(const FewArgs& a, FewShared& sh, int warp, int lan
 }
 
 template <int kRing>
-__global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int cap) {
+__global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   FewShared& sh = *reinterpret_cast<FewShared*>(smem);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
-  const bool identity = a.rows <= cap;
-  const int cols = identity ? a.rows : cap;
-  const int log_pitch = cols > 4 ? 3 : cols > 2 ? 2 : cols - 1, pitch = 1 << log_pitch;
+  const int cols = min(a.rows, kCols);
+  const bool identity = a.rows <= kCols;
   uint8_t* ring = smem + ((sizeof(FewShared) + 127) & ~static_cast<size_t>(127));
   float* red = reinterpret_cast<float*>(ring + kRing * kWarps * kSlotBytes);
-  const int red_floats = kWarps * 32 * pitch;
+  const int red_floats = kWarps * 32 * cols;
   uint8_t* columns = reinterpret_cast<uint8_t*>(red + kBufs * red_floats);
   if (tid == 0) {
     sh.abort = 0u;
@@ -601,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
       return;
     }
   }
-  route_and_select(a, sh, ring, cap, identity);
+  route_and_select(a, sh, ring, identity);
   const int entries = __shfl_sync(0xffffffffu, sh.entries, 0);
   if (blockIdx.x == 0 && tid == 0) {
     a.error_word[0] = sh.bad ? static_cast<uint32_t>(kErrBadExpert) : 0u;
@@ -628,8 +632,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
 #pragma unroll 1
     for (int i = 0; i < kRing - 1; ++i) issue();
     uint32_t tail = st.ring;
-    const uint32_t lane_columns = smem_addr(columns) + (min(lane >> 2, cols - 1) * 4 + (lane & 3)) * 16;
-    const int scale_at = 2048 - lane * 8 + (lane & 1) * 2;
+    const int lane_token = lane >> 4;                  // of the product column this lane brings, and whether it has values
+    const bool mine = ((lane >> 2) & 3) == (lane & 3) && lane_token < cols;
+    const uint32_t lane_columns = smem_addr(columns) + (lane_token * 4 + (lane & 3)) * 16;
+    const int scale_at = 2048 - lane * 8;
+    uint32_t b[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) b[i] = 0u;
     int n = 0;                     // items so far: buffer n % kBufs, its round n / kBufs
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
@@ -638,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
       const FewPass p = a.pass[pass];
       const int kwi = warp & (p.kw - 1);
       int entry = -1, j = s.entry, u = s.first;
-      float f0 = 1.0f, f1 = 1.0f;
+      float factor = 1.0f;
 #pragma unroll 1
       for (int it = s.begin; it < s.end; ++it) {
         if (j != entry) {
@@ -646,16 +655,14 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
             if (!identity) load_hidden_columns(a, sh, columns, j, cols, false);
           } else {
             load_act_columns(a, sh, columns, j, cols, p.kw);
-            f16_factor(sh.act_amax[kwi][2 * (lane & 3)], &f0);
-            f16_factor(sh.act_amax[kwi][2 * (lane & 3) + 1], &f1);
+            f16_factor(sh.act_amax[kwi][(lane & 3) >> 1], &factor);
           }
           entry = j;
         }
-        float acc[2][4] = {};
+        float acc[2][2] = {};
 #pragma unroll 1
         for (int k = kwi; k < p.units; k += p.kw) {
-          uint32_t b[16];
-          load_b(b, lane_columns, k, cols);
+          load_b(b, lane_columns, k, cols, mine);
           cp_async_wait<kRing - 2>();
           multiply_slot(acc, tail, tail + scale_at, b);
           tail += kSlotBytes;
@@ -666,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
         // barrier; until then the warp keeps step with the others, which meet it at the barriers around their columns.
         const int buf = n % kBufs;
         if (tc::mbar_wait_warp(&sh.empty[buf], ((n / kBufs) & 1) ^ 1u, &sh.abort)) {
-          store_partial(red + buf * red_floats + warp * 32 * pitch, acc, f0, f1, lane, pitch, cols);
+          store_partial(red + buf * red_floats + warp * 32 * cols, acc, factor, lane, cols);
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&sh.full[buf]);
         }
@@ -699,14 +706,15 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a, int c
         alive = tc::mbar_wait_warp(&sh.full[mine], ((base + i) / kBufs) & 1, &sh.abort);
         if (!alive) break;
 #pragma unroll 1
-        for (int q = 0; q < rw * cols; ++q) {
-          const int r = q / cols, c = q - r * cols;
+        for (int q = 0; q < rw * kCols; ++q) {
+          const int r = q / kCols, c = q % kCols;
+          if (c >= cols) continue;
           const int route = sh.ent_route[j][c];
           if (route < 0) continue;
-          const float* src = part + (r * p.kw * 32 + lane) * pitch + c;
+          const float* src = part + (r * p.kw * 32 + lane) * cols + c;
           float sum = 0.0f;
 #pragma unroll 4
-          for (int w = 0; w < warps_k; ++w) sum += src[w * 32 * pitch];
+          for (int w = 0; w < warps_k; ++w) sum += src[w * 32 * cols];
           if (pass == 0) {                             // lanes 0..15 gate, 16..31 up
             sum *= scale2 * sh.x_inv[sh.route_token[route]];
             const float up = __shfl_down_sync(0xffffffffu, sum, 16);
@@ -833,14 +841,13 @@ FewPass few_pass(int k, int groups) {
 namespace {
 size_t few_smem(int ring, int cols, int k) {
   const size_t fixed = (sizeof(FewShared) + 127) & ~static_cast<size_t>(127);
-  const int pitch = cols > 4 ? 8 : cols > 2 ? 4 : cols;
-  return fixed + static_cast<size_t>(ring) * kWarps * kSlotBytes + static_cast<size_t>(kBufs) * kWarps * 32 * pitch * 4 +
+  return fixed + static_cast<size_t>(ring) * kWarps * kSlotBytes + static_cast<size_t>(kBufs) * kWarps * 32 * cols * 4 +
          static_cast<size_t>(cols) * k * 2;
 }
 constexpr size_t kSmemMost = 227 * 1024;
 
 template <int kRing>
-glmrt_status_t launch_ring(const FewArgs& a, int cap, size_t smem, int sm_count, cudaStream_t s) {
+glmrt_status_t launch_ring(const FewArgs& a, size_t smem, int sm_count, cudaStream_t s) {
   static std::atomic<uint64_t> configured{0};
   GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, few_layer_kernel<kRing>, kSmemMost, "cudaFuncSetAttribute(few_layer_kernel)"));
   cudaLaunchConfig_t cfg{};
@@ -855,28 +862,25 @@ glmrt_status_t launch_ring(const FewArgs& a, int cap, size_t smem, int sm_count,
   cfg.numAttrs = 1;
   FewArgs args = a;
   args.grid_step = static_cast<uint32_t>(((uint64_t{1} << 32) + sm_count - 1) / sm_count);
-  cudaError_t err = cudaLaunchKernelEx(&cfg, few_layer_kernel<kRing>, args, cap);
+  cudaError_t err = cudaLaunchKernelEx(&cfg, few_layer_kernel<kRing>, args);
   if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "few_layer_kernel", err);
   GLMRT_LAUNCH_CHECK("few_layer_kernel");
   return GLMRT_STATUS_OK;
 }
 }  // namespace
 
-// Columns per pass over an expert and depth of the stream, from what fits into shared memory: the
-// selection's scratch (36 bytes an expert) lies in the ring, and at least
-// three slots are needed.
+// What fits into shared memory decides the depth of the stream; the selection's scratch (36 bytes an expert) lies in
+// its ring, and at least three slots are needed.
 bool few_fused_supported(const FewArgs& a) {
   static_assert(1024 * 36 <= 3 * kWarps * kSlotBytes, "selection scratch fits the ring");
   // (per_entry < 4096 makes the multiplication by its inverse exact: at most 256 entries)
-  return few_smem(3, 1, std::max(a.hidden, a.inter)) <= kSmemMost && a.experts <= 1024 && a.pass[0].per_entry > 1 &&
+  return few_smem(3, std::min(a.rows, kCols), std::max(a.hidden, a.inter)) <= kSmemMost && a.experts <= 1024 && a.pass[0].per_entry > 1 &&
          a.pass[0].per_entry < 4096 && a.pass[1].per_entry > 1 && a.pass[1].per_entry < 4096;
 }
 glmrt_status_t launch_few_fused(const FewArgs& a, int sm_count, cudaStream_t s) {
-  const int k = std::max(a.hidden, a.inter);
-  int cap = std::min(a.rows, 4);
-  while (cap > 1 && few_smem(3, cap, k) > kSmemMost) --cap;
-  if (few_smem(4, cap, k) <= kSmemMost) return launch_ring<4>(a, cap, few_smem(4, cap, k), sm_count, s);
-  return launch_ring<3>(a, cap, few_smem(3, cap, k), sm_count, s);
+  const size_t four = few_smem(4, std::min(a.rows, kCols), std::max(a.hidden, a.inter));
+  if (four <= kSmemMost) return launch_ring<4>(a, four, sm_count, s);
+  return launch_ring<3>(a, few_smem(3, std::min(a.rows, kCols), std::max(a.hidden, a.inter)), sm_count, s);
 }
 
 glmrt_status_t launch_few_simt(const FewArgs& a, cudaStream_t s) {
