@@ -123,14 +123,21 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 // All CTAs of the grid (co-resident: cooperative launch).  The arrivals of one barrier add up to 2^31: every CTA
 // adds one, the first what is missing.  So the top bit flips when the last has come, and nothing has to be
 // reset.  False when the wait ran out.
-__device__ bool grid_barrier(uint32_t* count, volatile uint32_t* abort) {
+// Arriving and waiting are apart, so that work may lie between them; thread 0 keeps what it saw.
+__device__ __forceinline__ uint32_t grid_arrive(uint32_t* count) {
+  uint32_t old = 0u;
   __syncthreads();
   if (threadIdx.x == 0) {
     const uint32_t add = blockIdx.x == 0 ? 0x80000000u - (gridDim.x - 1) : 1u;
-    uint32_t old, now;
     asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(old) : "l"(count), "r"(add) : "memory");
+  }
+  return old;
+}
+__device__ bool grid_wait(uint32_t* count, uint32_t old, volatile uint32_t* abort) {
+  if (threadIdx.x == 0) {
     uint64_t t0 = 0;
     for (uint32_t spin = 1;; ++spin) {
+      uint32_t now;
       asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(count) : "memory");
       if ((old ^ now) >> 31) break;
       if ((spin & 255u) == 0u) {
@@ -142,6 +149,9 @@ __device__ bool grid_barrier(uint32_t* count, volatile uint32_t* abort) {
   }
   __syncthreads();
   return *abort == 0u;
+}
+__device__ __forceinline__ bool grid_barrier(uint32_t* count, volatile uint32_t* abort) {
+  return grid_wait(count, grid_arrive(count), abort);
 }
 
 // A CTA's share of one of the two weight passes.  How an item of rows is shared by the warps (FewPass: kw along K,
@@ -583,7 +593,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
   if (tid < kFewMaxRows) sh.x_amax[tid] = 0u;
   __syncthreads();
 
-  if (a.scores != nullptr) score_experts(a, sh, warp, lane);
+  uint32_t arrived = 0u;
+  if (a.scores != nullptr) {
+    score_experts(a, sh, warp, lane);
+    arrived = grid_arrive(a.sync);
+  }
   // the rows' largest magnitudes, 256 values a warp
   const int row_pieces = a.hidden / 256;
 #pragma unroll 1
@@ -600,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
   if (tid < a.rows) f16_factor(sh.x_amax[tid], &sh.x_inv[tid]);
   if (identity && warp < kWarps) load_hidden_columns(a, sh, columns, 0, cols, true);    // needs no routes
   if (a.scores != nullptr) {
-    if (!grid_barrier(a.sync, &sh.abort)) {
+    if (!grid_wait(a.sync, arrived, &sh.abort)) {
       if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
       return;
     }
