@@ -20,13 +20,17 @@ _DTYPES = {torch.bfloat16: N.DTYPE_BF16, torch.float32: N.DTYPE_F32}
 _ARGS = struct.Struct("@" + launch.BUFFER * 7 + "8Q2I2f")      # glmrt_b200_block_norm_args_t
 
 
-def _rows(t: torch.Tensor, like: torch.Tensor, rows: int, width: int, what: str) -> tuple[tuple, int]:
+_SIZES = {torch.bfloat16: 2, torch.float32: 4}
+
+
+def _rows(t: torch.Tensor, shape, dtype: torch.dtype, index: int, what: str) -> tuple[tuple, int]:
     """Packed buffer and row stride of a [rows, width] tensor whose rows are contiguous inside."""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
         raise ValueError(f"block_norm: {what} must have the shape, type and device of residual")
-    if width > 1 and t.stride(1) != 1:
+    rows, width = shape
+    if not launch.inner_contiguous(t, width):
         raise ValueError(f"block_norm: {what} must be contiguous along its rows")
-    return launch.rows_buffer(t, rows, width)
+    return launch.rows_buffer(t, rows, width, _SIZES[dtype])
 
 
 def block_norm(residual: torch.Tensor, delta: torch.Tensor | None = None, *, norm_weight: torch.Tensor,
@@ -39,47 +43,55 @@ def block_norm(residual: torch.Tensor, delta: torch.Tensor | None = None, *, nor
     ``normalized`` may be given, also in the place of ``residual`` or ``delta``.  Without ``delta``
     the residual comes back as it is.
     """
-    dtype = _DTYPES.get(residual.dtype)
-    if residual.dim() != 2 or dtype is None:
+    dtype = residual.dtype
+    code = _DTYPES.get(dtype)
+    if residual.dim() != 2 or code is None:
         raise ValueError("block_norm: residual must be [rows, width], bfloat16 or float32")
     if not residual.is_cuda:
         raise ValueError("block_norm: tensors must be on a CUDA device")
-    rows, width = residual.shape
+    shape, index = residual.shape, residual.get_device()
+    rows, width = shape
     if delta is None and (post_weight is not None or gate is not None or residual_out is not None):
         raise ValueError("block_norm: post_weight, gate and residual_out need a delta")
-    wdtype = _DTYPES.get(norm_weight.dtype)
+    wdtype = norm_weight.dtype
+    wcode = _DTYPES.get(wdtype)
     for name, w in (("norm_weight", norm_weight), ("post_weight", post_weight)):
         if w is None:
             continue
-        if w.shape != (width,) or wdtype is None or w.device != residual.device or not w.is_contiguous():
+        if w.dim() != 1 or w.shape[0] != width or wcode is None or w.get_device() != index or not w.is_contiguous():
             raise ValueError(f"block_norm: {name} must be a contiguous [{width}] bfloat16 or float32 tensor on the rows' device")
-        if w.dtype != norm_weight.dtype:
+        if w.dtype is not wdtype:
             raise ValueError("block_norm: norm_weight and post_weight must have one type")
     gate_buf, gate_rs, gate_cs = launch.NO_BUFFER, 0, 0
     if gate is not None:
         if gate.dim() != 2 or gate.shape[0] not in (1, rows) or gate.shape[1] not in (1, width):
             raise ValueError("block_norm: gate must be [rows, 1], [1, width] or [rows, width]")
-        if gate.dtype != residual.dtype or gate.device != residual.device:
+        if gate.dtype is not dtype or gate.get_device() != index:
             raise ValueError("block_norm: gate must have the type and device of residual")
         gate_rs = gate.stride(0) if gate.shape[0] > 1 else 0
         gate_cs = gate.stride(1) if gate.shape[1] > 1 else 0
         if gate_cs > 1:
             raise ValueError("block_norm: gate must be contiguous along its rows")
         span = (gate.shape[0] - 1) * gate_rs + (gate.shape[1] - 1) * gate_cs + 1
-        gate_buf = (gate.data_ptr(), span * gate.element_size(), 0, 0)
+        gate_buf = (gate.data_ptr(), span * _SIZES[dtype], 0, 0)
+    like = residual if residual.is_contiguous() else None
     if normalized is None:
-        normalized = residual.new_empty((rows, width))
-    res, res_stride = _rows(residual, residual, rows, width, "residual")
-    norm, norm_stride = _rows(normalized, residual, rows, width, "normalized")
+        normalized = residual.new_empty(shape) if like is None else torch.empty_like(like)
+        norm, norm_stride = (normalized.data_ptr(), normalized.nbytes, 0, 0), width
+    else:
+        norm, norm_stride = _rows(normalized, shape, dtype, index, "normalized")
+    res, res_stride = _rows(residual, shape, dtype, index, "residual")
     dlt, dlt_stride, out, out_stride = launch.NO_BUFFER, 0, launch.NO_BUFFER, 0
     if delta is not None:
+        dlt, dlt_stride = _rows(delta, shape, dtype, index, "delta")
         if residual_out is None:
-            residual_out = residual.new_empty((rows, width))
-        dlt, dlt_stride = _rows(delta, residual, rows, width, "delta")
-        out, out_stride = _rows(residual_out, residual, rows, width, "residual_out")
+            residual_out = residual.new_empty(shape) if like is None else torch.empty_like(like)
+            out, out_stride = (residual_out.data_ptr(), residual_out.nbytes, 0, 0), width
+        else:
+            out, out_stride = _rows(residual_out, shape, dtype, index, "residual_out")
     if rows:
         launch.call(lib, "glmrt_b200_block_norm_async",
                     _ARGS.pack(*res, *dlt, *launch.buffer(norm_weight), *launch.buffer(post_weight), *gate_buf, *out, *norm,
                                rows, width, res_stride, dlt_stride, gate_rs, gate_cs, out_stride, norm_stride,
-                               dtype, wdtype, scale, eps), residual.device)
+                               code, wcode, scale, eps), index)
     return (residual if delta is None else residual_out), normalized

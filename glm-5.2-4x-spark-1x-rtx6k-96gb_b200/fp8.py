@@ -18,6 +18,8 @@ from . import native as N
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
+_CODE_TYPES = (E4M3, torch.uint8)
+_ROW_TYPES = (torch.bfloat16,)
 _QUANT_ARGS = struct.Struct("@" + launch.BUFFER * 3 + "3QI4x")       # glmrt_b200_fp8_quantize_rows_args_t
 _LINEAR_ARGS = struct.Struct("@" + launch.BUFFER * 5 + "4QI4x")      # glmrt_b200_fp8_block_linear_args_t
 _MLP_ARGS = struct.Struct("@" + launch.BUFFER * 9 + "4Q")            # glmrt_b200_fp8_gated_mlp_args_t
@@ -32,16 +34,16 @@ def _check_rows(x: torch.Tensor, k: int, types: tuple, what: str) -> None:
         raise ValueError(f"{what} must be [rows, {k}] of type {' or '.join(str(t) for t in types)}")
     if not x.is_cuda:
         raise ValueError(f"{what} must be on a CUDA device")
-    if k > 1 and x.stride(1) != 1:
+    if not launch.inner_contiguous(x, k):
         raise ValueError(f"{what} must be contiguous along its rows")
 
 
-def _check_weight(codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, device: torch.device, what: str) -> None:
-    if codes.shape != (n, k) or codes.dtype not in (E4M3, torch.uint8) or not codes.is_contiguous():
+def _check_weight(codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, index: int, what: str) -> None:
+    if codes.shape != (n, k) or codes.dtype not in _CODE_TYPES or not codes.is_contiguous():
         raise ValueError(f"{what} codes must be a contiguous E4M3 (or uint8) tensor [{n}, {k}]")
-    if scales.shape != (_blocks(n), _blocks(k)) or scales.dtype != torch.float32 or not scales.is_contiguous():
+    if scales.shape != (_blocks(n), _blocks(k)) or scales.dtype is not torch.float32 or not scales.is_contiguous():
         raise ValueError(f"{what} scales must be a contiguous float32 tensor [{_blocks(n)}, {_blocks(k)}]")
-    if codes.device != device or scales.device != device:
+    if codes.get_device() != index or scales.get_device() != index:
         raise ValueError(f"{what} must be on the device of the rows")
 
 
@@ -60,12 +62,12 @@ def quantize_rows(x: torch.Tensor, lib: N.NativeLibrary | None = None) -> tuple[
     """The rows' codes ``[rows, k]`` (E4M3) and scales ``[ceil(k/128), rows]``; x bf16 or float32."""
     rows, k = x.shape if x.dim() == 2 else (0, 0)
     _check_rows(x, k, (torch.bfloat16, torch.float32), "quantize_rows: x")
-    buf, stride = launch.rows_buffer(x, rows, k)
+    buf, stride = launch.rows_buffer(x, rows, k, x.element_size())
     codes = torch.empty((rows, k), dtype=E4M3, device=x.device)
     scales = torch.empty((_blocks(k), rows), dtype=torch.float32, device=x.device)
     launch.call(lib, "glmrt_b200_fp8_quantize_rows_async",
                 _QUANT_ARGS.pack(*buf, *launch.buffer(codes), *launch.buffer(scales), rows, k, stride,
-                                 N.DTYPE_BF16 if x.dtype == torch.bfloat16 else N.DTYPE_F32), x.device)
+                                 N.DTYPE_BF16 if x.dtype == torch.bfloat16 else N.DTYPE_F32), x.get_device())
     return codes, scales
 
 
@@ -78,10 +80,14 @@ def _workspace_bytes(lib: N.NativeLibrary, symbol: str, *sizes: int) -> int:
 
 def _output(out: torch.Tensor | None, rows: int, n: int, dtype: torch.dtype, x: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty((rows, n), dtype=dtype, device=x.device)
-    if out.shape != (rows, n) or out.dtype != dtype or out.device != x.device or not out.is_contiguous():
+        return x.new_empty((rows, n)) if dtype is x.dtype else x.new_empty((rows, n), dtype=dtype)
+    if out.shape != (rows, n) or out.dtype is not dtype or out.get_device() != x.get_device() or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {dtype} tensor [{rows}, {n}] on the rows' device")
     return out
+
+
+def _workspace(lib: N.NativeLibrary, symbol: str, x: torch.Tensor, *sizes: int) -> torch.Tensor:
+    return x.new_empty((_workspace_bytes(lib, symbol, *sizes) + 1) // 2)      # of bf16 rows: two bytes each
 
 
 def block_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None = None,
@@ -93,15 +99,16 @@ def block_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out
     n, k = codes.shape
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("block_linear: out_dtype must be bfloat16 or float32")
-    _check_rows(x, k, (torch.bfloat16,), "block_linear: x")
-    _check_weight(codes, scales, n, k, x.device, "block_linear: weight")
+    _check_rows(x, k, _ROW_TYPES, "block_linear: x")
+    index = x.get_device()
+    _check_weight(codes, scales, n, k, index, "block_linear: weight")
     rows = x.shape[0]
-    buf, stride = launch.rows_buffer(x, rows, k)
+    buf, stride = launch.rows_buffer(x, rows, k, 2)
     out = _output(out, rows, n, out_dtype, x)
-    ws = torch.empty(_workspace_bytes(lib, "glmrt_b200_fp8_block_linear_workspace", rows, n, k), dtype=torch.uint8, device=x.device)
+    ws = _workspace(lib, "glmrt_b200_fp8_block_linear_workspace", x, rows, n, k)
     launch.call(lib, "glmrt_b200_fp8_block_linear_async",
                 _LINEAR_ARGS.pack(*buf, *launch.buffer(codes), *launch.buffer(scales), *launch.buffer(out), *launch.buffer(ws),
-                                  rows, n, k, stride, N.DTYPE_BF16 if out_dtype == torch.bfloat16 else N.DTYPE_F32), x.device)
+                                  rows, n, k, stride, N.DTYPE_BF16 if out_dtype is torch.bfloat16 else N.DTYPE_F32), index)
     return out
 
 
@@ -114,16 +121,17 @@ def gated_mlp(x: torch.Tensor, gate_codes: torch.Tensor, gate_scales: torch.Tens
     if gate_codes.dim() != 2:
         raise ValueError("gated_mlp: gate codes must be [inter, hidden]")
     inter, hidden = gate_codes.shape
-    _check_rows(x, hidden, (torch.bfloat16,), "gated_mlp: x")
-    _check_weight(gate_codes, gate_scales, inter, hidden, x.device, "gated_mlp: gate")
-    _check_weight(up_codes, up_scales, inter, hidden, x.device, "gated_mlp: up")
-    _check_weight(down_codes, down_scales, hidden, inter, x.device, "gated_mlp: down")
+    _check_rows(x, hidden, _ROW_TYPES, "gated_mlp: x")
+    index = x.get_device()
+    _check_weight(gate_codes, gate_scales, inter, hidden, index, "gated_mlp: gate")
+    _check_weight(up_codes, up_scales, inter, hidden, index, "gated_mlp: up")
+    _check_weight(down_codes, down_scales, hidden, inter, index, "gated_mlp: down")
     rows = x.shape[0]
-    buf, stride = launch.rows_buffer(x, rows, hidden)
+    buf, stride = launch.rows_buffer(x, rows, hidden, 2)
     out = _output(out, rows, hidden, torch.bfloat16, x)
-    ws = torch.empty(_workspace_bytes(lib, "glmrt_b200_fp8_gated_mlp_workspace", rows, hidden, inter), dtype=torch.uint8, device=x.device)
+    ws = _workspace(lib, "glmrt_b200_fp8_gated_mlp_workspace", x, rows, hidden, inter)
     b = launch.buffer
     launch.call(lib, "glmrt_b200_fp8_gated_mlp_async",
                 _MLP_ARGS.pack(*buf, *b(gate_codes), *b(gate_scales), *b(up_codes), *b(up_scales), *b(down_codes),
-                               *b(down_scales), *b(out), *b(ws), rows, hidden, inter, stride), x.device)
+                               *b(down_scales), *b(out), *b(ws), rows, hidden, inter, stride), index)
     return out

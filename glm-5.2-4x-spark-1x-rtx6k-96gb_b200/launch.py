@@ -20,20 +20,29 @@ def buffer(t: torch.Tensor | None) -> tuple:
     return NO_BUFFER if t is None else (t.data_ptr(), t.nbytes, 0, 0)
 
 
-def rows_buffer(t: torch.Tensor, rows: int, width: int) -> tuple[tuple, int]:
-    """Packed fields and row stride (elements) of [rows, width] with rows contiguous inside."""
-    stride = t.stride(0) if rows > 1 else width
-    return (t.data_ptr(), ((rows - 1) * stride + width) * t.element_size() if rows else 0, 0, 0), stride
+def rows_buffer(t: torch.Tensor, rows: int, width: int, size: int) -> tuple[tuple, int]:
+    """Packed fields and row stride (elements) of [rows, width] with rows contiguous inside, `size` bytes a value."""
+    if rows == 1 or t.is_contiguous():
+        return (t.data_ptr(), rows * width * size, 0, 0), width
+    stride = t.stride(0)
+    return (t.data_ptr(), ((rows - 1) * stride + width) * size if rows else 0, 0, 0), stride
 
 
-def call(lib: N.NativeLibrary | None, symbol: str, packed: bytes, device: torch.device) -> None:
+def inner_contiguous(t: torch.Tensor, width: int) -> bool:
+    return width <= 1 or t.is_contiguous() or t.stride(1) == 1
+
+
+def call(lib: N.NativeLibrary | None, symbol: str, packed: bytes, index: int) -> None:
+    """``symbol(packed, current stream of device index)``; raises what NativeLibrary.call raises."""
     lib = lib or N.library()
-    index = device.index
+    fn = lib.symbol(symbol)
     if index == torch.cuda.current_device():
-        lib.call(symbol, packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
+        status = fn(packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
     else:
         with torch.cuda.device(index):
-            lib.call(symbol, packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
+            status = fn(packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
+    if status != 0:
+        raise N.GlmrtError(symbol, status, lib.last_error())
 
 
 def check(lib: N.NativeLibrary | None = None) -> None:
