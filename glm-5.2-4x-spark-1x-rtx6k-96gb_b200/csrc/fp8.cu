@@ -133,7 +133,7 @@ extern "C" glmrt_status_t glmrt_b200_fp8_quantize_rows_async(const glmrt_b200_fp
 extern "C" glmrt_status_t glmrt_b200_fp8_block_linear_workspace(size_t rows, size_t n, size_t k, size_t* out_bytes) {
   if (out_bytes == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "fp8_block_linear_workspace: null output");
   GLMRT_RETURN_IF_ERROR(check_dims(rows, n, k, "fp8_block_linear"));
-  *out_bytes = rows_bytes(rows, k);
+  *out_bytes = rows <= kFp8OwnRows ? 0 : rows_bytes(rows, k);
   return ok();
 }
 
@@ -149,15 +149,16 @@ extern "C" glmrt_status_t glmrt_b200_fp8_block_linear_async(const glmrt_b200_fp8
   GLMRT_RETURN_IF_ERROR(check_buffer(weight_codes, n * k, 16, "fp8_block_linear weight_codes"));
   GLMRT_RETURN_IF_ERROR(check_buffer(weight_scales, blocks_of(n) * blocks_of(k) * 4, 4, "fp8_block_linear weight_scales"));
   GLMRT_RETURN_IF_ERROR(check_buffer(output, rows * n * osize, osize, "fp8_block_linear output"));
-  GLMRT_RETURN_IF_ERROR(check_buffer(workspace, rows_bytes(rows, k), 256, "fp8_block_linear workspace"));
+  if (rows > kFp8OwnRows) GLMRT_RETURN_IF_ERROR(check_buffer(workspace, rows_bytes(rows, k), 256, "fp8_block_linear workspace"));
   GLMRT_RETURN_IF_ERROR(require_cuda());
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   uint8_t* codes = static_cast<uint8_t*>(workspace.ptr);
   float* scales = reinterpret_cast<float*>(codes + round256(rows * k));
-  GLMRT_RETURN_IF_ERROR(launch_quantize(x_bf16.ptr, GLMRT_B200_DTYPE_BF16, x_row_stride, codes, scales, rows, k, padded(rows), s));
+  const bool own = rows <= kFp8OwnRows;      // the product quantises so few rows itself
+  if (!own) GLMRT_RETURN_IF_ERROR(launch_quantize(x_bf16.ptr, GLMRT_B200_DTYPE_BF16, x_row_stride, codes, scales, rows, k, padded(rows), s));
   Fp8Gemm g{codes, scales, static_cast<const uint8_t*>(weight_codes.ptr), nullptr, static_cast<const float*>(weight_scales.ptr),
             nullptr, output.ptr, nullptr, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k),
-            static_cast<int>(padded(rows)), 0};
+            static_cast<int>(padded(rows)), 0, own ? static_cast<const uint16_t*>(x_bf16.ptr) : nullptr, x_row_stride};
   GLMRT_RETURN_IF_ERROR(launch_fp8_gemm(g, out_dtype == GLMRT_B200_DTYPE_BF16 ? 0 : 1, s));
   return ok();
 }
@@ -166,7 +167,7 @@ extern "C" glmrt_status_t glmrt_b200_fp8_gated_mlp_workspace(size_t rows, size_t
   if (out_bytes == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "fp8_gated_mlp_workspace: null output");
   GLMRT_RETURN_IF_ERROR(check_dims(rows, inter, hidden, "fp8_gated_mlp"));
   GLMRT_RETURN_IF_ERROR(check_dims(rows, hidden, inter, "fp8_gated_mlp"));
-  *out_bytes = rows_bytes(rows, hidden) + rows_bytes(rows, inter);
+  *out_bytes = (rows <= kFp8OwnRows ? 0 : rows_bytes(rows, hidden)) + rows_bytes(rows, inter);
   return ok();
 }
 
@@ -193,12 +194,14 @@ extern "C" glmrt_status_t glmrt_b200_fp8_gated_mlp_async(const glmrt_b200_fp8_ga
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   uint8_t* xq = static_cast<uint8_t*>(workspace.ptr);
   float* xs = reinterpret_cast<float*>(xq + round256(rows * hidden));
-  uint8_t* aq = xq + rows_bytes(rows, hidden);
+  uint8_t* aq = rows <= kFp8OwnRows ? xq : xq + rows_bytes(rows, hidden);
   float* as = reinterpret_cast<float*>(aq + round256(rows * inter));
-  GLMRT_RETURN_IF_ERROR(launch_quantize(x_bf16.ptr, GLMRT_B200_DTYPE_BF16, x_row_stride, xq, xs, rows, hidden, padded(rows), s));
+  const bool own = rows <= kFp8OwnRows;      // the product quantises so few rows itself
+  if (!own) GLMRT_RETURN_IF_ERROR(launch_quantize(x_bf16.ptr, GLMRT_B200_DTYPE_BF16, x_row_stride, xq, xs, rows, hidden, padded(rows), s));
   const int m = static_cast<int>(rows), h = static_cast<int>(hidden), i = static_cast<int>(inter), pad = static_cast<int>(padded(rows));
   const Fp8Gemm up{xq, xs, static_cast<const uint8_t*>(gate_codes.ptr), static_cast<const uint8_t*>(up_codes.ptr),
-                   static_cast<const float*>(gate_scales.ptr), static_cast<const float*>(up_scales.ptr), aq, as, m, i, h, pad, pad};
+                   static_cast<const float*>(gate_scales.ptr), static_cast<const float*>(up_scales.ptr), aq, as, m, i, h, pad, pad,
+                   own ? static_cast<const uint16_t*>(x_bf16.ptr) : nullptr, x_row_stride};
   const Fp8Gemm down{aq, as, static_cast<const uint8_t*>(down_codes.ptr), nullptr, static_cast<const float*>(down_scales.ptr),
                      nullptr, output_bf16.ptr, nullptr, m, h, i, pad, 0};
   GLMRT_RETURN_IF_ERROR(launch_fp8_gemm(up, 2, s));

@@ -30,6 +30,25 @@ using namespace tc;
 
 __device__ uint32_t g_fp8_error;       // kErrWaitTimeout when a bounded wait ran out (glmrt_b200_operators_check)
 
+// Brings a box into the L2.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+// Eight bf16 values as float32, zeros past the row's end (rows are multiples of 16 values).
+__device__ __forceinline__ void quantise_load(const uint16_t* src, bool in, bool vec, float (&v)[8]) {
+  uint16_t t[8] = {};
+  if (in) {
+    if (vec) {
+      *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(src);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = src[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = bf16_bits_to_f32(t[i]);
+}
+
 __device__ __forceinline__ void tc_mma_fp8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -349,48 +368,57 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
 // Few rows
 // ---------------------------------------------------------------------------------------------------
 struct WeightsArgs {
-  const float* xs;            // [blocks][xs_stride]
+  const float* xs;            // [blocks][xs_stride] (quantised in the kernel: unused)
+  const uint16_t* x;          // bf16 rows x_stride apart, quantised in the kernel; else unused
+  size_t x_stride;
+  int x_vector;               // the rows start on 16-byte boundaries
   const float *ws0, *ws1;
   void* out;
   float* out_scales;
   int rows, n, k, xs_stride, out_stride;
 };
 
-template <int kMode, int kN>
+// kOwnX: the rows are bf16 and every CTA quantises the blocks it needs itself (a few rows: one launch less than
+// quantising them first, and no workspace); their codes lie beside the ring, kXBlocks blocks at a time.
+template <int kMode, int kN, bool kOwnX>
 struct WCfg {
   static constexpr int kMats = kMode == 2 ? 2 : 1;
-  static constexpr int kStageBytes = kMats * kTileBytes + kN * kFp8Block;
+  static constexpr int kStageBytes = kMats * kTileBytes + (kOwnX ? 0 : kN * kFp8Block);
+  static constexpr int kXBlocks = kMode == 2 ? 6 : 8;
+  static constexpr int kXBytes = kOwnX ? kXBlocks * kN * kFp8Block : 0;
   static constexpr int kAccCols = kMats * kN;                       // of one block
   // Two CTAs on an SM where the sums leave the registers for it: twice as many chains of copy, product and
   // read-out side by side, and twice as many splits of a tile.
   static constexpr int kPerSm = kAccCols <= 64 ? 2 : 1;
-  static constexpr int kRingBytes = kPerSm == 2 ? 104448 : 184320;
+  static constexpr int kRingBytes = (kPerSm == 2 ? (kOwnX ? 111616 : 104448) : 184320) - kXBytes;
   static constexpr int kStages = kRingBytes / kStageBytes < 8 ? kRingBytes / kStageBytes : 8;
-  static constexpr int kScaleBlocks = 16;                           // blocks whose scales are kept in shared memory
+  static constexpr int kScaleBlocks = kOwnX ? kXBlocks : 16;        // blocks whose scales are kept in shared memory
   static constexpr int kTmemCols = 2 * kAccCols < 32 ? 32 : 2 * kAccCols;
   static constexpr int kParts = kAccCols > 64 ? 2 : 1;              // epilogue warps per tensor-memory quadrant, by columns
   static constexpr int kEpiWarps = 4 * kParts;
   static constexpr int kCols = kN / kParts;                         // of each matrix, per thread
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
-  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + 1024 + 512 + kScaleBlocks * (kN + kMats) * 4;
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kXBytes + 1024 + 512 + kScaleBlocks * (kN + kMats) * 4;
   static_assert(static_cast<size_t>(kStages) * kStageBytes >= static_cast<size_t>(kMats) * kN * 128 * 4, "partial sums reuse the ring");
 };
 
 // grid (weight tiles, splits, row tiles), cluster (1, splits, 1).
-template <int kMode, int kN>
-__global__ void __launch_bounds__(WCfg<kMode, kN>::kThreads, WCfg<kMode, kN>::kPerSm)
+template <int kMode, int kN, bool kOwnX>
+__global__ void __launch_bounds__(WCfg<kMode, kN, kOwnX>::kThreads, WCfg<kMode, kN, kOwnX>::kPerSm)
 fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w0,
                    const __grid_constant__ CUtensorMap map_w1) {
-  using C = WCfg<kMode, kN>;
+  using C = WCfg<kMode, kN, kOwnX>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes);
+  uint8_t* x_codes = smem + static_cast<size_t>(C::kStages) * C::kStageBytes;      // kOwnX: [kXBlocks] tiles of kN rows
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(x_codes + C::kXBytes);
   uint64_t* empty_bar = full_bar + C::kStages;
   uint64_t* acc_full = empty_bar + C::kStages;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* x_full = acc_empty + 2;                                                 // kOwnX: a group of blocks is quantised
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_full + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  float* sx_all = reinterpret_cast<float*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes + 512);   // [kScaleBlocks][kN]
+  float* sx_all = reinterpret_cast<float*>(x_codes + C::kXBytes + 512);   // [kScaleBlocks][kN]
   float* sw_all = sx_all + C::kScaleBlocks * kN;                              // [kMats][kScaleBlocks]
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -413,6 +441,7 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], C::kEpiWarps);
     }
+    mbar_init(x_full, C::kEpiWarps);
     *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -424,8 +453,9 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
-    // The weights do not come from the previous kernel, and that kernel let this one start only after everything
-    // before it had finished: the first stages' weights are asked for before its rows are waited for.
+    // The previous kernel of this call let this one start only after everything before it had finished, and wrote no
+    // weights: the first stages' weights are asked for before its rows are waited for.  Where this kernel is the
+    // call's first, they are only brought into the L2 until then.
     const uint64_t pol = policy_evict_first();
     auto load_w = [&](int stage, int b) {
       const uint32_t s_a = smem_u32(smem + static_cast<size_t>(stage) * C::kStageBytes);
@@ -439,12 +469,22 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
     };
     const int ahead = min(C::kStages, b1 - b0);
     if (elect_one())
-      for (int i = 0; i < ahead; ++i) load_w(i, b0 + i);
+      for (int i = 0; i < ahead; ++i) {
+        if constexpr (kOwnX) {
+          tma_prefetch_2d(&map_w0, (b0 + i) * kFp8Block, w0);
+          if (kMode == 2) tma_prefetch_2d(&map_w1, (b0 + i) * kFp8Block, w0);
+        } else {
+          load_w(i, b0 + i);
+        }
+      }
     __syncwarp();
     pdl_wait();
     pdl_launch_dependents();
     if (elect_one())
-      for (int i = 0; i < ahead; ++i) load_x(i, b0 + i);
+      for (int i = 0; i < ahead; ++i) {
+        if constexpr (kOwnX) load_w(i, b0 + i);
+        else load_x(i, b0 + i);
+      }
     __syncwarp();
     int stage = 0;
     uint32_t phase = 0;
@@ -452,7 +492,7 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
       if (!mbar_wait_hot(&empty_bar[stage], phase, abort_flag)) break;
       if (elect_one()) {
         load_w(stage, b);
-        load_x(stage, b);
+        if constexpr (!kOwnX) load_x(stage, b);
       }
       __syncwarp();
       if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
@@ -462,12 +502,17 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
     int stage = 0, abuf = 0;
     uint32_t phase = 0, aphase = 0;
     const uint32_t idesc = idesc_fp8(kN);
+    uint32_t xphase = 0;
     for (int b = b0; b < b1; ++b) {
+      if (kOwnX && (b - b0) % C::kXBlocks == 0) {
+        if (!mbar_wait_hot(x_full, xphase, abort_flag)) break;
+        xphase ^= 1u;
+      }
       if (!mbar_wait_hot(&acc_empty[abuf], aphase ^ 1u, abort_flag) ||
           !mbar_wait_hot(&full_bar[stage], phase, abort_flag)) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t s_a = smem_u32(smem + static_cast<size_t>(stage) * C::kStageBytes), s_x = s_a + C::kMats * kTileBytes;
+        const uint32_t s_a = smem_u32(smem + static_cast<size_t>(stage) * C::kStageBytes), s_x = kOwnX ? smem_u32(x_codes) + (b - b0) % C::kXBlocks * kN * kFp8Block : s_a + C::kMats * kTileBytes;
 #pragma unroll
         for (int mat = 0; mat < C::kMats; ++mat)
 #pragma unroll
@@ -502,9 +547,34 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
       if (at == 0) {              // the scales of the next blocks (rows padded to whole tiles)
         const int count = min(C::kScaleBlocks, b1 - b);
         asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kEpiWarps) : "memory");
-        for (int i = tid; i < count * (kN / 4); i += 32 * C::kEpiWarps)
-          reinterpret_cast<float4*>(sx_all)[i] = *reinterpret_cast<const float4*>(
-              a.xs + static_cast<size_t>(b + i / (kN / 4)) * a.xs_stride + m0 + (i % (kN / 4)) * 4);
+        if constexpr (kOwnX) {
+          // The products of the blocks before have all been read out, so their codes may go.  Half a warp per (row,
+          // block), eight values a lane, stored where the 128-byte swizzle puts them.
+          const int sub = tid % 16, rows = min(kN, a.rows - m0);
+          for (int i = tid / 16; i < count * rows; i += 2 * C::kEpiWarps) {
+            const int row = i / count, bb = i - row * count, c = (b + bb) * kFp8Block + sub * 8;
+            float v[8];
+            quantise_load(a.x + static_cast<size_t>(m0 + row) * a.x_stride + c, c < a.k, a.x_vector != 0, v);
+            uint32_t amax = 0u;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(v[e]) & 0x7fffffffu);
+            const uint32_t half = 0xffffu << (threadIdx.x & 16);       // the lanes of this row and block
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(half, amax, o));
+            float inv;
+            const float scale = fp8_block_scale(amax, &inv);
+            *reinterpret_cast<uint2*>(x_codes + bb * kN * kFp8Block + row * kFp8Block + (((sub >> 1) ^ (row & 7)) << 4) + (sub & 1) * 8) =
+                make_uint2(fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv), fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+            if (sub == 0) sx_all[bb * kN + row] = scale;
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(x_full);
+        } else {
+          for (int i = tid; i < count * (kN / 4); i += 32 * C::kEpiWarps)
+            reinterpret_cast<float4*>(sx_all)[i] = *reinterpret_cast<const float4*>(
+                a.xs + static_cast<size_t>(b + i / (kN / 4)) * a.xs_stride + m0 + (i % (kN / 4)) * 4);
+        }
         if (tid < count) {
           sw_all[tid] = __ldg(a.ws0 + wb + b + tid);
           if (kMode == 2) sw_all[(C::kMats - 1) * C::kScaleBlocks + tid] = __ldg(a.ws1 + wb + b + tid);
@@ -634,9 +704,9 @@ constexpr int kMaxDevices = 64;
 
 // Clusters of `splits` CTAs that run at once on the current device (they must fit into one GPC each, so this is
 // less than the SMs divided by the size); asked once per device.
-template <int kMode, int kN>
+template <int kMode, int kN, bool kOwnX>
 int active_clusters(int splits) {
-  using C = WCfg<kMode, kN>;
+  using C = WCfg<kMode, kN, kOwnX>;
   static std::atomic<int> known[kMaxDevices][9];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -652,7 +722,7 @@ int active_clusters(int splits) {
     attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = static_cast<unsigned>(splits); attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, fp8_weights_kernel<kMode, kN>, &cfg) != cudaSuccess) {
+    if (cudaOccupancyMaxActiveClusters(&n, fp8_weights_kernel<kMode, kN, kOwnX>, &cfg) != cudaSuccess) {
       cudaGetLastError();
       return 0;
     }
@@ -664,34 +734,35 @@ int active_clusters(int splits) {
 // CTAs of a cluster that share a tile's K blocks: the number with the shortest estimated time.  A wave of CTAs
 // costs about 3 us beside its blocks (set-up, first copies, joining), a block 0.42 us and 0.0015 us per column of
 // the sum (measured at 16 to 256 rows and 2048 to 6144 columns of K).
-template <int kMode, int kN>
+template <int kMode, int kN, bool kOwnX>
 int weight_splits(int tiles, int blocks, float* estimate_us) {
   int best = 1;
   float best_us = 0.0f;
   for (int s = 1; s <= 8 && s <= blocks; ++s) {
-    const int active = active_clusters<kMode, kN>(s);
+    const int active = active_clusters<kMode, kN, kOwnX>(s);
     if (active <= 0) continue;
     const float us = static_cast<float>((tiles + active - 1) / active) *
-                     (3.0f + (s > 1 ? 0.7f : 0.0f) + static_cast<float>((blocks + s - 1) / s) * (0.42f + 0.0015f * WCfg<kMode, kN>::kAccCols));
+                     (3.0f + (s > 1 ? 0.7f : 0.0f) + static_cast<float>((blocks + s - 1) / s) * (0.42f + 0.0015f * WCfg<kMode, kN, kOwnX>::kAccCols));
     if (best_us == 0.0f || us < best_us) { best = s; best_us = us; }
   }
   *estimate_us = best_us;
   return best;
 }
 
-template <int kMode, int kN>
+template <int kMode, int kN, bool kOwnX = false>
 glmrt_status_t launch_weights(const Fp8Gemm& g, cudaStream_t s) {
-  using C = WCfg<kMode, kN>;
+  using C = WCfg<kMode, kN, kOwnX>;
   static std::atomic<uint64_t> configured{0};
-  GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, fp8_weights_kernel<kMode, kN>, C::kSmem, "cudaFuncSetAttribute(fp8_weights_kernel)"));
+  GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, fp8_weights_kernel<kMode, kN, kOwnX>, C::kSmem, "cudaFuncSetAttribute(fp8_weights_kernel)"));
   float us = 0.0f;
-  const int splits = weight_splits<kMode, kN>((g.n + 127) / 128 * ((g.rows + kN - 1) / kN), (g.k + kFp8Block - 1) / kFp8Block, &us);
+  const int splits = weight_splits<kMode, kN, kOwnX>((g.n + 127) / 128 * ((g.rows + kN - 1) / kN), (g.k + kFp8Block - 1) / kFp8Block, &us);
   CUtensorMap mx, m0, m1;
-  GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&mx, g.x, g.rows, g.k, kN));
   GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&m0, g.w0, g.n, g.k, 128));
   if (kMode == 2) GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&m1, g.w1, g.n, g.k, 128));
   else m1 = m0;
-  WeightsArgs a{g.xs, g.ws0, g.ws1, g.out, g.out_scales, g.rows, g.n, g.k, g.xs_stride, g.out_stride};
+  if (kOwnX) mx = m0;
+  else GLMRT_RETURN_IF_ERROR(make_bytes_tensor_map(&mx, g.x, g.rows, g.k, kN));
+  WeightsArgs a{g.xs, g.x_bf16, g.x_stride, g.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(g.x_bf16) % 16 == 0, g.ws0, g.ws1, g.out, g.out_scales, g.rows, g.n, g.k, g.xs_stride, g.out_stride};
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>((g.n + 127) / 128), static_cast<unsigned>(splits), static_cast<unsigned>((g.rows + kN - 1) / kN));
   cfg.blockDim = dim3(C::kThreads);
@@ -704,7 +775,7 @@ glmrt_status_t launch_weights(const Fp8Gemm& g, cudaStream_t s) {
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaError_t err = cudaLaunchKernelEx(&cfg, fp8_weights_kernel<kMode, kN>, a, mx, m0, m1);
+  cudaError_t err = cudaLaunchKernelEx(&cfg, fp8_weights_kernel<kMode, kN, kOwnX>, a, mx, m0, m1);
   if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "fp8_weights_kernel", err);
   GLMRT_LAUNCH_CHECK("fp8_weights_kernel");
   return GLMRT_STATUS_OK;
@@ -750,6 +821,7 @@ constexpr int kWeightsMostRows = 1024;
 template <int kMode>
 glmrt_status_t launch_mode(const Fp8Gemm& g, cudaStream_t s) {
   constexpr int kMostN = kMode == 2 ? 64 : 128;
+  if (g.x_bf16 != nullptr) return launch_weights<kMode, 16, true>(g, s);      // at most kFp8OwnRows rows
   if (g.rows <= 16) return launch_weights<kMode, 16>(g, s);
   if (g.rows <= 32) return launch_weights<kMode, 32>(g, s);
   if (g.rows <= 64) return launch_weights<kMode, 64>(g, s);
@@ -757,14 +829,14 @@ glmrt_status_t launch_mode(const Fp8Gemm& g, cudaStream_t s) {
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev);
   if (g.rows <= kWeightsMostRows) {
-    using C = WCfg<kMode, kMostN>;
+    using C = WCfg<kMode, kMostN, false>;
     static std::atomic<uint64_t> configured{0};
-    GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, fp8_weights_kernel<kMode, kMostN>, C::kSmem, "cudaFuncSetAttribute(fp8_weights_kernel)"));
+    GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, fp8_weights_kernel<kMode, kMostN, false>, C::kSmem, "cudaFuncSetAttribute(fp8_weights_kernel)"));
     const int blocks = (g.k + kFp8Block - 1) / kFp8Block, per_tile = kMode == 2 ? 128 : kPairN;
     const int tiles = (g.n + 127) / 128 * ((g.rows + kMostN - 1) / kMostN);
     const int row_tiles = (g.n + per_tile - 1) / per_tile * ((g.rows + 255) / 256), pairs = sm_count / 2;
     float us = 0.0f;
-    weight_splits<kMode, kMostN>(tiles, blocks, &us);
+    weight_splits<kMode, kMostN, false>(tiles, blocks, &us);
     if (us < static_cast<float>((row_tiles + pairs - 1) / pairs) * (4.0f + 0.48f * static_cast<float>(blocks)))
       return launch_weights<kMode, kMostN>(g, s);
   }

@@ -75,7 +75,7 @@ def quantize_rows(x: torch.Tensor, lib: N.NativeLibrary | None = None) -> tuple[
 def _workspace_bytes(lib: N.NativeLibrary, symbol: str, *sizes: int) -> int:
     need = C.c_size_t(0)
     lib.call(symbol, *[C.c_size_t(v) for v in sizes], C.byref(need))
-    return max(need.value, 1)
+    return need.value
 
 
 def _output(out: torch.Tensor | None, rows: int, n: int, dtype: torch.dtype, x: torch.Tensor) -> torch.Tensor:
@@ -86,8 +86,9 @@ def _output(out: torch.Tensor | None, rows: int, n: int, dtype: torch.dtype, x: 
     return out
 
 
-def _workspace(lib: N.NativeLibrary, symbol: str, x: torch.Tensor, *sizes: int) -> torch.Tensor:
-    return x.new_empty((_workspace_bytes(lib, symbol, *sizes) + 1) // 2)      # of bf16 rows: two bytes each
+def _workspace(lib: N.NativeLibrary, symbol: str, x: torch.Tensor, *sizes: int) -> torch.Tensor | None:
+    need = _workspace_bytes(lib, symbol, *sizes)
+    return x.new_empty((need + 1) // 2) if need else None                     # of bf16 rows: two bytes each
 
 
 def block_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None = None,

@@ -427,7 +427,8 @@ glmrt_status_t glmrt_b200_operators_check(void* cuda_stream);
 /* as 2^-100; a block with a NaN or an infinity makes its row's outputs NaN).      */
 /* float32 sums.  k is a multiple of 16 and weight codes are 16-byte aligned;     */
 /* rows, n and the last block may be ragged, rows 0 is accepted.  `workspace` is   */
-/* 256-byte aligned device memory of the stated size; it carries nothing from one  */
+/* 256-byte aligned device memory of the stated size (null where that is 0, as for */
+/* a linear of at most 4 rows); it carries nothing from one                        */
 /* call to the next, and calls that may overlap need one each.                     */
 /* ------------------------------------------------------------------------ */
 /* bf16 / float32 rows (input_row_stride elements apart) -> codes [rows, cols], scales

@@ -228,7 +228,7 @@ def test_fp8_row_blocks_of_zeros_tiny_values_and_non_finite_values(mods):
     assert (y[0] == 0).all()
 
 
-LINEAR = [(1, 1, 16), (1, 4096, 6144), (2, 128, 128), (7, 130, 272), (16, 257, 2048), (17, 384, 144), (33, 1500, 2000),
+LINEAR = [(1, 1, 16), (1, 4096, 6144), (2, 128, 128), (3, 140, 16384), (4, 6144, 2064), (4, 20000, 272), (5, 200, 400), (7, 130, 272), (16, 257, 2048), (17, 384, 144), (33, 1500, 2000),
           (64, 640, 6144), (65, 96, 512), (128, 512, 1040), (129, 1000, 256), (197, 1500, 2000), (300, 6144, 2048),
           (777, 516, 400), (2048, 768, 1024), (1, 8, 16384), (520, 4100, 144)]
 
@@ -306,7 +306,7 @@ def mlp_ref(x, gate, up, down):
     return xq @ wd.T, (near + flip) @ wd.abs().T + roundings(inter) * ULP * (xq.abs() @ wd.abs().T)
 
 
-@pytest.mark.parametrize("rows,hidden,inter", [(1, 6144, 2048), (1, 128, 128), (3, 256, 144), (16, 1024, 400), (40, 528, 640),
+@pytest.mark.parametrize("rows,hidden,inter", [(1, 6144, 2048), (1, 128, 128), (3, 256, 144), (4, 8192, 1536), (5, 1024, 400), (16, 1024, 400), (40, 528, 640),
                                                (64, 6144, 2048), (65, 512, 272), (300, 2048, 1040), (1030, 1536, 768)])
 def test_fp8_gated_mlp(mods, rows, hidden, inter):
     x = randn(rows, rows, hidden, dtype=torch.bfloat16)

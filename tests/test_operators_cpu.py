@@ -68,10 +68,11 @@ def test_fp8_refusals(lib):
     assert lib.call_status("glmrt_b200_fp8_block_linear_workspace", Z(4), Z(64), Z(128), None) == 1
     for rows, n, k in ((4, 0, 128), (4, 64, 0), (4, 64, 120), (1 << 25, 64, 128), (4, 1 << 25, 128), (4, 64, 1 << 25)):
         assert lib.call_status("glmrt_b200_fp8_block_linear_workspace", Z(rows), Z(n), Z(k), C.byref(need)) == 1
-    assert lib.call_status("glmrt_b200_fp8_block_linear_workspace", Z(4), Z(64), Z(128), C.byref(need)) == 0 and need.value > 0
+    assert lib.call_status("glmrt_b200_fp8_block_linear_workspace", Z(4), Z(64), Z(128), C.byref(need)) == 0 and need.value == 0
+    assert lib.call_status("glmrt_b200_fp8_block_linear_workspace", Z(17), Z(64), Z(128), C.byref(need)) == 0 and need.value > 0
     ws = buf(0x100000, need.value)
 
-    def linear(x=buf(0x10000, 1024), c=buf(0x20000, 64 * 128), s=buf(0x30000, 4), o=buf(0x40000, 512), w=ws, rows=4, n=64, k=128,
+    def linear(x=buf(0x10000, 17 * 256), c=buf(0x20000, 64 * 128), s=buf(0x30000, 4), o=buf(0x40000, 17 * 128), w=ws, rows=17, n=64, k=128,
                stride=128, dtype=0):
         return lib.call_status("glmrt_b200_fp8_block_linear_async", C.byref(N.Fp8BlockLinearArgs(x, c, s, o, w, rows, n, k, stride, dtype)), None)
 
@@ -79,9 +80,9 @@ def test_fp8_refusals(lib):
     assert linear(dtype=2) == 1 and linear(stride=127) == 1 and linear(k=120) == 1
     for name in "xcsow":
         assert linear(**{name: null}) == 1, name
-    assert linear(x=buf(0x10000, 1023)) == 2 and linear(c=buf(0x20000, 8191)) == 2 and linear(s=buf(0x30000, 3)) == 2
-    assert linear(o=buf(0x40000, 511)) == 2 and linear(w=buf(0x100000, need.value - 1)) == 2
-    assert linear(o=buf(0x40000, 512), dtype=1) == 2
+    assert linear(x=buf(0x10000, 17 * 256 - 1)) == 2 and linear(c=buf(0x20000, 8191)) == 2 and linear(s=buf(0x30000, 3)) == 2
+    assert linear(o=buf(0x40000, 17 * 128 - 1)) == 2 and linear(w=buf(0x100000, need.value - 1)) == 2
+    assert linear(o=buf(0x40000, 17 * 128), dtype=1) == 2
     assert linear(c=buf(0x20008, 64 * 128)) == 1 and linear(w=buf(0x100010, need.value)) == 1
 
     def rows(x=buf(0x10000, 1024), c=buf(0x20000, 512), s=buf(0x30000, 16), n=4, cols=128, stride=128, dtype=0):
