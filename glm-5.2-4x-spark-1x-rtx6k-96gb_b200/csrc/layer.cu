@@ -811,11 +811,11 @@ bool few_fused(const Layer* l, const FewArgs& a) {
 
 }  // namespace
 
-extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_async(
-    void* layer, glmrt_device_buffer_t hidden_bf16, size_t rows, glmrt_device_buffer_t residual_bf16,
-    glmrt_device_buffer_t shared_delta_bf16, glmrt_device_buffer_t output_bf16, glmrt_device_buffer_t topk_indices,
-    glmrt_device_buffer_t topk_weights, void* cuda_stream) {
+extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_async(void* layer, const glmrt_b200_few_args_t* args,
+                                                                 void* cuda_stream) {
   Layer* l = static_cast<Layer*>(layer);
+  if (args == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "forward_few: null arguments");
+  const auto& [hidden_bf16, residual_bf16, shared_delta_bf16, output_bf16, topk_indices, topk_weights, rows] = *args;
   FewArgs a{};
   GLMRT_RETURN_IF_ERROR(few_args(l, hidden_bf16, rows, residual_bf16, shared_delta_bf16, output_bf16, &a));
   const size_t routes = rows * l->cfg.top_k;
@@ -844,11 +844,11 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_async(
   return ok();
 }
 
-extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_routed_async(
-    void* layer, glmrt_device_buffer_t hidden_bf16, size_t rows, glmrt_device_buffer_t topk_indices,
-    glmrt_device_buffer_t topk_weights, glmrt_device_buffer_t residual_bf16, glmrt_device_buffer_t shared_delta_bf16,
-    glmrt_device_buffer_t output_bf16, void* cuda_stream) {
+extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_routed_async(void* layer, const glmrt_b200_few_args_t* args,
+                                                                        void* cuda_stream) {
   Layer* l = static_cast<Layer*>(layer);
+  if (args == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "forward_few_routed: null arguments");
+  const auto& [hidden_bf16, residual_bf16, shared_delta_bf16, output_bf16, topk_indices, topk_weights, rows] = *args;
   FewArgs a{};
   GLMRT_RETURN_IF_ERROR(few_args(l, hidden_bf16, rows, residual_bf16, shared_delta_bf16, output_bf16, &a));
   const size_t routes = rows * l->cfg.top_k;

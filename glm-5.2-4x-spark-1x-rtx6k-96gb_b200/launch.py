@@ -1,4 +1,4 @@
-"""How the wrappers of the stateless operators reach the library.
+"""How the wrappers of the operators around the routed experts reach the library.
 
 A call's arguments travel as one packed struct (``struct.Struct`` costs a tenth of building ctypes objects
 field by field), on the current stream of the tensors' device, with that device current.
@@ -32,15 +32,15 @@ def inner_contiguous(t: torch.Tensor, width: int) -> bool:
     return width <= 1 or t.is_contiguous() or t.stride(1) == 1
 
 
-def call(lib: N.NativeLibrary | None, symbol: str, packed: bytes, index: int) -> None:
-    """``symbol(packed, current stream of device index)``; raises what NativeLibrary.call raises."""
+def call(lib: N.NativeLibrary | None, symbol: str, packed: bytes, index: int, *handle) -> None:
+    """``symbol(*handle, packed, current stream of device index)``; raises what NativeLibrary.call raises."""
     lib = lib or N.library()
     fn = lib.symbol(symbol)
     if index == torch.cuda.current_device():
-        status = fn(packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
+        status = fn(*handle, packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
     else:
         with torch.cuda.device(index):
-            status = fn(packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
+            status = fn(*handle, packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
     if status != 0:
         raise N.GlmrtError(symbol, status, lib.last_error())
 

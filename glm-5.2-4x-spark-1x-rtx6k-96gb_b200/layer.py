@@ -6,10 +6,12 @@ process groups.  Every computation happens inside libglmrt_b200.so.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 import torch
 
+from . import launch
 from . import native as N
 
 
@@ -169,45 +171,42 @@ class MoeLayer:
         return out
 
     FEW_MAX_ROWS = 16
+    _FEW_ARGS = struct.Struct("@" + launch.BUFFER * 6 + "Q")     # glmrt_b200_few_args_t
 
     def forward_few(self, hidden_bf16: torch.Tensor, out: torch.Tensor | None = None,
                     residual_bf16: torch.Tensor | None = None, shared_delta_bf16: torch.Tensor | None = None,
                     want_routes: bool = False):
         """The whole layer for at most ``FEW_MAX_ROWS`` rows on bf16 activations (no activation
         quantisation), out = bf16(residual + shared_delta + routed), rounded once."""
-        rows = self._few_rows(hidden_bf16, residual_bf16, shared_delta_bf16, out)
-        if out is None:
-            out = torch.empty_like(hidden_bf16)
         idx = w = None
         if want_routes:
+            rows = hidden_bf16.shape[0]
             idx = torch.empty((rows, self.top_k), dtype=torch.int32, device=self.device)
             w = torch.empty((rows, self.top_k), dtype=torch.float32, device=self.device)
-        opt = lambda t: N.DeviceBuffer.null() if t is None else _buf(t)  # noqa: E731
-        self.lib.call("glmrt_b200_moe_layer_forward_few_async", self.handle, _buf(hidden_bf16), C.c_size_t(rows),
-                      opt(residual_bf16), opt(shared_delta_bf16), _buf(out), opt(idx), opt(w), _stream())
+        out = self._few("glmrt_b200_moe_layer_forward_few_async", hidden_bf16, out, residual_bf16, shared_delta_bf16, idx, w)
         return (out, idx, w) if want_routes else out
 
     def forward_few_routed(self, hidden_bf16: torch.Tensor, idx: torch.Tensor, w: torch.Tensor,
                            out: torch.Tensor | None = None, residual_bf16: torch.Tensor | None = None,
                            shared_delta_bf16: torch.Tensor | None = None) -> torch.Tensor:
         """``forward_few`` with the routes given; index -1 is no route."""
-        rows = self._few_rows(hidden_bf16, residual_bf16, shared_delta_bf16, out)
-        assert idx.shape == (rows, self.top_k) and w.shape == (rows, self.top_k)
-        if out is None:
-            out = torch.empty_like(hidden_bf16)
-        idx = idx.to(torch.int32).contiguous()
-        w = w.to(torch.float32).contiguous()
-        opt = lambda t: N.DeviceBuffer.null() if t is None else _buf(t)  # noqa: E731
-        self.lib.call("glmrt_b200_moe_layer_forward_few_routed_async", self.handle, _buf(hidden_bf16), C.c_size_t(rows),
-                      _buf(idx), _buf(w), opt(residual_bf16), opt(shared_delta_bf16), _buf(out), _stream())
-        return out
+        assert idx.shape == (hidden_bf16.shape[0], self.top_k) and w.shape == idx.shape
+        assert idx.device == self.device and w.device == self.device
+        return self._few("glmrt_b200_moe_layer_forward_few_routed_async", hidden_bf16, out, residual_bf16, shared_delta_bf16,
+                         idx.to(torch.int32).contiguous(), w.to(torch.float32).contiguous())
 
-    def _few_rows(self, hidden: torch.Tensor, *others) -> int:
-        assert hidden.dim() == 2 and hidden.dtype == torch.bfloat16 and hidden.shape[1] == self.hidden
-        for t in (hidden, *others):
+    def _few(self, symbol, hidden, out, residual, shared, idx, w) -> torch.Tensor:
+        assert hidden.dim() == 2 and hidden.shape[1] == self.hidden
+        if out is None:
+            out = torch.empty_like(hidden)
+        shape, index = hidden.shape, self.device.index
+        for t in (hidden, out, residual, shared):
             if t is not None:
-                assert t.shape == hidden.shape and t.dtype == torch.bfloat16 and t.device == self.device
-        return hidden.shape[0]
+                assert t.shape == shape and t.dtype is torch.bfloat16 and t.get_device() == index and t.is_contiguous()
+        b = launch.buffer
+        launch.call(self.lib, symbol, self._FEW_ARGS.pack(*b(hidden), *b(residual), *b(shared), *b(out), *b(idx), *b(w), shape[0]),
+                    index, self.handle)
+        return out
 
     def forward_host(self, hidden_host: torch.Tensor, out_host: torch.Tensor) -> None:
         """Host buffers in, host buffers out (pinned memory recommended); synchronises."""

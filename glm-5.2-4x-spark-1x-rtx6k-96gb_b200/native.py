@@ -123,6 +123,12 @@ class Fp8GatedMlpArgs(C.Structure):
                 + [(n, C.c_size_t) for n in ("rows", "hidden", "inter", "x_row_stride")])
 
 
+class FewArgs(C.Structure):
+    """glmrt_b200_few_args_t."""
+    _fields_ = ([(n, DeviceBuffer) for n in ("hidden_bf16", "residual_bf16", "shared_delta_bf16", "output_bf16",
+                                             "topk_indices", "topk_weights")] + [("rows", C.c_size_t)])
+
+
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
 

@@ -556,19 +556,18 @@ glmrt_status_t glmrt_b200_moe_layer_forward_residual_async(
  * output = bf16(residual + shared_delta + routed), rounded once (nearest even).  residual, shared_delta,
  * topk_indices and topk_weights may be null; output may be residual or shared_delta, and no other input.
  * Needs ep_world == 1.  Results differ from glmrt_b200_moe_layer_forward_async, which quantises the
- * activations; an expert's sums do not depend on the other rows of the call. */
+ * activations.  A row's result does not depend on the other rows of the call, and two calls give the same bits. */
 #define GLMRT_B200_FEW_MAX_ROWS 16
-glmrt_status_t glmrt_b200_moe_layer_forward_few_async(
-    void* layer, glmrt_device_buffer_t hidden_bf16, size_t rows, glmrt_device_buffer_t residual_bf16,
-    glmrt_device_buffer_t shared_delta_bf16, glmrt_device_buffer_t output_bf16, glmrt_device_buffer_t topk_indices,
-    glmrt_device_buffer_t topk_weights, void* cuda_stream);
-/* The same with the routes given: topk_indices [rows, top_k] (0xffffffff: no route; any other id outside the
- * layer is skipped and reported by glmrt_b200_moe_layer_check), topk_weights [rows, top_k].  An expert may be
- * named more than once in a row. */
-glmrt_status_t glmrt_b200_moe_layer_forward_few_routed_async(
-    void* layer, glmrt_device_buffer_t hidden_bf16, size_t rows, glmrt_device_buffer_t topk_indices,
-    glmrt_device_buffer_t topk_weights, glmrt_device_buffer_t residual_bf16, glmrt_device_buffer_t shared_delta_bf16,
-    glmrt_device_buffer_t output_bf16, void* cuda_stream);
+typedef struct glmrt_b200_few_args_t {
+  glmrt_device_buffer_t hidden_bf16, residual_bf16, shared_delta_bf16, output_bf16; /* [rows, hidden_dim] */
+  glmrt_device_buffer_t topk_indices, topk_weights;                                 /* [rows, top_k] */
+  size_t rows;
+} glmrt_b200_few_args_t;
+glmrt_status_t glmrt_b200_moe_layer_forward_few_async(void* layer, const glmrt_b200_few_args_t* args, void* cuda_stream);
+/* The same with the routes given: topk_indices (0xffffffff: no route; any other id outside the layer is skipped and
+ * reported by glmrt_b200_moe_layer_check) and topk_weights.  An expert may be named more than once in a row. */
+glmrt_status_t glmrt_b200_moe_layer_forward_few_routed_async(void* layer, const glmrt_b200_few_args_t* args,
+                                                             void* cuda_stream);
 /* Same with host buffers: copies the rows in from `hidden_host`, runs the layer, copies the
  * result out to `output_host` and synchronises the stream.  Host memory may be pageable;
  * pinned memory makes the copies asynchronous. */

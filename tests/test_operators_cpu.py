@@ -110,10 +110,11 @@ def test_fp8_refusals(lib):
 
 def test_packed_arguments_have_the_layout_of_the_structs(pkg):
     """The wrappers pack their arguments with struct; the C side reads the structs of the header."""
-    from glmrt_b200 import block_norm, fp8, native as N
+    from glmrt_b200 import block_norm, fp8, layer, native as N
     import ctypes
     for packer, cls, nbuf in ((block_norm._ARGS, N.BlockNormArgs, 7), (fp8._QUANT_ARGS, N.Fp8QuantizeRowsArgs, 3),
-                              (fp8._LINEAR_ARGS, N.Fp8BlockLinearArgs, 5), (fp8._MLP_ARGS, N.Fp8GatedMlpArgs, 9)):
+                              (fp8._LINEAR_ARGS, N.Fp8BlockLinearArgs, 5), (fp8._MLP_ARGS, N.Fp8GatedMlpArgs, 9),
+                              (layer.MoeLayer._FEW_ARGS, N.FewArgs, 6)):
         assert packer.size == ctypes.sizeof(cls)
         values = [0] * (4 * nbuf)
         for i in range(nbuf):
@@ -131,10 +132,10 @@ def test_null_argument_structs(lib):
 
 def test_few_refusals(lib):
     from glmrt_b200 import native as N
-    null = N.DeviceBuffer.null()
-    for name, args in (("glmrt_b200_moe_layer_forward_few_async", (null, C.c_size_t(1), null, null, null, null, null, None)),
-                       ("glmrt_b200_moe_layer_forward_few_routed_async", (null, C.c_size_t(1), null, null, null, null, null, None))):
-        assert lib.call_status(name, None, *args) == 1 and "null" in lib.last_error()
+    for name in ("forward_few", "forward_few_routed"):
+        assert lib.call_status(f"glmrt_b200_moe_layer_{name}_async", None, None, None) == 1
+        assert lib.call_status(f"glmrt_b200_moe_layer_{name}_async", None, C.byref(N.FewArgs(rows=1)), None) == 1
+        assert "null" in lib.last_error()
 
 
 def test_wrappers_refuse_host_tensors_and_wrong_shapes(pkg):
