@@ -720,24 +720,29 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
         alive = tc::mbar_wait_warp(&sh.full[mine], ((base + i) / kBufs) & 1, &sh.abort);
         if (!alive) break;
 #pragma unroll 1
-        for (int q = 0; q < rw * kCols; ++q) {
-          const int r = q / kCols, c = q % kCols;
-          if (c >= cols) continue;
-          const int route = sh.ent_route[j][c];
-          if (route < 0) continue;
-          const float* src = part + (r * p.kw * 32 + lane) * cols + c;
-          float sum = 0.0f;
-#pragma unroll 4
-          for (int w = 0; w < warps_k; ++w) sum += src[w * 32 * cols];
-          if (pass == 0) {                             // lanes 0..15 gate, 16..31 up
-            sum *= scale2 * sh.x_inv[sh.route_token[route]];
-            const float up = __shfl_down_sync(0xffffffffu, sum, 16);
-            const float v = sh.ent_w[j][c] * (__fdividef(sum, 1.0f + __expf(-sum)) * up);
-            if (lane < 16)
-              a.act[static_cast<size_t>(route) * a.inter + unit_row(u * rw + r) + (lane & 7) + (lane >> 3) * 32] = v;
-          } else {
-            a.route_out[static_cast<size_t>(route) * a.hidden + unit_row((u * rw + r) * 2 + (lane >> 4)) + (lane & 7) +
-                        ((lane >> 3) & 1) * 32] = sum * scale2;
+        for (int q0 = 0; q0 < rw * kCols; q0 += 4) {   // four sums (row group, column) side by side
+          float sum[4] = {};
+          const float* src = part + ((q0 / kCols) * p.kw * 32 + lane) * cols;
+#pragma unroll 2
+          for (int w = 0; w < warps_k; ++w)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (q0 + x < rw * kCols && x % kCols < cols) sum[x] += src[((x / kCols) * p.kw + w) * 32 * cols + x % kCols];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int r = (q0 + x) / kCols, c = x % kCols;
+            const int route = r < rw && c < cols ? sh.ent_route[j][c] : -1;
+            if (route < 0) continue;
+            if (pass == 0) {                           // lanes 0..15 gate, 16..31 up
+              const float v = sum[x] * (scale2 * sh.x_inv[sh.route_token[route]]);
+              const float up = __shfl_down_sync(0xffffffffu, v, 16);
+              if (lane < 16)
+                a.act[static_cast<size_t>(route) * a.inter + unit_row(u * rw + r) + (lane & 7) + (lane >> 3) * 32] =
+                    sh.ent_w[j][c] * (__fdividef(v, 1.0f + __expf(-v)) * up);
+            } else {
+              a.route_out[static_cast<size_t>(route) * a.hidden + unit_row((u * rw + r) * 2 + (lane >> 4)) + (lane & 7) +
+                          ((lane >> 3) & 1) * 32] = sum[x] * scale2;
+            }
           }
         }
         __syncwarp();
