@@ -7,6 +7,8 @@
 //   weights      E4M3 [n, k] and one float32 scale per 128 x 128 block
 //   product      y[m, n] = sum over blocks b of sx[m, b] sw[n / 128, b] sum over k in b of q[m, k] w[n, k],
 //                float32 sums
+#include <initializer_list>
+
 #include "common.cuh"
 #include "fp8.cuh"
 #include "internal.h"
@@ -93,6 +95,18 @@ glmrt_status_t check_buffer(const glmrt_device_buffer_t& b, size_t need, size_t 
   return GLMRT_STATUS_OK;
 }
 
+// What a call writes (its first `need` bytes) must lie apart from everything it reads and from its workspace: tiles of
+// the output are written while others still read the rows.
+struct Span { const void* ptr; size_t bytes; };
+glmrt_status_t check_apart(const Span& out, std::initializer_list<Span> others, const char* what) {
+  const uintptr_t o = reinterpret_cast<uintptr_t>(out.ptr);
+  for (const Span& s : others) {
+    const uintptr_t i = reinterpret_cast<uintptr_t>(s.ptr);
+    if (i < o + out.bytes && o < i + s.bytes) return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string(what) + ": overlaps another buffer of the call");
+  }
+  return GLMRT_STATUS_OK;
+}
+
 glmrt_status_t launch_quantize(const void* in, uint32_t dtype, size_t stride, uint8_t* codes, float* scales, size_t rows,
                                size_t cols, size_t scale_stride, cudaStream_t s) {
   const size_t size = dtype == GLMRT_B200_DTYPE_BF16 ? 2 : 4, units = rows * blocks_of(cols);
@@ -124,6 +138,9 @@ extern "C" glmrt_status_t glmrt_b200_fp8_quantize_rows_async(const glmrt_b200_fp
   GLMRT_RETURN_IF_ERROR(check_buffer(input, ((rows - 1) * input_row_stride + cols) * size, size, "fp8_quantize_rows input"));
   GLMRT_RETURN_IF_ERROR(check_buffer(codes, rows * cols, 16, "fp8_quantize_rows codes"));
   GLMRT_RETURN_IF_ERROR(check_buffer(scales, rows * blocks_of(cols) * 4, 4, "fp8_quantize_rows scales"));
+  const Span in{input.ptr, ((rows - 1) * input_row_stride + cols) * size}, sc{scales.ptr, rows * blocks_of(cols) * 4};
+  GLMRT_RETURN_IF_ERROR(check_apart({codes.ptr, rows * cols}, {in, sc}, "fp8_quantize_rows codes"));
+  GLMRT_RETURN_IF_ERROR(check_apart(sc, {in}, "fp8_quantize_rows scales"));
   GLMRT_RETURN_IF_ERROR(require_cuda());
   GLMRT_RETURN_IF_ERROR(launch_quantize(input.ptr, dtype, input_row_stride, static_cast<uint8_t*>(codes.ptr),
                                         static_cast<float*>(scales.ptr), rows, cols, rows, static_cast<cudaStream_t>(cuda_stream)));
@@ -149,12 +166,16 @@ extern "C" glmrt_status_t glmrt_b200_fp8_block_linear_async(const glmrt_b200_fp8
   GLMRT_RETURN_IF_ERROR(check_buffer(weight_codes, n * k, 16, "fp8_block_linear weight_codes"));
   GLMRT_RETURN_IF_ERROR(check_buffer(weight_scales, blocks_of(n) * blocks_of(k) * 4, 4, "fp8_block_linear weight_scales"));
   GLMRT_RETURN_IF_ERROR(check_buffer(output, rows * n * osize, osize, "fp8_block_linear output"));
-  if (rows > kFp8OwnRows) GLMRT_RETURN_IF_ERROR(check_buffer(workspace, rows_bytes(rows, k), 256, "fp8_block_linear workspace"));
+  const bool own = rows <= kFp8OwnRows;      // the product quantises so few rows itself
+  if (!own) GLMRT_RETURN_IF_ERROR(check_buffer(workspace, rows_bytes(rows, k), 256, "fp8_block_linear workspace"));
+  const Span x{x_bf16.ptr, ((rows - 1) * x_row_stride + k) * 2}, wc{weight_codes.ptr, n * k}, wsc{weight_scales.ptr, blocks_of(n) * blocks_of(k) * 4},
+      out{output.ptr, rows * n * osize};
+  GLMRT_RETURN_IF_ERROR(check_apart(out, {x, wc, wsc}, "fp8_block_linear output"));
+  if (!own) GLMRT_RETURN_IF_ERROR(check_apart({workspace.ptr, rows_bytes(rows, k)}, {x, wc, wsc, out}, "fp8_block_linear workspace"));
   GLMRT_RETURN_IF_ERROR(require_cuda());
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   uint8_t* codes = static_cast<uint8_t*>(workspace.ptr);
   float* scales = reinterpret_cast<float*>(codes + round256(rows * k));
-  const bool own = rows <= kFp8OwnRows;      // the product quantises so few rows itself
   if (!own) GLMRT_RETURN_IF_ERROR(launch_quantize(x_bf16.ptr, GLMRT_B200_DTYPE_BF16, x_row_stride, codes, scales, rows, k, padded(rows), s));
   Fp8Gemm g{codes, scales, static_cast<const uint8_t*>(weight_codes.ptr), nullptr, static_cast<const float*>(weight_scales.ptr),
             nullptr, output.ptr, nullptr, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k),
@@ -190,6 +211,12 @@ extern "C" glmrt_status_t glmrt_b200_fp8_gated_mlp_async(const glmrt_b200_fp8_ga
   GLMRT_RETURN_IF_ERROR(check_buffer(down_scales, scale_bytes, 4, "fp8_gated_mlp down_scales"));
   GLMRT_RETURN_IF_ERROR(check_buffer(output_bf16, rows * hidden * 2, 2, "fp8_gated_mlp output"));
   GLMRT_RETURN_IF_ERROR(check_buffer(workspace, need, 256, "fp8_gated_mlp workspace"));
+  const Span x{x_bf16.ptr, ((rows - 1) * x_row_stride + hidden) * 2}, gc{gate_codes.ptr, hidden * inter}, gs{gate_scales.ptr, scale_bytes},
+      uc{up_codes.ptr, hidden * inter}, us{up_scales.ptr, scale_bytes}, dc{down_codes.ptr, hidden * inter}, ds{down_scales.ptr, scale_bytes},
+      out{output_bf16.ptr, rows * hidden * 2};
+  // (the rows have been read when the last product starts, so the output may take their place where they are whole)
+  GLMRT_RETURN_IF_ERROR(check_apart(out, {gc, gs, uc, us, dc, ds}, "fp8_gated_mlp output"));
+  GLMRT_RETURN_IF_ERROR(check_apart({workspace.ptr, need}, {x, gc, gs, uc, us, dc, ds, out}, "fp8_gated_mlp workspace"));
   GLMRT_RETURN_IF_ERROR(require_cuda());
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   uint8_t* xq = static_cast<uint8_t*>(workspace.ptr);

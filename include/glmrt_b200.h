@@ -429,7 +429,9 @@ glmrt_status_t glmrt_b200_operators_check(void* cuda_stream);
 /* rows, n and the last block may be ragged, rows 0 is accepted.  `workspace` is   */
 /* 256-byte aligned device memory of the stated size (null where that is 0, as for */
 /* a linear of at most 4 rows); it carries nothing from one                        */
-/* call to the next, and calls that may overlap need one each.                     */
+/* call to the next, and calls that may overlap need one each.  What a call writes */
+/* overlaps nothing that it reads (refused), but for the gated MLP's rows: its     */
+/* output may lie over them.                                                       */
 /* ------------------------------------------------------------------------ */
 /* bf16 / float32 rows (input_row_stride elements apart) -> codes [rows, cols], scales
  * [ceil(cols/128), rows]. */

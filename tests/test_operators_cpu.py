@@ -108,6 +108,43 @@ def test_fp8_refusals(lib):
         assert mlp(**{name: buf(good[name].ptr, good[name].bytes - 1)}) == 2, name
 
 
+def test_fp8_refuses_outputs_over_inputs(lib):
+    from glmrt_b200 import native as N
+    Z = C.c_size_t
+    buf = N.DeviceBuffer.of
+    need = Z(0)
+    assert lib.call_status("glmrt_b200_fp8_block_linear_workspace", Z(17), Z(128), Z(128), C.byref(need)) == 0
+    places = dict(x=buf(0x10000, 17 * 256), c=buf(0x20000, 128 * 128), s=buf(0x30000, 4), w=buf(0x100000, need.value))
+
+    def linear(o, rows=17, w=places["w"]):
+        return lib.call_status("glmrt_b200_fp8_block_linear_async",
+                               C.byref(N.Fp8BlockLinearArgs(places["x"], places["c"], places["s"], o, w, rows, 128, 128, 128, 0)), None)
+
+    for rows in (1, 17):
+        for name in ("x", "c", "s"):
+            assert linear(buf(places[name].ptr, 17 * 256), rows) == 1 and "overlaps" in lib.last_error(), (rows, name)
+            assert linear(buf(places[name].ptr - 2, 17 * 256), rows) == 1 and "overlaps" in lib.last_error(), (rows, name)
+    assert linear(buf(places["w"].ptr + 512, 17 * 256)) == 1 and "overlaps" in lib.last_error()
+    assert linear(buf(0x40000, 17 * 256), w=buf(0x10000, need.value)) == 1 and "overlaps" in lib.last_error()
+
+    def rows(x=buf(0x10000, 1024), c=buf(0x20000, 512), s=buf(0x30000, 16)):
+        return lib.call_status("glmrt_b200_fp8_quantize_rows_async", C.byref(N.Fp8QuantizeRowsArgs(x, c, s, 4, 128, 128, 0)), None)
+
+    for bad in (dict(c=buf(0x10000, 512)), dict(s=buf(0x10400 - 4, 16)), dict(s=buf(0x20000 + 508, 16))):
+        assert rows(**bad) == 1 and "overlaps" in lib.last_error(), bad
+
+    assert lib.call_status("glmrt_b200_fp8_gated_mlp_workspace", Z(4), Z(128), Z(64), C.byref(need)) == 0
+    names = ["x", "gc", "gs", "uc", "us", "dc", "ds", "o", "w"]
+    good = dict(zip(names, (buf(0x10000, 1024), buf(0x20000, 8192), buf(0x30000, 4), buf(0x40000, 8192), buf(0x50000, 4),
+                            buf(0x60000, 8192), buf(0x70000, 4), buf(0x80000, 1024), buf(0x100000, need.value))))
+    for out, others in (("o", names[1:7] + ["w"]), ("w", names[:8])):
+        for name in others:
+            b = {**good, out: buf(good[name].ptr & ~0xff, good[out].bytes)}
+            assert lib.call_status("glmrt_b200_fp8_gated_mlp_async",
+                                   C.byref(N.Fp8GatedMlpArgs(*[b[n] for n in names], 4, 128, 64, 128)), None) == 1, (out, name)
+            assert "overlaps" in lib.last_error(), (out, name)
+
+
 def test_packed_arguments_have_the_layout_of_the_structs(pkg):
     """The wrappers pack their arguments with struct; the C side reads the structs of the header."""
     from glmrt_b200 import block_norm, fp8, layer, native as N
