@@ -889,11 +889,12 @@ glmrt_status_t launch_ring(const FewArgs& a, size_t smem, int sm_count, cudaStre
 }  // namespace
 
 // What fits into shared memory decides the depth of the stream; the selection's scratch (36 bytes an expert) lies in
-// its ring, and at least three slots are needed.
+// its ring, and at least three slots are needed.  Whether it fits is asked for the widest entries, also where one row
+// would do with less: a row's result must not depend on how many rows the call has.
 bool few_fused_supported(const FewArgs& a) {
   static_assert(1024 * 36 <= 3 * kWarps * kSlotBytes, "selection scratch fits the ring");
   // (per_entry < 4096 makes the multiplication by its inverse exact: at most 256 entries)
-  return few_smem(3, std::min(a.rows, kCols), std::max(a.hidden, a.inter)) <= kSmemMost && a.experts <= 1024 && a.pass[0].per_entry > 1 &&
+  return few_smem(3, kCols, std::max(a.hidden, a.inter)) <= kSmemMost && a.experts <= 1024 && a.pass[0].per_entry > 1 &&
          a.pass[0].per_entry < 4096 && a.pass[1].per_entry > 1 && a.pass[1].per_entry < 4096;
 }
 glmrt_status_t launch_few_fused(const FewArgs& a, int sm_count, cudaStream_t s) {

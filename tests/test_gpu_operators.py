@@ -104,6 +104,18 @@ def test_block_norm_many_rows(mods, dtype, wdtype, rows, width):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and (out[:, width:] == 7).all()
 
 
+def test_block_norm_beyond_32_bit_offsets(mods):
+    rows, width = 350300, 6144
+    few = randn(1, 1000, width, dtype=torch.bfloat16)
+    nw = 1 + randn(2, width, std=0.1, dtype=torch.bfloat16)
+    want = mods["block_norm"].block_norm(few.repeat(2, 1), few.repeat(2, 1), norm_weight=nw, scale=0.5)
+    many = few.repeat(-(-rows // 1000), 1)[:rows]
+    got = mods["block_norm"].block_norm(many, many, norm_weight=nw, scale=0.5)
+    for at in range(0, rows, 1000):
+        n = min(1000, rows - at)
+        assert all(torch.equal(g[at:at + n], v[:n]) for g, v in zip(got, want)), at
+
+
 def test_block_norm_strides_and_alignment(mods):
     """Padded rows, rows that start off a 16-byte boundary, an expanded gate."""
     rows, width = 9, 520
@@ -284,6 +296,18 @@ def test_fp8_calls_on_two_streams_and_in_a_graph(mods, rows):
         xin.zero_()
 
 
+@pytest.mark.parametrize("rows,n,k", [(350300, 16, 6144), (140001, 16384, 16)])
+def test_fp8_linear_beyond_32_bit_offsets(mods, rows, n, k):
+    """More than 2^31 values in the rows, or in the output: every row as it comes out among a few."""
+    assert max(rows * n, rows * k) > 2 ** 31
+    few = randn(1, 1000, k, dtype=torch.bfloat16)
+    w = mods["fp8"].quantize_weight(randn(2, n, k, std=0.02))
+    want = mods["fp8"].block_linear(few.repeat(2, 1), *w)[:1000]       # (on the many rows' kernel)
+    got = mods["fp8"].block_linear(few.repeat(-(-rows // 1000), 1)[:rows], *w)
+    for at in range(0, rows, 1000):
+        assert torch.equal(got[at:at + 1000], want[:min(1000, rows - at)]), at
+
+
 def mlp_ref(x, gate, up, down):
     """y, and a bound on what float32 can change: sums, and codes whose border is within the error."""
     (g, mg), (u, mu) = product_ref(x, weight_ref(*gate)), product_ref(x, weight_ref(*up))
@@ -321,6 +345,7 @@ def test_fp8_gated_mlp(mods, rows, hidden, inter):
     wide = torch.nn.functional.pad(x, (0, 8))
     out = torch.empty_like(got)
     assert mods["fp8"].gated_mlp(wide[:, :hidden], *gate, *up, *down, out=out) is out and torch.equal(out, got)
+    assert torch.equal(mods["fp8"].gated_mlp(x, *gate, *up, *down, out=x), got), "in the rows' place"
 
 
 # ---- the layer for a few tokens ------------------------------------------------------------------
@@ -549,6 +574,84 @@ def test_few_full_size_layer(mods):
             assert idx1.tolist() == idx[2:3].tolist()
             within(one, out, half(torch.bfloat16) * (out.abs() + err) + err, "alone")
     layer.close()
+
+
+def test_few_many_experts_and_most_routes(mods):
+    """More than 256 experts, 16 slots, every row its own experts: 256 entries at once."""
+    h, i, e, top_k = 512, 256, 330, 16
+    ref = O.make_layer(13, h, i, e)
+    layer, weights = make_layer(mods, ref, top_k), layer_weights(ref)
+    x = randn(1, 16, h, dtype=torch.bfloat16)
+    _, idx, _ = check_few(layer, weights, x)
+    assert torch.equal(idx.sort(1).values, layer.forward(x, want_routes=True)[1].sort(1).values)
+    idx, w = torch.arange(256).view(16, 16) + 70, randn(2, 16, 16).abs() + 0.1
+    got = layer.forward_few_routed(x, idx.cuda(), w)
+    layer.check()
+    out, err = few_ref(weights, x, idx, w.cpu())
+    within(got, out, half(torch.bfloat16) * (out.abs() + err) + err)
+    layer.close()
+
+
+def test_few_shapes_beyond_the_fused_kernel(mods):
+    """Rows too long for the fused kernel's shared memory: right, and the same for one row as among others."""
+    h, i, e = 24576, 256, 3
+    ref = O.make_layer(14, h, i, e)
+    layer, weights = make_layer(mods, ref, 2), layer_weights(ref)
+    x = randn(1, 5, h, dtype=torch.bfloat16)
+    got, idx, w = check_few(layer, weights, x)
+    for r in range(5):
+        assert torch.equal(layer.forward_few_routed(x[r:r + 1], idx[r:r + 1], w[r:r + 1]), got[r:r + 1])
+    layer.close()
+
+
+def test_few_weights_beyond_4_gib(mods):
+    """Stacks of more than 2^32 bytes: the experts at their end, against 64 bits."""
+    h, i, e = 6144, 2048, 720
+    layer = mods["layer"].MoeLayer(h, i, e, 2, max_tokens=4)
+    layer.set_router(randn(1, e, h, std=0.02), randn(2, e, std=0.01))
+    layer.fill_synthetic(15)
+    assert e * h * i // 2 > 2 ** 32
+    x, w = randn(3, 3, h, dtype=torch.bfloat16), torch.ones(3, 2, device="cuda")
+    experts = [e - 1, 0, 683, e - 2]
+    pick = torch.tensor([[0, 1], [2, 3], [3, 0]])
+    got = layer.forward_few_routed(x, torch.tensor(experts)[pick].cuda(), w)
+    layer.check()
+    parts = [layer.read_expert(v) for v in experts]
+    grid = torch.tensor(GRID, dtype=torch.float64, device="cuda")
+    weights = [torch.stack([grid[torch.from_numpy(p[j][0]).cuda().long()]
+                            * torch.from_numpy(p[j][1].copy()).cuda().view(torch.float8_e4m3fn).double().repeat_interleave(16, 1) * p[j][2]
+                            for p in parts]) for j in range(3)]
+    out, err = few_ref(weights, x, pick, w.cpu())
+    within(got, out, half(torch.bfloat16) * (out.abs() + err) + err)
+    layer.close()
+
+
+def test_operators_on_three_streams_at_once(mods):
+    """Two lanes of a layer, 8-bit products and norms side by side: everybody gets what they get alone."""
+    ref = O.make_layer(16, 1024, 512, 32)
+    layer = make_layer(mods, ref, 4)
+    lane = layer.create_lane(16)
+    x, rows = randn(1, 7, 1024, dtype=torch.bfloat16), randn(2, 3000, 4096, dtype=torch.bfloat16)
+    w = mods["fp8"].quantize_weight(randn(3, 1000, 4096, std=0.02))
+    few, lin = layer.forward_few(x), {m: mods["fp8"].block_linear(rows[:m], *w) for m in (2, 40, 3000)}
+    nw = 1 + randn(4, 4096, std=0.1)
+    norm = mods["block_norm"].block_norm(rows, rows, norm_weight=nw)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(8):
+        for s, l in zip(streams, (layer, lane)):
+            with torch.cuda.stream(s):
+                got.append((l.forward_few(x), few))
+        with torch.cuda.stream(streams[2]):
+            got += [(mods["fp8"].block_linear(rows[:m], *w), lin[m]) for m in lin]
+            got += zip(mods["block_norm"].block_norm(rows, rows, norm_weight=nw), norm)
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g, want in got)
+    for l in (lane, layer):
+        l.check()
+        l.close()
+    import importlib
+    importlib.import_module("glmrt_b200.launch").check()
 
 
 # ---- all of them together ------------------------------------------------------------------------
