@@ -1,5 +1,6 @@
 // Number formats and the activation quantiser's block arithmetic of the 8-bit products (fp8.cu).
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -60,7 +61,8 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   return lo | (hi << 16);
 }
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-  return static_cast<uint32_t>(f32_to_bf16_rne(lo)) | (static_cast<uint32_t>(f32_to_bf16_rne(hi)) << 16);
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);       // one conversion for both
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ float fp8_swiglu(float g, float u) {
   // fast exponential and division: a few units in the last place, against codes of four bits

@@ -60,6 +60,12 @@ __device__ __forceinline__ void tc_mma_fp8(uint32_t d_tmem, uint64_t a_desc, uin
 // E4M3 x E4M3 -> float32, both operands K-major, M = 128, N = n.
 __device__ __forceinline__ uint32_t idesc_fp8(uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((128u >> 4) << 24); }
 
+// Keeps a CTA until the others of the cluster have read its shared memory: what they read went into what they stored,
+// so nothing has to be made visible.  (A releasing arrival also waits for the stores to global memory: half a microsecond.)
+__device__ __forceinline__ void cluster_leave() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
 constexpr int kTileBytes = 128 * kFp8Block;            // 128 rows of one K block
 
 // ---------------------------------------------------------------------------------------------------
@@ -97,6 +103,12 @@ __device__ __forceinline__ void tc_mma_fp8_pair(uint32_t d_tmem, uint64_t a_desc
       "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+// Arrives on the barrier at this place in both CTAs of the pair once every earlier product is done.
+__device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
 }
 // Arrival on the leader's barrier after reading tensor memory: the reads are complete (wait::ld) and ordered by the
 // tcgen05 fence before it, no other memory has to become visible.  With .release.cluster the same arrival made the
@@ -210,18 +222,17 @@ fp8_rows_kernel(RowsArgs a, const __grid_constant__ CUtensorMap map_x, const __g
       const uint32_t idesc = (1u << 4) | ((static_cast<uint32_t>(kPairN) >> 3) << 17) | ((256u >> 4) << 24);
       for (int tile = pair; tile < tiles && alive; tile += pairs)
         for (int b = 0; b < blocks; ++b) {
-          if (!mbar_wait_hot(&acc_empty[abuf], aphase ^ 1u, abort_flag) ||
-              !mbar_wait_hot(&full_bar[stage], phase, abort_flag)) { alive = false; break; }
+          // (the copies are early, the sums' buffer is what the next product waits for: its wait comes last)
+          if (!mbar_wait_hot(&full_bar[stage], phase, abort_flag) ||
+              !mbar_wait_hot(&acc_empty[abuf], aphase ^ 1u, abort_flag)) { alive = false; break; }
           tc_fence_after();
           if (elect_one()) {
             const uint32_t s_a = smem_u32(smem + static_cast<size_t>(stage) * kPairStageBytes), s_b = s_a + kTileBytes;
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               tc_mma_fp8_pair(tmem_base + abuf * kPairN, desc_sw128(s_a + kk * 32), desc_sw128(s_b + kk * 32), idesc, kk != 0 ? 1u : 0u);
-            tc_commit_pair(smem_u32(&empty_bar[stage]));
-            tc_commit_pair(cluster_addr(smem_u32(&empty_bar[stage]), 1));
-            tc_commit_pair(smem_u32(&acc_full[abuf]));
-            tc_commit_pair(cluster_addr(smem_u32(&acc_full[abuf]), 1));
+            tc_commit_both(&acc_full[abuf]);
+            tc_commit_both(&empty_bar[stage]);
           }
           __syncwarp();
           if (++stage == kPairStages) { stage = 0; phase ^= 1u; }
@@ -615,15 +626,9 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
     }
   }
 
-  // ---- the splits' sums meet: [matrix][row of x][weight row] in each CTA's ring, whose copies have all been used ----
-  __syncthreads();
-  if (*abort_flag != 0u) {
-    for (int i = 0; i < 200; ++i) __nanosleep(1000);   // let copies in flight land
-    if (threadIdx.x == 0) atomicOr(&g_fp8_error, static_cast<uint32_t>(kErrWaitTimeout));
-  }
+  // ---- the splits' sums meet: [matrix][row of x][weight row] in each CTA's ring.  An epilogue warp has seen the last
+  // product done, so nobody reads the ring any more and all its copies have landed. ----
   tc_fence_before();
-  __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem_base, C::kTmemCols);
   float* part = reinterpret_cast<float*>(smem);
   if (warp >= 2)
 #pragma unroll
@@ -631,7 +636,13 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
 #pragma unroll
       for (int j = 0; j < C::kCols; ++j) part[(mat * kN + part_col + j) * 128 + lane_row] = acc[mat][j];
   if (splits > 1) cluster_sync_all();
-  else if (warp >= 2) asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kEpiWarps) : "memory");
+  else __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, C::kTmemCols);
+  if (*abort_flag != 0u) {
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);   // let copies in flight land
+    if (threadIdx.x == 0) atomicOr(&g_fp8_error, static_cast<uint32_t>(kErrWaitTimeout));
+  }
   // This CTA finishes rows j0 .. j1 of the tile, one warp a row and four features a lane, the splits added in order.
   // A load from another CTA's shared memory takes most of a microsecond, so a lane has all splits' in flight.
   const int valid = min(kN, a.rows - m0);
@@ -697,7 +708,7 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
       }
     }
   }
-  if (splits > 1) cluster_sync_all();       // nobody leaves while its sums may still be read
+  if (splits > 1) cluster_leave();          // nobody leaves while its sums may still be read
 }
 
 constexpr int kMaxDevices = 64;
@@ -733,13 +744,16 @@ int active_clusters(int splits) {
 
 // CTAs of a cluster that share a tile's K blocks: the number with the shortest estimated time.  A wave of CTAs
 // costs about 3 us beside its blocks (set-up, first copies, joining), a block 0.42 us and 0.0015 us per column of
-// the sum (measured at 16 to 256 rows and 2048 to 6144 columns of K).
+// the sum (measured at 16 to 256 rows and 2048 to 6144 columns of K).  The driver's count is that of one CTA an SM.
+// With rows quantised here a second one beside it helps, since each CTA then has fewer blocks of them (1 row, n x k:
+// 4096 x 6144 4 splits 8.9 us, 6 splits 7.0; 12288 x 4096 1 split 16.9, 2 splits 13.3); otherwise it does not (16 rows,
+// 4096 x 6144: 4 splits 9.4, 6 splits 10.0).
 template <int kMode, int kN, bool kOwnX>
 int weight_splits(int tiles, int blocks, float* estimate_us) {
   int best = 1;
   float best_us = 0.0f;
   for (int s = 1; s <= 8 && s <= blocks; ++s) {
-    const int active = active_clusters<kMode, kN, kOwnX>(s);
+    const int active = active_clusters<kMode, kN, kOwnX>(s) * (kOwnX ? WCfg<kMode, kN, kOwnX>::kPerSm : 1);
     if (active <= 0) continue;
     const float us = static_cast<float>((tiles + active - 1) / active) *
                      (3.0f + (s > 1 ? 0.7f : 0.0f) + static_cast<float>((blocks + s - 1) / s) * (0.42f + 0.0015f * WCfg<kMode, kN, kOwnX>::kAccCols));
