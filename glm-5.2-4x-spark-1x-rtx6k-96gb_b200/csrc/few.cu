@@ -122,24 +122,27 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 
 // All CTAs of the grid (co-resident: cooperative launch).  The arrivals of one barrier add up to 2^31: every CTA
 // adds one, the first what is missing.  So the top bit flips when the last has come, and nothing has to be
-// reset.  False when the wait ran out.
-// Arriving and waiting are apart, so that work may lie between them; thread 0 keeps what it saw.
-__device__ __forceinline__ uint32_t grid_arrive(uint32_t* count) {
-  uint32_t old = 0u;
+// reset.  Thread 0 knows the bit from before its first arrival (it cannot flip without it), so an arrival needs no
+// answer.  Arriving and waiting are apart, so that work may lie between them; false when the wait ran out.
+__device__ __forceinline__ uint32_t grid_bit(const uint32_t* count) {
+  uint32_t now;
+  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(count) : "memory");
+  return now & 0x80000000u;
+}
+__device__ __forceinline__ void grid_arrive(uint32_t* count) {
   __syncthreads();
   if (threadIdx.x == 0) {
     const uint32_t add = blockIdx.x == 0 ? 0x80000000u - (gridDim.x - 1) : 1u;
-    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(old) : "l"(count), "r"(add) : "memory");
+    asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(count), "r"(add) : "memory");
   }
-  return old;
 }
-__device__ bool grid_wait(uint32_t* count, uint32_t old, volatile uint32_t* abort) {
+__device__ bool grid_wait(uint32_t* count, uint32_t& bit, volatile uint32_t* abort) {
   if (threadIdx.x == 0) {
     uint64_t t0 = 0;
     for (uint32_t spin = 1;; ++spin) {
       uint32_t now;
       asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(count) : "memory");
-      if ((old ^ now) >> 31) break;
+      if ((bit ^ now) >> 31) break;
       if ((spin & 255u) == 0u) {
         const uint64_t t = tc::global_timer_ns();
         if (t0 == 0) t0 = t;
@@ -147,11 +150,13 @@ __device__ bool grid_wait(uint32_t* count, uint32_t old, volatile uint32_t* abor
       }
     }
   }
+  bit ^= 0x80000000u;
   __syncthreads();
   return *abort == 0u;
 }
-__device__ __forceinline__ bool grid_barrier(uint32_t* count, volatile uint32_t* abort) {
-  return grid_wait(count, grid_arrive(count), abort);
+__device__ __forceinline__ bool grid_barrier(uint32_t* count, uint32_t& bit, volatile uint32_t* abort) {
+  grid_arrive(count);
+  return grid_wait(count, bit, abort);
 }
 
 // A CTA's share of one of the two weight passes.  How an item of rows is shared by the warps (FewPass: kw along K,
@@ -337,11 +342,13 @@ __device__ void load_act_columns(const FewArgs& a, FewShared& sh, uint8_t* dst, 
     const float4 x = __ldcg(src), y = __ldcg(src + 1);
     v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
   };
-  for (int i = threadIdx.x; i < cols * per_col; i += kMainThreads) {        // a unit is 16 neighbouring lanes (k % 256 == 0)
+  const int pieces = cols * per_col;
+  const bool keep = pieces <= kMainThreads;      // a piece a thread: read once
+  float v[8];
+  for (int i = threadIdx.x; i < pieces; i += kMainThreads) {        // a unit is 16 neighbouring lanes (k % 256 == 0)
     const int c = i / per_col, o = i - c * per_col, route = sh.ent_route[entry][c];
     uint32_t m = 0u;
     if (route >= 0) {
-      float v[8];
       read(route, o, v);
 #pragma unroll
       for (int n = 0; n < 8; ++n) m = max(m, __float_as_uint(v[n]) & 0x7fffffffu);
@@ -351,12 +358,12 @@ __device__ void load_act_columns(const FewArgs& a, FewShared& sh, uint8_t* dst, 
     if ((threadIdx.x & 15) == 0) atomicMax(&sh.act_amax[(o >> 4) & (kw - 1)][c], m);
   }
   main_sync();
-  for (int i = threadIdx.x; i < cols * per_col; i += kMainThreads) {
+  for (int i = threadIdx.x; i < pieces; i += kMainThreads) {
     const int c = i / per_col, o = i - c * per_col, route = sh.ent_route[entry][c];
     if (route < 0) continue;
     const int unit = o >> 4, t = (o >> 2) & 3, q = o & 3;
-    float v[8], inv;
-    read(route, o, v);
+    float inv;
+    if (!keep) read(route, o, v);
     const float f = f16_factor(sh.act_amax[unit & (kw - 1)][c], &inv);
     uint32_t h[4];
 #pragma unroll
@@ -470,7 +477,7 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
     live = e < static_cast<uint32_t>(a.experts);
     if (!live && e != kNoRoute) sh.bad = 1;
     const uint32_t* row = sh.route_expert + token * a.top_k;
-    for (int s = 0; s < a.top_k; ++s) {
+    for (int s = 0; s < a.top_k && a.scores == nullptr; ++s) {      // (the selection names nobody twice)
       if (s == slot || row[s] != e) continue;
       if (s < slot) live = false;                 // the row has named this expert before: its weight went there
       else w += sh.route_w[token * a.top_k + s];
@@ -593,10 +600,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
   if (tid < kFewMaxRows) sh.x_amax[tid] = 0u;
   __syncthreads();
 
-  uint32_t arrived = 0u;
+  uint32_t bit = tid == 0 ? grid_bit(a.sync) : 0u;
   if (a.scores != nullptr) {
     score_experts(a, sh, warp, lane);
-    arrived = grid_arrive(a.sync);
+    grid_arrive(a.sync);
   }
   // the rows' largest magnitudes, 256 values a warp
   const int row_pieces = a.hidden / 256;
@@ -614,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
   if (tid < a.rows) f16_factor(sh.x_amax[tid], &sh.x_inv[tid]);
   if (identity && warp < kWarps) load_hidden_columns(a, sh, columns, 0, cols, true);    // needs no routes
   if (a.scores != nullptr) {
-    if (!grid_wait(a.sync, arrived, &sh.abort)) {
+    if (!grid_wait(a.sync, bit, &sh.abort)) {
       if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
       return;
     }
@@ -656,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
     int n = 0;                     // items so far: buffer n % kBufs, its round n / kBufs
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
-      if (pass == 1) grid_barrier(a.sync, &sh.abort);
+      if (pass == 1) grid_barrier(a.sync, bit, &sh.abort);
       const Share s = pass == 0 ? s1 : s2;
       const FewPass p = a.pass[pass];
       const int kwi = warp & (p.kw - 1);
@@ -749,10 +756,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
         if (lane == 0) tc::mbar_arrive(&sh.empty[mine]);
       }
       base += items;
-      if (pass == 0) grid_barrier(a.sync, &sh.abort);
+      if (pass == 0) grid_barrier(a.sync, bit, &sh.abort);
     }
   }
-  if (!grid_barrier(a.sync, &sh.abort)) {
+  if (!grid_barrier(a.sync, bit, &sh.abort)) {
     if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
     return;
   }
