@@ -27,10 +27,13 @@ def _rows(t: torch.Tensor, shape, dtype: torch.dtype, index: int, what: str) -> 
     """Packed buffer and row stride of a [rows, width] tensor whose rows are contiguous inside."""
     if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
         raise ValueError(f"block_norm: {what} must have the shape, type and device of residual")
-    rows, width = shape
-    if not launch.inner_contiguous(t, width):
-        raise ValueError(f"block_norm: {what} must be contiguous along its rows")
-    return launch.rows_buffer(t, rows, width, _SIZES[dtype])
+    return launch.rows_buffer(t, shape[0], shape[1], _SIZES[dtype], "block_norm: " + what)
+
+
+def _weight(w: torch.Tensor, width: int, index: int, what: str) -> tuple:
+    if w.shape != (width,) or w.get_device() != index or not w.is_contiguous():
+        raise ValueError(f"block_norm: {what} must be a contiguous [{width}] tensor on the rows' device")
+    return w.data_ptr(), w.nbytes, 0, 0
 
 
 def block_norm(residual: torch.Tensor, delta: torch.Tensor | None = None, *, norm_weight: torch.Tensor,
@@ -55,12 +58,13 @@ def block_norm(residual: torch.Tensor, delta: torch.Tensor | None = None, *, nor
         raise ValueError("block_norm: post_weight, gate and residual_out need a delta")
     wdtype = norm_weight.dtype
     wcode = _DTYPES.get(wdtype)
-    for name, w in (("norm_weight", norm_weight), ("post_weight", post_weight)):
-        if w is None:
-            continue
-        if w.dim() != 1 or w.shape[0] != width or wcode is None or w.get_device() != index or not w.is_contiguous():
-            raise ValueError(f"block_norm: {name} must be a contiguous [{width}] bfloat16 or float32 tensor on the rows' device")
-        if w.dtype is not wdtype:
+    if wcode is None:
+        raise ValueError("block_norm: norm_weight must be bfloat16 or float32")
+    norm_w = _weight(norm_weight, width, index, "norm_weight")
+    post_w = launch.NO_BUFFER
+    if post_weight is not None:
+        post_w = _weight(post_weight, width, index, "post_weight")
+        if post_weight.dtype is not wdtype:
             raise ValueError("block_norm: norm_weight and post_weight must have one type")
     gate_buf, gate_rs, gate_cs = launch.NO_BUFFER, 0, 0
     if gate is not None:
@@ -74,24 +78,24 @@ def block_norm(residual: torch.Tensor, delta: torch.Tensor | None = None, *, nor
             raise ValueError("block_norm: gate must be contiguous along its rows")
         span = (gate.shape[0] - 1) * gate_rs + (gate.shape[1] - 1) * gate_cs + 1
         gate_buf = (gate.data_ptr(), span * _SIZES[dtype], 0, 0)
-    like = residual if residual.is_contiguous() else None
+    res, res_stride = launch.rows_buffer(residual, rows, width, _SIZES[dtype], "block_norm: residual")
+    whole = residual.is_contiguous()          # empty_like is the cheapest allocation
     if normalized is None:
-        normalized = residual.new_empty(shape) if like is None else torch.empty_like(like)
-        norm, norm_stride = (normalized.data_ptr(), normalized.nbytes, 0, 0), width
+        normalized = torch.empty_like(residual) if whole else residual.new_empty(shape)
+        norm, norm_stride = (normalized.data_ptr(), rows * width * _SIZES[dtype], 0, 0), width
     else:
         norm, norm_stride = _rows(normalized, shape, dtype, index, "normalized")
-    res, res_stride = _rows(residual, shape, dtype, index, "residual")
     dlt, dlt_stride, out, out_stride = launch.NO_BUFFER, 0, launch.NO_BUFFER, 0
     if delta is not None:
         dlt, dlt_stride = _rows(delta, shape, dtype, index, "delta")
         if residual_out is None:
-            residual_out = residual.new_empty(shape) if like is None else torch.empty_like(like)
-            out, out_stride = (residual_out.data_ptr(), residual_out.nbytes, 0, 0), width
+            residual_out = torch.empty_like(residual) if whole else residual.new_empty(shape)
+            out, out_stride = (residual_out.data_ptr(), rows * width * _SIZES[dtype], 0, 0), width
         else:
             out, out_stride = _rows(residual_out, shape, dtype, index, "residual_out")
     if rows:
         launch.call(lib, "glmrt_b200_block_norm_async",
-                    _ARGS.pack(*res, *dlt, *launch.buffer(norm_weight), *launch.buffer(post_weight), *gate_buf, *out, *norm,
+                    _ARGS.pack(*res, *dlt, *norm_w, *post_w, *gate_buf, *out, *norm,
                                rows, width, res_stride, dlt_stride, gate_rs, gate_cs, out_stride, norm_stride,
                                code, wcode, scale, eps), index)
     return (residual if delta is None else residual_out), normalized

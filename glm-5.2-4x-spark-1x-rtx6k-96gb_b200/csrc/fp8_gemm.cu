@@ -716,11 +716,9 @@ constexpr int kMaxDevices = 64;
 // Clusters of `splits` CTAs that run at once on the current device (they must fit into one GPC each, so this is
 // less than the SMs divided by the size); asked once per device.
 template <int kMode, int kN, bool kOwnX>
-int active_clusters(int splits) {
+int active_clusters(int dev, int splits) {
   using C = WCfg<kMode, kN, kOwnX>;
   static std::atomic<int> known[kMaxDevices][9];
-  int dev = 0;
-  cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices) return 0;
   int n = known[dev][splits].load(std::memory_order_relaxed);
   if (n == 0) {
@@ -750,10 +748,11 @@ int active_clusters(int splits) {
 // 4096 x 6144: 4 splits 9.4, 6 splits 10.0).
 template <int kMode, int kN, bool kOwnX>
 int weight_splits(int tiles, int blocks, float* estimate_us) {
-  int best = 1;
+  int best = 1, dev = 0;
+  cudaGetDevice(&dev);
   float best_us = 0.0f;
   for (int s = 1; s <= 8 && s <= blocks; ++s) {
-    const int active = active_clusters<kMode, kN, kOwnX>(s) * (kOwnX ? WCfg<kMode, kN, kOwnX>::kPerSm : 1);
+    const int active = active_clusters<kMode, kN, kOwnX>(dev, s) * (kOwnX ? WCfg<kMode, kN, kOwnX>::kPerSm : 1);
     if (active <= 0) continue;
     const float us = static_cast<float>((tiles + active - 1) / active) *
                      (3.0f + (s > 1 ? 0.7f : 0.0f) + static_cast<float>((blocks + s - 1) / s) * (0.42f + 0.0015f * WCfg<kMode, kN, kOwnX>::kAccCols));

@@ -29,22 +29,27 @@ def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def _check_rows(x: torch.Tensor, k: int, types: tuple, what: str) -> None:
+def _rows(x: torch.Tensor, k: int, types: tuple, what: str) -> tuple[int, tuple, int]:
+    """Number, packed buffer and row stride of the rows."""
     if x.dim() != 2 or x.shape[1] != k or x.dtype not in types:
         raise ValueError(f"{what} must be [rows, {k}] of type {' or '.join(str(t) for t in types)}")
     if not x.is_cuda:
         raise ValueError(f"{what} must be on a CUDA device")
-    if not launch.inner_contiguous(x, k):
-        raise ValueError(f"{what} must be contiguous along its rows")
+    rows = x.shape[0]
+    buf, stride = launch.rows_buffer(x, rows, k, x.itemsize, what)
+    return rows, buf, stride
 
 
-def _check_weight(codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, index: int, what: str) -> None:
+def _weight(codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, index: int, what: str) -> tuple:
+    """Packed buffers of a weight's codes and scales."""
+    nb, kb = -(-n // BLOCK), -(-k // BLOCK)
     if codes.shape != (n, k) or codes.dtype not in _CODE_TYPES or not codes.is_contiguous():
         raise ValueError(f"{what} codes must be a contiguous E4M3 (or uint8) tensor [{n}, {k}]")
-    if scales.shape != (_blocks(n), _blocks(k)) or scales.dtype is not torch.float32 or not scales.is_contiguous():
-        raise ValueError(f"{what} scales must be a contiguous float32 tensor [{_blocks(n)}, {_blocks(k)}]")
+    if scales.shape != (nb, kb) or scales.dtype is not torch.float32 or not scales.is_contiguous():
+        raise ValueError(f"{what} scales must be a contiguous float32 tensor [{nb}, {kb}]")
     if codes.get_device() != index or scales.get_device() != index:
         raise ValueError(f"{what} must be on the device of the rows")
+    return codes.data_ptr(), n * k, 0, 0, scales.data_ptr(), nb * kb * 4, 0, 0
 
 
 def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -60,9 +65,8 @@ def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def quantize_rows(x: torch.Tensor, lib: N.NativeLibrary | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The rows' codes ``[rows, k]`` (E4M3) and scales ``[ceil(k/128), rows]``; x bf16 or float32."""
-    rows, k = x.shape if x.dim() == 2 else (0, 0)
-    _check_rows(x, k, (torch.bfloat16, torch.float32), "quantize_rows: x")
-    buf, stride = launch.rows_buffer(x, rows, k, x.element_size())
+    k = x.shape[1] if x.dim() == 2 else 0
+    rows, buf, stride = _rows(x, k, (torch.bfloat16, torch.float32), "quantize_rows: x")
     codes = torch.empty((rows, k), dtype=E4M3, device=x.device)
     scales = torch.empty((_blocks(k), rows), dtype=torch.float32, device=x.device)
     launch.call(lib, "glmrt_b200_fp8_quantize_rows_async",
@@ -100,15 +104,13 @@ def block_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out
     n, k = codes.shape
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("block_linear: out_dtype must be bfloat16 or float32")
-    _check_rows(x, k, _ROW_TYPES, "block_linear: x")
+    rows, buf, stride = _rows(x, k, _ROW_TYPES, "block_linear: x")
     index = x.get_device()
-    _check_weight(codes, scales, n, k, index, "block_linear: weight")
-    rows = x.shape[0]
-    buf, stride = launch.rows_buffer(x, rows, k, 2)
+    weight = _weight(codes, scales, n, k, index, "block_linear: weight")
     out = _output(out, rows, n, out_dtype, x)
     ws = _workspace(lib, "glmrt_b200_fp8_block_linear_workspace", x, rows, n, k)
     launch.call(lib, "glmrt_b200_fp8_block_linear_async",
-                _LINEAR_ARGS.pack(*buf, *launch.buffer(codes), *launch.buffer(scales), *launch.buffer(out), *launch.buffer(ws),
+                _LINEAR_ARGS.pack(*buf, *weight, *launch.buffer(out), *launch.buffer(ws),
                                   rows, n, k, stride, N.DTYPE_BF16 if out_dtype is torch.bfloat16 else N.DTYPE_F32), index)
     return out
 
@@ -122,17 +124,13 @@ def gated_mlp(x: torch.Tensor, gate_codes: torch.Tensor, gate_scales: torch.Tens
     if gate_codes.dim() != 2:
         raise ValueError("gated_mlp: gate codes must be [inter, hidden]")
     inter, hidden = gate_codes.shape
-    _check_rows(x, hidden, _ROW_TYPES, "gated_mlp: x")
+    rows, buf, stride = _rows(x, hidden, _ROW_TYPES, "gated_mlp: x")
     index = x.get_device()
-    _check_weight(gate_codes, gate_scales, inter, hidden, index, "gated_mlp: gate")
-    _check_weight(up_codes, up_scales, inter, hidden, index, "gated_mlp: up")
-    _check_weight(down_codes, down_scales, hidden, inter, index, "gated_mlp: down")
-    rows = x.shape[0]
-    buf, stride = launch.rows_buffer(x, rows, hidden, 2)
+    gate = _weight(gate_codes, gate_scales, inter, hidden, index, "gated_mlp: gate")
+    up = _weight(up_codes, up_scales, inter, hidden, index, "gated_mlp: up")
+    down = _weight(down_codes, down_scales, hidden, inter, index, "gated_mlp: down")
     out = _output(out, rows, hidden, torch.bfloat16, x)
     ws = _workspace(lib, "glmrt_b200_fp8_gated_mlp_workspace", x, rows, hidden, inter)
-    b = launch.buffer
     launch.call(lib, "glmrt_b200_fp8_gated_mlp_async",
-                _MLP_ARGS.pack(*buf, *b(gate_codes), *b(gate_scales), *b(up_codes), *b(up_scales), *b(down_codes),
-                               *b(down_scales), *b(out), *b(ws), rows, hidden, inter, stride), index)
+                _MLP_ARGS.pack(*buf, *gate, *up, *down, *launch.buffer(out), *launch.buffer(ws), rows, hidden, inter, stride), index)
     return out

@@ -20,24 +20,25 @@ def buffer(t: torch.Tensor | None) -> tuple:
     return NO_BUFFER if t is None else (t.data_ptr(), t.nbytes, 0, 0)
 
 
-def rows_buffer(t: torch.Tensor, rows: int, width: int, size: int) -> tuple[tuple, int]:
+def rows_buffer(t: torch.Tensor, rows: int, width: int, size: int, what: str) -> tuple[tuple, int]:
     """Packed fields and row stride (elements) of [rows, width] with rows contiguous inside, `size` bytes a value."""
-    if rows == 1 or t.is_contiguous():
+    if t.is_contiguous():
         return (t.data_ptr(), rows * width * size, 0, 0), width
+    if width > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what} must be contiguous along its rows")
+    if rows == 1:
+        return (t.data_ptr(), width * size, 0, 0), width
     stride = t.stride(0)
-    return (t.data_ptr(), ((rows - 1) * stride + width) * size if rows else 0, 0, 0), stride
-
-
-def inner_contiguous(t: torch.Tensor, width: int) -> bool:
-    return width <= 1 or t.is_contiguous() or t.stride(1) == 1
+    return (t.data_ptr(), ((rows - 1) * stride + width) * size, 0, 0), stride
 
 
 def call(lib: N.NativeLibrary | None, symbol: str, packed: bytes, index: int, *handle) -> None:
     """``symbol(*handle, packed, current stream of device index)``; raises what NativeLibrary.call raises."""
     lib = lib or N.library()
     fn = lib.symbol(symbol)
-    if index == torch.cuda.current_device():
-        status = fn(*handle, packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
+    if index == torch._C._cuda_getDevice():
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        status = fn(*handle, packed, C.c_void_p(stream) if stream else None)
     else:
         with torch.cuda.device(index):
             status = fn(*handle, packed, C.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
