@@ -440,12 +440,12 @@ __device__ __forceinline__ void select_row(const FewArgs& a, FewShared& sh, int 
   }
 }
 
-// Routes of all rows, then the list of entries (sh.ent_*).  `scratch`: for every expert a word and 16 half-words.
+// Routes of all rows, then the list of entries (sh.ent_*).  `scratch`: for every expert a word and a half-word.
 __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scratch, bool identity) {
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int routes = a.rows * a.top_k;
   uint32_t* mask = reinterpret_cast<uint32_t*>(scratch);                            // rows that name an expert
-  uint16_t* entry_of = reinterpret_cast<uint16_t*>(mask + a.experts);               // [expert][16]
+  uint16_t* first_entry = reinterpret_cast<uint16_t*>(mask + a.experts);            // [expert]
   for (int i = tid; i < a.experts; i += kThreads) mask[i] = 0u;
   for (int i = tid; i < routes * kCols; i += kThreads) {    // at most one entry per route
     sh.ent_route[i / kCols][i % kCols] = -1;
@@ -492,27 +492,33 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
     }
   }
   __syncthreads();
-  const int rank = live ? __popc(mask[e] & ((1u << token) - 1u)) : 0;
-  const bool opens = live && (identity ? rank == 0 : rank % kCols == 0);
-  const uint32_t votes = __ballot_sync(0xffffffffu, opens);
-  if (lane == 0) sh.warp_count[warp] = __popc(votes);
+  // An expert's entries follow each other, so that their passes over its weights run side by side and meet in the L2.
+  const uint32_t rows_of = live ? mask[e] : 0u;
+  const int rank = __popc(rows_of & ((1u << token) - 1u));
+  const int opens = !live || rank != 0 ? 0 : identity ? 1 : (__popc(rows_of) + kCols - 1) / kCols;      // entries from here
+  int upto = opens;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) sh.warp_count[warp] = upto;
   __syncthreads();
-  int before = __popc(votes & ((1u << lane) - 1u)), total = 0;
+  int before = upto - opens, total = 0;
 #pragma unroll
   for (int i = 0; i < kMaxRoutes / 32; ++i) {
     if (i < warp) before += sh.warp_count[i];
     total += sh.warp_count[i];
   }
-  const int group = identity ? 0 : rank / kCols;
-  if (opens) {
-    entry_of[e * 16 + group] = static_cast<uint16_t>(before);
-    sh.ent_expert[before] = static_cast<uint16_t>(e);
-    if (rank == 0) atomicAdd(&sh.distinct, 1);
+  if (opens > 0) {
+    first_entry[e] = static_cast<uint16_t>(before);
+    atomicAdd(&sh.distinct, 1);
   }
   if (tid == 0) sh.entries = total;
   __syncthreads();
   if (live) {
-    const int entry = entry_of[e * 16 + group], col = identity ? token : rank - group * kCols;
+    const int entry = first_entry[e] + (identity ? 0 : rank / kCols), col = identity ? token : rank % kCols;
+    sh.ent_expert[entry] = static_cast<uint16_t>(e);
     sh.ent_route[entry][col] = static_cast<int16_t>(tid);
     sh.ent_w[entry][col] = w;
   }
@@ -895,11 +901,11 @@ glmrt_status_t launch_ring(const FewArgs& a, size_t smem, int sm_count, cudaStre
 }
 }  // namespace
 
-// What fits into shared memory decides the depth of the stream; the selection's scratch (36 bytes an expert) lies in
+// What fits into shared memory decides the depth of the stream; the selection's scratch (6 bytes an expert) lies in
 // its ring, and at least three slots are needed.  Whether it fits is asked for the widest entries, also where one row
 // would do with less: a row's result must not depend on how many rows the call has.
 bool few_fused_supported(const FewArgs& a) {
-  static_assert(1024 * 36 <= 3 * kWarps * kSlotBytes, "selection scratch fits the ring");
+  static_assert(1024 * 6 <= 3 * kWarps * kSlotBytes, "selection scratch fits the ring");
   // (per_entry < 4096 makes the multiplication by its inverse exact: at most 256 entries)
   return few_smem(3, kCols, std::max(a.hidden, a.inter)) <= kSmemMost && a.experts <= 1024 && a.pass[0].per_entry > 1 &&
          a.pass[0].per_entry < 4096 && a.pass[1].per_entry > 1 && a.pass[1].per_entry < 4096;
