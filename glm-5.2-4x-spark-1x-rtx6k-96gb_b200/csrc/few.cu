@@ -68,6 +68,7 @@ constexpr int kLogitShares = kThreads / 32 / kLogitExperts;
 constexpr uint64_t kBarrierLimitNs = 2000000000ull;
 
 struct FewShared {
+  uint4 zero;
   uint16_t ent_expert[kMaxEntries];
   int16_t ent_route[kMaxEntries][kCols];     // column -> route, or -1
   float ent_w[kMaxEntries][kCols];           // column -> weight
@@ -118,6 +119,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same from zero.
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // All CTAs of the grid (co-resident: cooperative launch).  The arrivals of one barrier add up to 2^31: every CTA
@@ -261,13 +270,12 @@ __device__ __forceinline__ void multiply_slot(float (&acc)[2][2], uint32_t slot,
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[m][half][i] = 0.0f;
-#pragma unroll
       for (int i = 2 * half; i < 2 * half + 2; ++i) {
         uint32_t d0[4], d1[4];
         e2m1x8_to_f16(w[2 * m][i], d0);
         e2m1x8_to_f16(w[2 * m + 1][i], d1);
-        mma16816(c[m][half], d0[0], d1[0], d0[1], d1[1], b[4 * i], b[4 * i + 1]);
+        if (i == 2 * half) mma16816_first(c[m][half], d0[0], d1[0], d0[1], d1[1], b[4 * i], b[4 * i + 1]);
+        else mma16816(c[m][half], d0[0], d1[0], d0[1], d1[1], b[4 * i], b[4 * i + 1]);
         mma16816(c[m][half], d0[2], d1[2], d0[3], d1[3], b[4 * i + 2], b[4 * i + 3]);
       }
     }
@@ -376,15 +384,14 @@ __device__ void load_act_columns(const FewArgs& a, FewShared& sh, uint8_t* dst, 
   main_sync();
 }
 
-// Lane (g, t) holds the values of lane t in product column g = 4 token + t': they are the token's where t' = t (`mine`),
-// else zero (and b stays as it was set).
-__device__ __forceinline__ void load_b(uint32_t (&b)[16], uint32_t lane_columns, int unit, int cols, bool mine) {
-  if (!mine) return;
-  const uint32_t step = cols * 64, at = lane_columns + unit * 4 * step;
+// Lane (g, t) holds the values of lane t in product column g = 4 token + t': they are the token's where t' = t, else
+// zero (read from FewShared::zero, with a step of nothing).
+__device__ __forceinline__ void load_b(uint32_t (&b)[16], uint32_t lane_columns, int unit, uint32_t lane_step) {
+  const uint32_t at = lane_columns + unit * 4 * lane_step;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t q[4];
-    lds128(q, at + i * step);
+    lds128(q, at + i * lane_step);
     b[4 * i] = q[0]; b[4 * i + 1] = q[1]; b[4 * i + 2] = q[2]; b[4 * i + 3] = q[3];
   }
 }
@@ -598,6 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
   uint8_t* columns = reinterpret_cast<uint8_t*>(red + kBufs * red_floats);
   if (tid == 0) {
     sh.abort = 0u;
+    sh.zero = make_uint4(0u, 0u, 0u, 0u);
     for (int i = 0; i < kBufs; ++i) {
       tc::mbar_init(&sh.full[i], kWarps);
       tc::mbar_init(&sh.empty[i], 1);
@@ -661,11 +669,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
     uint32_t tail = st.ring;
     const int lane_token = lane >> 4;                  // of the product column this lane brings, and whether it has values
     const bool mine = ((lane >> 2) & 3) == (lane & 3) && lane_token < cols;
-    const uint32_t lane_columns = smem_addr(columns) + (lane_token * 4 + (lane & 3)) * 16;
+    const uint32_t lane_columns = mine ? smem_addr(columns) + (lane_token * 4 + (lane & 3)) * 16 : smem_addr(&sh.zero);
+    const uint32_t lane_step = mine ? cols * 64 : 0;
     const int scale_at = 2048 - lane * 8;
     uint32_t b[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) b[i] = 0u;
     int n = 0;                     // items so far: buffer n % kBufs, its round n / kBufs
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
@@ -689,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
         float acc[2][2] = {};
 #pragma unroll 1
         for (int k = kwi; k < p.units; k += p.kw) {
-          load_b(b, lane_columns, k, cols, mine);
+          load_b(b, lane_columns, k, lane_step);
           cp_async_wait<kRing - 2>();
           multiply_slot(acc, tail, tail + scale_at, b);
           tail += kSlotBytes;
@@ -699,7 +706,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
         // The item's partial sums go to a summing warp.  A wait that ran out is seen by everybody at the grid's next
         // barrier; until then the warp keeps step with the others, which meet it at the barriers around their columns.
         const int buf = n % kBufs;
-        if (tc::mbar_wait_warp(&sh.empty[buf], ((n / kBufs) & 1) ^ 1u, &sh.abort)) {
+        const uint32_t empty_parity = ((n / kBufs) & 1) ^ 1u;
+        if (__all_sync(0xffffffffu, tc::mbar_try_wait(&sh.empty[buf], empty_parity)) || tc::mbar_wait_warp(&sh.empty[buf], empty_parity, &sh.abort)) {
           store_partial(red + buf * red_floats + warp * 32 * cols, acc, factor, lane, cols);
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&sh.full[buf]);
