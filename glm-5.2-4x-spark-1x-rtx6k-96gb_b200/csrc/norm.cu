@@ -42,9 +42,9 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ uint16_t from_f32<uint16_t>(float v) { return f32_to_bf16_rne(v); }
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 
-// kVec consecutive values as they lie in memory: 16 aligned bytes, or one value.
+// kVec consecutive values as they lie in memory: 16 or 8 aligned bytes, or one value.
 template <typename T, int kVec>
-struct alignas(kVec == 1 ? sizeof(T) : 16) Piece {
+struct alignas(kVec * sizeof(T)) Piece {
   T t[kVec];
   __device__ __forceinline__ static Piece load(const T* p) { return *reinterpret_cast<const Piece*>(p); }
   __device__ __forceinline__ void unpack(float (&v)[kVec]) const {
@@ -61,11 +61,11 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[kVec]) {
   for (int i = 0; i < kVec; ++i) q.t[i] = from_f32<T>(v[i]);
   *reinterpret_cast<Piece<T, kVec>*>(p) = q;
 }
-// Weights may be wider or narrower than the rows: kVec of them, vectorised where they are whole 16-byte pieces.
+// Weights may be wider or narrower than the rows: kVec of them, at most 16 bytes a load.
 template <typename W, int kVec>
 __device__ __forceinline__ void load_weight(const W* p, float (&v)[kVec]) {
-  constexpr int kPer = 16 / sizeof(W);
-  if constexpr (kVec % kPer == 0 && kVec > 1) {
+  constexpr int kPer = std::min<int>(16 / sizeof(W), kVec);
+  if constexpr (kVec > 1) {
 #pragma unroll
     for (int i = 0; i < kVec; i += kPer) {
       float t[kPer];
@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(NormArgs a) {
 
 // Many wide bf16 rows: a CTA takes every gridDim-th row; bulk copies bring the next rows into a ring in shared
 // memory while one is worked on, and the weights stay in registers (8192 x 6144: 71 us; four streams of 100 MB at the
-// copy rate are 61).  Rows whose pieces are 16 bytes, aligned; two pieces a thread.
+// copy rate are 61).  Rows whose pieces are 16 bytes, aligned; two pieces a thread; no norm of the branch (its sum
+// would make the chain of a row longer, and only two rows are under way on an SM).
 template <typename W>
 __global__ void __launch_bounds__(512, 2) block_norm_stream_kernel(NormArgs a, int stages, uint32_t row_bytes, uint32_t* error_word) {
   using T = uint16_t;
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(512, 2) block_norm_stream_kernel(NormArgs a, i
     }
   const float inv_width = 1.0f / static_cast<float>(a.width);
   auto column = [&](int n) { return (n * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * kVec; };
-  uint4 norm_w[kNv][kVec / kPer], post_w[kNv][kVec / kPer];
+  uint4 norm_w[kNv][kVec / kPer];
   auto take = [&](const void* w, uint4 (&q)[kVec / kPer], int c) {
 #pragma unroll
     for (int i = 0; i < kVec / kPer; ++i) q[i] = *reinterpret_cast<const uint4*>(static_cast<const W*>(w) + c + i * kPer);
@@ -237,10 +238,7 @@ __global__ void __launch_bounds__(512, 2) block_norm_stream_kernel(NormArgs a, i
   auto weight_at = [&](const uint4 (&q)[kVec / kPer], int i) { return to_f32(reinterpret_cast<const W*>(&q[i / kPer])[i % kPer]); };
 #pragma unroll
   for (int n = 0; n < kNv; ++n)
-    if (column(n) < a.width) {
-      take(a.norm_w, norm_w[n], column(n));
-      if (a.post_w != nullptr) take(a.post_w, post_w[n], column(n));
-    }
+    if (column(n) < a.width) take(a.norm_w, norm_w[n], column(n));
   int stage = 0;
   uint32_t phase = 0;
   for (long long row_i = blockIdx.x; row_i < a.rows; row_i += gridDim.x) {
@@ -263,35 +261,20 @@ __global__ void __launch_bounds__(512, 2) block_norm_stream_kernel(NormArgs a, i
       const long long next = row_i + static_cast<long long>(stages) * gridDim.x;
       if (next < a.rows) fetch(static_cast<int>(next), stage);
     }
-    if (branch) {
-      if (a.post_w != nullptr) {
-        float ss = 0.0f;
+    if (branch && a.gate != nullptr) {
+      const T* g = static_cast<const T*>(a.gate) + row * a.gate_rs;
 #pragma unroll
-        for (int n = 0; n < kNv; ++n)
+      for (int n = 0; n < kNv; ++n) {
+        if (column(n) >= a.width) continue;
+        float s[kVec];
+        if (a.gate_cs == 0) {
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) ss += v[n][i] * v[n][i];
-        const float rs = rsqrtf(row_sum(ss, scratch) * inv_width + a.eps);
-#pragma unroll
-        for (int n = 0; n < kNv; ++n)
-          if (column(n) < a.width)
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) v[n][i] *= rs * weight_at(post_w[n], i);
-      }
-      if (a.gate != nullptr) {
-        const T* g = static_cast<const T*>(a.gate) + row * a.gate_rs;
-#pragma unroll
-        for (int n = 0; n < kNv; ++n) {
-          if (column(n) >= a.width) continue;
-          float s[kVec];
-          if (a.gate_cs == 0) {
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) s[i] = to_f32(*g);
-          } else {
-            load_vec<T, kVec>(g + column(n), s);
-          }
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) v[n][i] *= s[i];
+          for (int i = 0; i < kVec; ++i) s[i] = to_f32(*g);
+        } else {
+          load_vec<T, kVec>(g + column(n), s);
         }
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[n][i] *= s[i];
       }
     }
     float ss = 0.0f;
@@ -345,22 +328,31 @@ glmrt_status_t launch_stream(const NormArgs& a, int stages, uint32_t row_bytes, 
   return GLMRT_STATUS_OK;
 }
 
+// Rows of one residual stream are at least this many values (8 MB of bf16) before bf16 rows are taken in 8-byte pieces.
+constexpr long long kManyValues = 1ll << 22;
+
 template <typename T, typename W, int kVec>
 glmrt_status_t dispatch(const NormArgs& a, cudaStream_t s) {
   const int pieces = (a.width + kVec - 1) / kVec;
   constexpr int kMost = 32 / kVec;            // accesses per thread at 32 values
+  constexpr bool kBf16 = sizeof(T) == 2;
+  const bool many = static_cast<long long>(a.rows) * a.width >= kManyValues;
   if constexpr (kVec == 8) {
-    // bf16 rows of 8 to 16 KB, at least four for each of the 296 CTAs: the kernel above holds 16 values a thread there
-    // and too few rows on an SM (measured, rows x width: 1200 x 6144 13.8 against 15.4 us, 8192 x 6144 71 / 87,
-    // 8192 x 8192 93 / 127, 8192 x 4096 55 / 62; but 8192 x 2048 47 / 30, and float32 8192 x 4096 90 / 80).
+    // bf16 rows of 10 to 16 KB without a norm of the branch, at least four for each of the 296 CTAs (rows x width,
+    // against the form below: 8192 x 6144 71 / 74 us, 8192 x 8192 93 / 106, 1200 x 8192 16.8 / 19.3; 8192 x 4096 55 / 52,
+    // and with a norm of the branch 8192 x 6144 108 / 91).
     const uint32_t row_bytes = static_cast<uint32_t>(a.width) * sizeof(T);
     const int ctas = 2 * 148, stages = std::min<int>(8, kStreamRing / (row_bytes * (a.delta != nullptr ? 2 : 1)));
-    if (a.rows >= 4 * ctas && pieces >= 512 && pieces <= 1024) return launch_stream<W>(a, stages, row_bytes, ctas, s);
+    if (a.post_w == nullptr && a.rows >= 4 * ctas && pieces >= 640 && pieces <= 1024) return launch_stream<W>(a, stages, row_bytes, ctas, s);
+    // Many bf16 values: four pieces of 8 bytes a thread do better than two of 16 (with a norm of the branch, two / four:
+    // 8192 x 2048 35 / 31 us, 8192 x 4096 75 / 64, 8192 x 6144 107 / 91, 8192 x 8192 156 / 132; but 1200 x 1024 4.0 / 4.7).
+    if (many) return dispatch<T, W, 4>(a, s);
   }
   // A few rows: as many threads per row as it has pieces, for the latency.  More rows than SMs: two pieces a thread,
   // so that several rows share an SM and their loads overlap each other's reductions (measured at 333 x 5120 bf16
   // with both norms and a gate: one piece 5.9 us, two 5.1, four 8.9).
   int nv = 1;
+  if (kBf16 && kVec == 4 && many) nv = 4;
   while (nv < kMost && (pieces + nv - 1) / nv > 1024) nv *= 2;
   if (a.rows > 2 * 148 && nv == 1 && pieces >= 256) nv = 2;
   const int threads = ((pieces + nv - 1) / nv + 31) / 32 * 32;
@@ -376,9 +368,13 @@ glmrt_status_t dispatch(const NormArgs& a, cudaStream_t s) {
   return GLMRT_STATUS_OK;
 }
 
+// align: bytes that every row and weight piece may be read at once
 template <typename T, typename W>
-glmrt_status_t dispatch_vec(const NormArgs& a, bool vec, cudaStream_t s) {
-  return vec ? dispatch<T, W, 16 / static_cast<int>(sizeof(T))>(a, s) : dispatch<T, W, 1>(a, s);
+glmrt_status_t dispatch_vec(const NormArgs& a, int align, cudaStream_t s) {
+  if (align == 16) return dispatch<T, W, 16 / static_cast<int>(sizeof(T))>(a, s);
+  if constexpr (sizeof(T) == 2)
+    if (align == 8) return dispatch<T, W, 4>(a, s);
+  return dispatch<T, W, 1>(a, s);
 }
 
 struct Span { uintptr_t lo, hi; size_t stride; };
@@ -407,7 +403,11 @@ extern "C" glmrt_status_t glmrt_b200_block_norm_async(const glmrt_b200_block_nor
   const bool branch = p->delta.ptr != nullptr;
   if (!branch && (p->post_weight.ptr != nullptr || p->gate.ptr != nullptr || p->residual_out.ptr != nullptr))
     return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm: post_weight, gate and residual_out need a delta");
-  bool vec = p->width % (16 / size) == 0;
+  // the widest access that the width, every address and every stride allow: 16 bytes, 8 bytes (bf16 rows) or one value
+  int align = p->width % (16 / size) == 0 ? 16 : p->width % (8 / size) == 0 ? 8 : 0;
+  auto aligned_to = [&](uintptr_t v) {
+    while (align != 0 && v % static_cast<uintptr_t>(align) != 0) align = align == 16 ? 8 : 0;
+  };
   Span spans[4];                              // residual, delta, residual_out, normalized
   auto rows_ok = [&](const glmrt_device_buffer_t& b, size_t row_stride, Span* span, const char* what) {
     if (b.ptr == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string("block_norm ") + what + ": null buffer");
@@ -417,7 +417,8 @@ extern "C" glmrt_status_t glmrt_b200_block_norm_async(const glmrt_b200_block_nor
       return fail(GLMRT_STATUS_BUFFER_TOO_SMALL, std::string("block_norm ") + what + ": buffer too small");
     const uintptr_t at = reinterpret_cast<uintptr_t>(b.ptr);
     if (at % size != 0) return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string("block_norm ") + what + ": misaligned");
-    vec = vec && at % 16 == 0 && row_stride % (16 / size) == 0;
+    aligned_to(at);
+    if (p->rows > 1) aligned_to(row_stride * size);
     *span = Span{at, at + (need + p->width) * size, row_stride};
     return GLMRT_STATUS_OK;
   };
@@ -443,7 +444,9 @@ extern "C" glmrt_status_t glmrt_b200_block_norm_async(const glmrt_b200_block_nor
     const Span s{at, at + p->width * wsize, 0};
     if (overlap(s, spans[3]) || (branch && overlap(s, spans[2])))
       return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string("block_norm ") + what + ": overlaps an output");
-    vec = vec && at % 16 == 0;
+    // (the narrower pieces are four values: 8 bytes of bf16 weights, 16 of float32)
+    if (wsize == 4 && at % 16 != 0) align = 0;
+    else aligned_to(at);
     return GLMRT_STATUS_OK;
   };
   if (p->norm_weight.ptr == nullptr) return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm norm_weight: null buffer");
@@ -460,7 +463,10 @@ extern "C" glmrt_status_t glmrt_b200_block_norm_async(const glmrt_b200_block_nor
     const Span s{at, at + (need + (p->gate_col_stride ? p->width : 1)) * size, 0};
     if (overlap(s, spans[2]) || overlap(s, spans[3]))
       return fail(GLMRT_STATUS_INVALID_ARGUMENT, "block_norm gate: overlaps an output");
-    if (p->gate_col_stride != 0) vec = vec && at % 16 == 0 && p->gate_row_stride % (16 / size) == 0;
+    if (p->gate_col_stride != 0) {
+      aligned_to(at);
+      aligned_to(p->gate_row_stride * size);
+    }
   }
   GLMRT_RETURN_IF_ERROR(require_cuda());
   NormArgs a{};
@@ -471,8 +477,8 @@ extern "C" glmrt_status_t glmrt_b200_block_norm_async(const glmrt_b200_block_nor
   a.rows = static_cast<int>(p->rows); a.width = static_cast<int>(p->width);
   a.scale = p->scale; a.eps = p->eps;
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-  GLMRT_RETURN_IF_ERROR(size == 2 ? (wsize == 2 ? dispatch_vec<uint16_t, uint16_t>(a, vec, s) : dispatch_vec<uint16_t, float>(a, vec, s))
-                                  : (wsize == 2 ? dispatch_vec<float, uint16_t>(a, vec, s) : dispatch_vec<float, float>(a, vec, s)));
+  GLMRT_RETURN_IF_ERROR(size == 2 ? (wsize == 2 ? dispatch_vec<uint16_t, uint16_t>(a, align, s) : dispatch_vec<uint16_t, float>(a, align, s))
+                                  : (wsize == 2 ? dispatch_vec<float, uint16_t>(a, align, s) : dispatch_vec<float, float>(a, align, s)));
   GLMRT_LAUNCH_CHECK("block_norm_kernel");
   return ok();
 }

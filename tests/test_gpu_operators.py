@@ -70,7 +70,7 @@ def check_norm(mods, res, delta, nw, pw=None, gate=None, scale=1.0, eps=1e-5, **
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,width", [(1, 6144), (3, 1), (5, 7), (2, 256), (700, 264), (1, 32768), (3, 32767), (301, 6144),
-                                        (2, 1025), (299, 5001), (7, 16384)])
+                                        (2, 1025), (299, 5001), (7, 16384), (4, 4100), (350, 12), (600, 2052), (2, 32764)])
 def test_block_norm_sizes(mods, dtype, wdtype, rows, width):
     res, delta = randn(1, rows, width, std=2.0, dtype=dtype), randn(2, rows, width, dtype=dtype)
     nw, pw = 1 + randn(3, width, std=0.1), 1 + randn(4, width, std=0.1)
@@ -85,9 +85,9 @@ def test_block_norm_sizes(mods, dtype, wdtype, rows, width):
 
 @pytest.mark.parametrize("dtype,wdtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
                                           (torch.float32, torch.bfloat16), (torch.float32, torch.float32)])
-@pytest.mark.parametrize("rows,width", [(1183, 4096), (1184, 4096), (1185, 4104), (2371, 520), (4737, 256), (2368, 8192), (1300, 8200), (3001, 6144)])
+@pytest.mark.parametrize("rows,width", [(1183, 4096), (1184, 4096), (1185, 4104), (2371, 520), (4737, 256), (2368, 8192), (1300, 8200), (3001, 6144), (1279, 4100), (17000, 252), (300, 16380)])
 def test_block_norm_many_rows(mods, dtype, wdtype, rows, width):
-    """The streaming form (rows in a ring of shared memory) at its borders, with every term and in place."""
+    """The forms for many rows (a ring in shared memory, narrow pieces) at their borders, with every term and in place."""
     res, delta = randn(1, rows, width, std=2.0, dtype=dtype), randn(2, rows, width, dtype=dtype)
     nw, pw = (1 + randn(3, width, std=0.1)).to(wdtype), (1 + randn(4, width, std=0.1)).to(wdtype)
     want = check_norm(mods, res, delta, nw)
@@ -120,7 +120,7 @@ def test_block_norm_strides_and_alignment(mods):
     """Padded rows, rows that start off a 16-byte boundary, an expanded gate."""
     rows, width = 9, 520
     base = randn(1, rows, 3, width + 12, dtype=torch.bfloat16)
-    for off in (0, 1, 8):
+    for off in (0, 1, 4, 8):
         res, delta = base[:, 0, off:off + width], base[:, 1, off:off + width]
         out = torch.full((rows, width + 5), 7.0, device="cuda", dtype=torch.bfloat16)
         nw = (1 + randn(2, width + 1, std=0.1)).bfloat16()[1 - off % 2:][:width]
