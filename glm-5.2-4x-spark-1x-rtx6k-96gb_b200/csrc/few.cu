@@ -34,7 +34,9 @@ __device__ __forceinline__ float warp_sum(float v) {
 //   combine    residual + (shared + sum over the slots, in slot order)
 //
 // What bounds it is the experts' weights (9/16 byte each, read once); everything else is arranged so
-// that they never stop arriving.  Each lane copies its own pieces of the weights into shared memory
+// that they never stop arriving.  Measured at 6144 / 2048, 256 experts, top-8, back to back: 1 row 50 us (170 MB; 9 us
+// until the routes are known, 20 us gate / up, 2 us barrier, 11 us down, 5 us barrier and combine), 4 rows 134, 8 rows
+// 250, 16 rows 425 to 455 us (2.2 GB: 4.8 to 5.1 TB/s, by then bound by issue slots, 295 instructions a slot).  Each lane copies its own pieces of the weights into shared memory
 // (cp.async), kRing - 1 slots ahead, and only itself reads them back, so the stream needs no barrier
 // between warps; it runs on from the gate / up rows into the down rows while the CTA waits at the
 // barrier between them.
