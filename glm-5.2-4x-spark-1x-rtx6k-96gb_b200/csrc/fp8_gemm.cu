@@ -415,7 +415,7 @@ struct WCfg {
   static constexpr int kEpiWarps = 4 * kParts;
   static constexpr int kCols = kN / kParts;                         // of each matrix, per thread
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
-  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kXBytes + 1024 + 512 + kScaleBlocks * (kN + kMats) * 4;
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kXBytes + 1024 + 512 + kScaleBlocks * kN * kMats * 4;
   static_assert(static_cast<size_t>(kStages) * kStageBytes >= static_cast<size_t>(kMats) * kN * 128 * 4, "partial sums reuse the ring");
 };
 
@@ -438,8 +438,8 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
   uint64_t* x_full = acc_empty + 2;                                                 // kOwnX: a group of blocks is quantised
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_full + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  float* sx_all = reinterpret_cast<float*>(x_codes + C::kXBytes + 512);   // [kScaleBlocks][kN]
-  float* sw_all = sx_all + C::kScaleBlocks * kN;                              // [kMats][kScaleBlocks]
+  // scales of the next blocks, row's times weight's (a power of two: exact): [kMats][kScaleBlocks][kN]
+  float* scale_all = reinterpret_cast<float*>(x_codes + C::kXBytes + 512);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int blocks = (a.k + kFp8Block - 1) / kFp8Block;
@@ -585,46 +585,50 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
             const float scale = fp8_block_scale(amax, &inv);
             *reinterpret_cast<uint2*>(x_codes + bb * kN * kFp8Block + row * kFp8Block + (((sub >> 1) ^ (row & 7)) << 4) + (sub & 1) * 8) =
                 make_uint2(fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv), fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
-            if (sub == 0) sx_all[bb * kN + row] = scale;
+            if (sub == 0) {
+              scale_all[bb * kN + row] = scale * __ldg(a.ws0 + wb + b + bb);
+              if (kMode == 2) scale_all[(C::kScaleBlocks + bb) * kN + row] = scale * __ldg(a.ws1 + wb + b + bb);
+            }
           }
           fence_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(x_full);
         } else {
-          for (int i = tid; i < count * (kN / 4); i += 32 * C::kEpiWarps)
-            reinterpret_cast<float4*>(sx_all)[i] = *reinterpret_cast<const float4*>(
-                a.xs + static_cast<size_t>(b + i / (kN / 4)) * a.xs_stride + m0 + (i % (kN / 4)) * 4);
-        }
-        if (tid < count) {
-          sw_all[tid] = __ldg(a.ws0 + wb + b + tid);
-          if (kMode == 2) sw_all[(C::kMats - 1) * C::kScaleBlocks + tid] = __ldg(a.ws1 + wb + b + tid);
+          for (int i = tid; i < count * (kN / 4); i += 32 * C::kEpiWarps) {
+            const int bb = i / (kN / 4);
+            const float4 sx = *reinterpret_cast<const float4*>(a.xs + static_cast<size_t>(b + bb) * a.xs_stride + m0 + (i % (kN / 4)) * 4);
+#pragma unroll
+            for (int mat = 0; mat < C::kMats; ++mat) {
+              const float sw = __ldg((mat == 0 ? a.ws0 : a.ws1) + wb + b + bb);
+              reinterpret_cast<float4*>(scale_all)[mat * C::kScaleBlocks * (kN / 4) + i] = make_float4(sx.x * sw, sx.y * sw, sx.z * sw, sx.w * sw);
+            }
+          }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kEpiWarps) : "memory");
       }
-      const float* xs = sx_all + at * kN + part_col;
+      const float* scales = scale_all + at * kN + part_col;
       mbar_wait_hot(&acc_full[abuf], aphase, abort_flag);      // on a time-out it keeps step, computing nothing valid
       tc_fence_after();
-      constexpr int kChunk = C::kCols >= 32 ? 32 : 16;        // columns in flight, per matrix
+      // Chunks of all matrices' columns, the next one's on their way while one is added.
+      constexpr int kChunk = C::kCols >= 32 ? 32 : 16, kChunks = C::kMats * C::kCols / kChunk;
+      uint32_t v[2][kChunk];
+      auto load = [&](int c, uint32_t (&dst)[kChunk]) {
+        const uint32_t at_col = t_lane + abuf * C::kAccCols + c * kChunk / C::kCols * kN + c * kChunk % C::kCols;
+        if constexpr (kChunk == 32) tc_load32(at_col, dst);
+        else tc_load16(at_col, dst);
+      };
+      load(0, v[0]);
 #pragma unroll
-      for (int c = 0; c < C::kCols / kChunk; ++c) {
-        uint32_t v[C::kMats][kChunk];
-#pragma unroll
-        for (int mat = 0; mat < C::kMats; ++mat) {
-          if constexpr (kChunk == 32) tc_load32(t_lane + abuf * C::kAccCols + mat * kN + c * kChunk, v[mat]);
-          else tc_load16(t_lane + abuf * C::kAccCols + mat * kN + c * kChunk, v[mat]);
-        }
+      for (int c = 0; c < kChunks; ++c) {
         tc_wait_ld();
+        if (c + 1 < kChunks) load(c + 1, v[(c + 1) & 1]);
+        const int mat = c * kChunk / C::kCols, col = c * kChunk % C::kCols;
 #pragma unroll
         for (int i = 0; i < kChunk; i += 4) {
-          const float4 q = *reinterpret_cast<const float4*>(xs + c * kChunk + i);
-          const float sx[4] = {q.x, q.y, q.z, q.w};
+          const float4 q = *reinterpret_cast<const float4*>(scales + mat * C::kScaleBlocks * kN + col + i);
+          const float f[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-          for (int mat = 0; mat < C::kMats; ++mat) {
-            const float sw = sw_all[mat * C::kScaleBlocks + at];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              acc[mat][c * kChunk + i + e] = fmaf(__uint_as_float(v[mat][i + e]), sx[e] * sw, acc[mat][c * kChunk + i + e]);
-          }
+          for (int e = 0; e < 4; ++e) acc[mat][col + i + e] = fmaf(__uint_as_float(v[c & 1][i + e]), f[e], acc[mat][col + i + e]);
         }
       }
       tc_fence_before();
