@@ -11,8 +11,8 @@
 //       rows, the K blocks of a tile split over a cluster of up to eight CTAs, whose sums meet in
 //       shared memory.  Bound by the weight bytes, so what counts is that every SM streams.
 //
-// Measured (rows x n x k, in a chain of calls, the quantiser included): 8192 x 4096 x 6144 208 us = 1.98 PFLOP/s,
-// 8192 x 6144 x 2048 115 us; 256 x 4096 x 6144 22 us, 16 rows 9.1 us; one row 6.7 us = 3.8 TB/s of weights from launch to
+// Measured (rows x n x k, in a chain of calls, the quantiser included): 8192 x 4096 x 6144 197 us = 2.09 PFLOP/s,
+// 8192 x 6144 x 2048 111 us; 256 x 4096 x 6144 17.8 us, 16 rows 8.9 us; one row 6.7 us = 3.8 TB/s of weights from launch to
 // launch, 5.6 between the first and the last copy.
 //
 // Each in two forms: the plain product, and gate / up with the SwiGLU and the next quantisation in the
@@ -68,6 +68,17 @@ __device__ __forceinline__ uint32_t idesc_fp8(uint32_t n) { return (1u << 4) | (
 // so nothing has to be made visible.  (A releasing arrival also waits for the stores to global memory: half a microsecond.)
 __device__ __forceinline__ void cluster_leave() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// Two sums at once (fma.rn of each; for the few rows' kernel, 256 x 4096 x 6144 18.9 -> 17.8 us.  The many rows' has no
+// register to spare for the pairs: 198 -> 252 us).
+__device__ __forceinline__ void fma_pair(float& a0, float& a1, uint32_t v0, uint32_t v1, float s0, float s1) {
+  asm("{\n\t.reg .b64 a, v, s;\n\t"
+      "mov.b64 a, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 s, {%4, %5};\n\t"
+      "fma.rn.f32x2 a, v, s, a;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "r"(v0), "r"(v1), "f"(s0), "f"(s1));
 }
 
 constexpr int kTileBytes = 128 * kFp8Block;            // 128 rows of one K block
@@ -626,9 +637,8 @@ fp8_weights_kernel(WeightsArgs a, const __grid_constant__ CUtensorMap map_x, con
 #pragma unroll
         for (int i = 0; i < kChunk; i += 4) {
           const float4 q = *reinterpret_cast<const float4*>(scales + mat * C::kScaleBlocks * kN + col + i);
-          const float f[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[mat][col + i + e] = fmaf(__uint_as_float(v[c & 1][i + e]), f[e], acc[mat][col + i + e]);
+          fma_pair(acc[mat][col + i], acc[mat][col + i + 1], v[c & 1][i], v[c & 1][i + 1], q.x, q.y);
+          fma_pair(acc[mat][col + i + 2], acc[mat][col + i + 3], v[c & 1][i + 2], v[c & 1][i + 3], q.z, q.w);
         }
       }
       tc_fence_before();
@@ -840,8 +850,8 @@ glmrt_status_t launch_rows(const Fp8Gemm& g, int sm_count, cudaStream_t s) {
 
 // Tiles of 16, 32 and 64 rows for batches that small.  Above, the larger of the weight-row tiles or the row tiles,
 // by their estimates: a wave of row tiles costs about 4 us and 0.48 us a block, whatever part of its 256 rows is
-// filled (measured: 256 rows, n = 6144, k = 2048: 14 against 20 us on weight-row tiles; n = 1500, k = 2000: 16
-// against 10 us).
+// filled (measured, row tiles against weight-row tiles: 256 rows, n = 6144, k = 2048 12.3 / 13.8 us; n = 4096, k = 6144
+// 24 / 18; n = 1500, k = 2000 15 / 9; 600 rows, n = 4096, k = 6144 26 / 49).
 constexpr int kWeightsMostRows = 1024;
 
 template <int kMode>
