@@ -804,6 +804,12 @@ glmrt_status_t few_args(Layer* l, const glmrt_device_buffer_t& hidden, size_t ro
   return GLMRT_STATUS_OK;
 }
 
+glmrt_status_t few_routes(const glmrt_device_buffer_t& buffer, size_t routes, const char* what) {
+  GLMRT_RETURN_IF_ERROR(check_buf(buffer, routes * 4, what));
+  if (reinterpret_cast<uintptr_t>(buffer.ptr) % 4 != 0) return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string(what) + ": misaligned buffer");
+  return GLMRT_STATUS_OK;
+}
+
 // One fused kernel, except on the verification engine and for shapes beyond its shared memory.
 bool few_fused(const Layer* l, const FewArgs& a) {
   return !(l->cfg.flags & GLMRT_B200_LAYER_ENGINE_SIMT) && few_fused_supported(a);
@@ -819,8 +825,8 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_async(void* layer, co
   FewArgs a{};
   GLMRT_RETURN_IF_ERROR(few_args(l, hidden_bf16, rows, residual_bf16, shared_delta_bf16, output_bf16, &a));
   const size_t routes = rows * l->cfg.top_k;
-  if (topk_indices.ptr != nullptr) GLMRT_RETURN_IF_ERROR(check_buf(topk_indices, routes * 4, "forward_few topk_indices"));
-  if (topk_weights.ptr != nullptr) GLMRT_RETURN_IF_ERROR(check_buf(topk_weights, routes * 4, "forward_few topk_weights"));
+  if (topk_indices.ptr != nullptr) GLMRT_RETURN_IF_ERROR(few_routes(topk_indices, routes, "forward_few topk_indices"));
+  if (topk_weights.ptr != nullptr) GLMRT_RETURN_IF_ERROR(few_routes(topk_weights, routes, "forward_few topk_weights"));
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   const uint64_t before = launches_total();
   if (few_fused(l, a)) {
@@ -852,8 +858,8 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_routed_async(void* la
   FewArgs a{};
   GLMRT_RETURN_IF_ERROR(few_args(l, hidden_bf16, rows, residual_bf16, shared_delta_bf16, output_bf16, &a));
   const size_t routes = rows * l->cfg.top_k;
-  GLMRT_RETURN_IF_ERROR(check_buf(topk_indices, routes * 4, "forward_few_routed topk_indices"));
-  GLMRT_RETURN_IF_ERROR(check_buf(topk_weights, routes * 4, "forward_few_routed topk_weights"));
+  GLMRT_RETURN_IF_ERROR(few_routes(topk_indices, routes, "forward_few_routed topk_indices"));
+  GLMRT_RETURN_IF_ERROR(few_routes(topk_weights, routes, "forward_few_routed topk_weights"));
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   const uint64_t before = launches_total();
   a.topk_idx = static_cast<uint32_t*>(topk_indices.ptr);

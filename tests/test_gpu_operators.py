@@ -576,6 +576,33 @@ def test_few_full_size_layer(mods):
     layer.close()
 
 
+def test_few_refuses_what_the_wrapper_cannot_pass(mods):
+    """C entry points: too many rows, an output over the rows, buffers off their boundaries."""
+    import ctypes as C
+    from glmrt_b200 import native as N
+    layer = make_layer(mods, O.make_layer(18, 256, 256, 4), 2)
+    x, out = randn(1, 17, 256, dtype=torch.bfloat16), torch.empty(17, 256, device="cuda", dtype=torch.bfloat16)
+    idx, w = torch.zeros(17, 2, dtype=torch.int32, device="cuda"), torch.ones(17, 2, device="cuda")
+    buf, null = lambda t, off=0, less=0: N.DeviceBuffer.of(t.data_ptr() + off, t.nbytes - off - less), N.DeviceBuffer.null()
+
+    def status(name, hidden=buf(x), out=buf(out), idx=buf(idx), w=buf(w), residual=null, rows=4):
+        a = N.FewArgs(hidden, residual, null, out, idx, w, rows)
+        return layer.lib.call_status(f"glmrt_b200_moe_layer_{name}_async", layer.handle, C.byref(a), None)
+
+    for name in ("forward_few", "forward_few_routed"):
+        assert status(name) == 0
+        for bad in (dict(rows=17), dict(rows=0), dict(hidden=null), dict(out=null), dict(out=buf(x)), dict(out=buf(x, 512)), dict(hidden=buf(x, 8)),
+                    dict(out=buf(out, 2)), dict(residual=buf(out, 512)), dict(idx=buf(idx, 2)), dict(w=buf(w, 1))):
+            assert status(name, **bad) == 1, (name, bad)
+        for small in (dict(hidden=buf(x, 0, x.nbytes - 4 * 512 + 1)), dict(out=buf(out, 0, out.nbytes - 4 * 512 + 1)), dict(idx=buf(idx, 0, idx.nbytes - 31)),
+                      dict(w=buf(w, 0, w.nbytes - 31))):
+            assert status(name, **small) == 2, (name, small)
+    assert status("forward_few", idx=null, w=null) == 0
+    assert status("forward_few_routed", idx=null) == 1 and status("forward_few_routed", w=null) == 1
+    layer.check()
+    layer.close()
+
+
 def test_few_many_experts_and_most_routes(mods):
     """More than 256 experts, 16 slots, every row its own experts: 256 entries at once."""
     h, i, e, top_k = 512, 256, 330, 16
@@ -652,6 +679,87 @@ def test_operators_on_three_streams_at_once(mods):
         l.close()
     import importlib
     importlib.import_module("glmrt_b200.launch").check()
+
+
+def test_operators_from_two_host_threads(mods):
+    """Two threads, a stream and a lane each, sizes that take different kernels; one thread's refused calls between."""
+    import threading
+    from glmrt_b200 import native as N
+    ref = O.make_layer(17, 512, 256, 16)
+    layer = make_layer(mods, ref, 4)
+    lanes = [layer, layer.create_lane(16)]
+    w = mods["fp8"].quantize_weight(randn(1, 700, 512, std=0.05))
+    xs = {m: randn(m, m, 512, dtype=torch.bfloat16) for m in (1, 6, 16, 90, 1500)}
+    nw = torch.ones(512, device="cuda")
+
+    def work(l):
+        out = []
+        for m, x in xs.items():
+            out += [mods["fp8"].block_linear(x, *w), *mods["block_norm"].block_norm(x, x, norm_weight=nw)]
+            if m <= 16:
+                out.append(l.forward_few(x))
+        return out
+
+    want = work(layer)
+    torch.cuda.synchronize()
+    failures = []
+
+    def run(l, refused):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got = work(l)
+                if refused:
+                    try:
+                        mods["fp8"].block_linear(xs[6], *w, out=torch.empty(6, 699, device="cuda", dtype=torch.bfloat16))
+                        failures.append("not refused")
+                    except ValueError:
+                        pass
+                    try:
+                        l.forward_few(xs[16].repeat(2, 1))
+                        failures.append("not refused")
+                    except N.GlmrtError:
+                        pass
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(g, v) for g, v in zip(got, want)):
+                    failures.append("differs")
+
+    threads = [threading.Thread(target=run, args=(l, i == 1)) for i, l in enumerate(lanes)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    for l in reversed(lanes):
+        l.check()
+        l.close()
+
+
+def test_first_calls_of_a_process_may_be_captured(pkg):
+    """Nothing has to run before a capture: every operator's first call is inside one."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from __graft_entry__ import load_package
+load_package()
+from glmrt_b200 import fp8
+from glmrt_b200.block_norm import block_norm
+x = {m: torch.ones(m, 6144, device="cuda", dtype=torch.bfloat16) for m in (1, 40, 100, 2000)}
+w = fp8.quantize_weight(torch.linspace(-1, 1, 640 * 6144, device="cuda").view(640, 6144))
+d = fp8.quantize_weight(torch.linspace(-1, 1, 6144 * 640, device="cuda").view(6144, 640))
+nw = torch.ones(6144, device="cuda")
+def run():
+    return [t for v in x.values() for t in (fp8.block_linear(v, *w), fp8.gated_mlp(v, *w, *w, *d), *block_norm(v, v, norm_weight=nw))]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = run()
+g.replay()
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
 
 
 # ---- all of them together ------------------------------------------------------------------------
