@@ -491,9 +491,9 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
       if (s < slot) live = false;                 // the row has named this expert before: its weight went there
       else w += sh.route_w[token * a.top_k + s];
     }
-    if (a.out_idx != nullptr && blockIdx.x == 0) {
-      a.out_idx[tid] = e;
-      a.out_w[tid] = sh.route_w[tid];
+    if (blockIdx.x == 0) {                        // either may be wanted alone
+      if (a.out_idx != nullptr) a.out_idx[tid] = e;
+      if (a.out_w != nullptr) a.out_w[tid] = sh.route_w[tid];
     }
     if (live) {
       atomicOr(&mask[e], 1u << token);

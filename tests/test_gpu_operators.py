@@ -603,6 +603,28 @@ def test_few_refuses_what_the_wrapper_cannot_pass(mods):
     layer.close()
 
 
+@pytest.mark.parametrize("engine", ["simt", "tc"])
+def test_few_writes_either_route_buffer_alone(mods, engine):
+    """Through C: indices, weights, both or neither may be asked for."""
+    import ctypes as C
+    from glmrt_b200 import native as N
+    layer = make_layer(mods, O.make_layer(19, 256, 256, 12), 3, engine)
+    x = randn(1, 5, 256, dtype=torch.bfloat16)
+    want, want_idx, want_w = layer.forward_few(x, want_routes=True)
+    buf, null = lambda t: N.DeviceBuffer.of(t.data_ptr(), t.nbytes), N.DeviceBuffer.null()
+    for has_idx, has_w in ((True, True), (True, False), (False, True), (False, False)):
+        out = torch.zeros_like(x)
+        idx, w = torch.full((6, 3), 77, dtype=torch.int32, device="cuda"), torch.full((6, 3), 77.0, device="cuda")
+        a = N.FewArgs(buf(x), null, null, buf(out), buf(idx) if has_idx else null, buf(w) if has_w else null, 5)
+        assert layer.lib.call_status("glmrt_b200_moe_layer_forward_few_async", layer.handle, C.byref(a), None) == 0
+        layer.check()
+        assert torch.equal(out, want), (has_idx, has_w)
+        assert torch.equal(idx[:5], want_idx) if has_idx else (idx[:5] == 77).all()
+        assert torch.equal(w[:5], want_w) if has_w else (w[:5] == 77).all()
+        assert (idx[5] == 77).all() and (w[5] == 77).all()
+    layer.close()
+
+
 def test_few_many_experts_and_most_routes(mods):
     """More than 256 experts, 16 slots, every row its own experts: 256 entries at once."""
     h, i, e, top_k = 512, 256, 330, 16
