@@ -135,9 +135,12 @@ __device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint3
 // adds one, the first what is missing.  So the top bit flips when the last has come, and nothing has to be
 // reset.  Thread 0 knows the bit from before its first arrival (it cannot flip without it), so an arrival needs no
 // answer.  Arriving and waiting are apart, so that work may lie between them; false when the wait ran out.
-__device__ __forceinline__ uint32_t grid_bit(const uint32_t* count) {
+// CTAs that gave up arrive no more, so the count is then short and a later call could pass a barrier early.  They
+// leave that in the word behind the count (kCntFewExpired), and every call that finds it set does nothing until the
+// layer's check has reported it and cleared both.
+__device__ __forceinline__ uint32_t grid_bit(const uint32_t* count, uint32_t& expired) {
   uint32_t now;
-  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(count) : "memory");
+  asm volatile("ld.relaxed.gpu.global.v2.u32 {%0, %1}, [%2];" : "=r"(now), "=r"(expired) : "l"(count) : "memory");
   return now & 0x80000000u;
 }
 __device__ __forceinline__ void grid_arrive(uint32_t* count) {
@@ -616,11 +619,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
   if (tid < kFewMaxRows) sh.x_amax[tid] = 0u;
   __syncthreads();
 
-  uint32_t bit = tid == 0 ? grid_bit(a.sync) : 0u;
+  uint32_t* sync = a.counters + kCntFewBarrier;
+  uint32_t expired = 0u, bit = tid == 0 ? grid_bit(sync, expired) : 0u;
   if (a.scores != nullptr) {
     score_experts(a, sh, warp, lane);
-    grid_arrive(a.sync);
+    grid_arrive(sync);
   }
+  if (expired != 0u) sh.abort = 1u;
   // the rows' largest magnitudes, 256 values a warp
   const int row_pieces = a.hidden / 256;
 #pragma unroll 1
@@ -634,11 +639,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
     if (lane == 0) atomicMax(&sh.x_amax[i / row_pieces], m);
   }
   __syncthreads();
+  if (sh.abort != 0u) return;            // an earlier call's: nothing is written
   if (tid < a.rows) f16_factor(sh.x_amax[tid], &sh.x_inv[tid]);
   if (identity && warp < kWarps) load_hidden_columns(a, sh, columns, 0, cols, true);    // needs no routes
   if (a.scores != nullptr) {
-    if (!grid_wait(a.sync, bit, &sh.abort)) {
-      if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
+    if (!grid_wait(sync, bit, &sh.abort)) {
+      if (tid == 0) atomicOr(a.counters + kCntFewExpired, static_cast<uint32_t>(kErrWaitTimeout));
       return;
     }
   }
@@ -678,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
     int n = 0;                     // items so far: buffer n % kBufs, its round n / kBufs
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
-      if (pass == 1) grid_barrier(a.sync, bit, &sh.abort);
+      if (pass == 1) grid_barrier(sync, bit, &sh.abort);
       const Share s = pass == 0 ? s1 : s2;
       const FewPass p = a.pass[pass];
       const int kwi = warp & (p.kw - 1);
@@ -772,11 +778,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
         if (lane == 0) tc::mbar_arrive(&sh.empty[mine]);
       }
       base += items;
-      if (pass == 0) grid_barrier(a.sync, bit, &sh.abort);
+      if (pass == 0) grid_barrier(sync, bit, &sh.abort);
     }
   }
-  if (!grid_barrier(a.sync, bit, &sh.abort)) {
-    if (tid == 0) atomicOr(a.error_word, static_cast<uint32_t>(kErrWaitTimeout));
+  if (!grid_barrier(sync, bit, &sh.abort)) {
+    if (tid == 0) atomicOr(a.counters + kCntFewExpired, static_cast<uint32_t>(kErrWaitTimeout));
     return;
   }
 

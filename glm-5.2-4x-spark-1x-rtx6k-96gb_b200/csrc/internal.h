@@ -27,7 +27,9 @@ enum Counter : int {
   kCntLocalRoutes = 4,
   kCntRouterError = 5,   // error word of the tensor-core router kernel (cleared by that kernel)
   kCntTicket = 6,        // last-CTA ticket of the router's selection kernel (zero between launches)
-  kCntWords = 8,
+  kCntFewBarrier = 8,    // barrier count of the few-token kernel (few.cu), then kErrWaitTimeout when one of its waits
+  kCntFewExpired = 9,    // ran out: only the layer's check clears them, and until it has, such calls do nothing
+  kCntWords = 16,
 };
 
 struct Chunk {      // one (expert, block of <= BN tokens) work item
@@ -331,7 +333,6 @@ struct FewArgs {
   uint32_t* out_idx;                                        // where the routes are written, or nullptr
   float* out_w;
   float* route_out;                                         // [rows * top_k, hidden] float32 result rows
-  uint32_t* sync;                                           // barrier count
   uint32_t* counters;
 };
 FewPass few_pass(int k, int groups);

@@ -81,11 +81,9 @@ struct Layer {
   uint16_t* route_rows = nullptr;
   uint16_t** slot_out = nullptr;
   uint32_t* slot_weight = nullptr;   // route weight per slot (fused combine of large batches)
-  // few-token path: weighted SwiGLU rows, one float32 result row per route, scores, the count of
-  // its kernel's barriers
+  // few-token path: weighted SwiGLU rows, one float32 result row per route, scores
   float *few_act = nullptr, *few_out = nullptr;
   uint2* few_scores = nullptr;
-  uint32_t* few_sync = nullptr;
   uint32_t* fc_sync = nullptr;       // hand-over words between the decode FC1 and FC2 kernels
   uint16_t *hidden_stage = nullptr, *out_stage = nullptr;
   // scratch for weight loading
@@ -479,7 +477,6 @@ glmrt_status_t alloc_workspace(Layer* l) {
     A(dev_alloc(b, &l->few_act, F * K * I));
     A(dev_alloc(b, &l->few_out, F * K * H));
     A(dev_alloc(b, &l->few_scores, F * c.experts));
-    A(dev_alloc(b, &l->few_sync, 1, true));
   }
   A(dev_alloc(b, &l->hidden_stage, T * H));
   A(dev_alloc(b, &l->out_stage, T * H));
@@ -798,7 +795,6 @@ glmrt_status_t few_args(Layer* l, const glmrt_device_buffer_t& hidden, size_t ro
   a.route_out = l->few_out;
   a.pass[0] = few_pass(a.hidden, a.inter / 16);
   a.pass[1] = few_pass(a.inter, a.hidden / 32);
-  a.sync = l->few_sync;
   a.counters = l->counters;
   *out = a;
   return GLMRT_STATUS_OK;
@@ -951,11 +947,11 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_check(void* layer, void* cuda_str
   cudaError_t err = cudaStreamSynchronize(static_cast<cudaStream_t>(cuda_stream));
   if (err == cudaSuccess) err = cudaMemcpy(host, l->counters, sizeof(host), cudaMemcpyDeviceToHost);
   if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_COPY_FAILED, "layer check", err);
-  const uint32_t e = host[kCntError] | host[kCntRouterError];
+  const uint32_t e = host[kCntError] | host[kCntRouterError] | host[kCntFewExpired];
   if (e == 0) return ok();
-  // a few-token kernel that gave up leaves its barrier count uneven: nothing runs now, so it is cleared
-  if ((e & kErrWaitTimeout) && l->few_sync != nullptr &&
-      (err = cudaMemset(l->few_sync, 0, sizeof(*l->few_sync))) != cudaSuccess)
+  // a few-token kernel that gave up leaves its barrier count uneven, and every later one leaves at once; nothing runs
+  // now, so both are cleared
+  if (host[kCntFewExpired] != 0 && (err = cudaMemset(l->counters + kCntFewBarrier, 0, 8)) != cudaSuccess)
     return fail_cuda(GLMRT_STATUS_COPY_FAILED, "layer check", err);
   std::string msg = "device reported:";
   if (e & kErrWaitTimeout) msg += " a bounded wait expired;";
@@ -1015,7 +1011,7 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_stats(void* layer, glmrt_b200_lay
   out->chunks = host[kCntChunks];
   out->slots = host[kCntSlots];
   out->distinct_experts = host[kCntDistinct];
-  out->device_error = host[kCntError] | host[kCntRouterError];
+  out->device_error = host[kCntError] | host[kCntRouterError] | host[kCntFewExpired];
   return ok();
 }
 

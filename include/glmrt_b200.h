@@ -586,7 +586,9 @@ glmrt_status_t glmrt_b200_moe_layer_forward_routed_async(
     glmrt_device_buffer_t topk_weights, glmrt_device_buffer_t output_bf16, void* cuda_stream);
 
 /* Device-side error word of the last forward (0 = none): bounded waits that gave up and
- * capacity overflows are reported here instead of hanging or faulting.  Synchronises. */
+ * capacity overflows are reported here instead of hanging or faulting.  Synchronises.
+ * A wait that ran out in a forward_few stays reported whatever runs after it; until this call has
+ * reported it, every forward_few of the workspace leaves its outputs as they are. */
 glmrt_status_t glmrt_b200_moe_layer_check(void* layer, void* cuda_stream);
 
 /* Introspection for tests and profiling. */
@@ -598,7 +600,7 @@ typedef enum glmrt_b200_debug_buffer_t {
   GLMRT_B200_DEBUG_ACT2_CODES = 4,   /* [slots, I/2] requantised SwiGLU output */
   GLMRT_B200_DEBUG_ACT2_SF = 5,
   GLMRT_B200_DEBUG_ROUTE_ROWS = 6,   /* bf16 [rows * top_k, H] per-route FC2 output */
-  GLMRT_B200_DEBUG_COUNTERS = 7,     /* uint32 [8]: chunks, slots, error, ... */
+  GLMRT_B200_DEBUG_COUNTERS = 7,     /* uint32 [16]: chunks, slots, error, ... */
   GLMRT_B200_DEBUG_CHUNKS = 8,       /* int32 [chunks][4]: expert, slot_base, tokens, 0 */
   GLMRT_B200_DEBUG_EXPERT_COUNTS = 9, /* int32 [local experts] routes per expert */
   GLMRT_B200_DEBUG_GATE_CODES = 10,   /* [local experts * I, H/2] */

@@ -625,6 +625,48 @@ def test_few_writes_either_route_buffer_alone(mods, engine):
     layer.close()
 
 
+def test_few_expired_wait_is_reported_once_and_healed(mods):
+    """What a barrier that ran out leaves (the word set, the count short) outlives the calls after it: they leave their
+    outputs alone, the check reports it, and then everything is right again.  The state is set from the host."""
+    from glmrt_b200 import native as N
+    import ctypes as C
+    ref = O.make_layer(20, 512, 256, 16)
+    layer = make_layer(mods, ref, 4, "tc-ordered", max_tokens=300)      # (whose large batches repeat bit by bit)
+    stacked = layer.create_stacked()                    # shares the workspace
+    stacked.load_quantized_layer(ref)
+    lane = layer.create_lane(3)                         # has its own
+    x, big = randn(1, 3, 512, dtype=torch.bfloat16), randn(2, 300, 512, dtype=torch.bfloat16)
+    want, idx, w = layer.forward_few(x, want_routes=True)
+    want_routed = layer.forward_few_routed(x, idx, w)
+    want_big = layer.forward(big)
+    b = N.DeviceBuffer()
+    layer.lib.call("glmrt_b200_moe_layer_debug_buffer", layer.handle, C.c_uint32(N.DEBUG["COUNTERS"]), C.byref(b))
+    for short in (1, 7, 147):
+        layer.check()
+        torch.cuda.synchronize()
+        words = np.array([2 ** 32 - short, 1], np.uint32)     # barrier count, expired
+        layer.lib.call("glmrt_copy_h2d", N.DeviceBuffer.of(b.ptr + 32, 8), C.c_void_p(words.ctypes.data), C.c_size_t(8))
+        out = torch.full_like(x, 7.0)
+        for l in (layer, stacked, layer):
+            l.forward_few(x, out=out, residual_bf16=x)
+            l.forward_few_routed(x, idx, w, out=out)
+            assert torch.equal(layer.forward(big), want_big)
+        torch.cuda.synchronize()
+        assert (out == 7).all()
+        assert torch.equal(lane.forward_few(x), want)
+        lane.check()
+        assert layer.stats().device_error == 1
+        with pytest.raises(N.GlmrtError, match="bounded wait"):
+            layer.check()
+        layer.check()
+        assert layer.debug("COUNTERS", np.uint32)[8:10].tolist() == [0, 0]
+        for l in (layer, stacked):
+            assert torch.equal(l.forward_few(x), want) and torch.equal(l.forward_few_routed(x, idx, w), want_routed)
+    layer.check()
+    for l in (lane, stacked, layer):
+        l.close()
+
+
 def test_few_many_experts_and_most_routes(mods):
     """More than 256 experts, 16 slots, every row its own experts: 256 entries at once."""
     h, i, e, top_k = 512, 256, 330, 16
