@@ -85,6 +85,7 @@ struct FewShared {
   uint64_t full[kBufs], empty[kBufs];
   int warp_count[kThreads / 32];
   int entries, distinct, bad;
+  int short_row;                             // a row has fewer finite scores than slots
   uint32_t abort;
 };
 
@@ -414,7 +415,8 @@ __device__ __forceinline__ void store_partial(float* red, const float (&acc)[2][
     }
 }
 
-// Top-k of one row by one warp: the largest keys, the lower id first among equal ones.
+// Top-k of one row by one warp: the largest keys, the lower id first among equal ones.  Slots that no key is left
+// for name expert 0 with weight 0, as in the router (router.cu); such a row may name it more than once.
 template <int kKeys>
 __device__ __forceinline__ void select_row(const FewArgs& a, FewShared& sh, int row, int lane) {
   uint2 v[kKeys];            // key, score
@@ -433,6 +435,10 @@ __device__ __forceinline__ void select_row(const FewArgs& a, FewShared& sh, int 
 #pragma unroll
       for (int i = 0; i < h; ++i) best[i] = max(best[i], best[i + h]);
     const uint32_t top = __reduce_max_sync(0xffffffffu, best[0]);
+    if (top == 0u) {
+      if (lane == 0) sh.short_row = 1;
+      break;
+    }
     uint32_t id = 0xffffffffu, score = 0u;
 #pragma unroll
     for (int i = kKeys - 1; i >= 0; --i)
@@ -477,6 +483,7 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
   __syncthreads();
   // Entries, in the order of the first route that names each: an expert's rows in groups of kCols
   // (identity: all rows are one group and a row's column is its number).
+  const bool search = a.scores == nullptr || sh.short_row != 0;      // else the selection names nobody twice
   uint32_t e = kNoRoute;
   int slot = 0, token = 0;
   bool live = false;
@@ -489,7 +496,7 @@ __device__ void route_and_select(const FewArgs& a, FewShared& sh, uint8_t* scrat
     live = e < static_cast<uint32_t>(a.experts);
     if (!live && e != kNoRoute) sh.bad = 1;
     const uint32_t* row = sh.route_expert + token * a.top_k;
-    for (int s = 0; s < a.top_k && a.scores == nullptr; ++s) {      // (the selection names nobody twice)
+    for (int s = 0; s < a.top_k && search; ++s) {
       if (s == slot || row[s] != e) continue;
       if (s < slot) live = false;                 // the row has named this expert before: its weight went there
       else w += sh.route_w[token * a.top_k + s];
@@ -588,10 +595,11 @@ __device__ void score_experts(const FewArgs& a, FewShared& sh, int warp, int lan
       float s = 0.0f;
 #pragma unroll
       for (int i = 0; i < kLogitShares; ++i) s += sh.logit_part[h][i][t];
-      // a key that orders like score + bias (a NaN last, zero for no expert) and the score
+      // a key that orders like score + bias and the score; zero, as for no expert, where they are not finite: the
+      // router picks none of those (a finite value's key is at least 2^23)
       const float score = sigmoid_f32(s), rank = score + __ldg(a.router_b + e);
       const uint32_t u = __float_as_uint(rank == 0.0f ? 0.0f : rank);
-      a.scores[t * a.experts + e] = make_uint2(rank != rank ? 1u : ((u >> 31) ? ~u : u | 0x80000000u), __float_as_uint(score));
+      a.scores[t * a.experts + e] = make_uint2(!isfinite(rank) ? 0u : ((u >> 31) ? ~u : u | 0x80000000u), __float_as_uint(score));
     }
     __syncthreads();
   }
@@ -610,6 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
   uint8_t* columns = reinterpret_cast<uint8_t*>(red + kBufs * red_floats);
   if (tid == 0) {
     sh.abort = 0u;
+    sh.short_row = 0;
     sh.zero = make_uint4(0u, 0u, 0u, 0u);
     for (int i = 0; i < kBufs; ++i) {
       tc::mbar_init(&sh.full[i], kWarps);

@@ -667,6 +667,63 @@ def test_few_expired_wait_is_reported_once_and_healed(mods):
         l.close()
 
 
+@pytest.mark.parametrize("engine", ["simt", "tc"])
+@pytest.mark.parametrize("experts", [20, 300])
+def test_few_picks_the_experts_that_the_router_picks(mods, engine, experts):
+    """Equal scores go to the lower id; scores or biases that are not finite are never picked, and slots without a
+    candidate name expert 0 with weight 0: the rule of the layer's router, whose routes `forward` returns."""
+    h, top_k = 256, 6
+    ref = O.make_layer(21, h, 256, experts)
+    w0, b0 = torch.from_numpy(ref.router_w).cuda(), torch.from_numpy(ref.bias).cuda()
+    layer, weights = make_layer(mods, ref, top_k, engine), layer_weights(ref)
+    x = randn(1, 16, h, dtype=torch.bfloat16)
+    inf, nan = float("inf"), float("nan")
+
+    def equal_rows(w, b):               # every expert the same score
+        w[:], b[:] = w[0], 0.0
+
+    def pairs(w, b):                    # neighbours share theirs
+        w[1::2], b[1::2] = w[0::2], b[0::2]
+
+    def zero_and_above(w, b):           # sums of score and bias at zero, and one quarter
+        w[:], b[:] = 0.0, -0.5
+        b[experts // 2:] = -0.25
+
+    def infinite(w, b):
+        b[3], b[5], w[7, 2], w[8] = inf, -inf, nan, inf
+        b[experts - 1] = nan
+
+    def three_left(w, b):
+        b[:], b[[2, 9, experts - 2]] = -inf, torch.tensor([0.1, 0.0, 0.2], device="cuda")
+
+    def zero_and_one_left(w, b):
+        b[:], b[[0, 11]] = nan, torch.tensor([0.1, 0.2], device="cuda")
+
+    def none_left(w, b):
+        b[:] = inf
+
+    for change in (equal_rows, pairs, zero_and_above, infinite, three_left, zero_and_one_left, none_left):
+        w, b = w0.clone(), b0.clone()
+        change(w, b)
+        layer.set_router(w, b)
+        for rows in (1, 2, 16):
+            want_idx, want_w = layer.forward(x[:rows], want_routes=True)[1:]
+            got, idx, rw = check_few(layer, weights, x[:rows])
+            assert torch.equal(idx, want_idx), (change.__name__, rows)
+            # weights: float32 logits of h terms in another order, their exponential, and their share of the sum
+            assert float((rw - want_w).abs().max()) <= 2.5 * 2 ** -14, (change.__name__, rows)
+            assert torch.equal(layer.forward_few_routed(x[:rows], idx, rw), got), (change.__name__, rows)
+    layer.set_router(w0, b0)
+    bad = x.clone()
+    bad[2, 5], bad[4, 7] = nan, -inf
+    got, idx, rw = layer.forward_few(bad, want_routes=True)
+    want, want_idx, want_w = layer.forward_few(x, want_routes=True)
+    assert (idx[2] == 0).all() and (rw[2] == 0).all() and got[2].isnan().all() and not got[4].isfinite().any()
+    keep = [r for r in range(16) if r not in (2, 4)]
+    assert torch.equal(got[keep], want[keep]) and torch.equal(idx[keep], want_idx[keep]) and torch.equal(rw[keep], want_w[keep])
+    layer.close()
+
+
 def test_few_many_experts_and_most_routes(mods):
     """More than 256 experts, 16 slots, every row its own experts: 256 entries at once."""
     h, i, e, top_k = 512, 256, 330, 16
