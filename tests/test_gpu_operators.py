@@ -608,8 +608,8 @@ def test_few_writes_either_route_buffer_alone(mods, engine):
     """Through C: indices, weights, both or neither may be asked for."""
     import ctypes as C
     from glmrt_b200 import native as N
-    layer = make_layer(mods, O.make_layer(19, 256, 256, 12), 3, engine)
-    x = randn(1, 5, 256, dtype=torch.bfloat16)
+    layer = make_layer(mods, O.make_layer(19, 512, 256, 12), 3, engine)
+    x = randn(1, 5, 512, dtype=torch.bfloat16)
     want, want_idx, want_w = layer.forward_few(x, want_routes=True)
     buf, null = lambda t: N.DeviceBuffer.of(t.data_ptr(), t.nbytes), N.DeviceBuffer.null()
     for has_idx, has_w in ((True, True), (True, False), (False, True), (False, False)):
@@ -618,6 +618,7 @@ def test_few_writes_either_route_buffer_alone(mods, engine):
         a = N.FewArgs(buf(x), null, null, buf(out), buf(idx) if has_idx else null, buf(w) if has_w else null, 5)
         assert layer.lib.call_status("glmrt_b200_moe_layer_forward_few_async", layer.handle, C.byref(a), None) == 0
         layer.check()
+        assert engine == "simt" or layer.stats().launches_last_forward == 1, "not the one-kernel form"
         assert torch.equal(out, want), (has_idx, has_w)
         assert torch.equal(idx[:5], want_idx) if has_idx else (idx[:5] == 77).all()
         assert torch.equal(w[:5], want_w) if has_w else (w[:5] == 77).all()
@@ -672,7 +673,7 @@ def test_few_expired_wait_is_reported_once_and_healed(mods):
 def test_few_picks_the_experts_that_the_router_picks(mods, engine, experts):
     """Equal scores go to the lower id; scores or biases that are not finite are never picked, and slots without a
     candidate name expert 0 with weight 0: the rule of the layer's router, whose routes `forward` returns."""
-    h, top_k = 256, 6
+    h, top_k = 512, 6
     ref = O.make_layer(21, h, 256, experts)
     w0, b0 = torch.from_numpy(ref.router_w).cuda(), torch.from_numpy(ref.bias).cuda()
     layer, weights = make_layer(mods, ref, top_k, engine), layer_weights(ref)
@@ -709,6 +710,7 @@ def test_few_picks_the_experts_that_the_router_picks(mods, engine, experts):
         for rows in (1, 2, 16):
             want_idx, want_w = layer.forward(x[:rows], want_routes=True)[1:]
             got, idx, rw = check_few(layer, weights, x[:rows])
+            assert engine == "simt" or layer.stats().launches_last_forward == 1, "not the one-kernel form"
             assert torch.equal(idx, want_idx), (change.__name__, rows)
             # weights: float32 logits of h terms in another order, their exponential, and their share of the sum
             assert float((rw - want_w).abs().max()) <= 2.5 * 2 ** -14, (change.__name__, rows)
