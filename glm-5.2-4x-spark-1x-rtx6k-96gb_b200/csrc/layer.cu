@@ -20,6 +20,7 @@
 // handles that share a workspace must be used on one stream, in order.
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <new>
 #include <vector>
@@ -800,9 +801,18 @@ glmrt_status_t few_args(Layer* l, const glmrt_device_buffer_t& hidden, size_t ro
   return GLMRT_STATUS_OK;
 }
 
-glmrt_status_t few_routes(const glmrt_device_buffer_t& buffer, size_t routes, const char* what) {
+// A buffer of indices or weights.  Routes that the call returns are written while its rows are still read, given ones are
+// read until the output is written: they lie apart from `others` (buffers of `bytes` bytes, or null).
+glmrt_status_t few_routes(const glmrt_device_buffer_t& buffer, size_t routes, const char* what,
+                          std::initializer_list<const void*> others, size_t bytes) {
   GLMRT_RETURN_IF_ERROR(check_buf(buffer, routes * 4, what));
-  if (reinterpret_cast<uintptr_t>(buffer.ptr) % 4 != 0) return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string(what) + ": misaligned buffer");
+  const uintptr_t r = reinterpret_cast<uintptr_t>(buffer.ptr);
+  if (r % 4 != 0) return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string(what) + ": misaligned buffer");
+  for (const void* p : others) {
+    const uintptr_t o = reinterpret_cast<uintptr_t>(p);
+    if (p != nullptr && r < o + bytes && o < r + routes * 4)
+      return fail(GLMRT_STATUS_INVALID_ARGUMENT, std::string(what) + ": overlaps another buffer of the call");
+  }
   return GLMRT_STATUS_OK;
 }
 
@@ -820,9 +830,14 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_async(void* layer, co
   const auto& [hidden_bf16, residual_bf16, shared_delta_bf16, output_bf16, topk_indices, topk_weights, rows] = *args;
   FewArgs a{};
   GLMRT_RETURN_IF_ERROR(few_args(l, hidden_bf16, rows, residual_bf16, shared_delta_bf16, output_bf16, &a));
-  const size_t routes = rows * l->cfg.top_k;
-  if (topk_indices.ptr != nullptr) GLMRT_RETURN_IF_ERROR(few_routes(topk_indices, routes, "forward_few topk_indices"));
-  if (topk_weights.ptr != nullptr) GLMRT_RETURN_IF_ERROR(few_routes(topk_weights, routes, "forward_few topk_weights"));
+  const size_t routes = rows * l->cfg.top_k, bytes = rows * static_cast<size_t>(l->cfg.hidden_dim) * 2;
+  const auto apart = {static_cast<const void*>(a.hidden_rows), static_cast<const void*>(a.residual), static_cast<const void*>(a.shared),
+                      static_cast<const void*>(a.out)};
+  if (topk_indices.ptr != nullptr) GLMRT_RETURN_IF_ERROR(few_routes(topk_indices, routes, "forward_few topk_indices", apart, bytes));
+  if (topk_weights.ptr != nullptr) {
+    GLMRT_RETURN_IF_ERROR(few_routes(topk_weights, routes, "forward_few topk_weights", apart, bytes));
+    GLMRT_RETURN_IF_ERROR(few_routes(topk_weights, routes, "forward_few topk_weights", {topk_indices.ptr}, routes * 4));
+  }
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   const uint64_t before = launches_total();
   if (few_fused(l, a)) {
@@ -854,8 +869,9 @@ extern "C" glmrt_status_t glmrt_b200_moe_layer_forward_few_routed_async(void* la
   FewArgs a{};
   GLMRT_RETURN_IF_ERROR(few_args(l, hidden_bf16, rows, residual_bf16, shared_delta_bf16, output_bf16, &a));
   const size_t routes = rows * l->cfg.top_k;
-  GLMRT_RETURN_IF_ERROR(few_routes(topk_indices, routes, "forward_few_routed topk_indices"));
-  GLMRT_RETURN_IF_ERROR(few_routes(topk_weights, routes, "forward_few_routed topk_weights"));
+  const size_t bytes = rows * static_cast<size_t>(l->cfg.hidden_dim) * 2;
+  GLMRT_RETURN_IF_ERROR(few_routes(topk_indices, routes, "forward_few_routed topk_indices", {a.out}, bytes));
+  GLMRT_RETURN_IF_ERROR(few_routes(topk_weights, routes, "forward_few_routed topk_weights", {a.out}, bytes));
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   const uint64_t before = launches_total();
   a.topk_idx = static_cast<uint32_t*>(topk_indices.ptr);

@@ -556,7 +556,8 @@ glmrt_status_t glmrt_b200_moe_layer_forward_residual_async(
  * router, expert FFN with the NVFP4 weights and unquantised activations (W4A16: the arithmetic of the
  * reference's decode kernels, native/cuda/kernels/b12x_direct.cu:171-201,989-1541), weighted combine;
  * output = bf16(residual + shared_delta + routed), rounded once (nearest even).  residual, shared_delta,
- * topk_indices and topk_weights may be null; output may be residual or shared_delta, and no other input.
+ * topk_indices and topk_weights may each be null and lie apart from every other buffer; output may be residual or
+ * shared_delta, and no other input.
  * Needs ep_world == 1.  Results differ from glmrt_b200_moe_layer_forward_async, which quantises the
  * activations.  A row's result does not depend on the other rows of the call, and two calls give the same bits. */
 #define GLMRT_B200_FEW_MAX_ROWS 16

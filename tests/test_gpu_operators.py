@@ -726,6 +726,33 @@ def test_few_picks_the_experts_that_the_router_picks(mods, engine, experts):
     layer.close()
 
 
+def test_few_refuses_route_buffers_over_others(mods):
+    """Through C: returned routes over the rows, the residual, the output or each other; an output over given routes."""
+    import ctypes as C
+    from glmrt_b200 import native as N
+    layer = make_layer(mods, O.make_layer(22, 512, 256, 12), 3)
+    x, res, sh = (randn(s, 4, 512, dtype=torch.bfloat16) for s in (1, 2, 3))
+    out, idx, w = torch.empty_like(x), torch.zeros(4, 3, dtype=torch.int32, device="cuda"), torch.ones(4, 3, device="cuda")
+    buf = lambda t, off=0: N.DeviceBuffer.of(t.data_ptr() + off, t.nbytes - off)
+
+    def status(name, **kw):
+        b = {**dict(hidden=buf(x), residual=buf(res), shared=buf(sh), out=buf(out), idx=buf(idx), w=buf(w)), **kw}
+        return layer.lib.call_status(f"glmrt_b200_moe_layer_{name}_async", layer.handle, C.byref(N.FewArgs(*b.values(), 4)), None)
+
+    assert status("forward_few") == 0 and status("forward_few_routed") == 0
+    for t in (x, res, sh, out):
+        for name in ("idx", "w"):
+            for off in (0, 512, t.nbytes - 48):
+                assert status("forward_few", **{name: buf(t, off)}) == 1 and "overlaps" in layer.lib.last_error(), (name, off)
+    assert status("forward_few", w=buf(idx)) == 1 and "overlaps" in layer.lib.last_error()
+    for name in ("idx", "w"):
+        assert status("forward_few_routed", **{name: buf(out, 1024)}) == 1 and "overlaps" in layer.lib.last_error()
+    both = torch.zeros(2, 4, 3, dtype=torch.int32, device="cuda")           # side by side is apart
+    assert status("forward_few", idx=buf(both[0]), w=buf(both[1])) == 0
+    layer.check()
+    layer.close()
+
+
 def test_few_many_experts_and_most_routes(mods):
     """More than 256 experts, 16 slots, every row its own experts: 256 entries at once."""
     h, i, e, top_k = 512, 256, 330, 16
