@@ -69,9 +69,11 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
   if (ok != 0u) (void)mbar_try_wait(bar, parity);
   return ok != 0u;
 }
-// The same for waits on the critical path of every block of a product: every lane polls, and the clock is read
-// only once 256 polls have failed (reading it costs a good part of a microsecond).
-__device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
+// For waits on the critical path of every block of a product: every lane polls, and the clock is read only once 256
+// polls have failed (reading it costs a good part of a microsecond).  The answer is the lane's own: when a wait runs out,
+// lanes may come back apart and some of them with true.  So whoever calls this brings the warp together again
+// (elect.sync, __syncwarp) before anything that whole warps issue, and votes before it leaves its loop.
+__device__ __forceinline__ bool mbar_wait_lane(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
   uint64_t t0 = 0;
   for (uint32_t spin = 1;; ++spin) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -85,6 +87,10 @@ __device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, vo
       }
     }
   }
+}
+// The same with one answer for the whole warp, which leaves it converged.
+__device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait_lane(bar, parity, abort_flag));
 }
 // One leader lane of a converged warp (the form the compiler recognises as warp-uniform issue).
 __device__ __forceinline__ bool elect_one() {
