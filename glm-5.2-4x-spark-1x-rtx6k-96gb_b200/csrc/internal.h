@@ -346,21 +346,6 @@ glmrt_status_t launch_few_simt(const FewArgs& a, cudaStream_t stream);
 glmrt_status_t norm_take_error(uint32_t* out);
 glmrt_status_t fp8_take_error(uint32_t* out);
 #ifdef __CUDACC__
-constexpr int kMaxErrorDevices = 64;
-template <typename Symbol>
-glmrt_status_t error_word_of(const Symbol& symbol, uint32_t** out) {
-  static std::atomic<void*> known[kMaxErrorDevices];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  void* p = dev >= 0 && dev < kMaxErrorDevices ? known[dev].load(std::memory_order_relaxed) : nullptr;
-  if (p == nullptr) {
-    cudaError_t err = cudaGetSymbolAddress(&p, symbol);
-    if (err != cudaSuccess) return fail_cuda(GLMRT_STATUS_INTERNAL_ERROR, "cudaGetSymbolAddress(error word)", err);
-    if (dev >= 0 && dev < kMaxErrorDevices) known[dev].store(p, std::memory_order_relaxed);
-  }
-  *out = static_cast<uint32_t*>(p);
-  return GLMRT_STATUS_OK;
-}
 template <typename Symbol>
 glmrt_status_t take_error_word(Symbol& symbol, uint32_t* out) {
   const uint32_t zero = 0;

@@ -28,6 +28,8 @@ namespace {
 
 constexpr int kMaxWidth = 32768;      // 1024 threads x 32 values
 
+__device__ uint32_t g_norm_error;     // kErrWaitTimeout when a bounded wait ran out (glmrt_b200_operators_check)
+
 struct NormArgs {
   const void *residual, *delta, *norm_w, *post_w, *gate;
   void *residual_out, *normalized;
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(NormArgs a) {
 // copy rate are 61).  Rows whose pieces are 16 bytes, aligned; two pieces a thread; no norm of the branch (its sum
 // would make the chain of a row longer, and only two rows are under way on an SM).
 template <typename W>
-__global__ void __launch_bounds__(512, 2) block_norm_stream_kernel(NormArgs a, int stages, uint32_t row_bytes, uint32_t* error_word) {
+__global__ void __launch_bounds__(512, 2) block_norm_stream_kernel(NormArgs a, int stages, uint32_t row_bytes) {
   using T = uint16_t;
   constexpr int kVec = 8, kNv = 2, kPer = 16 / static_cast<int>(sizeof(W));
   extern __shared__ __align__(128) uint8_t ring[];
@@ -302,11 +304,9 @@ __global__ void __launch_bounds__(512, 2) block_norm_stream_kernel(NormArgs a, i
   }
   if (threadIdx.x == 0 && abort_word != 0u) {
     for (int i = 0; i < 200; ++i) __nanosleep(1000);    // let copies in flight land
-    atomicOr(error_word, static_cast<uint32_t>(kErrWaitTimeout));
+    atomicOr(&g_norm_error, static_cast<uint32_t>(kErrWaitTimeout));
   }
 }
-
-__device__ uint32_t g_norm_error;
 
 template <typename T, typename W, int kVec, int kNv>
 void launch(const NormArgs& a, int threads, cudaStream_t s) {
@@ -321,11 +321,9 @@ template <typename W>
 glmrt_status_t launch_stream(const NormArgs& a, int stages, uint32_t row_bytes, int ctas, cudaStream_t s) {
   static std::atomic<uint64_t> configured{0};
   GLMRT_RETURN_IF_ERROR(ensure_smem_limit(configured, block_norm_stream_kernel<W>, kStreamRing, "cudaFuncSetAttribute(block_norm_stream_kernel)"));
-  uint32_t* error_word = nullptr;
-  GLMRT_RETURN_IF_ERROR(error_word_of(g_norm_error, &error_word));
   const int pieces = a.width / 8;
   launch_pdl(block_norm_stream_kernel<W>, dim3(static_cast<unsigned>(ctas)), dim3(static_cast<unsigned>(((pieces + 1) / 2 + 31) / 32 * 32)),
-             static_cast<size_t>(stages) * row_bytes * (a.delta != nullptr ? 2 : 1), s, a, stages, row_bytes, error_word);
+             static_cast<size_t>(stages) * row_bytes * (a.delta != nullptr ? 2 : 1), s, a, stages, row_bytes);
   return GLMRT_STATUS_OK;
 }
 
