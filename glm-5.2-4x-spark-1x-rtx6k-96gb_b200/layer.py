@@ -189,20 +189,25 @@ class MoeLayer:
     def forward_few_routed(self, hidden_bf16: torch.Tensor, idx: torch.Tensor, w: torch.Tensor,
                            out: torch.Tensor | None = None, residual_bf16: torch.Tensor | None = None,
                            shared_delta_bf16: torch.Tensor | None = None) -> torch.Tensor:
-        """``forward_few`` with the routes given; index -1 is no route."""
-        assert idx.shape == (hidden_bf16.shape[0], self.top_k) and w.shape == idx.shape
-        assert idx.device == self.device and w.device == self.device
+        """``forward_few`` with the routes given: whole numbers ``[rows, top_k]``, index -1 is no route."""
+        if idx.shape != (hidden_bf16.shape[0], self.top_k) or w.shape != idx.shape:
+            raise ValueError(f"forward_few_routed: idx and w must be [rows, {self.top_k}]")
+        if idx.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
+            raise ValueError("forward_few_routed: idx must be whole numbers")
+        if idx.device != self.device or w.device != self.device:
+            raise ValueError("forward_few_routed: idx and w must be on the layer's device")
         return self._few("glmrt_b200_moe_layer_forward_few_routed_async", hidden_bf16, out, residual_bf16, shared_delta_bf16,
                          idx.to(torch.int32).contiguous(), w.to(torch.float32).contiguous())
 
     def _few(self, symbol, hidden, out, residual, shared, idx, w) -> torch.Tensor:
-        assert hidden.dim() == 2 and hidden.shape[1] == self.hidden
+        if hidden.dim() != 2 or hidden.shape[1] != self.hidden:
+            raise ValueError(f"forward_few: hidden must be [rows, {self.hidden}]")
         if out is None:
             out = torch.empty_like(hidden)
         shape, index = hidden.shape, self.device.index
         for t in (hidden, out, residual, shared):
-            if t is not None:
-                assert t.shape == shape and t.dtype is torch.bfloat16 and t.get_device() == index and t.is_contiguous()
+            if t is not None and (t.shape != shape or t.dtype is not torch.bfloat16 or t.get_device() != index or not t.is_contiguous()):
+                raise ValueError("forward_few: rows must be contiguous bfloat16 tensors of hidden's shape on the layer's device")
         b = launch.buffer
         launch.call(self.lib, symbol, self._FEW_ARGS.pack(*b(hidden), *b(residual), *b(shared), *b(out), *b(idx), *b(w), shape[0]),
                     index, self.handle)

@@ -210,3 +210,31 @@ def test_quantize_weight_against_the_definition(pkg):
             back = codes[128 * i:128 * i + 128, 128 * j:128 * j + 128].float() * scales[i, j]
             # half a step of E4M3: 2^-4 of the value, or half the smallest step (2^-10) of the scale
             assert ((back - b).abs() <= 2 ** -4 * b.abs() * 1.001 + 2 ** -10 * s).all()
+
+
+def test_few_wrapper_raises_on_rows_and_routes_it_cannot_pass(pkg, monkeypatch):
+    """ValueError, also where asserts are off, before anything reaches the library."""
+    import types
+    from glmrt_b200 import launch
+    from glmrt_b200.layer import MoeLayer
+    layer = object.__new__(MoeLayer)
+    layer.hidden, layer.top_k, layer.lib, layer.handle = 64, 2, None, None
+    layer.device = types.SimpleNamespace(index=-1)              # what get_device says of a host tensor
+    calls = []
+    monkeypatch.setattr(launch, "call", lambda lib, symbol, packed, index, *handle: calls.append(symbol))
+    x = torch.zeros(3, 64, dtype=torch.bfloat16)
+    layer.forward_few(x, out=x, residual_bf16=x, shared_delta_bf16=x)
+    assert len(calls) == 1
+    for bad in (x[0], x[:, :32], x.float(), x.T.contiguous().T, x.view(torch.float16)):
+        with pytest.raises(ValueError, match="forward_few"):
+            layer.forward_few(bad)
+    for bad in (x[:2], x.float(), torch.zeros(3, 128, dtype=torch.bfloat16)[:, :64]):
+        for name in ("out", "residual_bf16", "shared_delta_bf16"):
+            with pytest.raises(ValueError, match="forward_few"):
+                layer.forward_few(x, **{name: bad})
+    idx, w = torch.zeros(3, 2, dtype=torch.int64), torch.ones(3, 2)
+    layer.device = torch.device("cpu")
+    for i, v in ((idx[:2], w), (idx, w[:, :1]), (idx.float(), w), (idx.bool(), w), (idx.to("meta"), w), (idx, w.to("meta"))):
+        with pytest.raises(ValueError, match="forward_few_routed"):
+            layer.forward_few_routed(x, i, v)
+    assert len(calls) == 1
