@@ -196,6 +196,8 @@ class MoeLayer:
             raise ValueError("forward_few_routed: idx must be whole numbers")
         if idx.device != self.device or w.device != self.device:
             raise ValueError("forward_few_routed: idx and w must be on the layer's device")
+        if idx.dtype is torch.int64:      # ids outside 32 bits stay ids outside the layer
+            idx = idx.clamp(-2 ** 31, 2 ** 31 - 1)
         return self._few("glmrt_b200_moe_layer_forward_few_routed_async", hidden_bf16, out, residual_bf16, shared_delta_bf16,
                          idx.to(torch.int32).contiguous(), w.to(torch.float32).contiguous())
 

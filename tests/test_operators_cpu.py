@@ -238,3 +238,13 @@ def test_few_wrapper_raises_on_rows_and_routes_it_cannot_pass(pkg, monkeypatch):
         with pytest.raises(ValueError, match="forward_few_routed"):
             layer.forward_few_routed(x, i, v)
     assert len(calls) == 1
+
+
+def test_few_wrapper_keeps_ids_outside_32_bits_outside(pkg, monkeypatch):
+    from glmrt_b200.layer import MoeLayer
+    layer = object.__new__(MoeLayer)
+    layer.hidden, layer.top_k, layer.device, layer.lib, layer.handle = 64, 4, torch.device("cpu"), None, None
+    seen = []
+    monkeypatch.setattr(MoeLayer, "_few", lambda self, symbol, hidden, out, residual, shared, idx, w: seen.append(idx))
+    layer.forward_few_routed(torch.zeros(1, 64, dtype=torch.bfloat16), torch.tensor([[2 ** 32, -2 ** 32 - 1, -1, 5]]), torch.ones(1, 4))
+    assert seen[0].dtype == torch.int32 and seen[0].tolist() == [[2 ** 31 - 1, -2 ** 31, -1, 5]]
