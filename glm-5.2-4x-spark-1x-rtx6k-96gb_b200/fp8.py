@@ -57,8 +57,8 @@ def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     n, k = weight.shape
     pad = torch.nn.functional.pad(weight.float(), (0, -k % BLOCK, 0, -n % BLOCK))
     b = pad.view(_blocks(n), BLOCK, _blocks(k), BLOCK)
-    amax = b.abs().amax(dim=(1, 3))
-    scales = torch.where(amax > 0, amax / 448.0, torch.ones_like(amax))
+    scales = b.abs().amax(dim=(1, 3)) / 448.0
+    scales = torch.where(scales > 0, scales, torch.ones_like(scales))       # of zeros, or so small that the quotient is zero
     codes = (b / scales[:, None, :, None]).reshape(pad.shape)[:n, :k].clamp(-448, 448).to(E4M3)
     return codes.contiguous(), scales
 

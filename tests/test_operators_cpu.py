@@ -248,3 +248,15 @@ def test_few_wrapper_keeps_ids_outside_32_bits_outside(pkg, monkeypatch):
     monkeypatch.setattr(MoeLayer, "_few", lambda self, symbol, hidden, out, residual, shared, idx, w: seen.append(idx))
     layer.forward_few_routed(torch.zeros(1, 64, dtype=torch.bfloat16), torch.tensor([[2 ** 32, -2 ** 32 - 1, -1, 5]]), torch.ones(1, 4))
     assert seen[0].dtype == torch.int32 and seen[0].tolist() == [[2 ** 31 - 1, -2 ** 31, -1, 5]]
+
+
+def test_quantize_weight_of_blocks_below_the_smallest_scale(pkg):
+    """Largest magnitudes whose 448th part rounds to zero in float32: zeros stay zeros and nothing is NaN."""
+    from glmrt_b200 import fp8
+    w = torch.zeros(130, 256)
+    w[0, 0], w[1, 1], w[129, 3], w[0, 200] = 1e-44, -3e-43, 2e-40, 1.0
+    codes, scales = fp8.quantize_weight(w)
+    assert codes.float().isfinite().all() and (scales > 0).all()
+    back = codes.float() * scales.repeat_interleave(128, 0)[:130].repeat_interleave(128, 1)
+    # E4M3's half step, and float32's smallest value: half of it per code of a scale that is itself subnormal
+    assert ((back - w).abs().double() <= 2 ** -4 * w.abs().double() + 448 * 2.0 ** -150).all()
