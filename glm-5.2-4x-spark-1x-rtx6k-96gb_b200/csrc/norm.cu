@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(NormArgs a) {
   __shared__ float scratch[32];
   pdl_launch_dependents();
   pdl_wait();
-  const int row_i = blockIdx.x * blockDim.y + threadIdx.y;
-  if (row_i >= a.rows) return;        // blockDim.y > 1 only with one warp per row: whole warps leave
+  const uint32_t row_i = blockIdx.x * blockDim.y + threadIdx.y;
+  if (row_i >= static_cast<uint32_t>(a.rows)) return;        // blockDim.y > 1 only with one warp per row: whole warps leave
   const size_t row = static_cast<size_t>(row_i);
   const T* res = static_cast<const T*>(a.residual) + row * a.residual_stride;
   const float inv_width = 1.0f / static_cast<float>(a.width);
@@ -310,9 +310,9 @@ __global__ void __launch_bounds__(512, 2) block_norm_stream_kernel(NormArgs a, i
 
 template <typename T, typename W, int kVec, int kNv>
 void launch(const NormArgs& a, int threads, cudaStream_t s) {
-  const int ty = threads == 32 ? 8 : 1;
-  launch_pdl(block_norm_kernel<T, W, kVec, kNv>, dim3(static_cast<unsigned>((a.rows + ty - 1) / ty)),
-             dim3(static_cast<unsigned>(threads), static_cast<unsigned>(ty)), 0, s, a);
+  const unsigned ty = threads == 32 ? 8 : 1;
+  launch_pdl(block_norm_kernel<T, W, kVec, kNv>, dim3((static_cast<unsigned>(a.rows) + ty - 1) / ty),     // rows < 2^31
+             dim3(static_cast<unsigned>(threads), ty), 0, s, a);
 }
 
 constexpr int kStreamRing = 104 * 1024;       // a CTA's rows in shared memory, two CTAs on an SM

@@ -116,6 +116,20 @@ def test_block_norm_beyond_32_bit_offsets(mods):
         assert all(torch.equal(g[at:at + n], v[:n]) for g, v in zip(got, want)), at
 
 
+def test_block_norm_of_the_most_rows(mods):
+    """2^31 - 1 rows of one value: the last ones too."""
+    rows, few = 2 ** 31 - 1, 2 ** 20
+    x = randn(1, few, 1, dtype=torch.bfloat16)
+    nw = torch.full((1,), 1.5, device="cuda")
+    want = mods["block_norm"].block_norm(x, norm_weight=nw, eps=0.5)[1]
+    y = x.double() * torch.rsqrt(x.double() ** 2 + 0.5) * 1.5
+    within(want, y, (half(torch.bfloat16) + 2 ** -18) * y.abs() + 1e-38)
+    got = mods["block_norm"].block_norm(x.repeat(2048, 1)[:rows], norm_weight=nw, eps=0.5)[1]
+    for at in range(0, rows, 64 * few):
+        part = got[at:at + 64 * few]
+        assert torch.equal(part, want.repeat(64, 1)[:len(part)]), at
+
+
 def test_block_norm_strides_and_alignment(mods):
     """Padded rows, rows that start off a 16-byte boundary, an expanded gate."""
     rows, width = 9, 520
