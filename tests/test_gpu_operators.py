@@ -926,6 +926,58 @@ assert all(torch.equal(a, b) for a, b in zip(got, run()))
     subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
 
 
+def test_first_few_row_calls_of_a_process_may_be_captured(pkg):
+    """The few-row layer's first calls, routes chosen and routes given, inside a capture (the layer is made before)."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from __graft_entry__ import load_package
+load_package()
+from glmrt_b200.layer import MoeLayer
+layer = MoeLayer(512, 256, 16, 4, max_tokens=16)
+layer.set_router(torch.linspace(-1, 1, 16 * 512, device="cuda").sin().view(16, 512), torch.zeros(16, device="cuda"))
+layer.fill_synthetic(3)
+x = {m: torch.linspace(-2, 2, m * 512, device="cuda").cos().view(m, 512).bfloat16() for m in (1, 5, 16)}
+idx = {m: torch.arange(4 * m, device="cuda", dtype=torch.int32).view(m, 4) % 16 for m in x}
+w = {m: torch.full((m, 4), 0.5, device="cuda") for m in x}
+def run():
+    return [t for m in x for t in (*layer.forward_few(x[m], want_routes=True), layer.forward_few_routed(x[m], idx[m], w[m], residual_bf16=x[m]))]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = run()
+for _ in range(2):
+    for t in got:
+        t.zero_()
+    g.replay()
+    layer.check()
+    assert layer.stats().launches_last_forward == 1
+    assert all(torch.equal(a, b) for a, b in zip(got, run())) and any(t.any() for t in got)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
+
+
+def test_few_rows_of_the_full_size_layer_do_not_depend_on_their_batch(mods):
+    """The model's own shape: outputs, indices and weights bit by bit, alone and among others, routes chosen and given."""
+    h, e = 6144, 256
+    layer = mods["layer"].MoeLayer(h, 2048, e, 8, max_tokens=16)
+    layer.set_router(randn(1, e, h, std=0.02), randn(2, e, std=0.01))
+    layer.fill_synthetic(23)
+    x, res = randn(3, 16, h, dtype=torch.bfloat16), randn(4, 16, h, dtype=torch.bfloat16)
+    want = layer.forward_few(x, residual_bf16=res, want_routes=True)
+    layer.check()
+    for at, rows in ((0, 1), (2, 1), (15, 1), (3, 2), (5, 3), (9, 7), (0, 16)):
+        part = slice(at, at + rows)
+        got = layer.forward_few(x[part], residual_bf16=res[part], want_routes=True)
+        assert all(torch.equal(g, v[part]) for g, v in zip(got, want)), (at, rows)
+        assert torch.equal(layer.forward_few_routed(x[part], want[1][part], want[2][part], residual_bf16=res[part]), want[0][part]), (at, rows)
+    layer.check()
+    layer.close()
+
+
 # ---- all of them together ------------------------------------------------------------------------
 @pytest.mark.parametrize("rows", [1, 5, 16, 17, 200])
 def test_sparse_block_runs_the_operators_together(mods, rows):
