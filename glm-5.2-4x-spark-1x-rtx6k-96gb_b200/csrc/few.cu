@@ -435,16 +435,12 @@ __device__ __forceinline__ void select_row(const FewArgs& a, FewShared& sh, int 
 #pragma unroll
       for (int i = 0; i < h; ++i) best[i] = max(best[i], best[i + h]);
     const uint32_t top = __reduce_max_sync(0xffffffffu, best[0]);
-    if (top == 0u) {
-      if (lane == 0) sh.short_row = 1;
-      break;
-    }
     uint32_t id = 0xffffffffu, score = 0u;
 #pragma unroll
     for (int i = kKeys - 1; i >= 0; --i)
       if (v[i].x == top) { id = lane + 32 * i; score = v[i].y; }
-    const uint32_t first = __reduce_min_sync(0xffffffffu, id);
-    const float chosen = __uint_as_float(__shfl_sync(0xffffffffu, score, first & 31));
+    const uint32_t first = top != 0u ? __reduce_min_sync(0xffffffffu, id) : kNoRoute;
+    const float chosen = top != 0u ? __uint_as_float(__shfl_sync(0xffffffffu, score, first & 31)) : 0.0f;
 #pragma unroll
     for (int i = 0; i < kKeys; ++i)
       if (lane + 32 * i == static_cast<int>(first)) v[i].x = 0u;
@@ -453,7 +449,9 @@ __device__ __forceinline__ void select_row(const FewArgs& a, FewShared& sh, int 
   }
   if (lane < a.top_k) {
     const int r = row * a.top_k + lane;
-    sh.route_expert[r] = mine;
+    const bool none = mine == kNoRoute;
+    if (none) sh.short_row = 1;
+    sh.route_expert[r] = none ? 0u : mine;
     sh.route_w[r] = my_score * (a.scaling / fmaxf(sum, 1e-12f));
   }
 }
@@ -628,11 +626,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
   if (tid < kFewMaxRows) sh.x_amax[tid] = 0u;
   __syncthreads();
 
-  uint32_t* sync = a.counters + kCntFewBarrier;
-  uint32_t expired = 0u, bit = tid == 0 ? grid_bit(sync, expired) : 0u;
+  uint32_t expired = 0u, bit = tid == 0 ? grid_bit(a.sync, expired) : 0u;
   if (a.scores != nullptr) {
     score_experts(a, sh, warp, lane);
-    grid_arrive(sync);
+    grid_arrive(a.sync);
   }
   if (expired != 0u) sh.abort = 1u;
   // the rows' largest magnitudes, 256 values a warp
@@ -652,8 +649,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
   if (tid < a.rows) f16_factor(sh.x_amax[tid], &sh.x_inv[tid]);
   if (identity && warp < kWarps) load_hidden_columns(a, sh, columns, 0, cols, true);    // needs no routes
   if (a.scores != nullptr) {
-    if (!grid_wait(sync, bit, &sh.abort)) {
-      if (tid == 0) atomicOr(a.counters + kCntFewExpired, static_cast<uint32_t>(kErrWaitTimeout));
+    if (!grid_wait(a.sync, bit, &sh.abort)) {
+      if (tid == 0) atomicOr(a.sync + 1, static_cast<uint32_t>(kErrWaitTimeout));
       return;
     }
   }
@@ -693,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
     int n = 0;                     // items so far: buffer n % kBufs, its round n / kBufs
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
-      if (pass == 1) grid_barrier(sync, bit, &sh.abort);
+      if (pass == 1) grid_barrier(a.sync, bit, &sh.abort);
       const Share s = pass == 0 ? s1 : s2;
       const FewPass p = a.pass[pass];
       const int kwi = warp & (p.kw - 1);
@@ -787,11 +784,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_layer_kernel(FewArgs a) {
         if (lane == 0) tc::mbar_arrive(&sh.empty[mine]);
       }
       base += items;
-      if (pass == 0) grid_barrier(sync, bit, &sh.abort);
+      if (pass == 0) grid_barrier(a.sync, bit, &sh.abort);
     }
   }
-  if (!grid_barrier(sync, bit, &sh.abort)) {
-    if (tid == 0) atomicOr(a.counters + kCntFewExpired, static_cast<uint32_t>(kErrWaitTimeout));
+  if (!grid_barrier(a.sync, bit, &sh.abort)) {
+    if (tid == 0) atomicOr(a.sync + 1, static_cast<uint32_t>(kErrWaitTimeout));
     return;
   }
 

@@ -333,6 +333,7 @@ struct FewArgs {
   uint32_t* out_idx;                                        // where the routes are written, or nullptr
   float* out_w;
   float* route_out;                                         // [rows * top_k, hidden] float32 result rows
+  uint32_t* sync;                                           // counters + kCntFewBarrier
   uint32_t* counters;
 };
 FewPass few_pass(int k, int groups);

@@ -796,6 +796,7 @@ glmrt_status_t few_args(Layer* l, const glmrt_device_buffer_t& hidden, size_t ro
   a.route_out = l->few_out;
   a.pass[0] = few_pass(a.hidden, a.inter / 16);
   a.pass[1] = few_pass(a.inter, a.hidden / 32);
+  a.sync = l->counters + kCntFewBarrier;
   a.counters = l->counters;
   *out = a;
   return GLMRT_STATUS_OK;
