@@ -36,10 +36,6 @@ __device__ __forceinline__ float fp8_input(float v) { return v; }
 __device__ __forceinline__ void fp8_store(uint16_t* p, float v) { *p = f32_to_bf16_rne(v); }
 __device__ __forceinline__ void fp8_store(float* p, float v) { *p = v; }
 
-__device__ __forceinline__ float e4m3_to_f32_nan(uint8_t b) {
-  return (b & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : e4m3_to_f32(b);
-}
-
 // Scale of a block whose largest magnitude has the bits `amax`: the smallest power of two with
 // amax / scale <= 448 = 1.75 * 2^8, so one exponent comparison decides it.  Blocks below 2^-100 are
 // scaled as if they reached it (their codes are then zero or tiny); a block with an infinity or a NaN gets

@@ -286,11 +286,11 @@ struct TensorMaps {
   CUtensorMap act1, act2;       // activation codes (box rows = chunk_tokens)
   CUtensorMap act1_sf, gate_sf, up_sf, act2_sf, down_sf;   // tiled scales seen as rows of 128 bytes, 2 KB boxes (CTA-pair kernels)
 };
-// Encodes a 2D uint8 tensor map [rows, row_bytes] with a {128 B, box_rows} box and 128-byte swizzle.
-// Bytes in rows of row_bytes (a multiple of 16), read in boxes of box_rows x 128 bytes with the 128-byte
-// swizzle; what lies past the rows' and the tensor's end reads as zero.
+// Encodes a 2D uint8 tensor map [rows, row_bytes] (row_bytes a multiple of 16) with a {128 B, box_rows} box and
+// 128-byte swizzle; what lies past the rows' and the tensor's end reads as zero.
 glmrt_status_t make_bytes_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes,
                                      uint32_t box_rows);
+// The same for codes in whole 128-byte pieces (row_bytes a multiple of 128).
 glmrt_status_t make_codes_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes,
                                      uint32_t box_rows);
 // Encodes a byte range as [bytes / 128, 128] with a {128 B, 16 rows} box and no swizzle: one box = 2 KB of scale tiles.
