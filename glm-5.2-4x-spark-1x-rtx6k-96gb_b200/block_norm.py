@@ -43,8 +43,8 @@ def block_norm(residual: torch.Tensor, delta: torch.Tensor | None = None, *, nor
     """``(residual + scale * branch, its RMSNorm)``; rows bf16 or float32, weights bf16 or float32.
 
     ``gate``: [rows, 1], [1, width] or [rows, width] of the rows' type.  ``residual_out`` and
-    ``normalized`` may be given, also in the place of ``residual`` or ``delta``.  Without ``delta``
-    the residual comes back as it is.
+    ``normalized`` may be given, also in the place of ``residual`` or ``delta``; rows of an output may not
+    interleave with those of another tensor of the call.  Without ``delta`` the residual comes back as it is.
     """
     dtype = residual.dtype
     code = _DTYPES.get(dtype)

@@ -5,8 +5,8 @@
 //   act[r]  = weight[r] * silu(gate x) * (up x)          r = (token, slot), float32
 //   out[t]  = residual[t] + (shared[t] + sum over slots down act[t, slot])
 //
-// with W = E2M1 code * E4M3 block scale * scale_2.  Nothing is rounded between the bf16 rows and the
-// bf16 result except where a comment says so.
+// with W = E2M1 code * E4M3 block scale * scale_2.  Between the bf16 rows and the bf16 result only the SwiGLU rows are
+// rounded to fewer bits than float32, and rows of very wide range (both below); the verification form rounds neither.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -34,9 +34,9 @@ __device__ __forceinline__ float warp_sum(float v) {
 //   combine    residual + (shared + sum over the slots, in slot order)
 //
 // What bounds it is the experts' weights (9/16 byte each, read once); everything else is arranged so
-// that they never stop arriving.  Measured at 6144 / 2048, 256 experts, top-8, back to back: 1 row 50 us (170 MB; 9 us
-// until the routes are known, 20 us gate / up, 2 us barrier, 11 us down, 5 us barrier and combine), 4 rows 134, 8 rows
-// 250, 16 rows 425 to 455 us (2.2 GB: 4.8 to 5.1 TB/s, by then bound by issue slots, 295 instructions a slot).  Each lane copies its own pieces of the weights into shared memory
+// that they never stop arriving.  Measured at 6144 / 2048, 256 experts, top-8, back to back: 1 row 48 us (170 MB; 9 us
+// until the routes are known, 19 us gate / up, 2 us barrier, 11 us down, 5 us barrier and combine), 4 rows 130, 8 rows
+// 235 to 250, 16 rows 429 to 459 us (2.2 GB: 4.7 to 5.1 TB/s, by then bound by issue slots, 295 instructions a slot).  Each lane copies its own pieces of the weights into shared memory
 // (cp.async), kRing - 1 slots ahead, and only itself reads them back, so the stream needs no barrier
 // between warps; it runs on from the gate / up rows into the down rows while the CTA waits at the
 // barrier between them.
@@ -53,8 +53,9 @@ __device__ __forceinline__ float warp_sum(float v) {
 // with them, 10.5 without; the conversions take 12 on another pipe).
 //
 // The rows as fp16: times a power of two per token that brings the largest magnitude to 2^14, which is
-// exact for everything within 2^28 of it and off by 2^-39 of it below.  The SwiGLU rows likewise, rounded
-// from float32 to fp16's 11 bits (2^-12 of a value: a sixteenth of the bf16 result's rounding).
+// exact for everything within 2^28 of it and off by at most 2^-39 of it below.  The SwiGLU rows likewise, rounded from
+// float32 to fp16's 11 bits, because the products take both operands in fp16: off by at most 2^-11 of a value (an eighth
+// of the bf16 result's rounding), or 2^-39 of the largest of its share for values more than 2^28 below that.
 // ------------------------------------------------------------------------------------------------
 constexpr int kWarps = 16;                   // that multiply
 constexpr int kSumWarps = 4;                 // that add the warps' partial sums up and finish the rows

@@ -20,8 +20,8 @@ constexpr int kBlock = kFp8Block;
 
 // Eight lanes per (row, 128-column block), sixteen values a lane (two 16-byte loads of bf16 in flight, one 16-byte store
 // of codes); a CTA takes eight rows of four neighbouring blocks, so that the scales leave as whole sectors.  Bound by
-// memory (bf16: 3 bytes a value): 8192 x 6144 25 us = 6.0 TB/s, 8192 x 2048 9.8 us (with eight values a lane, and blocks of
-// one row next to each other in a CTA, 33 and 12.9 us).  kVec: the rows' pieces of eight values are 16-byte aligned.
+// memory (3 bytes a bf16 value, 5 a float32 one): 8192 x 6144 bf16 25 us = 6.0 TB/s, float32 38 us = 6.6 TB/s (bf16 with eight
+// values a lane, and blocks of one row next to each other in a CTA, 33 us).  kVec: the rows' pieces of eight values are 16-byte aligned.
 constexpr int kQuantBlocks = 4, kQuantRows = 256 / 8 / kQuantBlocks;       // of a CTA
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(256) fp8_quantize_rows_kernel(const T* __restrict__ in, size_t stride, uint8_t* __restrict__ codes,

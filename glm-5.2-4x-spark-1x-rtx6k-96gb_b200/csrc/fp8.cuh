@@ -14,8 +14,9 @@ constexpr int kFp8Block = 128;   // columns per activation scale, rows and colum
 // mode 0: out bf16 [rows, n]; 1: float32; 2: silu(w0 x) * (w1 x) quantised: codes [rows, n], scales
 // out_scales [ceil(n / 128)][out_stride].
 // x_bf16: instead of x and xs, at most kFp8OwnRows rows of bf16 that the product quantises itself.
-// (Measured, n = 4096, k = 6144: 1 row 8.3 against 9.2 us with a quantiser before it, 4 rows 9.9 / 9.6, 16 rows 17 / 9.6;
-// and a launch less on the host.)
+// (Measured from a graph, against a quantiser before the product, 1 to 8 rows: n = 4096, k = 6144 6.8 / 8.2, 7.5 / 8.2,
+// 8.0 / 8.2, 8.4 / 8.3, 8.8 / 8.3, 9.3 / 8.3, 9.8 / 8.3, 10.2 / 8.2 us; n = 6144, k = 2048 5.3 / 6.8, 5.3 / 6.8, 5.8 / 6.8,
+// 6.0 / 6.9, 6.4 / 6.9, 6.6 / 6.9, 7.0 / 7.0, 7.0 / 6.8.  At four rows it loses 2 % there and wins 14 % here.)
 constexpr size_t kFp8OwnRows = 4;
 struct Fp8Gemm {
   const uint8_t* x;

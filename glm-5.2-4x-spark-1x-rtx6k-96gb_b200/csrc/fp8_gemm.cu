@@ -11,9 +11,9 @@
 //       rows, the K blocks of a tile split over a cluster of up to eight CTAs, whose sums meet in
 //       shared memory.  Bound by the weight bytes, so what counts is that every SM streams.
 //
-// Measured (rows x n x k, in a chain of calls, the quantiser included): 8192 x 4096 x 6144 197 us = 2.09 PFLOP/s,
-// 8192 x 6144 x 2048 111 us; 256 x 4096 x 6144 17.8 us, 16 rows 8.9 us; one row 6.7 us = 3.8 TB/s of weights from launch to
-// launch, 5.6 between the first and the last copy.
+// Measured (rows x n x k, in a chain of calls, the quantiser included): 8192 x 4096 x 6144 201 to 207 us = 2.0 PFLOP/s
+// (float32 out 229), 8192 x 6144 x 2048 112 us; 1000 x 4096 x 6144 29 us, 256 rows 18.7, 64 rows 10.8, 16 rows 8.4; one row 6.8 us
+// = 3.7 TB/s of weights from launch to launch, 5.6 between the first and the last copy.
 //
 // Each in two forms: the plain product, and gate / up with the SwiGLU and the next quantisation in the
 // epilogue (both matrices in one tile, so that a thread meets gate and up of the same feature).
@@ -769,8 +769,8 @@ int active_clusters(int dev, int splits) {
 // costs about 3 us beside its blocks (set-up, first copies, joining), a block 0.42 us and 0.0015 us per column of
 // the sum (measured at 16 to 256 rows and 2048 to 6144 columns of K).  The driver's count is that of one CTA an SM.
 // With rows quantised here a second one beside it helps, since each CTA then has fewer blocks of them (1 row, n x k:
-// 4096 x 6144 4 splits 8.9 us, 6 splits 7.0; 12288 x 4096 1 split 16.9, 2 splits 13.3); otherwise it does not (16 rows,
-// 4096 x 6144: 4 splits 9.4, 6 splits 10.0).
+// 4096 x 6144 4 splits 8.3 us, 6 splits 6.8; 12288 x 4096 1 split 15.9, 2 splits 10.6); otherwise it does not (16 rows,
+// 4096 x 6144: 4 splits 8.4, 6 splits 8.7; 64 rows 10.9 / 11.9).
 template <int kMode, int kN, bool kOwnX>
 int weight_splits(int tiles, int blocks, float* estimate_us) {
   int best = 1, dev = 0;

@@ -15,8 +15,8 @@
 //
 // Bound by memory: each value is read once and written once and does about ten operations.  One row
 // belongs to one group of threads that keeps all of it in registers (at most 32 values a thread)
-// between the loads and the second statistic, so nothing is read twice.  Measured: 1 x 6144 bf16 2.3 us, 1021 x 4100
-// float32 12.4 us = 5.4 TB/s, 8192 x 4096 float32 80 us = 6.7 TB/s, 8192 x 4100 bf16 56 us = 4.8 TB/s.
+// between the loads and the second statistic, so nothing is read twice.  Measured: 1 x 6144 bf16 2.3 to 2.8 us, 1021 x 4100
+// float32 12.5 us = 5.4 TB/s, 8192 x 4096 float32 80 us = 6.7 TB/s, 8192 x 4100 bf16 56 us = 4.8 TB/s.
 #include <algorithm>
 
 #include "common.cuh"

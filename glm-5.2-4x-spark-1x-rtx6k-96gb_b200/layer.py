@@ -176,8 +176,8 @@ class MoeLayer:
     def forward_few(self, hidden_bf16: torch.Tensor, out: torch.Tensor | None = None,
                     residual_bf16: torch.Tensor | None = None, shared_delta_bf16: torch.Tensor | None = None,
                     want_routes: bool = False):
-        """The whole layer for at most ``FEW_MAX_ROWS`` rows on bf16 activations (no activation
-        quantisation), out = bf16(residual + shared_delta + routed), rounded once."""
+        """The whole layer for at most ``FEW_MAX_ROWS`` rows on bf16 activations (no activation quantisation; the
+        SwiGLU rows are rounded to fp16's 11 bits), out = bf16(residual + shared_delta + routed), rounded once."""
         idx = w = None
         if want_routes:
             rows = hidden_bf16.shape[0]

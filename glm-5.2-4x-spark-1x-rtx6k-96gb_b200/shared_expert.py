@@ -74,8 +74,10 @@ class SparseBlock:
     residual stream and normalises it (``block_norm``), runs the shared expert and the routed experts on the
     normalised rows, and returns the new residual stream (glm_moe_dsa_layer_ref.py:157-206).
 
-    Batches of at most ``few_rows`` rows go through ``MoeLayer.forward_few`` (bf16 activations in the
-    experts), larger ones through ``forward_residual`` (NVFP4 activations); 0 keeps all on the latter.
+    Batches of at most ``few_rows`` rows (default: as many as it takes, 16) go through ``MoeLayer.forward_few`` (bf16
+    activations in the experts), larger ones through ``forward_residual`` (NVFP4 activations); 0 keeps all on the latter.
+    The default is for accuracy: of the layer 6144 / 2048 with 256 experts the former is the faster one up to 4 rows (1 row
+    48 against 57 us, 4 rows 130 / 134), even at 5 and slower above (8 rows 240 / 212, 16 rows 445 / 340).
     """
 
     def __init__(self, routed_layer, shared: DenseSharedExpert, norm_weight: torch.Tensor, eps: float = 1e-5,

@@ -393,8 +393,9 @@ glmrt_status_t glmrt_cuda_residual_add_shared_f32_delta_bf16_async(
 /* 0 = one row for all rows, column stride 0 = one value per row, else 1.        */
 /* Without a delta (null) post_weight, gate and residual_out must be null and    */
 /* only normalized is written.  An output may be one of the row inputs (same     */
-/* address and stride); other overlaps are refused.  width 1..32768; rows 0 is   */
-/* accepted and does nothing.                                                    */
+/* address and stride); other overlaps are refused (of the spans from first to   */
+/* last value, so the rows of two buffers may not interleave).  width 1..32768;  */
+/* rows 0 is accepted and does nothing.                                          */
 /* ------------------------------------------------------------------------ */
 typedef enum glmrt_b200_dtype_t {
   GLMRT_B200_DTYPE_BF16 = 0,
@@ -555,7 +556,9 @@ glmrt_status_t glmrt_b200_moe_layer_forward_residual_async(
 /* The whole sparse layer for a few rows (at most GLMRT_B200_FEW_MAX_ROWS and max_tokens) on bf16 activations:
  * router, expert FFN with the NVFP4 weights and unquantised activations (W4A16: the arithmetic of the
  * reference's decode kernels, native/cuda/kernels/b12x_direct.cu:171-201,989-1541), weighted combine;
- * output = bf16(residual + shared_delta + routed), rounded once (nearest even).  residual, shared_delta,
+ * output = bf16(residual + shared_delta + routed), rounded once (nearest even).  Sums are float32; the SwiGLU rows
+ * between the products are rounded to fp16's 11 bits with a power of two of their own (2^-11 of a value, or 2^-39 of a
+ * share's largest where a value is more than 2^28 below it).  Routes are the router's of the other forwards.  residual, shared_delta,
  * topk_indices and topk_weights may each be null and lie apart from every other buffer; output may be residual or
  * shared_delta, and no other input.
  * Needs ep_world == 1.  Results differ from glmrt_b200_moe_layer_forward_async, which quantises the
