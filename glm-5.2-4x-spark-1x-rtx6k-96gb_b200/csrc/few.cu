@@ -36,7 +36,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 // What bounds it is the experts' weights (9/16 byte each, read once); everything else is arranged so
 // that they never stop arriving.  Measured at 6144 / 2048, 256 experts, top-8, back to back: 1 row 48 us (170 MB; 9 us
 // until the routes are known, 19 us gate / up, 2 us barrier, 11 us down, 5 us barrier and combine), 4 rows 130, 8 rows
-// 235 to 250, 16 rows 429 to 459 us (2.2 GB: 4.7 to 5.1 TB/s, by then bound by issue slots, 295 instructions a slot).  Each lane copies its own pieces of the weights into shared memory
+// 235 to 262, 16 rows 429 to 462 us (2.2 GB: 4.7 to 5.1 TB/s, by then bound by issue slots, 295 instructions a slot).  Each lane copies its own pieces of the weights into shared memory
 // (cp.async), kRing - 1 slots ahead, and only itself reads them back, so the stream needs no barrier
 // between warps; it runs on from the gate / up rows into the down rows while the CTA waits at the
 // barrier between them.
