@@ -1,6 +1,7 @@
 """GPU test of a bounded wait that runs out: every lane of the warp gets the same answer."""
 import ctypes as C
 import os
+import shutil
 import subprocess
 
 import pytest
@@ -43,7 +44,8 @@ def test_expired_wait_has_one_answer_for_the_warp(pkg, tmp_path):
     csrc = os.path.join(os.path.dirname(pkg.__file__), "csrc")
     (tmp_path / "waits.cu").write_text(SOURCE)
     lib = tmp_path / "libwaits.so"
-    subprocess.run(["nvcc", "-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "--expt-relaxed-constexpr", "-shared",
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    subprocess.run([nvcc, "-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "--expt-relaxed-constexpr", "-shared",
                     "-Xcompiler", "-fPIC", "-I", csrc, "-I", os.path.join(csrc, "..", "..", "include"), "-o", str(lib), str(tmp_path / "waits.cu")],
                    check=True, timeout=300)
     out = torch.full((4, 32), 9, dtype=torch.int32, device="cuda")
